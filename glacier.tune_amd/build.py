@@ -51,6 +51,9 @@ SOURCES = {
     "proj_lora.hip": (),
     "proj_gemm.hip": (),
     "rmsnorm.hip": (),
+    "qk_norm.hip": (),
+    "cache_append.hip": (),
+    "cache_attn.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
     "lmhead.hip": (),
     "lora_file.cpp": (),
     "engine.cpp": (),

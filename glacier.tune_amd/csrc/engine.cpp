@@ -22,11 +22,13 @@
 #include <vector>
 
 #include "../../include/glacier_attn.h"
+#include "../../include/glacier_cache.h"
 #include "../../include/glacier_lmhead.h"
 #include "../../include/glacier_norm.h"
 #include "../../include/glacier_qkv.h"
 #include "attn_launch.hpp"
 #include "blas_lt.hpp"
+#include "cache_launch.hpp"
 #include "lmhead_launch.hpp"
 #include "lora_file.hpp"
 #include "noalloc.hpp"
@@ -522,6 +524,7 @@ class GpuAttentionEngine {
   int precision() const { return precision_; }
   KernelTimer& timer() { return timer_; }
   void activate() { check_hip(hipSetDevice(device_), "hipSetDevice"); }
+  int device() const { return device_; }
 
   // ---- device entry points --------------------------------------------
   // LaunchRopeBatch + LaunchAttnTrainFwd (GpuLoraEngine.Forward.cs:401-465).
@@ -824,6 +827,30 @@ class GpuAttentionEngine {
     check_hip(launch_rmsnorm_backward(a, stream(), &timer_), "rmsnorm backward launch");
   }
 
+  // ---- per-head norms of queries and keys, the paged cache ---------------
+  // (glacier_norm.h, glacier_cache.h)
+  void QkNormForward(const QkNorm& a, float base) {
+    if (a.T == 0) return;
+    check_hip(launch_qk_norm_forward(a, turn_rates(base, a.D), n_cu_, stream()), "q/k norm forward launch");
+  }
+  void QkNormBackward(const QkNorm& a, float base) {
+    if (a.T == 0) return;
+    check_hip(launch_qk_norm_backward(a, turn_rates(base, a.D), n_cu_, stream()),
+              "q/k norm backward launch");
+  }
+  void AppendToCache(const CacheAppend& a, float base) {
+    if (a.c.T == 0 || a.c.n_seqs == 0) return;
+    check_hip(launch_cache_append(a, turn_rates(base, a.c.D), n_cu_, stream()), "cache append launch");
+  }
+  CachePlan PlanCacheAttention(const CacheView& c, int hq, int max_new, int max_kv) const {
+    if (c.T == 0 || c.n_seqs == 0) return CachePlan{};
+    return cache_attn_plan(c, hq, max_new, max_kv, n_cu_);
+  }
+  void AttendToCache(const CacheAttn& a) {
+    if (a.c.T == 0 || a.c.n_seqs == 0) return;
+    check_hip(launch_cache_attn(a, stream()), "cache attention launch");
+  }
+
   // ---- LM-head cross-entropy (glacier_lmhead.h) -------------------------
   // FusedCrossEntropyLoss.ComputeLoss / ComputeLossAndGradients
   // (FusedCrossEntropyLoss.cs:38-364): the kept rows are found on the host
@@ -967,6 +994,18 @@ class GpuAttentionEngine {
     rope_base_ = base;
   }
 
+  // The rotation rates of head size D and theta = base (0: no rotation),
+  // formed again only when they change.
+  const TurnRates& turn_rates(float base, int D) {
+    if (base > 0.0f && (turn_base_ != base || turn_dim_ != D)) {
+      for (int i = 0; i < D / 2; ++i)
+        turn_.rev[i] = std::pow(static_cast<double>(base), -2.0 * i / D) / (2.0 * M_PI);
+      turn_base_ = base;
+      turn_dim_ = D;
+    }
+    return turn_;
+  }
+
   const TileSet& tiles_for(const Shape& s) {
     auto it = tile_cache_.find(s.cu);
     if (it != tile_cache_.end()) return *it->second;
@@ -1083,6 +1122,9 @@ class GpuAttentionEngine {
     a.shadow = need.shadow > 0 ? shadow_.ensure(need.shadow, "projection output") : nullptr;
   }
 
+  TurnRates turn_{};
+  float turn_base_ = 0.0f;
+  int turn_dim_ = 0;
   int device_;
   int precision_;
   hipStream_t own_stream_ = nullptr;
@@ -1290,6 +1332,159 @@ void norm_check(const glacier_norm_desc* desc) {
 void need_row_tensor(const void* p, const char* name, bool has_rows) {
   if (has_rows && p == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, std::string(name) + " is NULL");
   if (!aligned16(p)) fail(GLACIER_ATTN_ERR_UNSUPPORTED, std::string(name) + " must be 16-byte aligned");
+}
+
+// The engine's device for a call's duration; the caller's afterwards.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) {
+    check_hip(hipGetDevice(&old_), "hipGetDevice");
+    if (old_ != device) check_hip(hipSetDevice(device), "hipSetDevice");
+    changed_ = old_ != device;
+  }
+  ~DeviceScope() {
+    if (changed_) (void)hipSetDevice(old_);
+  }
+
+ private:
+  int old_ = 0;
+  bool changed_ = false;
+};
+
+bool overlaps(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a != nullptr && b != nullptr && x < y + bn && y < x + an;
+}
+
+// An output that shares memory with an input other than the one it may replace.
+void need_apart(const void* out, size_t out_bytes, const char* name, const void* in, size_t in_bytes,
+                const char* in_name, bool same_ok) {
+  if (same_ok && out == in) return;
+  if (overlaps(out, out_bytes, in, in_bytes))
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, std::string(name) + " overlaps " + in_name);
+}
+
+void need_base(float base) {
+  if (base != 0.0f && (!(base > 0.0f) || !std::isfinite(base)))
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "rope_freq_base must be positive and finite, or 0 for no rotation");
+}
+
+void need_head_dim(int d) {
+  if (d <= 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "head_dim must be positive");
+  if (d % 8 != 0 || d > kTurnMaxDim)
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 up to " +
+                                           std::to_string(kTurnMaxDim) + ", not " + std::to_string(d));
+}
+
+void need_workspace(const void* p, size_t have, size_t want) {
+  if (want == 0) return;
+  if (p == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "workspace is NULL");
+  if (have < want)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "workspace of " + std::to_string(have) + " bytes, the call needs " +
+                                                std::to_string(want));
+  if ((reinterpret_cast<uintptr_t>(p) & 255) != 0)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+}
+
+// Checks a glacier_rmsnorm_qk_desc and fills the shape part of the launch.
+QkNorm qk_norm_of(const glacier_rmsnorm_qk_desc* desc) {
+  if (desc == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "desc is NULL");
+  const glacier_rmsnorm_qk_desc& d = *desc;
+  if (d.total_tokens < 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "total_tokens must be >= 0");
+  if (d.n_heads_q <= 0 || d.n_heads_kv <= 0)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "head counts must be positive");
+  if (d.io_dtype != GLACIER_ATTN_IO_F32 && d.io_dtype != GLACIER_ATTN_IO_BF16)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "unknown io dtype " + std::to_string(d.io_dtype));
+  if (!std::isfinite(d.eps) || d.eps < 0.0f)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
+  need_base(d.rope_freq_base);
+  need_head_dim(d.head_dim);
+  if ((long long)d.total_tokens * ((long long)d.n_heads_q + d.n_heads_kv) >= (1LL << 31))
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
+  QkNorm a{};
+  a.T = d.total_tokens;
+  a.hq = d.n_heads_q;
+  a.hkv = d.n_heads_kv;
+  a.D = d.head_dim;
+  a.eps = d.eps;
+  a.io_bf16 = d.io_dtype == GLACIER_ATTN_IO_BF16;
+  a.rotate = d.rope_freq_base > 0.0f;
+  return a;
+}
+
+size_t qk_norm_workspace(const QkNorm& a) { return sizeof(float) * kQkMaxGroups * 2 * a.D; }
+
+// Checks a cache and a batch (not the device arrays' contents, which the
+// kernels bound) and fills their part of a launch.
+CacheView cache_view_of(const glacier_kv_cache* cache, const glacier_cache_batch* batch) {
+  if (cache == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "cache is NULL");
+  if (batch == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "batch is NULL");
+  const glacier_kv_cache& k = *cache;
+  const glacier_cache_batch& b = *batch;
+  if (k.n_pages < 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "n_pages must be >= 0");
+  if (k.n_heads_kv <= 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "head counts must be positive");
+  if (k.io_dtype != GLACIER_ATTN_IO_F32 && k.io_dtype != GLACIER_ATTN_IO_BF16)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "unknown io dtype " + std::to_string(k.io_dtype));
+  need_head_dim(k.head_dim);
+  if (k.page_size < 16 || k.page_size > 1024 || (k.page_size & (k.page_size - 1)) != 0)
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "page_size must be a power of two from 16 to 1024, not " +
+                                           std::to_string(k.page_size));
+  const long long page = (long long)k.n_heads_kv * k.page_size * k.head_dim;
+  if (k.page_stride < page)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "page_stride must be at least n_heads_kv page_size head_dim");
+  if (k.page_stride % 8 != 0) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "page_stride must be a multiple of 8");
+  if (k.page_stride >= (1LL << 40) || (long long)k.n_pages * k.page_stride >= (1LL << 46))
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "cache too large");
+  if (b.n_seqs < 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "n_seqs must be >= 0");
+  if (b.total_tokens < 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "total_tokens must be >= 0");
+  if (b.max_pages < 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "max_pages must be >= 0");
+  if (b.max_new < 0 || b.max_kv < 0)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "max_new and max_kv must be >= 0");
+  if (b.n_seqs > 1 && b.table_stride < b.max_pages)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "table_stride must be at least max_pages");
+  if ((long long)b.max_pages * k.page_size >= (1LL << 30))
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "max_pages page_size must be below 2^30");
+  CacheView c{};
+  c.k_pages = k.k_pages;
+  c.v_pages = k.v_pages;
+  c.page_stride = k.page_stride;
+  c.n_pages = k.n_pages;
+  for (c.page_shift = 4; (1 << c.page_shift) < k.page_size;) ++c.page_shift;
+  c.hkv = k.n_heads_kv;
+  c.D = k.head_dim;
+  c.io_bf16 = k.io_dtype == GLACIER_ATTN_IO_BF16;
+  c.cu = b.cu_tokens;
+  c.kv_lens = b.kv_lens;
+  c.table = b.page_table;
+  c.table_stride = b.table_stride;
+  c.n_seqs = b.n_seqs;
+  c.T = b.total_tokens;
+  c.max_pages = b.max_pages;
+  return c;
+}
+
+// The device pointers of a cache and batch that a call is going to use.
+void need_cache_arrays(const CacheView& c) {
+  if (c.T == 0 || c.n_seqs == 0) return;
+  if (c.cu == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "cu_tokens is NULL");
+  if (c.kv_lens == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "kv_lens is NULL");
+  if (c.table == nullptr && c.max_pages > 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "page_table is NULL");
+  need_row_tensor(c.k_pages, "k_pages", c.n_pages > 0);
+  need_row_tensor(c.v_pages, "v_pages", c.n_pages > 0);
+}
+
+// Query heads of a call over the cache.
+void need_heads_q(const CacheView& c, int hq) {
+  if (hq <= 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "head counts must be positive");
+  if (hq % c.hkv != 0)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT,
+         "n_heads_q (" + std::to_string(hq) + ") must be a multiple of n_heads_kv (" + std::to_string(c.hkv) + ")");
+}
+void need_cache_size(const CacheView& c, int heads) {
+  if ((long long)c.T * heads >= (1LL << 31) || c.n_seqs >= (1 << 30) ||
+      (long long)c.T * heads * c.D >= (1LL << 40))
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
+  if (c.hkv > 65535) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "more than 65535 KV heads");
 }
 
 void need(const void* p, const char* name) {
@@ -1564,6 +1759,167 @@ int glacier_rmsnorm_backward(glacier_attn_ctx* ctx, const glacier_norm_desc* des
     std::lock_guard<std::mutex> g(ctx->eng->lock());
     ctx->eng->activate();
     ctx->eng->NormBackward(a);
+  });
+}
+
+int glacier_rmsnorm_qk_forward(glacier_attn_ctx* ctx, const glacier_rmsnorm_qk_desc* desc, const void* q,
+                               const void* k, const float* q_weight, const float* k_weight,
+                               const int32_t* positions, void* q_out, void* k_out) {
+  return guarded([&] {
+    glacier::QkNorm a = glacier::qk_norm_of(desc);
+    const bool rows = a.T > 0;
+    glacier::need_row_tensor(q, "q", rows);
+    glacier::need_row_tensor(k, "k", rows);
+    glacier::need_row_tensor(q_out, "q_out", rows);
+    glacier::need_row_tensor(k_out, "k_out", rows);
+    if (rows) {
+      need(q_weight, "q_weight"); need(k_weight, "k_weight");
+    }
+    const size_t esz = a.io_bf16 ? 2 : 4;
+    const size_t qb = esz * a.T * a.hq * a.D, kb = esz * a.T * a.hkv * a.D;
+    glacier::need_apart(q_out, qb, "q_out", q, qb, "q", true);
+    glacier::need_apart(q_out, qb, "q_out", k, kb, "k", false);
+    glacier::need_apart(k_out, kb, "k_out", q, qb, "q", false);
+    glacier::need_apart(k_out, kb, "k_out", k, kb, "k", true);
+    glacier::need_apart(k_out, kb, "k_out", q_out, qb, "q_out", false);
+    need(ctx, "ctx");
+    a.q = q; a.k = k; a.wq = q_weight; a.wk = k_weight; a.positions = positions;
+    a.yq = q_out; a.yk = k_out;
+    std::lock_guard<std::mutex> g(ctx->eng->lock());
+    glacier::DeviceScope on(ctx->eng->device());
+    ctx->eng->QkNormForward(a, desc->rope_freq_base);
+  });
+}
+
+size_t glacier_rmsnorm_qk_workspace(const glacier_rmsnorm_qk_desc* desc) {
+  size_t bytes = 0;
+  (void)guarded([&] { bytes = glacier::qk_norm_workspace(glacier::qk_norm_of(desc)); });
+  return bytes;
+}
+
+int glacier_rmsnorm_qk_backward(glacier_attn_ctx* ctx, const glacier_rmsnorm_qk_desc* desc,
+                                const void* dq_out, const void* dk_out, const void* q, const void* k,
+                                const float* q_weight, const float* k_weight, const int32_t* positions,
+                                void* dq, void* dk, float* dq_weight, float* dk_weight, void* workspace,
+                                size_t workspace_bytes) {
+  return guarded([&] {
+    glacier::QkNorm a = glacier::qk_norm_of(desc);
+    const bool rows = a.T > 0;
+    glacier::need_row_tensor(dq_out, "dq_out", rows);
+    glacier::need_row_tensor(dk_out, "dk_out", rows);
+    glacier::need_row_tensor(q, "q", rows);
+    glacier::need_row_tensor(k, "k", rows);
+    glacier::need_row_tensor(dq, "dq", rows);
+    glacier::need_row_tensor(dk, "dk", rows);
+    if (rows) {
+      need(q_weight, "q_weight"); need(k_weight, "k_weight");
+    }
+    const size_t esz = a.io_bf16 ? 2 : 4;
+    const size_t qb = esz * a.T * a.hq * a.D, kb = esz * a.T * a.hkv * a.D;
+    glacier::need_apart(dq, qb, "dq", dq_out, qb, "dq_out", true);
+    glacier::need_apart(dq, qb, "dq", dk_out, kb, "dk_out", false);
+    glacier::need_apart(dq, qb, "dq", q, qb, "q", false);
+    glacier::need_apart(dq, qb, "dq", k, kb, "k", false);
+    glacier::need_apart(dk, kb, "dk", dq_out, qb, "dq_out", false);
+    glacier::need_apart(dk, kb, "dk", dk_out, kb, "dk_out", true);
+    glacier::need_apart(dk, kb, "dk", q, qb, "q", false);
+    glacier::need_apart(dk, kb, "dk", k, kb, "k", false);
+    glacier::need_apart(dk, kb, "dk", dq, qb, "dq", false);
+    const bool dw = dq_weight != nullptr || dk_weight != nullptr;
+    if (dw && dq_weight == dk_weight)
+      fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "dq_weight and dk_weight are the same array");
+    if (dw && rows) glacier::need_workspace(workspace, workspace_bytes, glacier::qk_norm_workspace(a));
+    need(ctx, "ctx");
+    a.dq_out = dq_out; a.dk_out = dk_out; a.q = q; a.k = k; a.wq = q_weight; a.wk = k_weight;
+    a.positions = positions; a.yq = dq; a.yk = dk; a.dwq = dq_weight; a.dwk = dk_weight;
+    a.partials = static_cast<float*>(workspace);
+    std::lock_guard<std::mutex> g(ctx->eng->lock());
+    glacier::DeviceScope on(ctx->eng->device());
+    ctx->eng->QkNormBackward(a, desc->rope_freq_base);
+  });
+}
+
+int glacier_attn_cache_append(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
+                              const glacier_cache_batch* batch, const void* k, const void* v,
+                              float rope_freq_base, int32_t n_heads_q, const void* q, void* q_rot) {
+  return guarded([&] {
+    glacier::CacheAppend a{};
+    a.c = glacier::cache_view_of(cache, batch);
+    glacier::need_base(rope_freq_base);
+    const bool rows = a.c.T > 0 && a.c.n_seqs > 0;
+    if (q != nullptr) {
+      glacier::need_heads_q(a.c, n_heads_q);
+      a.hq = n_heads_q;
+      if (rope_freq_base == 0.0f)
+        fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "q is given, but there is no rotation (rope_freq_base is 0)");
+      glacier::need_row_tensor(q_rot, "q_rot", rows);
+    }
+    glacier::need_cache_size(a.c, a.hq + 2 * a.c.hkv);
+    glacier::need_cache_arrays(a.c);
+    glacier::need_row_tensor(k, "k", rows);
+    glacier::need_row_tensor(v, "v", rows);
+    glacier::need_row_tensor(q, "q", false);
+    const size_t esz = a.c.io_bf16 ? 2 : 4;
+    const size_t qb = esz * a.c.T * a.hq * a.c.D, kb = esz * a.c.T * a.c.hkv * a.c.D;
+    if (q != nullptr) {
+      glacier::need_apart(q_rot, qb, "q_rot", q, qb, "q", true);
+      glacier::need_apart(q_rot, qb, "q_rot", k, kb, "k", false);
+      glacier::need_apart(q_rot, qb, "q_rot", v, kb, "v", false);
+    }
+    need(ctx, "ctx");
+    a.rotate = rope_freq_base > 0.0f;
+    a.k = k; a.v = v; a.q = q; a.q_rot = q_rot;
+    std::lock_guard<std::mutex> g(ctx->eng->lock());
+    glacier::DeviceScope on(ctx->eng->device());
+    ctx->eng->AppendToCache(a, rope_freq_base);
+  });
+}
+
+size_t glacier_attn_cache_workspace(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
+                                    const glacier_cache_batch* batch, int32_t n_heads_q) {
+  size_t bytes = 0;
+  (void)guarded([&] {
+    const glacier::CacheView c = glacier::cache_view_of(cache, batch);
+    glacier::need_heads_q(c, n_heads_q);
+    glacier::need_cache_size(c, n_heads_q);
+    need(ctx, "ctx");
+    bytes = ctx->eng->PlanCacheAttention(c, n_heads_q, batch->max_new, batch->max_kv).bytes;
+  });
+  return bytes;
+}
+
+int glacier_attn_cache_forward(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
+                               const glacier_cache_batch* batch, int32_t n_heads_q, const void* q, void* out,
+                               float* lse, void* workspace, size_t workspace_bytes) {
+  return guarded([&] {
+    glacier::CacheAttn a{};
+    a.c = glacier::cache_view_of(cache, batch);
+    glacier::need_heads_q(a.c, n_heads_q);
+    glacier::need_cache_size(a.c, n_heads_q);
+    glacier::need_cache_arrays(a.c);
+    const bool rows = a.c.T > 0 && a.c.n_seqs > 0;
+    glacier::need_row_tensor(q, "q", rows);
+    glacier::need_row_tensor(out, "out", rows);
+    const size_t qb = (a.c.io_bf16 ? 2 : 4) * (size_t)a.c.T * n_heads_q * a.c.D;
+    glacier::need_apart(out, qb, "out", q, qb, "q", true);
+    need(ctx, "ctx");
+    const glacier::CachePlan p = ctx->eng->PlanCacheAttention(a.c, n_heads_q, batch->max_new, batch->max_kv);
+    glacier::need_workspace(workspace, workspace_bytes, p.bytes);
+    a.hq = n_heads_q;
+    a.group = n_heads_q / a.c.hkv;
+    a.scale_log2 = glacier::kLog2e / std::sqrt(static_cast<float>(a.c.D));
+    a.q = q; a.out = out; a.lse = lse;
+    a.rows = p.rows;
+    a.n_splits = p.n_splits;
+    a.split_keys = p.split_keys;
+    if (p.n_splits > 1) {
+      const size_t sums = p.n_splits * (size_t)a.c.T * n_heads_q * a.c.D;
+      a.part_o = static_cast<float*>(workspace);
+      a.part_ml = reinterpret_cast<float2*>(a.part_o + sums);
+    }
+    std::lock_guard<std::mutex> g(ctx->eng->lock());
+    glacier::DeviceScope on(ctx->eng->device());
+    ctx->eng->AttendToCache(a);
   });
 }
 

@@ -1,0 +1,238 @@
+// qk_norm.hip -- the per-head RMS norms of a layer's queries and keys with the
+// position rotation in the same pass, forward and backward:
+//   forward   y = R(pos) (x r w),  r = 1 / sqrt(mean x^2 + eps)
+//   backward  g = R(-pos) dy,  dx = r w g - (r^3 / D) x sum w g x,
+//             dw += sum over tokens and heads of g x r
+// (the norms of TransformerBlock.cs:413, :421, :751 and :759, and the rotation
+// that follows them).
+//
+// HBM-bound: each row is read once and written once, a head's sums are one
+// fixed-order reduction over the lanes that hold it (turn.hpp), and queries and
+// keys share the launch.  Each lane reads its pieces before it writes them, so
+// outputs may lie on inputs.
+//
+// Weight gradients: a lane meets the same columns in every head and token, so
+// it sums them in registers; a workgroup's sums go to the workspace and a second
+// launch adds the workgroups in order.  No atomics: results are bitwise
+// repeatable.
+#include "turn.hpp"
+
+namespace glacier {
+namespace {
+
+constexpr int kWavesQk = 4;
+
+template <typename IO, int E, int L>
+__global__ __launch_bounds__(64 * kWavesQk) void qk_norm_fwd_kernel(QkNorm a, TurnRates rates) {
+  constexpr int H = 64 / L;  // heads per step
+  __shared__ float2 turns[kWavesQk][kTurnMaxDim / 2];
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  const int unit = blockIdx.x * kWavesQk + wave;
+  const int t = unit / a.parts, part = unit % a.parts;
+  if (t >= a.T) return;
+  const int half = a.D / 2, heads = a.hq + a.hkv;
+  const int ch = lane % L, col = ch * E;
+  const bool in_row = col < half;
+  if (a.rotate) turn_table(turns[wave], rates, half, a.positions != nullptr ? a.positions[t] : t, lane);
+  for (int h0 = part * H; h0 < heads; h0 += a.parts * H) {
+    const int h = h0 + lane / L;
+    const bool ok = in_row && h < heads, is_q = h < a.hq;
+    const long at = is_q ? ((long)t * a.hq + h) * a.D : ((long)t * a.hkv + (h - a.hq)) * a.D;
+    const float* w = is_q ? a.wq : a.wk;
+    float x0[E] = {}, x1[E] = {}, w0[E] = {}, w1[E] = {};
+    if (ok) {
+      const IO* x = static_cast<const IO*>(is_q ? a.q : a.k) + at + col;
+      Piece<IO, E> p0, p1;
+      p0.load(x);
+      p1.load(x + half);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        w0[e] = w[col + e];
+        w1[e] = w[half + col + e];
+      }
+      p0.get(x0);
+      p1.get(x1);
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss += x0[e] * x0[e] + x1[e] * x1[e];
+    const float r = 1.0f / sqrtf(lanes_sum<L>(ss) / (float)a.D + a.eps);
+    if (!ok) continue;
+    float y0[E], y1[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      y0[e] = (x0[e] * r) * w0[e];
+      y1[e] = (x1[e] * r) * w1[e];
+      if (a.rotate) {
+        const float2 cs = turns[wave][col + e];
+        rope_fwd(y0[e], y1[e], cs.x, cs.y, y0[e], y1[e]);
+      }
+    }
+    IO* y = static_cast<IO*>(is_q ? a.yq : a.yk) + at + col;
+    Piece<IO, E> o0, o1;
+    o0.set(y0);
+    o1.set(y1);
+    o0.store(y);
+    o1.store(y + half);
+  }
+}
+
+// DW: the weight gradients are formed.
+template <typename IO, int E, int L, bool DW>
+__global__ __launch_bounds__(64 * kWavesQk) void qk_norm_bwd_kernel(QkNorm a, TurnRates rates) {
+  constexpr int H = 64 / L;
+  __shared__ float2 turns[kWavesQk][kTurnMaxDim / 2];
+  __shared__ float sums[DW ? kWavesQk : 1][DW ? 2 * kTurnMaxDim : 1];
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  const int half = a.D / 2, heads = a.hq + a.hkv;
+  const int ch = lane % L, col = ch * E;
+  const bool in_row = col < half;
+  float dq0[E] = {}, dq1[E] = {}, dk0[E] = {}, dk1[E] = {};
+  const int units = a.T * a.parts;
+  for (int unit = blockIdx.x * kWavesQk + wave; unit < units; unit += gridDim.x * kWavesQk) {
+    const int t = unit / a.parts, part = unit % a.parts;
+    if (a.rotate) turn_table(turns[wave], rates, half, a.positions != nullptr ? a.positions[t] : t, lane);
+    for (int h0 = part * H; h0 < heads; h0 += a.parts * H) {
+      const int h = h0 + lane / L;
+      const bool ok = in_row && h < heads, is_q = h < a.hq;
+      const long at = is_q ? ((long)t * a.hq + h) * a.D : ((long)t * a.hkv + (h - a.hq)) * a.D;
+      const float* w = is_q ? a.wq : a.wk;
+      float x0[E] = {}, x1[E] = {}, g0[E] = {}, g1[E] = {}, w0[E] = {}, w1[E] = {};
+      if (ok) {
+        const IO* x = static_cast<const IO*>(is_q ? a.q : a.k) + at + col;
+        const IO* dy = static_cast<const IO*>(is_q ? a.dq_out : a.dk_out) + at + col;
+        Piece<IO, E> p0, p1, d0, d1;
+        p0.load(x);
+        p1.load(x + half);
+        d0.load(dy);
+        d1.load(dy + half);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          w0[e] = w[col + e];
+          w1[e] = w[half + col + e];
+        }
+        p0.get(x0);
+        p1.get(x1);
+        d0.get(g0);
+        d1.get(g1);
+      }
+      float ss = 0.0f, c = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (a.rotate && in_row) {
+          const float2 cs = turns[wave][col + e];
+          rope_inv(g0[e], g1[e], cs.x, cs.y, g0[e], g1[e]);
+        }
+        ss += x0[e] * x0[e] + x1[e] * x1[e];
+        c += (w0[e] * g0[e]) * x0[e] + (w1[e] * g1[e]) * x1[e];
+      }
+      ss = lanes_sum<L>(ss);
+      c = lanes_sum<L>(c);
+      if (!ok) continue;
+      const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+      const float kx = r * r * r / (float)a.D * c;
+      float o0[E], o1[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        o0[e] = r * (w0[e] * g0[e]) - kx * x0[e];
+        o1[e] = r * (w1[e] * g1[e]) - kx * x1[e];
+        if constexpr (DW) {
+          const float v0 = g0[e] * (x0[e] * r), v1 = g1[e] * (x1[e] * r);
+          dq0[e] += is_q ? v0 : 0.0f;
+          dq1[e] += is_q ? v1 : 0.0f;
+          dk0[e] += is_q ? 0.0f : v0;
+          dk1[e] += is_q ? 0.0f : v1;
+        }
+      }
+      IO* dx = static_cast<IO*>(is_q ? a.yq : a.yk) + at + col;
+      Piece<IO, E> s0, s1;
+      s0.set(o0);
+      s1.set(o1);
+      s0.store(dx);
+      s1.store(dx + half);
+    }
+  }
+  if constexpr (DW) {
+    // the lanes that hold the same columns (the wave's heads), then the waves
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+      for (int s = L; s < 64; s *= 2) {
+        dq0[e] += __shfl_xor(dq0[e], s);
+        dq1[e] += __shfl_xor(dq1[e], s);
+        dk0[e] += __shfl_xor(dk0[e], s);
+        dk1[e] += __shfl_xor(dk1[e], s);
+      }
+      if (lane < L && in_row) {
+        sums[wave][col + e] = dq0[e];
+        sums[wave][half + col + e] = dq1[e];
+        sums[wave][a.D + col + e] = dk0[e];
+        sums[wave][a.D + half + col + e] = dk1[e];
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * a.D; i += 64 * kWavesQk) {
+      float s = 0.0f;
+#pragma unroll
+      for (int u = 0; u < kWavesQk; ++u) s += sums[u][i];
+      a.partials[(long)blockIdx.x * 2 * a.D + i] = s;
+    }
+  }
+}
+
+// dw[i] += sum over the workgroups' partials, 8 groups of rows side by side.
+__global__ __launch_bounds__(256) void qk_norm_dw_kernel(QkNorm a, int groups) {
+  __shared__ float sums[8][32];
+  const int i = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+  float s = 0.0f;
+  if (i < 2 * a.D)
+    for (int g = part; g < groups; g += 8) s += a.partials[(long)g * 2 * a.D + i];
+  sums[part][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (part != 0 || i >= 2 * a.D) return;
+  float total = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) total += sums[u][threadIdx.x & 31];
+  float* dw = i < a.D ? a.dwq : a.dwk;
+  if (dw != nullptr) dw[i < a.D ? i : i - a.D] += total;
+}
+
+template <typename IO, int E, int L>
+hipError_t fwd(QkNorm& a, const TurnRates& r, int n_cu, hipStream_t st) {
+  a.parts = turn_parts(a.T, (a.hq + a.hkv + 64 / L - 1) / (64 / L), n_cu);
+  const long units = (long)a.T * a.parts;
+  hipLaunchKernelGGL((qk_norm_fwd_kernel<IO, E, L>), dim3((units + kWavesQk - 1) / kWavesQk),
+                     dim3(64 * kWavesQk), 0, st, a, r);
+  return hipGetLastError();
+}
+
+template <typename IO, int E, int L>
+hipError_t bwd(QkNorm& a, const TurnRates& r, int n_cu, hipStream_t st) {
+  a.parts = turn_parts(a.T, (a.hq + a.hkv + 64 / L - 1) / (64 / L), n_cu);
+  const long units = (long)a.T * a.parts;
+  const bool dw = a.dwq != nullptr || a.dwk != nullptr;
+  const int all = static_cast<int>((units + kWavesQk - 1) / kWavesQk);
+  const int groups = dw ? std::min(all, kQkMaxGroups) : all;
+  if (dw)
+    hipLaunchKernelGGL((qk_norm_bwd_kernel<IO, E, L, true>), dim3(groups), dim3(64 * kWavesQk), 0, st,
+                       a, r);
+  else
+    hipLaunchKernelGGL((qk_norm_bwd_kernel<IO, E, L, false>), dim3(groups), dim3(64 * kWavesQk), 0, st,
+                       a, r);
+  GL_CHECK(hipGetLastError());
+  if (!dw) return hipSuccess;
+  hipLaunchKernelGGL(qk_norm_dw_kernel, dim3((2 * a.D + 31) / 32), dim3(256), 0, st, a, groups);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_qk_norm_forward(QkNorm a, const TurnRates& r, int n_cu, hipStream_t st) {
+  GL_BY_HEAD(fwd, a.io_bf16, a.D, a, r, n_cu, st);
+}
+
+hipError_t launch_qk_norm_backward(QkNorm a, const TurnRates& r, int n_cu, hipStream_t st) {
+  GL_BY_HEAD(bwd, a.io_bf16, a.D, a, r, n_cu, st);
+}
+
+}  // namespace glacier

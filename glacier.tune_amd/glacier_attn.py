@@ -12,7 +12,11 @@ on host float32 numpy arrays, plus `forward` / `backward` on device-resident
 torch tensors (passed to the library as raw pointers, enqueued on torch's
 current stream), and `proj_forward` / `proj_backward`: the q/k/v projections
 with LoRA adapters on the device (include/glacier_qkv.h; GpuLoraEngine.ForwardQKV,
-GpuLoraEngine.Forward.cs:205-245, and LoraAdapter.Backward, LoraAdapter.cs:190-247).  Errors raise: InvalidArgument (a ValueError, where the C#
+GpuLoraEngine.Forward.cs:205-245, and LoraAdapter.Backward, LoraAdapter.cs:190-247).
+`qk_norm_forward` / `qk_norm_backward` are the per-head norms of queries and keys
+with the rotation (include/glacier_norm.h); `cache_append` and `cache_forward`
+the paged key/value cache that answers with the tuned model
+(include/glacier_cache.h).  Errors raise: InvalidArgument (a ValueError, where the C#
 engine throws ArgumentOutOfRangeException), Unsupported (the shape stays on
 the CPU path), DeviceError, OutOfMemory.  There is no fallback: if the
 library is missing or the device fails, the call raises.
@@ -28,8 +32,8 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libglacier_attn.so")
 HEADERS = [os.path.join(os.path.dirname(HERE), "include", h)
-           for h in ("glacier_attn.h", "glacier_qkv.h", "glacier_norm.h", "glacier_lmhead.h",
-                     "glacier_lora_file.h")]
+           for h in ("glacier_attn.h", "glacier_qkv.h", "glacier_norm.h", "glacier_cache.h",
+                     "glacier_lmhead.h", "glacier_lora_file.h")]
 
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_DEVICE, ERR_OUT_OF_MEMORY = 0, 1, 2, 3, 4
 PREC_FP32, PREC_BF16 = 0, 1
@@ -97,6 +101,48 @@ class NormDesc(ctypes.Structure):
         ("n", ctypes.c_int32),
         ("io_dtype", ctypes.c_int32),
         ("eps", ctypes.c_float),
+    ]
+
+
+class QkNormDesc(ctypes.Structure):
+    """glacier_rmsnorm_qk_desc (include/glacier_norm.h)."""
+    _fields_ = [
+        ("total_tokens", ctypes.c_int32),
+        ("n_heads_q", ctypes.c_int32),
+        ("n_heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("io_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("rope_freq_base", ctypes.c_float),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    """glacier_kv_cache (include/glacier_cache.h)."""
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("n_heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("io_dtype", ctypes.c_int32),
+    ]
+
+
+class CacheBatch(ctypes.Structure):
+    """glacier_cache_batch (include/glacier_cache.h)."""
+    _fields_ = [
+        ("cu_tokens", ctypes.c_void_p),
+        ("kv_lens", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("n_seqs", ctypes.c_int32),
+        ("total_tokens", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("max_new", ctypes.c_int32),
+        ("max_kv", ctypes.c_int32),
     ]
 
 
@@ -220,6 +266,16 @@ def load():
                                                ctypes.POINTER(ctypes.c_float), i32p]
     L.glacier_rmsnorm_forward.argtypes = [vp, ctypes.POINTER(NormDesc), vp, vp, vp, vp, vp]
     L.glacier_rmsnorm_backward.argtypes = [vp, ctypes.POINTER(NormDesc), vp, vp, vp, vp, vp, vp]
+    qp, kp, bp = ctypes.POINTER(QkNormDesc), ctypes.POINTER(KvCache), ctypes.POINTER(CacheBatch)
+    L.glacier_rmsnorm_qk_forward.argtypes = [vp, qp, vp, vp, vp, vp, vp, vp, vp]
+    L.glacier_rmsnorm_qk_workspace.argtypes = [qp]
+    L.glacier_rmsnorm_qk_workspace.restype = ctypes.c_size_t
+    L.glacier_rmsnorm_qk_backward.argtypes = [vp, qp] + [vp] * 12 + [ctypes.c_size_t]
+    L.glacier_attn_cache_append.argtypes = [vp, kp, bp, vp, vp, c_float, ctypes.c_int32, vp, vp]
+    L.glacier_attn_cache_workspace.argtypes = [vp, kp, bp, ctypes.c_int32]
+    L.glacier_attn_cache_workspace.restype = ctypes.c_size_t
+    L.glacier_attn_cache_forward.argtypes = [vp, kp, bp, ctypes.c_int32, vp, vp, vp, vp,
+                                             ctypes.c_size_t]
     L.glacier_proj_backward.argtypes = [vp, ctypes.POINTER(ProjDesc), vp,
                                         ctypes.POINTER(LoraProj), c_int, vp]
     _lib = L
@@ -375,6 +431,63 @@ def check_norm_args(x, weight, d_weight=None):
     _on_gpu(("x", x), ("weight", weight), ("d_weight", d_weight))
 
 
+def _address(t, name, shape, dtype, device):
+    """The address of a contiguous tensor of this shape and dtype on GPU `device`
+    (checked in that order)."""
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
+        _need(t, name, shape, dtype=dtype)
+    if t.get_device() != device:
+        raise TypeError(f"{name} must be on cuda:{device}, got {t.device}")
+    return t.data_ptr()
+
+
+def _optional(t, name, shape, dtype, device):
+    return None if t is None else _address(t, name, shape, dtype, device)
+
+
+def cache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, max_new, max_kv,
+               device):
+    """(glacier_kv_cache, glacier_cache_batch) of a cache and batch: pages
+    [n_pages, Hkv, page_size, D] of one dtype, each page contiguous and the
+    pages any one stride apart; cu_tokens [n + 1], kv_lens [n] and page_table
+    [n, max_pages] int32, the table's rows any stride apart."""
+    i32 = _torch().int32
+    if k_pages.dim() != 4:
+        raise TypeError("k_pages must be [n_pages, n_heads_kv, page_size, head_dim]")
+    n_pages, hkv, page, d = k_pages.shape
+    strides = []
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if t.shape != k_pages.shape or t.dtype is not k_pages.dtype:
+            raise TypeError(f"{name} must be {k_pages.dtype} of shape {tuple(k_pages.shape)}, got "
+                            f"{t.dtype} of {tuple(t.shape)}")
+        if n_pages < 2 or t.is_contiguous():
+            strides.append(hkv * page * d)
+        else:
+            strides.append(t.stride(0))
+        if not (t.is_contiguous() or (n_pages > 0 and t[0].is_contiguous())):
+            raise TypeError(f"{name}: each page must be contiguous")
+        if t.get_device() != device:
+            raise TypeError(f"{name} must be on cuda:{device}, got {t.device}")
+    if strides[0] != strides[1]:
+        raise TypeError(f"k_pages and v_pages must have one page stride, got {strides[0]} and {strides[1]}")
+    if page_table.dim() != 2 or page_table.dtype is not i32:
+        raise TypeError("page_table must be an int32 [n_seqs, max_pages] tensor")
+    n, most = page_table.shape
+    if most > 1 and page_table.stride(1) != 1:
+        raise TypeError("page_table's rows must be contiguous")
+    if page_table.get_device() != device:
+        raise TypeError(f"page_table must be on cuda:{device}, got {page_table.device}")
+    row = page_table.stride(0) if n > 1 else most
+    if row < most:
+        raise TypeError("page_table's rows must not overlap")
+    cache = KvCache(k_pages.data_ptr(), v_pages.data_ptr(), strides[0], n_pages, page, hkv, d,
+                    GpuAttentionEngine._io_of(k_pages))
+    batch = CacheBatch(_address(cu_tokens, "cu_tokens", (n + 1,), i32, device),
+                       _address(kv_lens, "kv_lens", (n,), i32, device), page_table.data_ptr(), row, n,
+                       total_tokens, most, int(max_new), int(max_kv))
+    return cache, batch
+
+
 class GpuAttentionEngine:
     """One library context: a device, a stream and grow-only scratch."""
 
@@ -384,6 +497,7 @@ class GpuAttentionEngine:
         _check(L.glacier_attn_create(int(device_ordinal), int(precision), ctypes.byref(h)))
         self._h = h
         self.precision = precision
+        self.device_ordinal = int(device_ordinal)
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -705,6 +819,134 @@ class GpuAttentionEngine:
                                                self._ptr(d_residual), self._ptr(dx),
                                                self._ptr(d_weight)))
         return dx
+
+    # ---- per-head norms of queries and keys (glacier_norm.h) ---------------
+    def _bind_device_stream(self):
+        """torch's current stream of this engine's device, whichever device is current."""
+        raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
+        dev = self.device_ordinal
+        stream = _torch_mod.cuda.current_stream(dev).cuda_stream if raw is None else raw(dev)
+        rc = load().glacier_attn_set_stream(self._h, stream)
+        if rc != OK:
+            _check(rc)
+
+    def _workspace(self, size):
+        """`size` bytes of torch's allocator on the current stream of the engine's
+        device (inside a capture: the graph's own memory)."""
+        if size == 0:
+            return None
+        return _torch().empty(size, dtype=_torch_mod.uint8, device=self.device_ordinal)
+
+    def _qk_args(self, q, k, q_weight, k_weight, eps, rope_freq_base, positions):
+        if q.dim() != 3 or k.dim() != 3:
+            raise TypeError("q must be [T, Hq, D] and k [T, Hkv, D]")
+        torch, dev = _torch(), self.device_ordinal
+        T, hq, d = q.shape
+        hkv = k.shape[1]
+        desc = QkNormDesc(T, hq, hkv, d, self._io_of(q), eps, rope_freq_base or 0.0)
+        return desc, (_address(q, "q", (T, hq, d), q.dtype, dev),
+                      _address(k, "k", (T, hkv, d), q.dtype, dev),
+                      _address(q_weight, "q_weight", (d,), torch.float32, dev),
+                      _address(k_weight, "k_weight", (d,), torch.float32, dev),
+                      _optional(positions, "positions", (T,), torch.int32, dev))
+
+    def qk_norm_forward(self, q, k, q_weight, k_weight, eps, rope_freq_base=None, positions=None,
+                        q_out=None, k_out=None):
+        """RMS norms of every head of q [T, Hq, D] and k [T, Hkv, D] (float32 or
+        bfloat16) with weights [D] (float32), then the rotation by positions
+        (int32 [T], None: 0 .. T - 1) unless rope_freq_base is None.  q_out may
+        be q and k_out k.  Returns (q_out, k_out)."""
+        desc, args = self._qk_args(q, k, q_weight, k_weight, eps, rope_freq_base, positions)
+        torch, dev = _torch_mod, self.device_ordinal
+        q_out = torch.empty_like(q) if q_out is None else q_out
+        k_out = torch.empty_like(k) if k_out is None else k_out
+        outs = (_address(q_out, "q_out", q.shape, q.dtype, dev),
+                _address(k_out, "k_out", k.shape, q.dtype, dev))
+        self._bind_device_stream()
+        _check(load().glacier_rmsnorm_qk_forward(self._h, ctypes.byref(desc), *args, *outs))
+        return q_out, k_out
+
+    def qk_norm_backward(self, dq_out, dk_out, q, k, q_weight, k_weight, eps, rope_freq_base=None,
+                         positions=None, dq=None, dk=None, dq_weight=None, dk_weight=None):
+        """Gradients of qk_norm_forward(q, k, ...) for upstream dq_out, dk_out:
+        returns (dq, dk); dq_weight and dk_weight (float32 [D], optional) are
+        accumulated.  dq may be dq_out and dk dk_out."""
+        desc, args = self._qk_args(q, k, q_weight, k_weight, eps, rope_freq_base, positions)
+        torch, dev = _torch_mod, self.device_ordinal
+        d = q.shape[2]
+        dq = torch.empty_like(q) if dq is None else dq
+        dk = torch.empty_like(k) if dk is None else dk
+        grads = (_address(dq_out, "dq_out", q.shape, q.dtype, dev),
+                 _address(dk_out, "dk_out", k.shape, q.dtype, dev))
+        outs = (_address(dq, "dq", q.shape, q.dtype, dev), _address(dk, "dk", k.shape, q.dtype, dev),
+                _optional(dq_weight, "dq_weight", (d,), torch.float32, dev),
+                _optional(dk_weight, "dk_weight", (d,), torch.float32, dev))
+        L, size, work = load(), 0, None
+        if dq_weight is not None or dk_weight is not None:
+            size = L.glacier_rmsnorm_qk_workspace(ctypes.byref(desc))
+            work = self._workspace(size)
+        self._bind_device_stream()
+        _check(L.glacier_rmsnorm_qk_backward(self._h, ctypes.byref(desc), *grads, *args, *outs,
+                                             self._ptr(work), size))
+        return dq, dk
+
+    # ---- paged key/value cache (glacier_cache.h) ---------------------------
+    def cache_append(self, k, v, k_pages, v_pages, cu_tokens, kv_lens, page_table,
+                     rope_freq_base=None, q=None, q_rot=None):
+        """Writes the new tokens' k and v [T, Hkv, D] into the pages
+        [n_pages, Hkv, page_size, D]: tokens cu_tokens[b] .. cu_tokens[b + 1] - 1
+        are the last ones of sequence b, whose length with them is kv_lens[b].
+        k is rotated by its positions unless rope_freq_base is None; then q
+        [T, Hq, D], if given, is rotated too, into q_rot (which may be q), and
+        returned."""
+        if k.dim() != 3:
+            raise TypeError("k must be [T, Hkv, D]")
+        dev, T = self.device_ordinal, k.shape[0]
+        cache, batch = cache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, T, 0, 0, dev)
+        shape, dt = (T, cache.n_heads_kv, cache.head_dim), k_pages.dtype
+        kp, vp = _address(k, "k", shape, dt, dev), _address(v, "v", shape, dt, dev)
+        hq, qp, rp = 0, None, None
+        if q is not None:
+            if q.dim() != 3:
+                raise TypeError("q must be [T, Hq, D]")
+            hq = q.shape[1]
+            q_rot = _torch_mod.empty_like(q) if q_rot is None else q_rot
+            qp = _address(q, "q", (T, hq, cache.head_dim), dt, dev)
+            rp = _address(q_rot, "q_rot", (T, hq, cache.head_dim), dt, dev)
+        self._bind_device_stream()
+        _check(load().glacier_attn_cache_append(self._h, ctypes.byref(cache), ctypes.byref(batch), kp,
+                                                vp, rope_freq_base or 0.0, hq, qp, rp))
+        return q_rot if q is not None else None
+
+    def cache_forward(self, q, k_pages, v_pages, cu_tokens, kv_lens, page_table, max_new=0, max_kv=0,
+                      out=None, lse=None, save=False):
+        """Attention of the new tokens' rotated queries q [T, Hq, D] over the
+        cached keys of their sequences up to their own position (arguments as
+        cache_append's).  max_new, max_kv: the longest chunk and sequence where
+        the caller knows them (0: not known); they steer the layout of the work,
+        not the result.  Returns (out, lse); lse float32 [Hq, T] is written when
+        given or save is set, else None.  Rows at or past cu_tokens[-1] are not
+        written."""
+        if q.dim() != 3:
+            raise TypeError("q must be [T, Hq, D]")
+        dev = self.device_ordinal
+        T, hq, _ = q.shape
+        cache, batch = cache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, T, max_new, max_kv,
+                                  dev)
+        shape, dt = (T, hq, cache.head_dim), k_pages.dtype
+        qp = _address(q, "q", shape, dt, dev)
+        torch = _torch_mod
+        out = torch.empty_like(q) if out is None else out
+        if lse is None and save:
+            lse = torch.empty((hq, T), dtype=torch.float32, device=q.device)
+        op = _address(out, "out", shape, dt, dev)
+        lp = _optional(lse, "lse", (hq, T), torch.float32, dev)
+        L, cp, bp = load(), ctypes.byref(cache), ctypes.byref(batch)
+        size = L.glacier_attn_cache_workspace(self._h, cp, bp, hq)
+        work = self._workspace(size)
+        self._bind_device_stream()
+        _check(L.glacier_attn_cache_forward(self._h, cp, bp, hq, qp, op, lp, self._ptr(work), size))
+        return out, lse
 
     # ---- LM-head cross-entropy (glacier_lmhead.h) -------------------------
     def _lmhead(self, hidden, targets, weight, d_hidden, grad, precision):

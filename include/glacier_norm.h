@@ -62,6 +62,49 @@ int glacier_rmsnorm_backward(glacier_attn_ctx *ctx, const glacier_norm_desc *des
                              const void *x, const float *weight, const void *d_residual, void *dx,
                              float *d_weight);
 
+/* ---- queries and keys of one layer --------------------------------------- */
+
+/* The per-head norms of a layer's queries and keys with the position rotation
+ * in the same pass:
+ *   forward   y = R(pos) (x r w),  r = 1 / sqrt(mean_i x_i^2 + eps) per token and head
+ *   backward  g = R(-pos) dy,  dx = r w g - (r^3 / D) x sum_j w_j g_j x_j,
+ *             d_weight += sum over tokens and heads of g x r
+ * (TransformerBlock.cs:413, :421, :751, :759, and the rotation of the call that
+ * follows them).  R turns the pairs (i, i + D/2) by pos * theta^(-2i/D), the
+ * angle reduced in 64 bits; rope_freq_base 0 leaves it out (for
+ * glacier_attn_forward, which rotates by itself).  The sums are fp32, and every
+ * result is rounded once. */
+typedef struct glacier_rmsnorm_qk_desc {
+  int32_t total_tokens;  /* T (may be 0) */
+  int32_t n_heads_q;     /* q [T][n_heads_q][D] */
+  int32_t n_heads_kv;    /* k [T][n_heads_kv][D] */
+  int32_t head_dim;      /* D: a multiple of 8, at most 256 */
+  int32_t io_dtype;      /* GLACIER_ATTN_IO_F32 or GLACIER_ATTN_IO_BF16 */
+  float eps;             /* finite and >= 0 */
+  float rope_freq_base;  /* theta, or 0 for no rotation */
+} glacier_rmsnorm_qk_desc;
+
+/* q_weight, k_weight [D] fp32; positions: device int32 [T], or NULL for
+ * 0 .. T - 1 (not read without a rotation).  q_out may be q, k_out may be k. */
+int glacier_rmsnorm_qk_forward(glacier_attn_ctx *ctx, const glacier_rmsnorm_qk_desc *desc,
+                               const void *q, const void *k, const float *q_weight,
+                               const float *k_weight, const int32_t *positions, void *q_out,
+                               void *k_out);
+
+/* Bytes of device workspace the backward needs when it forms weight gradients
+ * (0 if the arguments are not valid). */
+size_t glacier_rmsnorm_qk_workspace(const glacier_rmsnorm_qk_desc *desc);
+
+/* q, k: the forward's inputs.  dq, dk are overwritten and may be dq_out, dk_out.
+ * dq_weight, dk_weight [D] fp32 are accumulated (+=), each formed only when not
+ * NULL; then workspace holds at least glacier_rmsnorm_qk_workspace bytes,
+ * 256-byte aligned, the call's own until it has run. */
+int glacier_rmsnorm_qk_backward(glacier_attn_ctx *ctx, const glacier_rmsnorm_qk_desc *desc,
+                                const void *dq_out, const void *dk_out, const void *q,
+                                const void *k, const float *q_weight, const float *k_weight,
+                                const int32_t *positions, void *dq, void *dk, float *dq_weight,
+                                float *dk_weight, void *workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,286 @@
+"""The paged key/value cache (glacier_attn_cache_*), through the Python front
+end, against its definition in 64 bits."""
+import math
+
+import pytest
+
+import glacier_attn as ga
+
+torch = pytest.importorskip("torch")
+import cache_harness as ch  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+@pytest.fixture(scope="module")
+def eng():
+    assert torch.cuda.is_available(), "GPU tests need a ROCm GPU"
+    e = ga.GpuAttentionEngine(0, ga.PREC_BF16)
+    yield e
+    e.close()
+
+
+# (new tokens, tokens with them) per sequence; hq, hkv, D, page, rows behind
+BATCHES = {
+    "one_key": ([(1, 1)], 1, 1, 8, 16, 0),
+    "one_token": ([(1, 512)], 14, 2, 64, 16, 0),
+    "tokens": ([(1, 17), (1, 1), (1, 300), (1, 64), (1, 65)], 28, 4, 128, 16, 3),
+    "idle_among_them": ([(0, 40), (1, 33), (0, 0), (2, 2), (0, 7)], 8, 2, 96, 32, 1),
+    "whole_prompt": ([(77, 77)], 8, 8, 64, 64, 0),
+    "chunk": ([(50, 190)], 28, 4, 128, 32, 0),
+    "ragged_chunks": ([(5, 5), (130, 300), (1, 1000), (64, 64), (0, 10), (33, 97)], 32, 8, 128, 16, 19),
+    "odd_head": ([(3, 40), (20, 21)], 5, 1, 80, 128, 2),
+    "narrow_head": ([(9, 70), (1, 129)], 16, 4, 32, 16, 0),
+    "wide_head": ([(6, 50), (1, 200)], 8, 2, 256, 16, 0),
+    "between_heads": ([(4, 90)], 6, 3, 200, 64, 0),
+    "many_heads": ([(3, 50)], 40, 1, 64, 16, 0),
+    "long": ([(1, 9000), (2, 300)], 16, 4, 128, 256, 0),
+    "long_chunk": ([(40, 5000)], 14, 2, 64, 1024, 0),
+    "many_sequences": ([(1, 20 + i % 50) for i in range(150)], 4, 2, 64, 16, 5),
+}
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("name", sorted(BATCHES))
+def test_attention(eng, name, dt):
+    seqs, hq, hkv, d, page, pad = BATCHES[name]
+    p = ch.Paged(seqs, hq, hkv, d, page, DTYPES[dt], 5, pad)
+    q = p.q.cuda()
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((hq, p.tokens), 7.0, device="cuda")
+    ref = ch.attend_ref(p)
+    hints = dict(max_new=max(n for n, _ in seqs), max_kv=max(kv for _, kv in seqs))
+    for kw in ({}, hints):
+        eng.cache_forward(q, *p.arrays(), out=out, lse=lse, **kw)
+        ch.check("out", out, ref[0], ref[1])
+        ch.check("lse", lse, ref[2], ref[3])
+    if pad:  # rows behind the last sequence stay as they were
+        assert (out[-pad:] == 7.0).all() and (lse[:, -pad:] == 7.0).all()
+    again, none = eng.cache_forward(q, *p.arrays(), **hints)
+    live = slice(0, p.tokens - pad)
+    assert none is None and torch.equal(again[live], out[live])
+    eng.cache_forward(q, *p.arrays(), out=q, **hints)  # over its own queries
+    assert torch.equal(q[live], out[live])
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_wrong_hints_change_nothing_but_the_layout(eng, dt):
+    p = ch.Paged([(70, 400), (1, 2500)], 8, 2, 128, 16, DTYPES[dt], 6)
+    ref = ch.attend_ref(p)
+    for kw in (dict(max_new=1, max_kv=1), dict(max_new=70, max_kv=300), dict(max_new=10 ** 6, max_kv=10 ** 9)):
+        out, lse = eng.cache_forward(p.q.cuda(), *p.arrays(), save=True, **kw)
+        ch.check("out", out, ref[0], ref[1])
+        ch.check("lse", lse, ref[2], ref[3])
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_rows_without_a_key(eng, dt):
+    # a length below the number of new tokens leaves the first rows at negative
+    # positions: they see nothing, get 0 and -inf, and append nothing
+    p = ch.Paged([(6, 9), (3, 3)], 4, 2, 64, 16, DTYPES[dt], 7)
+    p.kv_lens[1] = 1
+    out, lse = eng.cache_forward(p.q.cuda(), *p.arrays(), save=True)
+    assert not out[6:8].any() and (lse[:, 6:8] == -math.inf).all()
+    q = ch.Paged([(6, 9), (3, 3)], 4, 2, 64, 16, DTYPES[dt], 7)
+    q.seqs = [(6, 9), (1, 1)]
+    q.q = torch.cat([p.q[:6], p.q[8:9]])
+    q.tokens = 7
+    q.k[1], q.v[1] = q.k[1][:1], q.v[1][:1]
+    ref = ch.attend_ref(q)
+    ch.check("out", torch.cat([out[:6], out[8:]]), ref[0], ref[1])
+    ch.check("lse", torch.cat([lse[:, :6], lse[:, 8:]], 1), ref[2], ref[3])
+    before = p.both.clone()
+    k = torch.ones(9, 2, 64, device="cuda", dtype=DTYPES[dt])
+    eng.cache_append(k, 2 * k, *p.arrays())
+    same = torch.eq(before, p.both) | (before.isnan() & p.both.isnan())
+    changed = (~same).any(-1).nonzero()  # page, k or v, head, row
+    last = int(p.table[1, 0])
+    assert {(int(r[0]), int(r[3])) for r in changed} == \
+        {(int(p.table[0, 0]), i) for i in range(3, 9)} | {(last, 0)}
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_bad_pages_hold_no_keys(eng, dt):
+    p = ch.Paged([(4, 150), (1, 64), (1, 5)], 8, 2, 64, 16, DTYPES[dt], 8)
+    bad = {(0, 2): -1, (0, 9): p.n_pages, (1, 0): 2 ** 31 - 1, (2, 0): -2 ** 31}
+    hidden = [(b, i) for (b, pg) in bad for i in range(16 * pg, min(16 * pg + 16, p.seqs[b][1]))]
+    for (b, pg), to in bad.items():
+        p.table[b, pg] = to
+    ref = ch.attend_ref(p, hidden)
+    out, lse = eng.cache_forward(p.q.cuda(), *p.arrays(), save=True)
+    assert (lse[:, 5] == -math.inf).all() and not out[5].any()
+    ch.check("out", out, ref[0], ref[1])
+    ch.check("lse", lse, ref[2], ref[3])
+    before = p.both.clone()
+    k = torch.ones(6, 2, 64, device="cuda", dtype=DTYPES[dt])
+    eng.cache_append(k, k, *p.arrays())  # sequences 0 and 2 end in a bad page
+    same = torch.eq(before, p.both) | (before.isnan() & p.both.isnan())
+    changed = {(int(r[0]), int(r[3])) for r in (~same).any(-1).nonzero()}
+    assert changed == {(int(p.table[1, 3]), 15)}
+
+
+def test_lengths_past_the_table(eng):
+    # positions the table has no column for hold no key
+    p = ch.Paged([(1, 64)], 4, 1, 64, 16, torch.bfloat16, 9)
+    table = p.table[:, :2]  # a view: rows further apart than they are long
+    ref = ch.attend_ref(p, [(0, j) for j in range(32, 64)])
+    out, lse = eng.cache_forward(p.q.cuda(), p.k_pages, p.v_pages, p.cu, p.kv_lens, table, save=True)
+    ch.check("out", out, ref[0], ref[1])
+    ch.check("lse", lse, ref[2], ref[3])
+    before = p.both.clone()
+    k = torch.ones(1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    eng.cache_append(k, k, p.k_pages, p.v_pages, p.cu, p.kv_lens, table)
+    assert torch.equal(before.nan_to_num(9.0), p.both.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("name", sorted(BATCHES))
+def test_append(eng, name, dt):
+    seqs, hq, hkv, d, page, pad = BATCHES[name]
+    p = ch.Paged(seqs, hq, hkv, d, page, DTYPES[dt], 11, pad)
+    k, v = (torch.randn(p.tokens, hkv, d).to(DTYPES[dt]) for _ in range(2))
+    for theta in (None, 5e5):
+        q, q_rot = p.q.cuda(), torch.full((p.tokens, hq, d), 7.0, device="cuda", dtype=DTYPES[dt])
+        before = p.both.clone()
+        got = eng.cache_append(k.cuda(), v.cuda(), *p.arrays(), rope_freq_base=theta,
+                               **({} if theta is None else dict(q=q, q_rot=q_rot)))
+        assert (got is None) == (theta is None)
+        pos = p.positions()
+        turned = ch.rotate(k.double(), pos, theta)
+        bound = (ch.half_step(DTYPES[dt]) * turned.abs() + 8 * ch.F * ch.pair_size(k.double())
+                 if theta else torch.zeros_like(turned))
+        kp, vp = p.k_pages.cpu(), p.v_pages.cpu()
+        was = before.cpu().nan_to_num(9.0)
+        t = 0
+        for b, (n, kv) in enumerate(seqs):
+            for i in range(n):
+                at, row = int(p.table[b, (kv - n + i) // page]), (kv - n + i) % page
+                ch.check("k", kp[at, :, row], turned[t], bound[t])
+                assert torch.equal(vp[at, :, row], v[t])
+                was[at, 0, :, row], was[at, 1, :, row] = kp[at, :, row], vp[at, :, row]
+                t += 1
+        assert torch.equal(was, p.both.cpu().nan_to_num(9.0)), "no other row changes"
+        if theta:
+            live = slice(0, p.tokens - pad)
+            want = ch.rotate(p.q.double(), pos, theta)
+            b = ch.half_step(DTYPES[dt]) * want.abs() + 8 * ch.F * ch.pair_size(p.q.double())
+            ch.check("q", q_rot[live], want[live], b[live])
+            assert (q_rot[p.tokens - pad:] == 7.0).all()
+            eng.cache_append(k.cuda(), v.cuda(), *p.arrays(), rope_freq_base=theta, q=q, q_rot=q)
+            assert torch.equal(q[live], q_rot[live])
+
+
+def test_empty_calls(eng):
+    p = ch.Paged([(0, 20), (0, 0)], 4, 2, 64, 16, torch.bfloat16, 12)
+    out, lse = eng.cache_forward(p.q.cuda(), *p.arrays(), save=True)  # no rows
+    assert out.shape == (0, 4, 64) and lse.shape == (4, 0)
+    none = torch.empty(0, 2, 64, device="cuda", dtype=torch.bfloat16)
+    eng.cache_append(none, none, *p.arrays())
+    # rows, but no sequence
+    q = torch.full((3, 4, 64), 5.0, device="cuda", dtype=torch.bfloat16)
+    zero = torch.zeros(1, device="cuda", dtype=torch.int32)
+    out = eng.cache_forward(q, p.k_pages, p.v_pages, zero, zero[:0], p.table[:0], out=q.clone())[0]
+    assert torch.equal(out, q)
+
+
+def test_refusals(eng):
+    p = ch.Paged([(1, 20)], 4, 2, 64, 16, torch.bfloat16, 13)
+    q = p.q.cuda()
+    k = torch.zeros(1, 2, 64, device="cuda", dtype=torch.bfloat16)
+    for change in (dict(cu_tokens=p.cu.long()), dict(kv_lens=p.kv_lens.float()), dict(page_table=p.table.cpu()),
+                   dict(q=q.float()), dict(q=q[:, :, :32]), dict(q=q.cpu()), dict(k_pages=p.k_pages.float()),
+                   dict(v_pages=p.v_pages[:-1]), dict(k_pages=p.k_pages.transpose(1, 2)),
+                   dict(v_pages=p.v_pages.contiguous()), dict(lse=torch.zeros(4, 2, device="cuda"))):
+        args = dict(q=q, k_pages=p.k_pages, v_pages=p.v_pages, cu_tokens=p.cu, kv_lens=p.kv_lens,
+                    page_table=p.table)
+        args.update(change)
+        with pytest.raises(TypeError):
+            eng.cache_forward(**args)
+    with pytest.raises(ga.InvalidArgument):  # q without a rotation
+        eng.cache_append(k, k, *p.arrays(), q=q)
+    with pytest.raises(ga.InvalidArgument):
+        eng.cache_append(k, k, *p.arrays(), rope_freq_base=-1.0)
+    with pytest.raises(ga.InvalidArgument):  # 3 query heads for 2 of the cache
+        eng.cache_forward(q[:, :3].contiguous(), *p.arrays())
+
+
+@pytest.mark.parametrize("normed", [False, True])
+def test_a_prompt_and_its_answer_as_one_sequence(eng, normed):
+    """A sequence given chunk by chunk and then token by token, through norms,
+    append and attention, has the rows that the whole sequence has in
+    glacier_attn_forward, which the training path uses."""
+    T, hq, hkv, d, page, theta = 150, 14, 2, 64, 16, 1.0e6
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn(T, h, d, device="cuda", generator=g).bfloat16() for h in (hq, hkv, hkv))
+    wq, wk = (1 + 0.1 * torch.randn(d, device="cuda", generator=g) for _ in range(2))
+    qn, kn = eng.qk_norm_forward(q, k, wq, wk, 1e-6) if normed else (q, k)
+    want = eng.forward(qn, kn, v, theta, save=False)[0].float()
+    pages = torch.zeros(2, 12, hkv, page, d, device="cuda", dtype=torch.bfloat16)
+    table = torch.randperm(12, device="cuda", generator=g).to(torch.int32)[None]
+    at = 0
+    for n in [64, 1, 37, 40] + [1] * 8:
+        rows = slice(at, at + n)
+        at += n
+        cu = torch.tensor([0, n], device="cuda", dtype=torch.int32)
+        lens = torch.tensor([at], device="cuda", dtype=torch.int32)
+        arrays = (pages[0], pages[1], cu, lens, table)
+        if normed:  # norms and rotation in one pass, keys appended as they are
+            pos = torch.arange(at - n, at, device="cuda", dtype=torch.int32)
+            q_rot, k_rot = eng.qk_norm_forward(q[rows].contiguous(), k[rows].contiguous(), wq, wk, 1e-6,
+                                               rope_freq_base=theta, positions=pos)
+            eng.cache_append(k_rot, v[rows], *arrays)
+        else:
+            q_rot = eng.cache_append(k[rows], v[rows], *arrays, rope_freq_base=theta, q=q[rows])
+        out = eng.cache_forward(q_rot, *arrays)[0].float()
+        # both sides hold bf16 weights, queries and outputs: the path's bf16 gate
+        assert (out - want[rows]).abs().max() <= 2e-2 * want.abs().max()
+    assert at == T
+
+
+def test_a_captured_step_follows_its_arrays(eng):
+    """One captured step of append and attention, replayed for growing
+    sequences by changing the device arrays only, between eager calls."""
+    hq, hkv, d, page, theta, B = 8, 2, 128, 16, 5e5, 3
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()  # noqa: E731
+    pages = n(2, 200, hkv, page, d)
+    mirror = pages.clone()
+    table = torch.randperm(200, device="cuda", generator=g)[:B * 60].view(B, 60).to(torch.int32)
+    q, k, v = n(B + 2, hq, d), n(B + 2, hkv, d), n(B + 2, hkv, d)
+    cu = torch.arange(B + 1, device="cuda", dtype=torch.int32)
+    lens = torch.tensor([1, 500, 900], device="cuda", dtype=torch.int32)
+    out, q_rot = torch.zeros_like(q), torch.zeros_like(q)
+
+    def step(store, to, rot):
+        eng.cache_append(k, v, store[0], store[1], cu, lens, table, rope_freq_base=theta, q=q, q_rot=rot)
+        eng.cache_forward(rot, store[0], store[1], cu, lens, table, max_new=1, max_kv=960, out=to)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(pages, out, q_rot)
+    for turn in range(4):
+        for t in (q, k, v):
+            t.copy_(n(*t.shape))
+        # rows behind the last sequence keep what the replay before left there
+        want, rot = out.clone(), torch.zeros_like(q)
+        step(mirror, want, rot)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(pages, mirror)
+        lens += 1
+        if turn == 1:  # one sequence rests
+            cu.copy_(torch.tensor([0, 1, 1, 2], dtype=torch.int32))
+
+
+def test_another_stream(eng):
+    p = ch.Paged([(20, 300), (1, 700)], 8, 2, 128, 16, torch.bfloat16, 14)
+    q = p.q.cuda()
+    want = eng.cache_forward(q, *p.arrays())[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = eng.cache_forward(q, *p.arrays())[0]
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
