@@ -54,6 +54,7 @@ SOURCES = {
     "qk_norm.hip": (),
     "cache_append.hip": (),
     "cache_attn.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
+    "cache_attn_wide.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
     "lmhead.hip": (),
     "lora_file.cpp": (),
     "engine.cpp": (),

@@ -18,14 +18,12 @@
 // Which tiles exist, which keys they see and how these are split follows from
 // device data (cu_tokens, kv_lens) by the same formulas in both launches; the
 // grid covers every batch of the call's size, and workgroups without work leave.
-#include "cache_view.hpp"
+#include "cache_tiles.hpp"
 
 namespace glacier {
 namespace {
 
 constexpr int kWavesCa = 4;
-constexpr int kMaxSplits = 64;    // one lane each in the join
-constexpr int kSplitUnit = 128;   // splits begin at multiples of it
 
 template <typename T>
 struct KeyBlock;
@@ -37,29 +35,6 @@ template <>
 struct KeyBlock<float> {
   static constexpr int KB = 16;  // two blocks of 256 columns and their copies fit the LDS
 };
-
-// The first tile number of sequence b: tiles of all sequences in a row, with
-// one number at most left unused per sequence.
-__device__ inline int first_tile(const CacheAttn& a, int b) {
-  return clamp_row(a.c.cu[b], a.c.T) * a.group / a.rows + b;
-}
-
-// The keys of a tile whose last row is token `last`, and how they are split.
-struct TileKeys {
-  int kend;  // keys 0 .. kend - 1
-  int per, active;
-};
-__device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int tile) {
-  TileKeys k;
-  const int last = min(s.n - 1, (tile * a.rows + a.rows - 1) / a.group);
-  const long cap = (long)a.c.max_pages << a.c.page_shift;
-  const long end = (long)s.pos0 + last + 1;
-  k.kend = static_cast<int>(end < 0 ? 0 : end < cap ? end : cap);
-  const int even = (k.kend + a.n_splits - 1) / a.n_splits;
-  k.per = max(a.split_keys, (even + kSplitUnit - 1) / kSplitUnit * kSplitUnit);
-  k.active = max(1, (k.kend + k.per - 1) / k.per);
-  return k;
-}
 
 template <typename T, int DP, int MB>
 struct CaLayout {
@@ -223,14 +198,14 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
           top = fmaxf(top, x);
         }
       const float mn = fmaxf(m[mb], col_max_swap(top));
-      const float alpha = exp2f(m[mb] - mn);
+      const float alpha = weight(m[mb] - mn);
       m[mb] = mn;
       float sum = 0.0f;
 #pragma unroll
       for (int p = 0; p < NS; ++p)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = exp2f(st[mb][p][r] - mn);
+          const float e = weight(st[mb][p][r] - mn);
           st[mb][p][r] = e;
           sum += e;
         }
@@ -304,7 +279,7 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
 #pragma unroll
     for (int u = 0; u < kWavesCa; ++u) {
       const float* reg = all + u * L::WAVE;
-      const float f = exp2f(reg[ROWS * L::OS + row] - mx);
+      const float f = weight(reg[ROWS * L::OS + row] - mx);
       total += f * reg[ROWS * (L::OS + 1) + row];
       const f32x4 v = *reinterpret_cast<const f32x4*>(reg + row * L::OS + d);
 #pragma unroll
@@ -348,7 +323,7 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttn a) {
   float mx = ml.x;
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x));
-  const float f = exp2f(ml.x - mx);
+  const float f = weight(ml.x - mx);
   float total = f * ml.y;
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
@@ -377,11 +352,13 @@ hipError_t attend(const CacheAttn& a, hipStream_t st) {
   using L = CaLayout<T, DP, MB>;
   auto* fn = &cache_attn_kernel<T, DP, MB>;
   GL_CHECK(allow_lds(fn, L::BYTES));
-  const unsigned tiles = static_cast<unsigned>((long)a.c.T * a.group / a.rows + a.c.n_seqs);
-  hipLaunchKernelGGL((cache_attn_kernel<T, DP, MB>), dim3(tiles, a.c.hkv, a.n_splits),
+  hipLaunchKernelGGL((cache_attn_kernel<T, DP, MB>), dim3(tile_numbers(a), a.c.hkv, a.n_splits),
                      dim3(64 * kWavesCa), L::BYTES, st, a);
-  GL_CHECK(hipGetLastError());
-  if (a.n_splits == 1) return hipSuccess;
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t join(const CacheAttn& a, hipStream_t st) {
   const long rows = (long)a.c.T * a.hq;
   hipLaunchKernelGGL(cache_attn_join_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0,
                      st, a);
@@ -402,11 +379,11 @@ hipError_t by_head(const CacheAttn& a, hipStream_t st) {
 
 CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, int n_cu) {
   CachePlan p{};
-  (void)max_new;
-  p.rows = 16;
   const long group = hq / c.hkv;
   const long cap = (long)c.max_pages << c.page_shift;
   const long keys = max_kv > 0 && max_kv < cap ? max_kv : cap;
+  const long longest = max_new > 0 && max_new < c.T ? max_new : c.T;  // chunk
+  p.rows = c.io_bf16 && c.D <= 128 && longest * group > 64 ? kCacheWideRows : 16;
   const long tiles = (c.T * group + p.rows - 1) / p.rows + std::min(c.T, c.n_seqs) / 2;
   // enough workgroups for two on each CU, of 256 keys or more
   const long want = 2L * n_cu / std::max(1L, tiles * c.hkv);
@@ -422,7 +399,12 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
 }
 
 hipError_t launch_cache_attn(const CacheAttn& a, hipStream_t st) {
-  return a.c.io_bf16 ? by_head<bf16>(a, st) : by_head<float>(a, st);
+  if (a.rows == kCacheWideRows)
+    GL_CHECK(launch_cache_attn_wide(a, st));
+  else
+    GL_CHECK(a.c.io_bf16 ? by_head<bf16>(a, st) : by_head<float>(a, st));
+  if (a.n_splits == 1) return hipSuccess;
+  return a.c.io_bf16 ? join<bf16>(a, st) : join<float>(a, st);
 }
 
 }  // namespace glacier

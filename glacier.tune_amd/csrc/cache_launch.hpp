@@ -79,4 +79,7 @@ struct CachePlan {
 CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, int n_cu);
 hipError_t launch_cache_attn(const CacheAttn& a, hipStream_t st);
 
+constexpr int kCacheWideRows = 128;  // rows of a tile of cache_attn_wide.hip
+hipError_t launch_cache_attn_wide(const CacheAttn& a, hipStream_t st);
+
 }  // namespace glacier
