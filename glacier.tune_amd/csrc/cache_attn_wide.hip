@@ -19,7 +19,6 @@
 // and the sums need no rescaling.  The result is the same: any reference value
 // cancels in out and lse.
 #include "cache_tiles.hpp"
-#include "lds_mfma.hpp"
 
 namespace glacier {
 namespace {
@@ -105,19 +104,23 @@ __global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(Cac
       }
   }
 
-  // this thread's share of a tile: rows row0 + RPI i, piece `piece`
+  // this thread's share of a tile: rows row0 + RPI i, piece `piece`.  The 16
+  // rows of a page piece are read through a buffer resource that ends with the
+  // last one that holds a key (none without a page): what lies past it, and
+  // past column D, arrives as zero, with no branch and no address arithmetic
+  // in vector registers.
   const int piece = threadIdx.x % W::PPR, row0 = threadIdx.x / W::PPR;
-  const int wrow0 = w * (64 / W::PPR);  // the wave's first row: 16 rows of it lie in one page piece
-  const bool in_row = 8 * piece < D;
+  const int wrow0 = w * (64 / W::PPR);  // the wave's rows of one load lie in one page piece
+  const int rowb = 2 * D;
+  const int loff = 8 * piece < D ? (row0 & 15) * rowb + 16 * piece : 1 << 20;
   int soff[W::NI];
 #pragma unroll
   for (int i = 0; i < W::NI; ++i) {
     const int row = row0 + i * W::RPI;
     soff[i] = row * W::RB + 16 * (piece ^ lds_sw<DP>(row));
   }
-  const bf16* const kp = static_cast<const bf16*>(c.k_pages) + 8 * piece;
-  const bf16* const vp = static_cast<const bf16*>(c.v_pages) + 8 * piece;
   const int in_page = (1 << c.page_shift) - 1;
+  const long head = ((long)kvh << c.page_shift) * rowb, strideb = 2 * c.page_stride;
   // the pages of a tile's four pieces of 16 keys, one a lane; none (-1) past k1
   auto look_up = [&](int j) {
     const int key = j + 16 * (lane & 3);
@@ -127,15 +130,12 @@ __global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(Cac
   auto fetch = [&](int j, int pages) {
 #pragma unroll
     for (int i = 0; i < W::NI; ++i) {
-      const int key = j + row0 + i * W::RPI;
+      const int key = j + (wrow0 + i * W::RPI) / 16 * 16;
       const int page = __builtin_amdgcn_readlane(pages, (wrow0 + i * W::RPI) / 16);
-      kr[i] = i32x4{0, 0, 0, 0};
-      vr[i] = i32x4{0, 0, 0, 0};
-      if (page >= 0 && key < k1 && in_row) {
-        const long off = page * c.page_stride + (((long)kvh << c.page_shift) + (key & in_page)) * D;
-        kr[i] = *reinterpret_cast<const i32x4*>(kp + off);
-        vr[i] = *reinterpret_cast<const i32x4*>(vp + off);
-      }
+      const long off = (page < 0 ? 0 : page) * strideb + head + (key & in_page) * rowb;
+      const int rows = page < 0 ? 0 : min(16, k1 - key);
+      kr[i] = load_within(static_cast<const char*>(c.k_pages) + off, rows * rowb, loff);
+      vr[i] = load_within(static_cast<const char*>(c.v_pages) + off, rows * rowb, loff);
     }
   };
   auto put = [&](int buf) {

@@ -4,6 +4,7 @@
 #pragma once
 
 #include "cache_view.hpp"
+#include "lds_mfma.hpp"
 
 namespace glacier {
 
@@ -41,5 +42,14 @@ __device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int 
 // exp2 of the weights: the instruction itself, whose results below 2^-126 are
 // zero (exp2f spends four more instructions to keep them).
 __device__ inline float weight(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 16 bytes at `off` of the wave's [base, base + bytes); zeros past its end.
+__device__ inline i32x4 load_within(const void* base, int bytes, int off) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_raw_buffer_load_b128(wave_rsrc(base, bytes), off, 0, 0);
+#else
+  return i32x4{0, 0, 0, 0};
+#endif
+}
 
 }  // namespace glacier
