@@ -50,7 +50,7 @@ __global__ __launch_bounds__(64 * kWavesAp) void cache_append_kernel(CacheAppend
   const int pos = s.pos0 + (t - s.tok0);
   const int page = cache_page(c, b, pos);
   const int row = pos & ((1 << c.page_shift) - 1);
-  if (a.rotate) turn_table(turns[wave], rates, half, pos, lane);
+  if (a.rotate) turn_table(turns[wave], LaneRates(rates, half, lane), half, pos, lane);
   for (int h0 = part * H; h0 < heads; h0 += a.parts * H) {
     const int h = h0 + lane / L;
     if (h0 != part * H) fetch(h);

@@ -19,7 +19,7 @@ struct TurnRates {
 };
 
 // ---- per-head norms of queries and keys (qk_norm.hip) ----------------------
-constexpr int kQkMaxGroups = 1024;  // workgroups (partial sums) of a backward with weight gradients
+constexpr int kQkMaxGroups = 512;  // workgroups of a backward, each with its partial sums
 
 struct QkNorm {
   int T, hq, hkv, D;

@@ -21,6 +21,7 @@ namespace glacier {
 namespace {
 
 constexpr int kWavesQk = 4;
+constexpr int kWavesQkBwd = 8;  // with kQkMaxGroups workgroups: 16 waves a CU
 
 template <typename IO, int E, int L>
 __global__ __launch_bounds__(64 * kWavesQk) void qk_norm_fwd_kernel(QkNorm a, TurnRates rates) {
@@ -33,7 +34,8 @@ __global__ __launch_bounds__(64 * kWavesQk) void qk_norm_fwd_kernel(QkNorm a, Tu
   const int half = a.D / 2, heads = a.hq + a.hkv;
   const int ch = lane % L, col = ch * E;
   const bool in_row = col < half;
-  if (a.rotate) turn_table(turns[wave], rates, half, a.positions != nullptr ? a.positions[t] : t, lane);
+  if (a.rotate)
+    turn_table(turns[wave], LaneRates(rates, half, lane), half, a.positions != nullptr ? a.positions[t] : t, lane);
   for (int h0 = part * H; h0 < heads; h0 += a.parts * H) {
     const int h = h0 + lane / L;
     const bool ok = in_row && h < heads, is_q = h < a.hq;
@@ -77,58 +79,101 @@ __global__ __launch_bounds__(64 * kWavesQk) void qk_norm_fwd_kernel(QkNorm a, Tu
   }
 }
 
-// DW: the weight gradients are formed.
+// DW: the weight gradients are formed.  The wave's steps (a token's heads, H at
+// a time) follow each other with the next step's rows requested before this
+// one's are used.
 template <typename IO, int E, int L, bool DW>
-__global__ __launch_bounds__(64 * kWavesQk) void qk_norm_bwd_kernel(QkNorm a, TurnRates rates) {
+__global__ __launch_bounds__(64 * kWavesQkBwd) void qk_norm_bwd_kernel(QkNorm a, TurnRates rates) {
   constexpr int H = 64 / L;
-  __shared__ float2 turns[kWavesQk][kTurnMaxDim / 2];
-  __shared__ float sums[DW ? kWavesQk : 1][DW ? 2 * kTurnMaxDim : 1];
+  __shared__ float2 turns[kWavesQkBwd][kTurnMaxDim / 2];
+  __shared__ float sums[DW ? kWavesQkBwd : 1][DW ? 2 * kTurnMaxDim : 1];
   const int wave = wave_id(), lane = threadIdx.x & 63;
   const int half = a.D / 2, heads = a.hq + a.hkv;
   const int ch = lane % L, col = ch * E;
   const bool in_row = col < half;
+  const LaneRates lane_rates(rates, half, lane);
   float dq0[E] = {}, dq1[E] = {}, dk0[E] = {}, dk1[E] = {};
   const int units = a.T * a.parts;
-  for (int unit = blockIdx.x * kWavesQk + wave; unit < units; unit += gridDim.x * kWavesQk) {
-    const int t = unit / a.parts, part = unit % a.parts;
-    if (a.rotate) turn_table(turns[wave], rates, half, a.positions != nullptr ? a.positions[t] : t, lane);
-    for (int h0 = part * H; h0 < heads; h0 += a.parts * H) {
-      const int h = h0 + lane / L;
-      const bool ok = in_row && h < heads, is_q = h < a.hq;
-      const long at = is_q ? ((long)t * a.hq + h) * a.D : ((long)t * a.hkv + (h - a.hq)) * a.D;
-      const float* w = is_q ? a.wq : a.wk;
-      float x0[E] = {}, x1[E] = {}, g0[E] = {}, g1[E] = {}, w0[E] = {}, w1[E] = {};
-      if (ok) {
-        const IO* x = static_cast<const IO*>(is_q ? a.q : a.k) + at + col;
-        const IO* dy = static_cast<const IO*>(is_q ? a.dq_out : a.dk_out) + at + col;
-        Piece<IO, E> p0, p1, d0, d1;
-        p0.load(x);
-        p1.load(x + half);
-        d0.load(dy);
-        d1.load(dy + half);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          w0[e] = w[col + e];
-          w1[e] = w[half + col + e];
-        }
-        p0.get(x0);
-        p1.get(x1);
-        d0.get(g0);
-        d1.get(g1);
-      }
-      float ss = 0.0f, c = 0.0f;
+
+  struct Step {
+    int unit, h0;
+  };
+  // a step's rows; the place of this lane's head is formed again where it is used
+  auto place = [&](const Step& s, bool& is_q) {
+    const int t = s.unit / a.parts, h = s.h0 + lane / L;
+    is_q = h < a.hq;
+    return (is_q ? (long)t * a.hq + h : (long)t * a.hkv + (h - a.hq)) * a.D + col;
+  };
+  struct Rows {
+    Piece<IO, E> x0, x1, d0, d1;
+  };
+  auto load = [&](const Step& s, Rows& r) {
+    bool is_q;
+    const long at = place(s, is_q);
+    if (s.unit >= units || !in_row || s.h0 + lane / L >= heads) return;
+    const IO* x = static_cast<const IO*>(is_q ? a.q : a.k) + at;
+    const IO* dy = static_cast<const IO*>(is_q ? a.dq_out : a.dk_out) + at;
+    r.x0.load(x);
+    r.x1.load(x + half);
+    r.d0.load(dy);
+    r.d1.load(dy + half);
+  };
+  auto after = [&](Step s) {
+    s.h0 += a.parts * H;
+    if (s.h0 >= heads) {
+      s.unit += gridDim.x * kWavesQkBwd;
+      s.h0 = s.unit % a.parts * H;
+    }
+    return s;
+  };
+  auto position = [&](int unit) {
+    const int t = unit / a.parts;
+    return a.positions != nullptr && a.rotate && unit < units ? a.positions[t] : t;
+  };
+
+  Step now;
+  now.unit = blockIdx.x * kWavesQkBwd + wave;
+  now.h0 = now.unit % a.parts * H;
+  Rows rows{}, ahead{};
+  load(now, rows);
+  int formed = -1, pos = position(now.unit);
+  while (now.unit < units) {
+    const Step next = after(now);
+    load(next, ahead);
+    if (now.unit != formed) {
+      if (a.rotate) turn_table(turns[wave], lane_rates, half, pos, lane);
+      formed = now.unit;
+      pos = position(now.unit + gridDim.x * kWavesQkBwd);
+    }
+    bool is_q;
+    const long at = place(now, is_q);
+    const bool ok = in_row && now.h0 + lane / L < heads;
+    const float* w = is_q ? a.wq : a.wk;
+    float x0[E] = {}, x1[E] = {}, g0[E] = {}, g1[E] = {}, w0[E] = {}, w1[E] = {};
+    if (ok) {
+      rows.x0.get(x0);
+      rows.x1.get(x1);
+      rows.d0.get(g0);
+      rows.d1.get(g1);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (a.rotate && in_row) {
-          const float2 cs = turns[wave][col + e];
-          rope_inv(g0[e], g1[e], cs.x, cs.y, g0[e], g1[e]);
-        }
-        ss += x0[e] * x0[e] + x1[e] * x1[e];
-        c += (w0[e] * g0[e]) * x0[e] + (w1[e] * g1[e]) * x1[e];
+        w0[e] = w[col + e];
+        w1[e] = w[half + col + e];
       }
-      ss = lanes_sum<L>(ss);
-      c = lanes_sum<L>(c);
-      if (!ok) continue;
+    }
+    float ss = 0.0f, c = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (a.rotate && in_row) {
+        const float2 cs = turns[wave][col + e];
+        rope_inv(g0[e], g1[e], cs.x, cs.y, g0[e], g1[e]);
+      }
+      ss += x0[e] * x0[e] + x1[e] * x1[e];
+      c += (w0[e] * g0[e]) * x0[e] + (w1[e] * g1[e]) * x1[e];
+    }
+    ss = lanes_sum<L>(ss);
+    c = lanes_sum<L>(c);
+    if (ok) {
       const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
       const float kx = r * r * r / (float)a.D * c;
       float o0[E], o1[E];
@@ -144,13 +189,15 @@ __global__ __launch_bounds__(64 * kWavesQk) void qk_norm_bwd_kernel(QkNorm a, Tu
           dk1[e] += is_q ? 0.0f : v1;
         }
       }
-      IO* dx = static_cast<IO*>(is_q ? a.yq : a.yk) + at + col;
+      IO* dx = static_cast<IO*>(is_q ? a.yq : a.yk) + at;
       Piece<IO, E> s0, s1;
       s0.set(o0);
       s1.set(o1);
       s0.store(dx);
       s1.store(dx + half);
     }
+    rows = ahead;
+    now = next;
   }
   if constexpr (DW) {
     // the lanes that hold the same columns (the wave's heads), then the waves
@@ -171,28 +218,32 @@ __global__ __launch_bounds__(64 * kWavesQk) void qk_norm_bwd_kernel(QkNorm a, Tu
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * a.D; i += 64 * kWavesQk) {
+    for (int i = threadIdx.x; i < 2 * a.D; i += 64 * kWavesQkBwd) {
       float s = 0.0f;
 #pragma unroll
-      for (int u = 0; u < kWavesQk; ++u) s += sums[u][i];
+      for (int u = 0; u < kWavesQkBwd; ++u) s += sums[u][i];
       a.partials[(long)blockIdx.x * 2 * a.D + i] = s;
     }
   }
 }
 
-// dw[i] += sum over the workgroups' partials, 8 groups of rows side by side.
-__global__ __launch_bounds__(256) void qk_norm_dw_kernel(QkNorm a, int groups) {
-  __shared__ float sums[8][32];
-  const int i = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+// dw[i] += sum over the workgroups' partials: 16 columns a workgroup, 64 rows
+// side by side, so that 512 rows are one round of loads deep.
+__global__ __launch_bounds__(1024) void qk_norm_dw_kernel(QkNorm a, int groups) {
+  __shared__ float sums[64][17];
+  const int x = threadIdx.x & 15, part = threadIdx.x >> 4, i = blockIdx.x * 16 + x;
   float s = 0.0f;
-  if (i < 2 * a.D)
-    for (int g = part; g < groups; g += 8) s += a.partials[(long)g * 2 * a.D + i];
-  sums[part][threadIdx.x & 31] = s;
+#pragma unroll
+  for (int u = 0; u < kQkMaxGroups / 64; ++u) {
+    const int g = part + 64 * u;
+    s += g < groups ? a.partials[(long)g * 2 * a.D + i] : 0.0f;
+  }
+  sums[part][x] = s;
   __syncthreads();
-  if (part != 0 || i >= 2 * a.D) return;
+  if (threadIdx.x >= 16) return;
   float total = 0.0f;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) total += sums[u][threadIdx.x & 31];
+  for (int u = 0; u < 64; ++u) total += sums[u][x];
   float* dw = i < a.D ? a.dwq : a.dwk;
   if (dw != nullptr) dw[i < a.D ? i : i - a.D] += total;
 }
@@ -211,17 +262,15 @@ hipError_t bwd(QkNorm& a, const TurnRates& r, int n_cu, hipStream_t st) {
   a.parts = turn_parts(a.T, (a.hq + a.hkv + 64 / L - 1) / (64 / L), n_cu);
   const long units = (long)a.T * a.parts;
   const bool dw = a.dwq != nullptr || a.dwk != nullptr;
-  const int all = static_cast<int>((units + kWavesQk - 1) / kWavesQk);
-  const int groups = dw ? std::min(all, kQkMaxGroups) : all;
+  const int groups = static_cast<int>(std::min<long>((units + kWavesQkBwd - 1) / kWavesQkBwd, kQkMaxGroups));
+  const dim3 block(64 * kWavesQkBwd);
   if (dw)
-    hipLaunchKernelGGL((qk_norm_bwd_kernel<IO, E, L, true>), dim3(groups), dim3(64 * kWavesQk), 0, st,
-                       a, r);
+    hipLaunchKernelGGL((qk_norm_bwd_kernel<IO, E, L, true>), dim3(groups), block, 0, st, a, r);
   else
-    hipLaunchKernelGGL((qk_norm_bwd_kernel<IO, E, L, false>), dim3(groups), dim3(64 * kWavesQk), 0, st,
-                       a, r);
+    hipLaunchKernelGGL((qk_norm_bwd_kernel<IO, E, L, false>), dim3(groups), block, 0, st, a, r);
   GL_CHECK(hipGetLastError());
   if (!dw) return hipSuccess;
-  hipLaunchKernelGGL(qk_norm_dw_kernel, dim3((2 * a.D + 31) / 32), dim3(256), 0, st, a, groups);
+  hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(2 * a.D / 16), dim3(1024), 0, st, a, groups);
   return hipGetLastError();
 }
 

@@ -50,10 +50,20 @@ __device__ inline void wave_lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// The rates of the pairs whose angles this lane forms.
+struct LaneRates {
+  double lo, hi;
+  __device__ inline LaneRates(const TurnRates& r, int half, int lane) {
+    lo = r.rev[lane < half ? lane : 0];
+    hi = half > 64 ? r.rev[lane + 64 < half ? lane + 64 : 0] : 0.0;
+  }
+};
+
 // This wave's angles of position pos into its LDS area [D/2].
-__device__ inline void turn_table(float2* area, const TurnRates& r, int half, int pos, int lane) {
+__device__ inline void turn_table(float2* area, const LaneRates& r, int half, int pos, int lane) {
   wave_lds_order();
-  for (int i = lane; i < half; i += 64) area[i] = turn_of(r.rev[i], pos);
+  if (lane < half) area[lane] = turn_of(r.lo, pos);
+  if (lane + 64 < half) area[lane + 64] = turn_of(r.hi, pos);
   wave_lds_order();
 }
 
