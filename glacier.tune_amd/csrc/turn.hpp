@@ -84,10 +84,10 @@ inline int lanes_of(int D, int E) {
   return l;
 }
 
-// F<IO, E, L> for the call's dtype and head size.
-#define GL_BY_HEAD(F, io_bf16, D, ...)                        \
+// F<IO, E, L> for the call's dtype, head size and piece.
+#define GL_BY_HEAD(F, io_bf16, D, piece, ...)                 \
   do {                                                        \
-    const int e_ = piece_elems(io_bf16, D);                   \
+    const int e_ = piece;                                     \
     const int l_ = lanes_of(D, e_);                           \
     if ((io_bf16) && e_ == 8) {                               \
       if (l_ == 4) return F<bf16, 8, 4>(__VA_ARGS__);         \
