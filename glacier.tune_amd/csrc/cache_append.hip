@@ -42,13 +42,11 @@ __global__ __launch_bounds__(64 * kWavesAp) void cache_append_kernel(CacheAppend
     p1.load(x + half + col);
   };
   fetch(part * H + lane / L);
-  // the sequences that end at or before this token
-  const int b = count_prefix(c.n_seqs, lane, [&](int i) { return c.cu[i + 1] <= t; });
-  if (b >= c.n_seqs) return;  // behind the last sequence
-  const CacheSeq s = cache_seq(c, b);
+  const CacheSeq s = seq_of_token(c, lane, t);
+  if (s.b >= c.n_seqs) return;  // behind the last sequence
   if (t < s.tok0) return;
   const int pos = s.pos0 + (t - s.tok0);
-  const int page = cache_page(c, b, pos);
+  const int page = cache_page(c, s.b, pos);
   const int row = pos & ((1 << c.page_shift) - 1);
   if (a.rotate) turn_table(turns[wave], LaneRates(rates, half, lane), half, pos, lane);
   for (int h0 = part * H; h0 < heads; h0 += a.parts * H) {

@@ -23,7 +23,6 @@
 namespace glacier {
 namespace {
 
-constexpr int kWavesCa = 4;
 
 template <typename T>
 struct KeyBlock;
@@ -36,14 +35,14 @@ struct KeyBlock<float> {
   static constexpr int KB = 16;  // two blocks of 256 columns and their copies fit the LDS
 };
 
-template <typename T, int DP, int MB>
+template <typename T, int DP, int MB, int WAVES>
 struct CaLayout {
   static constexpr int KB = KeyBlock<T>::KB;
   static constexpr int S = Lds<T, DP>::STRIDE;
-  static constexpr int TILES = kWavesCa * 2 * KB * S * static_cast<int>(sizeof(T));
+  static constexpr int TILES = WAVES * 2 * KB * S * static_cast<int>(sizeof(T));
   static constexpr int OS = DP + 4;  // row stride (floats) of a wave's sums in the join
   static constexpr int WAVE = 16 * MB * (OS + 2);  // sums, maxima, totals
-  static constexpr int JOIN = kWavesCa * WAVE * 4;
+  static constexpr int JOIN = WAVES * WAVE * 4;
   static constexpr int BYTES = TILES > JOIN ? TILES : JOIN;
   static_assert(BYTES <= 160 * 1024, "exceeds the LDS of a CU");
 };
@@ -58,17 +57,15 @@ struct BlockRegs {
   static constexpr int RPI = 64 / LPR;  // rows per instruction, at most 16
   static constexpr int N = KB / RPI;
   i32x4 w[N];
-  // rows of one page piece (16 keys) each from base[piece]; rows at or past
-  // nvalid, pieces without a page and columns at or past D read as zero
-  __device__ inline void load(const T* const (&base)[KB / 16], const bool (&held)[KB / 16], int D,
-                              int nvalid, int lane) {
-    const int ch = lane % LPR;
+  // 16 rows of each page piece from base[piece], of which rows[piece] hold
+  // keys; rows past them and columns past D arrive as zero (load_within).
+  // off: this lane's row lane / LPR and column, in bytes
+  __device__ inline void load(const char* const (&base)[KB / 16], const int (&rows)[KB / 16], int rowb,
+                              int off) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = i * RPI + lane / LPR;
-      w[i] = i32x4{0, 0, 0, 0};
-      if (held[i * RPI / 16] && r < nvalid && ch * CE < D)
-        w[i] = *reinterpret_cast<const i32x4*>(base[i * RPI / 16] + (long)(r & 15) * D + ch * CE);
+      constexpr int P = 16 / RPI;  // loads of a piece
+      w[i] = load_within(base[i / P], rows[i / P] * rowb, off + i % P * RPI * rowb);
     }
   }
   __device__ inline void store(T* lds, int lane) const {
@@ -86,21 +83,21 @@ __device__ inline void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <typename T, int DP, int MB>
-__global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) {
+template <typename T, int DP, int MB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   using M = Mfma<T>;
-  using L = CaLayout<T, DP, MB>;
-  constexpr int KB = L::KB, NS = KB / 16, NKD = DP / M::KSTEP, ROWS = 16 * MB;
+  using L = CaLayout<T, DP, MB, WAVES>;
+  constexpr int KB = L::KB, NS = KB / 16, ROWS = 16 * MB;
+  constexpr int NW = DP * sizeof(T) / 64;  // 16-byte words a lane holds of a row
   extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
   const int w = wave_id(), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int kvh = blockIdx.y, split = blockIdx.z, D = c.D;
 
-  const int b = __builtin_amdgcn_readfirstlane(count_prefix(
-      c.n_seqs, lane, [&](int i) { return first_tile(a, i + 1) <= static_cast<int>(blockIdx.x); }));
+  const CacheSeq s = seq_of_tile(a, lane, static_cast<int>(blockIdx.x));
+  const int b = s.b;
   if (b >= c.n_seqs) return;
-  const CacheSeq s = cache_seq(c, b);
-  const int tile = static_cast<int>(blockIdx.x) - first_tile(a, b);
+  const int tile = static_cast<int>(blockIdx.x) - first_tile(a, b, s.tok0);
   const int r0 = tile * ROWS, n_rows = s.n * a.group;
   if (tile < 0 || r0 >= n_rows) return;
   const TileKeys tk = tile_keys(a, s, tile);
@@ -108,21 +105,32 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
   const int k0 = split * tk.per, k1 = min(tk.kend, k0 + tk.per);
 
   // this lane's rows (one per 16-row block): operand fragments and last key
-  typename M::Frag qf[MB][NKD];
+  i32x4 qw[MB][NW];
   int limit[MB];
+  // the first of the 16 bytes of columns that this lane holds in word x of a
+  // row of Q or K: one k-step's 8 columns in bf16; in fp32, where a k-step takes
+  // one column a lane, those of four steps (step 4 x + e takes column
+  // 16 x + 4 g + e: a dot product may take its terms in any order)
+  auto first_col = [&](int x) { return sizeof(T) == 2 ? 32 * x + 8 * g : 16 * x + 4 * g; };
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     const int r = r0 + 16 * mb + col;
     const int i = r / a.group, h = kvh * a.group + (r - i * a.group);
     const bool ok = r < n_rows;
     limit[mb] = ok ? s.pos0 + i : -1;
-    const T* q = static_cast<const T*>(a.q) + ((long)(s.tok0 + i) * a.hq + h) * D;
+    // (loaded from the tile's first row where there is none, and cleared after
+    // all loads are under way)
+    const T* q = static_cast<const T*>(a.q) +
+                 (ok ? (long)(s.tok0 + i) * a.hq + h : (long)(s.tok0 + r0 / a.group) * a.hq) * D;
 #pragma unroll
-    for (int kk = 0; kk < NKD; ++kk) {
-      qf[mb][kk] = frag_zero<T>();
-      if (ok && kk * M::KSTEP + M::KPL * g < D) qf[mb][kk] = frag_global<T>(q, kk, g);
-    }
+    for (int x = 0; x < NW; ++x)
+      qw[mb][x] = *reinterpret_cast<const i32x4*>(q + (first_col(x) < D ? first_col(x) : 0));
   }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int x = 0; x < NW; ++x)
+      if (limit[mb] < 0 || first_col(x) >= D) qw[mb][x] = i32x4{0, 0, 0, 0};
 
   f32x4 acc[MB][DP / 16];
   float m[MB], l[MB];
@@ -137,37 +145,41 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
   T* const kt = reinterpret_cast<T*>(smem) + w * 2 * KB * L::S;
   T* const vt = kt + KB * L::S;
   BlockRegs<T, DP> kr, vr;
-  bool held[NS];
+  using R = BlockRegs<T, DP>;
+  const int rowb = D * static_cast<int>(sizeof(T));
+  const int off = lane % R::LPR * R::CE < D ? lane / R::LPR * rowb + lane % R::LPR * 16 : 1 << 20;
+  const long head = ((long)kvh << c.page_shift) * rowb, strideb = c.page_stride * sizeof(T);
+  int rows[NS];  // keys of the fetched block's pieces
   auto fetch = [&](int j) {
-    const T *kb[NS], *vb[NS];
+    const char *kb[NS], *vb[NS];
 #pragma unroll
     for (int p = 0; p < NS; ++p) {
       const int key = j + 16 * p;
       const int page = key < k1 ? __builtin_amdgcn_readfirstlane(cache_page(c, b, key)) : -1;
-      held[p] = page >= 0;
-      const long at = (page >= 0 ? page : 0) * c.page_stride +
-                      (((long)kvh << c.page_shift) + (key & ((1 << c.page_shift) - 1))) * D;
-      kb[p] = static_cast<const T*>(c.k_pages) + at;
-      vb[p] = static_cast<const T*>(c.v_pages) + at;
+      rows[p] = page < 0 ? 0 : min(16, k1 - key);
+      const long at = (page < 0 ? 0 : page) * strideb + head + (key & ((1 << c.page_shift) - 1)) * rowb;
+      kb[p] = static_cast<const char*>(c.k_pages) + at;
+      vb[p] = static_cast<const char*>(c.v_pages) + at;
     }
-    kr.load(kb, held, D, k1 - j, lane);
-    vr.load(vb, held, D, k1 - j, lane);
+    kr.load(kb, rows, rowb, off);
+    vr.load(vb, rows, rowb, off);
   };
   const int first_limit = s.pos0 + r0 / a.group;  // the tile's first row sees keys up to here
   int j = k0 + w * KB;
   if (j < k1) fetch(j);
-  for (; j < k1; j += kWavesCa * KB) {
+  for (; j < k1; j += WAVES * KB) {
     wave_lds_fence();
     kr.store(kt, lane);
     vr.store(vt, lane);
     wave_lds_fence();
-    bool here[NS], whole = j + KB - 1 <= first_limit && j + KB <= k1;
+    int here[NS];
+    bool whole = j + KB - 1 <= first_limit;
 #pragma unroll
     for (int p = 0; p < NS; ++p) {
-      here[p] = held[p];
-      whole = whole && held[p];
+      here[p] = rows[p];
+      whole = whole && rows[p] == 16;
     }
-    if (j + kWavesCa * KB < k1) fetch(j + kWavesCa * KB);
+    if (j + WAVES * KB < k1) fetch(j + WAVES * KB);
     // S^T: keys 16 p + 4 g + r of this block, row col of each 16-row block
     f32x4 st[MB][NS];
 #pragma unroll
@@ -177,10 +189,18 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
 #pragma unroll
     for (int p = 0; p < NS; ++p)
 #pragma unroll
-      for (int kk = 0; kk < NKD; ++kk) {
-        const auto kf = frag_rm<T, DP>(kt, 16 * p + col, kk, g);
+      for (int x = 0; x < NW; ++x) {
+        const i32x4 kw = *reinterpret_cast<const i32x4*>(kt + (16 * p + col) * L::S + first_col(x));
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) st[mb][p] = M::mma(kf, qf[mb][kk], st[mb][p]);
+        for (int mb = 0; mb < MB; ++mb) {
+          if constexpr (sizeof(T) == 2) {
+            st[mb][p] = M::mma(__builtin_bit_cast(bf16x8, kw), __builtin_bit_cast(bf16x8, qw[mb][x]), st[mb][p]);
+          } else {
+            const f32x4 kf = __builtin_bit_cast(f32x4, kw), qf = __builtin_bit_cast(f32x4, qw[mb][x]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st[mb][p] = M::mma(kf[e], qf[e], st[mb][p]);
+          }
+        }
       }
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
@@ -191,8 +211,8 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
         for (int r = 0; r < 4; ++r) {
           float x = st[mb][p][r] * a.scale_log2;
           if (!whole) {
-            const int key = j + 16 * p + 4 * g + r;
-            x = here[p] && key < k1 && key <= limit[mb] ? x : -INFINITY;
+            const int at = 4 * g + r;
+            x = at < here[p] && j + 16 * p + at <= limit[mb] ? x : -INFINITY;
           }
           st[mb][p][r] = x;
           top = fmaxf(top, x);
@@ -239,14 +259,29 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
         for (int mb = 0; mb < MB; ++mb) acc[mb][db] = M::mma(vf, pf[mb], acc[mb][db]);
       }
     } else {
+      // V in wide reads: row i of the four blocks 4 x .. 4 x + 3 is column
+      // 64 x + 4 i + their number, and of a last pair 64 x + 2 i + its number
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 4; ++r) {
+        const float* const vrow = vt + (4 * g + r) * L::S;
 #pragma unroll
-        for (int db = 0; db < DP / 16; ++db) {
-          const float vf = vt[(4 * g + r) * L::S + 16 * db + col];
+        for (int x = 0; x < DP / 64; ++x) {
+          const f32x4 vf = *reinterpret_cast<const f32x4*>(vrow + 64 * x + 4 * col);
 #pragma unroll
-          for (int mb = 0; mb < MB; ++mb) acc[mb][db] = M::mma(vf, st[mb][0][r], acc[mb][db]);
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+              acc[mb][4 * x + e] = M::mma(vf[e], st[mb][0][r], acc[mb][4 * x + e]);
         }
+        if constexpr (DP % 64 != 0) {
+          const float2 vf = *reinterpret_cast<const float2*>(vrow + DP / 64 * 64 + 2 * col);
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) {
+            acc[mb][DP / 16 - 2] = M::mma(vf.x, st[mb][0][r], acc[mb][DP / 16 - 2]);
+            acc[mb][DP / 16 - 1] = M::mma(vf.y, st[mb][0][r], acc[mb][DP / 16 - 1]);
+          }
+        }
+      }
     }
   }
 
@@ -257,9 +292,25 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
   for (int mb = 0; mb < MB; ++mb) {
     const float total = col_sum_swap(l[mb]);
     const int row = 16 * mb + col;
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int db = 0; db < DP / 16; ++db)
-      store4(mine + row * L::OS + 16 * db + 4 * g, acc[mb][db]);
+      for (int db = 0; db < DP / 16; ++db)
+        store4(mine + row * L::OS + 16 * db + 4 * g, acc[mb][db]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int x = 0; x < DP / 64; ++x) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[mb][4 * x + e][r];
+          store4(mine + row * L::OS + 64 * x + 16 * g + 4 * r, v);
+        }
+        if constexpr (DP % 64 != 0)
+          *reinterpret_cast<float2*>(mine + row * L::OS + DP / 64 * 64 + 8 * g + 2 * r) =
+              make_float2(acc[mb][DP / 16 - 2][r], acc[mb][DP / 16 - 1][r]);
+      }
+    }
     if (g == 0) {
       mine[ROWS * L::OS + row] = m[mb];
       mine[ROWS * (L::OS + 1) + row] = total;
@@ -268,16 +319,16 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
   __syncthreads();
   const float* const all = reinterpret_cast<const float*>(smem);
   constexpr int CPR = DP / 4;
-  for (int idx = threadIdx.x; idx < ROWS * CPR; idx += 64 * kWavesCa) {
+  for (int idx = threadIdx.x; idx < ROWS * CPR; idx += 64 * WAVES) {
     const int row = idx / CPR, d = 4 * (idx % CPR), r = r0 + row;
     if (r >= n_rows || d >= D) continue;
     float mx = kNegBig;
 #pragma unroll
-    for (int u = 0; u < kWavesCa; ++u) mx = fmaxf(mx, all[u * L::WAVE + ROWS * L::OS + row]);
+    for (int u = 0; u < WAVES; ++u) mx = fmaxf(mx, all[u * L::WAVE + ROWS * L::OS + row]);
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float total = 0.0f;
 #pragma unroll
-    for (int u = 0; u < kWavesCa; ++u) {
+    for (int u = 0; u < WAVES; ++u) {
       const float* reg = all + u * L::WAVE;
       const float f = weight(reg[ROWS * L::OS + row] - mx);
       total += f * reg[ROWS * (L::OS + 1) + row];
@@ -302,24 +353,32 @@ __global__ __launch_bounds__(64 * kWavesCa) void cache_attn_kernel(CacheAttn a) 
   }
 }
 
-// Joins the splits of a row: one wave each, four to a workgroup.
-template <typename T>
+// Joins the splits of a row.  A split's sums take ceil(D / 4) lanes of 4
+// columns, so a wave reads several splits at once where D <= 128, and up to
+// eight such loads are in flight.  WAVES waves share a row (1: few splits; 4:
+// many, so that 64 splits are one round of loads deep: one wave for them all
+// took 20 us of a 77 us call).
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttn a) {
+  __shared__ f32x4 part[4][64];
   const CacheView& c = a.c;
-  const int lane = threadIdx.x & 63;
-  const long at = (long)blockIdx.x * 4 + wave_id();
+  const int lane = threadIdx.x & 63, w = wave_id();
+  const long at = WAVES == 1 ? (long)blockIdx.x * 4 + w : blockIdx.x;
   if (at >= (long)c.T * a.hq) return;
   const int t = static_cast<int>(at / a.hq), h = static_cast<int>(at % a.hq);
-  const int b = __builtin_amdgcn_readfirstlane(
-      count_prefix(c.n_seqs, lane, [&](int i) { return c.cu[i + 1] <= t; }));
-  if (b >= c.n_seqs) return;
-  const CacheSeq s = cache_seq(c, b);
+  const CacheSeq s = seq_of_token(c, lane, t);
+  if (s.b >= c.n_seqs) return;
   if (t < s.tok0) return;
   const TileKeys tk = tile_keys(a, s, ((t - s.tok0) * a.group + h % a.group) / a.rows);
   if (tk.active <= 1) return;
   const long step = (long)c.T * a.hq;
   float2 ml = make_float2(kNegBig, 0.0f);
   if (lane < tk.active) ml = a.part_ml[lane * step + at];
+  // lanes of a split: a power of two that holds D / 4
+  const int lanes = c.D <= 32 ? 8 : c.D <= 64 ? 16 : c.D <= 128 ? 32 : 64;
+  const int per_load = 64 / lanes, d = 4 * (lane % lanes);
+  const int first = (WAVES == 1 ? 0 : w * per_load) + lane / lanes, stride = WAVES * per_load;
+  f32x4 v[8], o = {0.0f, 0.0f, 0.0f, 0.0f};
   float mx = ml.x;
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x));
@@ -327,18 +386,36 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttn a) {
   float total = f * ml.y;
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  const int d = 4 * lane;
-  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int u = 0; u < tk.active; ++u) {
-    const float fu = __shfl(f, u);
-    if (d < c.D) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_o + (u * step + at) * c.D + d);
+  for (int u0 = 0; u0 < tk.active; u0 += 8 * stride) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += fu * v[e];
+    for (int i = 0; i < 8; ++i) {
+      const int u = u0 + i * stride + first;
+      v[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (u < tk.active && d < c.D)
+        v[i] = *reinterpret_cast<const f32x4*>(a.part_o + (u * step + at) * c.D + d);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int u = u0 + i * stride + first;
+      const float fu = __shfl(f, u & 63);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += (u < tk.active ? fu : 0.0f) * v[i][e];
     }
   }
-  if (d < c.D) {
+  for (int x = lanes; x < 64; x *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
+  if constexpr (WAVES > 1) {
+    part[w][lane] = o;
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int u = 1; u < WAVES; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += part[u][lane][e];
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  if (lane < lanes && d < c.D) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] *= inv;
     store4(static_cast<T*>(a.out) + at * c.D + d, o);
@@ -347,32 +424,36 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttn a) {
     a.lse[(long)h * c.T + t] = total == 0.0f ? -INFINITY : (mx + log2f(total)) * kLn2;
 }
 
-template <typename T, int DP, int MB>
+template <typename T, int DP, int MB, int WAVES>
 hipError_t attend(const CacheAttn& a, hipStream_t st) {
-  using L = CaLayout<T, DP, MB>;
-  auto* fn = &cache_attn_kernel<T, DP, MB>;
+  using L = CaLayout<T, DP, MB, WAVES>;
+  auto* fn = &cache_attn_kernel<T, DP, MB, WAVES>;
   GL_CHECK(allow_lds(fn, L::BYTES));
-  hipLaunchKernelGGL((cache_attn_kernel<T, DP, MB>), dim3(tile_numbers(a), a.c.hkv, a.n_splits),
-                     dim3(64 * kWavesCa), L::BYTES, st, a);
+  hipLaunchKernelGGL((cache_attn_kernel<T, DP, MB, WAVES>), dim3(tile_numbers(a), a.c.hkv, a.n_splits),
+                     dim3(64 * WAVES), L::BYTES, st, a);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t join(const CacheAttn& a, hipStream_t st) {
   const long rows = (long)a.c.T * a.hq;
-  hipLaunchKernelGGL(cache_attn_join_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0,
-                     st, a);
+  if (a.n_splits <= 8)
+    hipLaunchKernelGGL((cache_attn_join_kernel<T, 1>), dim3(static_cast<unsigned>((rows + 3) / 4)),
+                       dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((cache_attn_join_kernel<T, 4>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t by_head(const CacheAttn& a, hipStream_t st) {
+  constexpr int WAVES = sizeof(T) == 2 ? 4 : 8;
   const int d = a.c.D;
-  if (d <= 32) return attend<T, 32, 1>(a, st);
-  if (d <= 64) return attend<T, 64, 1>(a, st);
-  if (d <= 96) return attend<T, 96, 1>(a, st);
-  if (d <= 128) return attend<T, 128, 1>(a, st);
-  return attend<T, 256, 1>(a, st);
+  if (d <= 32) return attend<T, 32, 1, WAVES>(a, st);
+  if (d <= 64) return attend<T, 64, 1, WAVES>(a, st);
+  if (d <= 96) return attend<T, 96, 1, WAVES>(a, st);
+  if (d <= 128) return attend<T, 128, 1, WAVES>(a, st);
+  return attend<T, 256, 1, 4>(a, st);  // eight waves' fp32 tiles exceed the LDS
 }
 
 }  // namespace
@@ -384,10 +465,23 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   const long keys = max_kv > 0 && max_kv < cap ? max_kv : cap;
   const long longest = max_new > 0 && max_new < c.T ? max_new : c.T;  // chunk
   p.rows = c.io_bf16 && c.D <= 128 && longest * group > 64 ? kCacheWideRows : 16;
-  const long tiles = (c.T * group + p.rows - 1) / p.rows + std::min(c.T, c.n_seqs) / 2;
-  // enough workgroups for two on each CU, of 256 keys or more
-  const long want = 2L * n_cu / std::max(1L, tiles * c.hkv);
-  const long most = (keys + 255) / 256;
+  // tiles, if the new tokens are spread evenly over the sequences
+  const long seqs = std::min(c.T, c.n_seqs);
+  const long tiles = seqs * ((c.T * group + seqs * p.rows - 1) / (seqs * p.rows));
+  // Splits of 512 keys or more, as many as fill the workgroups the CUs hold at
+  // once (by their LDS); none up to 1024 keys, where the second launch costs
+  // more than the shorter chain gives.  us a call, one token a sequence, 28/4
+  // heads of 128: one sequence of 2048 keys 11.8 in splits of 512, 15.5 of
+  // 1024, 19.4 whole; 8192 keys 12.2, 15.9, 23.2 in splits of 512, 1024, 2048;
+  // 32 sequences of up to 1024 keys 12.8 whole, 15.8 in two; of up to 8192 keys
+  // 93, 73, 77 for one, two and four workgroups a CU.  14/2 heads of 64, 64
+  // sequences of up to 4096 keys: 24.8, 23.2, 21.5.  Eight waves a workgroup
+  // instead of four: fp32 128 tokens over 4096 keys 37 -> 30; bf16 64 sequences
+  // of up to 512 keys 12.1 -> 15.1.
+  const long per_cu = p.rows == kCacheWideRows ? 4 : !c.io_bf16 ? 1 : c.D <= 64 ? 4 : c.D <= 128 ? 2 : 1;
+  const long want = per_cu * n_cu / (tiles * c.hkv);
+  const bool full = p.rows == kCacheWideRows && 2 * tiles * c.hkv >= 3L * n_cu;
+  const long most = keys <= 1024 || full ? 1 : (keys + 511) / 512;
   p.n_splits = static_cast<int>(std::max(1L, std::min({want, most, (long)kMaxSplits})));
   const long even = (keys + p.n_splits - 1) / p.n_splits;
   p.split_keys = static_cast<int>((even + kSplitUnit - 1) / kSplitUnit * kSplitUnit);

@@ -53,11 +53,10 @@ __global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(Cac
   // later tiles see more keys: they start first
   const int number = static_cast<int>(gridDim.x - 1 - blockIdx.x);
 
-  const int b = __builtin_amdgcn_readfirstlane(
-      count_prefix(c.n_seqs, lane, [&](int i) { return first_tile(a, i + 1) <= number; }));
+  const CacheSeq s = seq_of_tile(a, lane, number);
+  const int b = s.b;
   if (b >= c.n_seqs) return;
-  const CacheSeq s = cache_seq(c, b);
-  const int tile = number - first_tile(a, b);
+  const int tile = number - first_tile(a, b, s.tok0);
   const int r0 = tile * kRowsWide, n_rows = s.n * a.group;
   if (tile < 0 || r0 >= n_rows) return;
   const TileKeys tk = tile_keys(a, s, tile);
@@ -70,11 +69,17 @@ __global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(Cac
   const int limit = live ? s.pos0 + tok : -1;
   const long at = (long)(s.tok0 + tok) * a.hq + kvh * a.group + (r - tok * a.group);
   bf16x8 qf[W::NKK];
+  {
+    // (from the tile's first row where there is none, and cleared after all
+    // loads are under way)
+    const bf16* const q = static_cast<const bf16*>(a.q) +
+                          (live ? at : (long)(s.tok0 + r0 / a.group) * a.hq) * D;
 #pragma unroll
-  for (int kk = 0; kk < W::NKK; ++kk) {
-    qf[kk] = frag_zero<bf16>();
-    if (live && 16 * kk + 8 * h < D)
-      qf[kk] = *reinterpret_cast<const bf16x8*>(static_cast<const bf16*>(a.q) + at * D + 16 * kk + 8 * h);
+    for (int kk = 0; kk < W::NKK; ++kk)
+      qf[kk] = *reinterpret_cast<const bf16x8*>(q + (16 * kk + 8 * h < D ? 16 * kk + 8 * h : 0));
+#pragma unroll
+    for (int kk = 0; kk < W::NKK; ++kk)
+      if (!live || 16 * kk + 8 * h >= D) qf[kk] = frag_zero<bf16>();
   }
   // a wave's rows see keys first_limit at least, and none past last_limit
   const int wr = r0 + 32 * w;

@@ -11,10 +11,12 @@ namespace glacier {
 constexpr int kMaxSplits = 64;   // one lane each in the join
 constexpr int kSplitUnit = 128;  // splits begin at multiples of it
 
-// The first tile number of sequence b: tiles of all sequences in a row, with
-// one number at most left unused per sequence.
-__device__ inline int first_tile(const CacheAttn& a, int b) {
-  return clamp_row(a.c.cu[b], a.c.T) * a.group / a.rows + b;
+// Tiles are numbered through all sequences: sequence b's first one is
+// first_tile(a, b, cu[b]), which leaves room for every tile it can have.
+__device__ inline int first_tile(const CacheAttn& a, int b, int cu) { return cu * a.group / a.rows + b; }
+// The sequence of tile `number`.
+__device__ inline CacheSeq seq_of_tile(const CacheAttn& a, int lane, int number) {
+  return find_seq(a.c, lane, number, [&](int b, int to) { return first_tile(a, b, to); });
 }
 
 // How many tile numbers a batch of the call's size can use at most.
@@ -25,7 +27,7 @@ inline unsigned tile_numbers(const CacheAttn& a) {
 // The keys of a tile whose last row is token `last`, and how they are split.
 struct TileKeys {
   int kend;  // keys 0 .. kend - 1
-  int per, active;
+  int per, active;  // keys of a split, and how many splits have any
 };
 __device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int tile) {
   TileKeys k;
@@ -35,6 +37,9 @@ __device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int 
   k.kend = static_cast<int>(end < 0 ? 0 : end < cap ? end : cap);
   const int even = (k.kend + a.n_splits - 1) / a.n_splits;
   k.per = max(a.split_keys, (even + kSplitUnit - 1) / kSplitUnit * kSplitUnit);
+  k.active = max(1, (k.kend + k.per - 1) / k.per);
+  // as many splits as that, evenly
+  k.per = ((k.kend + k.active - 1) / k.active + kSplitUnit - 1) / kSplitUnit * kSplitUnit;
   k.active = max(1, (k.kend + k.per - 1) / k.per);
   return k;
 }

@@ -16,30 +16,33 @@ struct CacheSeq {
   int b, tok0, n, pos0;
 };
 
-// How many of 0 .. n_seqs - 1 satisfy the test (b), which holds for a prefix
-// of them: 64 at a time, one a lane, so that a search is one load deep.
-template <typename F>
-__device__ inline int count_prefix(int n_seqs, int lane, F test) {
-  int count = 0;
-  for (int b0 = 0; b0 < n_seqs; b0 += 64) {
-    const int b = b0 + lane;
-    const unsigned long long m = __ballot(b < n_seqs && test(b));
-    count += __popcll(m);
-    if (m != ~0ull) break;
-  }
-  return count;
-}
-
 __device__ inline int clamp_row(int r, int T) { return r < 0 ? 0 : r > T ? T : r; }
 
-__device__ inline CacheSeq cache_seq(const CacheView& c, int b) {
-  CacheSeq s;
-  s.b = b;
-  s.tok0 = clamp_row(c.cu[b], c.T);
-  const int end = clamp_row(c.cu[b + 1], c.T);
-  s.n = end > s.tok0 ? end - s.tok0 : 0;
-  s.pos0 = c.kv_lens[b] - s.n;
+// The sequence b with start(b, cu[b]) <= x < start(b + 1, cu[b + 1]), start
+// growing with b; b = n_seqs if there is none.  Every lane reads one sequence's
+// entries, 64 sequences at a time, and the lane that holds the sequence hands
+// them out: the search and the sequence's lengths are one load deep together.
+template <typename F>
+__device__ inline CacheSeq find_seq(const CacheView& c, int lane, int x, F start) {
+  CacheSeq s{c.n_seqs, 0, 0, 0};
+  for (int b0 = 0; b0 < c.n_seqs; b0 += 64) {
+    const int b = b0 + lane, i = b < c.n_seqs ? b : c.n_seqs - 1;
+    const int from = clamp_row(c.cu[i], c.T), to = clamp_row(c.cu[i + 1], c.T), len = c.kv_lens[i];
+    const int before = __popcll(__ballot(b < c.n_seqs && start(i + 1, to) <= x));
+    if (before == 64) continue;
+    if (b0 + before >= c.n_seqs) break;
+    s.b = b0 + before;
+    s.tok0 = __builtin_amdgcn_readlane(from, before);
+    const int end = __builtin_amdgcn_readlane(to, before);
+    s.n = end > s.tok0 ? end - s.tok0 : 0;
+    s.pos0 = __builtin_amdgcn_readlane(len, before) - s.n;
+    break;
+  }
   return s;
+}
+// The sequence that token row t belongs to.
+__device__ inline CacheSeq seq_of_token(const CacheView& c, int lane, int t) {
+  return find_seq(c, lane, t, [](int, int to) { return to; });
 }
 
 // The page of positions p .. (same page) of sequence b, or -1.
