@@ -30,17 +30,100 @@ constexpr float kGrowth = 8.0f;
 
 template <int DP>
 struct Wide {
-  static constexpr int RB = 2 * DP;           // bytes of an LDS row
-  static constexpr int PPR = DP / 8;          // 16-byte pieces of a row
-  static constexpr int RPI = 64 * kWavesWide / PPR;  // rows one load of all threads covers
-  static constexpr int NI = kKeysWide / RPI;  // loads per thread of a K or V tile
+  static constexpr int RB = 2 * DP;   // bytes of an LDS row
+  static constexpr int PPR = DP / 8;  // 16-byte pieces of a row
   static constexpr int TILE = kKeysWide * RB;
-  static constexpr int BYTES = 4 * TILE;  // K and V, two buffers
+  static constexpr int BYTES = 4 * TILE;  // K and V, two slots each
   static constexpr int NKK = DP / 16, NDB = DP / 32;
+  static constexpr int ND = 16 * RB / 1024;  // DMA instructions of a page piece
 };
 
 __device__ inline f32x16 mma16(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// 1 KB of a wave's [base, base + bytes) to LDS, lane l's 16 bytes from `off` to
+// to + 16 l; zeros past the end.
+__device__ inline void dma16(const void* base, int bytes, int off, unsigned char* to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(wave_rsrc(base, bytes), (GLACIER_LDS void*)to, 16, off, 0, 0, 0);
+#endif
+}
+
+// What a wave carries from tile to tile.
+template <int DP>
+struct WideState {
+  f32x16 o[DP / 32];  // O^T
+  float m, l, top;    // reference, sum, and the next tile's largest score
+};
+
+template <int DP>
+__device__ __forceinline__ void wide_scores(f32x16 (&st)[2], const unsigned char* kt, const int (&koff)[DP / 16],
+                                            const bf16x8 (&qf)[DP / 16]) {
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) st[kb][e] = 0.0f;
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+      st[kb] = mma16(*reinterpret_cast<const bf16x8*>(kt + koff[kk] + kb * 32 * 2 * DP), qf[kk], st[kb]);
+}
+
+__device__ __forceinline__ float wide_largest(const f32x16 (&st)[2]) {
+  float top = fmaxf(st[0][0], st[1][0]);
+#pragma unroll
+  for (int e = 1; e < 16; ++e) top = fmaxf(fmaxf(top, st[0][e]), st[1][e]);
+  return top;
+}
+
+// One tile: its scores st (formed a tile earlier) become weights and meet V,
+// while the next tile's scores are formed into sn.
+template <int DP>
+__device__ __forceinline__ void wide_step(WideState<DP>& w, f32x16 (&st)[2], f32x16 (&sn)[2],
+                                          const unsigned char* __restrict__ kt,
+                                          const unsigned char* __restrict__ vt, const int (&koff)[DP / 16],
+                                          const int (&voff)[DP / 32][2], const bf16x8 (&qf)[DP / 16],
+                                          float scale_log2) {
+  w.top = swap_max(w.top, false) * scale_log2;
+  if (__any(w.top > w.m + kGrowth)) {
+    const float mn = fmaxf(w.m, w.top);
+    const float f = weight(w.m - mn);
+    w.m = mn;
+    w.l *= f;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w.o[db][e] *= f;
+  }
+  wide_scores<DP>(sn, kt, koff, qf);
+  bf16x8 pf[4];
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      st[kb][e] = weight(fmaf(st[kb][e], scale_log2, -w.m));
+      pf[2 * kb + e / 8][e % 8] = (bf16)st[kb][e];
+    }
+#pragma unroll
+  for (int sp = 0; sp < 4; ++sp)
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+      const unsigned char* const p = vt + sp * 16 * 2 * DP;
+      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+          (bf16x4 GLACIER_LDS*)(const_cast<unsigned char*>(p + voff[db][0])));
+      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+          (bf16x4 GLACIER_LDS*)(const_cast<unsigned char*>(p + voff[db][1])));
+      w.o[db] = mma16(join8(lo, hi), pf[sp], w.o[db]);
+    }
+  float sum = 0.0f;
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum += st[kb][e];
+  w.l += sum;
+  w.top = wide_largest(sn);
 }
 
 template <int DP>
@@ -49,9 +132,9 @@ __global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(Cac
   extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
   const int w = wave_id(), lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
-  const int kvh = blockIdx.y, split = blockIdx.z, D = c.D;
+  const int kvh = blockIdx.x % c.hkv, split = blockIdx.y, D = c.D;
   // later tiles see more keys: they start first
-  const int number = static_cast<int>(gridDim.x - 1 - blockIdx.x);
+  const int number = static_cast<int>((gridDim.x - 1 - blockIdx.x) / c.hkv);
 
   const CacheSeq s = seq_of_tile(a, lane, number);
   const int b = s.b;
@@ -86,13 +169,6 @@ __global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(Cac
   const int first_limit = s.pos0 + wr / a.group;
   const int last_limit = wr < n_rows ? s.pos0 + min(s.n - 1, (wr + 31) / a.group) : -1;
 
-  f32x16 o[W::NDB];
-#pragma unroll
-  for (int db = 0; db < W::NDB; ++db)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
-  float m = kNegBig, l = 0.0f;
-
   // LDS offsets of this lane's reads: K pieces of row col; V pieces of rows
   // 4 h + 8 u + (lane % 16) / 4 at columns 32 db + 16 (lane / 16 % 2) + 4 (lane % 4)
   int koff[W::NKK], voff[W::NDB][2];
@@ -109,81 +185,78 @@ __global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(Cac
       }
   }
 
-  // this thread's share of a tile: rows row0 + RPI i, piece `piece`.  The 16
-  // rows of a page piece are read through a buffer resource that ends with the
-  // last one that holds a key (none without a page): what lies past it, and
-  // past column D, arrives as zero, with no branch and no address arithmetic
-  // in vector registers.
-  const int piece = threadIdx.x % W::PPR, row0 = threadIdx.x / W::PPR;
-  const int wrow0 = w * (64 / W::PPR);  // the wave's rows of one load lie in one page piece
+  // A tile is four page pieces of 16 keys; a wave brings one of them, of K and
+  // of V.  The piece is read through a buffer resource that
+  // ends with its last key (none without a page): what lies past it, and past
+  // column D, arrives as zero.
   const int rowb = 2 * D;
-  const int loff = 8 * piece < D ? (row0 & 15) * rowb + 16 * piece : 1 << 20;
-  int soff[W::NI];
+  int doff[W::ND];
 #pragma unroll
-  for (int i = 0; i < W::NI; ++i) {
-    const int row = row0 + i * W::RPI;
-    soff[i] = row * W::RB + 16 * (piece ^ lds_sw<DP>(row));
+  for (int n = 0; n < W::ND; ++n) {
+    const int row = n * (1024 / W::RB) + lane / W::PPR, piece = lane % W::PPR ^ lds_sw<DP>(row);
+    doff[n] = 8 * piece < D ? row * rowb + 16 * piece : 1 << 20;
   }
   const int in_page = (1 << c.page_shift) - 1;
   const long head = ((long)kvh << c.page_shift) * rowb, strideb = 2 * c.page_stride;
-  // the pages of a tile's four pieces of 16 keys, one a lane; none (-1) past k1
+  // the page of this wave's piece of tile j (-1: none), by a scalar load: a
+  // vector load would make the wave wait for every DMA it has in flight
+  const auto* const table = (const __attribute__((address_space(4))) int32_t*)(
+      reinterpret_cast<uintptr_t>(c.table + (long)b * c.table_stride));
   auto look_up = [&](int j) {
-    const int key = j + 16 * (lane & 3);
-    return key < k1 ? cache_page(c, b, key) : -1;
+    const int at = (j + 16 * w) >> c.page_shift;
+    const int page = table[min(at, c.max_pages - 1)];
+    return j + 16 * w < k1 && static_cast<unsigned>(page) < static_cast<unsigned>(c.n_pages) ? page : -1;
   };
-  i32x4 kr[W::NI], vr[W::NI];
-  auto fetch = [&](int j, int pages) {
+  auto bring = [&](const void* pages, unsigned char* to, int j, int page) {
+    const int key = j + 16 * w;
+    const long off = (page < 0 ? 0 : page) * strideb + head + (key & in_page) * rowb;
+    const int bytes = (page < 0 ? 0 : min(16, k1 - key)) * rowb;
 #pragma unroll
-    for (int i = 0; i < W::NI; ++i) {
-      const int key = j + (wrow0 + i * W::RPI) / 16 * 16;
-      const int page = __builtin_amdgcn_readlane(pages, (wrow0 + i * W::RPI) / 16);
-      const long off = (page < 0 ? 0 : page) * strideb + head + (key & in_page) * rowb;
-      const int rows = page < 0 ? 0 : min(16, k1 - key);
-      kr[i] = load_within(static_cast<const char*>(c.k_pages) + off, rows * rowb, loff);
-      vr[i] = load_within(static_cast<const char*>(c.v_pages) + off, rows * rowb, loff);
-    }
+    for (int n = 0; n < W::ND; ++n)
+      dma16(static_cast<const char*>(pages) + off, bytes, doff[n], to + w * 16 * W::RB + 1024 * n);
   };
-  auto put = [&](int buf) {
-    unsigned char* const t = smem + buf * 2 * W::TILE;
-#pragma unroll
-    for (int i = 0; i < W::NI; ++i) {
-      *reinterpret_cast<i32x4*>(t + soff[i]) = kr[i];
-      *reinterpret_cast<i32x4*>(t + W::TILE + soff[i]) = vr[i];
-    }
-  };
+  unsigned char* const ks[2] = {smem, smem + W::TILE};
+  unsigned char* const vs[2] = {smem + 2 * W::TILE, smem + 3 * W::TILE};
+  // whether every piece of the keys has a page (if not, each tile is looked at)
+  bool clean = true;
+  for (int p = (k0 >> c.page_shift) + lane; p <= (k1 - 1) >> c.page_shift; p += 64)
+    clean = clean && cache_page(c, b, p << c.page_shift) >= 0;
+  clean = __all(clean);
 
-  int next = look_up(k0), held = 0;  // held: which pieces of the tile in LDS have a page
+  WideState<DP> ws;
+#pragma unroll
+  for (int db = 0; db < W::NDB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ws.o[db][e] = 0.0f;
+  ws.m = kNegBig;
+  ws.l = 0.0f;
+  ws.top = kNegBig;
+  f32x16 sa[2], sb[2];
+  int v_page = -1, k_page = -1;  // of the next V tile and of the K tile after it
   if (k0 < k1) {
-    const int pages = next;
-    next = look_up(k0 + kKeysWide);
-    fetch(k0, pages);
-    held = static_cast<int>(__ballot(pages >= 0)) & 15;
-    put(0);
+    const int first = look_up(k0);
+    v_page = look_up(k0 + kKeysWide);
+    k_page = look_up(k0 + 2 * kKeysWide);
+    bring(c.k_pages, ks[0], k0, first);
+    bring(c.v_pages, vs[0], k0, first);
+    bring(c.k_pages, ks[1], k0 + kKeysWide, v_page);
+    vmw<0>();
+    wg_barrier();
+    wide_scores<DP>(sa, ks[0], koff, qf);
+    ws.top = wide_largest(sa);
+    lgkm<0>();
+    wg_barrier();
   }
-  __syncthreads();
-  int buf = 0;
-  for (int j = k0; j < k1; j += kKeysWide, buf ^= 1) {
-    const bool more = j + kKeysWide < k1;
-    int held_next = 0;
-    if (more) {
-      const int pages = next;
-      next = look_up(j + 2 * kKeysWide);
-      fetch(j + kKeysWide, pages);
-      held_next = static_cast<int>(__ballot(pages >= 0)) & 15;
-    }
+  auto tile_step = [&](f32x16 (&st)[2], f32x16 (&sn)[2], int j, int odd) {
+    bring(c.k_pages, ks[odd], j + 2 * kKeysWide, k_page);
+    bring(c.v_pages, vs[odd ^ 1], j + kKeysWide, v_page);
+    v_page = k_page;
+    k_page = look_up(j + 3 * kKeysWide);
+    __builtin_amdgcn_sched_barrier(0);
     if (j <= last_limit) {
-      const unsigned char* const kt = smem + buf * 2 * W::TILE;
-      const unsigned char* const vt = kt + W::TILE;
-      f32x16 st[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) st[kb][e] = 0.0f;
-#pragma unroll
-        for (int kk = 0; kk < W::NKK; ++kk)
-          st[kb] = mma16(*reinterpret_cast<const bf16x8*>(kt + koff[kk] + kb * 32 * W::RB), qf[kk], st[kb]);
-      }
-      if (j + kKeysWide - 1 > first_limit || j + kKeysWide > k1 || held != 15) {
+      if (j + kKeysWide - 1 > first_limit || j + kKeysWide > k1 || !clean) {
+        const int at = j + 16 * (lane & 3);
+        const int held = clean ? 15 : static_cast<int>(__ballot(at < k1 && cache_page(c, b, at) >= 0)) & 15;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -191,50 +264,21 @@ __global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(Cac
             const int key = j + 32 * kb + 8 * (e / 4) + 4 * h + e % 4;
             st[kb][e] = (held >> (2 * kb + e / 8) & 1) && key < k1 && key <= limit ? st[kb][e] : -INFINITY;
           }
+        ws.top = wide_largest(st);
       }
-      float top = st[0][0];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, st[kb][e]);
-      top = swap_max(top, false) * a.scale_log2;
-      if (__any(top > m + kGrowth)) {
-        const float mn = fmaxf(m, top);
-        const float f = weight(m - mn);
-        m = mn;
-        l *= f;
-#pragma unroll
-        for (int db = 0; db < W::NDB; ++db)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[db][e] *= f;
-      }
-      bf16x8 pf[4];
-      float sum = 0.0f;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = weight(fmaf(st[kb][e], a.scale_log2, -m));
-          sum += p;
-          pf[2 * kb + e / 8][e % 8] = (bf16)p;
-        }
-      l += sum;
-#pragma unroll
-      for (int sp = 0; sp < 4; ++sp)
-#pragma unroll
-        for (int db = 0; db < W::NDB; ++db) {
-          const unsigned char* const p = vt + sp * 16 * W::RB;
-          const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-              (bf16x4 GLACIER_LDS*)(const_cast<unsigned char*>(p + voff[db][0])));
-          const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-              (bf16x4 GLACIER_LDS*)(const_cast<unsigned char*>(p + voff[db][1])));
-          o[db] = mma16(join8(lo, hi), pf[sp], o[db]);
-        }
+      wide_step<DP>(ws, st, sn, ks[odd ^ 1], vs[odd], koff, voff, qf, a.scale_log2);
     }
-    if (more) put(buf ^ 1);
-    held = held_next;
-    __syncthreads();
+    vmw<0>();
+    lgkm<0>();
+    wg_barrier();
+  };
+  for (int j = k0; j < k1; j += 2 * kKeysWide) {
+    tile_step(sa, sb, j, 0);
+    if (j + kKeysWide < k1) tile_step(sb, sa, j + kKeysWide, 1);
   }
+  f32x16 (&o)[W::NDB] = ws.o;
+  const float m = ws.m;
+  float l = ws.l;
   if (!live) return;
   l = swap_sum(l, false);
   // elements 4 q .. 4 q + 3 of block db are columns 32 db + 8 q + 4 h ..
@@ -266,7 +310,7 @@ template <int DP>
 hipError_t attend(const CacheAttn& a, hipStream_t st) {
   auto* fn = &cache_attn_wide_kernel<DP>;
   GL_CHECK(allow_lds(fn, Wide<DP>::BYTES));
-  hipLaunchKernelGGL((cache_attn_wide_kernel<DP>), dim3(tile_numbers(a), a.c.hkv, a.n_splits),
+  hipLaunchKernelGGL((cache_attn_wide_kernel<DP>), dim3(tile_numbers(a) * a.c.hkv, a.n_splits),
                      dim3(64 * kWavesWide), Wide<DP>::BYTES, st, a);
   return hipGetLastError();
 }
