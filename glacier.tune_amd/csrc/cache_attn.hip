@@ -464,10 +464,20 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   const long cap = (long)c.max_pages << c.page_shift;
   const long keys = max_kv > 0 && max_kv < cap ? max_kv : cap;
   const long longest = max_new > 0 && max_new < c.T ? max_new : c.T;  // chunk
-  p.rows = c.io_bf16 && c.D <= 128 && longest * group > 64 ? kCacheWideRows : 16;
-  // tiles, if the new tokens are spread evenly over the sequences
+  // tiles of so many rows, if the new tokens are spread evenly over the sequences
   const long seqs = std::min(c.T, c.n_seqs);
-  const long tiles = seqs * ((c.T * group + seqs * p.rows - 1) / (seqs * p.rows));
+  auto tiles_of = [&](long rows) { return seqs * ((c.T * group + seqs * rows - 1) / (seqs * rows)); };
+  // Tiles of 128 rows for chunks that need more than one of 16, where tiles of 16
+  // would read enough keys (tiles x keys x D).  us a call, tiles of 16 and of 128:
+  // 28/4 heads of 128, 32 tokens over 1024 keys (7e6) 12.6, 18.3; 8 sequences of
+  // up to 4 over up to 2048 (17e6) 13.7, 18.3; 16 tokens over 8192 (29e6) 28.7,
+  // 20.2; 32 sequences of up to 8 over up to 2048 (134e6) 46, 30; 14/2 heads of
+  // 64, 8 sequences of up to 16 over up to 2048 (15e6) 12.9, 14.4; of up to 32
+  // (29e6) 18.4, 16.6.
+  const bool wide = c.io_bf16 && c.D <= 128 && longest * group > 16 &&
+                    (double)tiles_of(16) * c.hkv * keys * c.D > 25e6;
+  p.rows = wide ? kCacheWideRows : 16;
+  const long groups = tiles_of(p.rows) * c.hkv;
   // Splits of 512 keys or more, as many as fill the workgroups the CUs hold at
   // once (by their LDS); none up to 1024 keys, where the second launch costs
   // more than the shorter chain gives.  us a call, one token a sequence, 28/4
@@ -478,11 +488,21 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   // sequences of up to 4096 keys: 24.8, 23.2, 21.5.  Eight waves a workgroup
   // instead of four: fp32 128 tokens over 4096 keys 37 -> 30; bf16 64 sequences
   // of up to 512 keys 12.1 -> 15.1.
-  const long per_cu = p.rows == kCacheWideRows ? 4 : !c.io_bf16 ? 1 : c.D <= 64 ? 4 : c.D <= 128 ? 2 : 1;
-  const long want = per_cu * n_cu / (tiles * c.hkv);
-  const bool full = p.rows == kCacheWideRows && 2 * tiles * c.hkv >= 3L * n_cu;
-  const long most = keys <= 1024 || full ? 1 : (keys + 511) / 512;
-  p.n_splits = static_cast<int>(std::max(1L, std::min({want, most, (long)kMaxSplits})));
+  //
+  // Tiles of 128 rows, two to a CU: as many splits as fill it, of 256 keys or
+  // more (512 from 64 workgroups on, 2048 from 256 on), none up to 512 keys.  us
+  // a call, 28/4 heads of 128, whole and in 2, 4, 8 splits: 32 tokens over 8192
+  // keys (8 workgroups) 146, 83, 49, 35, and 25 in 32; 512 over 4096 (112) 80,
+  // 57, 52, 67; 512 over 512 19, 22; 2048 over 8192 (448) 232, 248, 260, 299;
+  // 16 chunks of up to 128 over up to 2048 (320) 55, 69; 8 of up to 256 over up
+  // to 4096 (320) 98, 87, 98, 119.
+  const long per_cu = wide ? 2 : !c.io_bf16 ? 1 : c.D <= 64 ? 4 : c.D <= 128 ? 2 : 1;
+  // (rounded up from the half where chunks differ and the estimate is high)
+  const long want = (per_cu * n_cu + (wide && c.n_seqs > 1 ? groups / 2 : 0)) / groups;
+  const long least = !wide ? 512 : groups < 64 ? 256 : groups < 256 ? 512 : 2048;
+  const long most = keys <= (wide ? 512 : 1024) ? 1 : keys / least;
+  const long cap_splits = wide && (long)c.T * hq > kCacheJoinRows ? kCacheTileJoin : kMaxSplits;
+  p.n_splits = static_cast<int>(std::max(1L, std::min({want, most, cap_splits})));
   const long even = (keys + p.n_splits - 1) / p.n_splits;
   p.split_keys = static_cast<int>((even + kSplitUnit - 1) / kSplitUnit * kSplitUnit);
   if (p.n_splits > 1) {
@@ -497,7 +517,8 @@ hipError_t launch_cache_attn(const CacheAttn& a, hipStream_t st) {
     GL_CHECK(launch_cache_attn_wide(a, st));
   else
     GL_CHECK(a.c.io_bf16 ? by_head<bf16>(a, st) : by_head<float>(a, st));
-  if (a.n_splits == 1) return hipSuccess;
+  // few splits of wide tiles are joined by tiles (launch_cache_attn_wide)
+  if (a.n_splits == 1 || (a.rows == kCacheWideRows && a.n_splits <= kCacheTileJoin)) return hipSuccess;
   return a.c.io_bf16 ? join<bf16>(a, st) : join<float>(a, st);
 }
 

@@ -306,6 +306,64 @@ __global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(Cac
     a.lse[(at % a.hq) * c.T + at / a.hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
+// Joins the splits of a tile's rows, 32 of them a workgroup: D / 4 lanes to a
+// row, four splits' sums in flight.  (A wave for each row, as after the 16-row
+// kernel, spends more on finding the row's sequence than on joining it: 84 us
+// for 16 sequences of up to 128 new tokens and 2048 keys that need 54 whole.)
+constexpr int kJoinRows = 32;
+__global__ __launch_bounds__(256) void cache_join_tiles_kernel(CacheAttn a) {
+  const CacheView& c = a.c;
+  const int lane = threadIdx.x & 63;
+  const int kvh = blockIdx.x % c.hkv, number = blockIdx.x / c.hkv;
+  const CacheSeq s = seq_of_tile(a, lane, number);
+  if (s.b >= c.n_seqs) return;
+  const int tile = number - first_tile(a, s.b, s.tok0);
+  const int r0 = tile * kRowsWide + blockIdx.y * kJoinRows, n_rows = s.n * a.group;
+  if (tile < 0 || r0 >= n_rows) return;
+  const TileKeys tk = tile_keys(a, s, tile);
+  if (tk.active <= 1) return;
+  const int lanes = c.D <= 64 ? 16 : 32, d = 4 * (threadIdx.x % lanes);
+  const long step = (long)c.T * a.hq;
+  for (int r = r0 + threadIdx.x / lanes; r < min(n_rows, r0 + kJoinRows); r += 256 / lanes) {
+    const int tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
+    const long t = s.tok0 + tok, at = t * a.hq + h;
+    float mx = kNegBig, total = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int u0 = 0; u0 < tk.active; u0 += 4) {
+      float2 ml[4];
+      f32x4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long slot = min(u0 + i, tk.active - 1) * step + at;
+        ml[i] = a.part_ml[slot];
+        v[i] = *reinterpret_cast<const f32x4*>(a.part_o + slot * c.D + (d < c.D ? d : 0));
+      }
+      float top = mx;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);
+      const float f = weight(mx - top);
+      mx = top;
+      total *= f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float g = u0 + i < tk.active ? weight(ml[i].x - mx) : 0.0f;
+        total += g * ml[i].y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += g * v[i][e];
+      }
+    }
+    if (d >= c.D) continue;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    store4(static_cast<bf16*>(a.out) + at * c.D + d, o);
+    if (a.lse != nullptr && d == 0)
+      a.lse[(long)h * c.T + t] = total == 0.0f ? -INFINITY : (mx + log2f(total)) * kLn2;
+  }
+}
+
 template <int DP>
 hipError_t attend(const CacheAttn& a, hipStream_t st) {
   auto* fn = &cache_attn_wide_kernel<DP>;
@@ -319,7 +377,11 @@ hipError_t attend(const CacheAttn& a, hipStream_t st) {
 
 hipError_t launch_cache_attn_wide(const CacheAttn& a, hipStream_t st) {
   static_assert(kRowsWide == kCacheWideRows, "rows of a wide tile");
-  return a.c.D <= 64 ? attend<64>(a, st) : attend<128>(a, st);
+  GL_CHECK(a.c.D <= 64 ? attend<64>(a, st) : attend<128>(a, st));
+  if (a.n_splits == 1 || a.n_splits > kCacheTileJoin) return hipSuccess;
+  hipLaunchKernelGGL(cache_join_tiles_kernel, dim3(tile_numbers(a) * a.c.hkv, kRowsWide / kJoinRows),
+                     dim3(256), 0, st, a);
+  return hipGetLastError();
 }
 
 }  // namespace glacier

@@ -80,6 +80,8 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
 hipError_t launch_cache_attn(const CacheAttn& a, hipStream_t st);
 
 constexpr int kCacheWideRows = 128;  // rows of a tile of cache_attn_wide.hip
+constexpr int kCacheTileJoin = 8;     // up to so many splits it joins them itself, tile by tile;
+constexpr int kCacheJoinRows = 2048;  // more, up to so many rows, go to a wave or four per row
 hipError_t launch_cache_attn_wide(const CacheAttn& a, hipStream_t st);
 
 }  // namespace glacier

@@ -73,16 +73,16 @@ class Paged:
     them) each; every page that a sequence needs is a random one of `spare`
     more than are needed; unused table entries are -1; K and V share one
     allocation, so that pages are more than a page apart.  Rows of a page that
-    hold no token are NaN."""
+    hold no token are NaN.  columns: of the page table, at least what is needed."""
 
-    def __init__(self, seqs, hq, hkv, d, page, dtype, seed, pad=0, spare=3, device="cuda"):
+    def __init__(self, seqs, hq, hkv, d, page, dtype, seed, pad=0, spare=3, device="cuda", columns=0):
         g = torch.Generator().manual_seed(seed)
         self.seqs, self.hq, self.hkv, self.d, self.page, self.dtype = seqs, hq, hkv, d, page, dtype
         self.tokens = sum(n for n, _ in seqs) + pad
         need = [-(-kv // page) for _, kv in seqs]
         order = torch.randperm(sum(need) + spare, generator=g)
         self.n_pages = len(order)
-        table = torch.full((len(seqs), max(need + [1]) + 1), -1, dtype=torch.int32)
+        table = torch.full((len(seqs), max(need + [columns - 1, 1]) + 1), -1, dtype=torch.int32)
         at = 0
         for b, k in enumerate(need):
             table[b, :k] = order[at:at + k].to(torch.int32)

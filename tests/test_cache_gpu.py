@@ -41,27 +41,62 @@ BATCHES = {
 }
 
 
+# The layout of the work follows from how many keys the page table or max_kv
+# allow: a table for 2^17 of them takes 128-row tiles (bf16, heads up to 128) and
+# many splits; the lengths themselves, mostly 16-row tiles.
+WIDE = 2 ** 17
+
+
+@pytest.mark.parametrize("columns", [0, WIDE])
 @pytest.mark.parametrize("dt", sorted(DTYPES))
 @pytest.mark.parametrize("name", sorted(BATCHES))
-def test_attention(eng, name, dt):
+def test_attention(eng, name, dt, columns):
     seqs, hq, hkv, d, page, pad = BATCHES[name]
-    p = ch.Paged(seqs, hq, hkv, d, page, DTYPES[dt], 5, pad)
+    p = ch.Paged(seqs, hq, hkv, d, page, DTYPES[dt], 5, pad, columns=columns // page)
     q = p.q.cuda()
     out = torch.full_like(q, 7.0)
     lse = torch.full((hq, p.tokens), 7.0, device="cuda")
     ref = ch.attend_ref(p)
     hints = dict(max_new=max(n for n, _ in seqs), max_kv=max(kv for _, kv in seqs))
-    for kw in ({}, hints):
+    few = dict(max_kv=20000)  # fewer splits than for 2^17 keys
+    for kw in (hints, few, {}):
         eng.cache_forward(q, *p.arrays(), out=out, lse=lse, **kw)
         ch.check("out", out, ref[0], ref[1])
         ch.check("lse", lse, ref[2], ref[3])
     if pad:  # rows behind the last sequence stay as they were
         assert (out[-pad:] == 7.0).all() and (lse[:, -pad:] == 7.0).all()
-    again, none = eng.cache_forward(q, *p.arrays(), **hints)
+    again, none = eng.cache_forward(q, *p.arrays())
     live = slice(0, p.tokens - pad)
     assert none is None and torch.equal(again[live], out[live])
-    eng.cache_forward(q, *p.arrays(), out=q, **hints)  # over its own queries
+    eng.cache_forward(q, *p.arrays(), out=q)  # over its own queries
     assert torch.equal(q[live], out[live])
+
+
+CHUNKS = {  # more than 16 rows a KV head: 128-row tiles where the table is wide
+    "d40": ([(30, 31), (129, 500), (0, 90)], 8, 2, 40, 16, 4),
+    "d64": ([(200, 900), (1, 3), (64, 64)], 14, 2, 64, 32, 0),
+    "d72": ([(65, 700)], 6, 2, 72, 64, 1),
+    "d8": ([(70, 200), (33, 40)], 8, 1, 8, 16, 0),
+    "d128_one_head_groups": ([(128, 128), (129, 130), (127, 1000)], 4, 4, 128, 16, 7),
+    "d128_group_of_40": ([(9, 3000), (5, 5)], 40, 1, 128, 128, 0),
+    "d128_many": ([(3 + i, 40 + 13 * i) for i in range(70)], 16, 2, 128, 16, 2),
+    "d120_long": ([(20, 6000)], 10, 2, 120, 512, 0),
+}
+
+
+@pytest.mark.parametrize("keys", [512, 1500, 3000, 9000, WIDE])
+@pytest.mark.parametrize("name", sorted(CHUNKS))
+def test_chunks_in_every_layout(eng, name, keys):
+    # max_kv only lays the work out: few or many splits, narrow or wide tiles
+    seqs, hq, hkv, d, page, pad = CHUNKS[name]
+    p = ch.Paged(seqs, hq, hkv, d, page, torch.bfloat16, 15, pad, columns=WIDE // page)
+    out = torch.full((p.tokens, hq, d), 7.0, device="cuda", dtype=torch.bfloat16)
+    lse = torch.full((hq, p.tokens), 7.0, device="cuda")
+    ref = ch.attend_ref(p)
+    eng.cache_forward(p.q.cuda(), *p.arrays(), max_kv=keys, out=out, lse=lse)
+    ch.check("out", out, ref[0], ref[1])
+    ch.check("lse", lse, ref[2], ref[3])
+    assert not pad or ((out[-pad:] == 7.0).all() and (lse[:, -pad:] == 7.0).all())
 
 
 @pytest.mark.parametrize("dt", sorted(DTYPES))
@@ -74,15 +109,16 @@ def test_wrong_hints_change_nothing_but_the_layout(eng, dt):
         ch.check("lse", lse, ref[2], ref[3])
 
 
+@pytest.mark.parametrize("columns", [0, WIDE // 16])
 @pytest.mark.parametrize("dt", sorted(DTYPES))
-def test_rows_without_a_key(eng, dt):
+def test_rows_without_a_key(eng, dt, columns):
     # a length below the number of new tokens leaves the first rows at negative
     # positions: they see nothing, get 0 and -inf, and append nothing
-    p = ch.Paged([(6, 9), (3, 3)], 4, 2, 64, 16, DTYPES[dt], 7)
+    p = ch.Paged([(6, 9), (3, 3)], 16, 2, 64, 16, DTYPES[dt], 7, columns=columns)
     p.kv_lens[1] = 1
     out, lse = eng.cache_forward(p.q.cuda(), *p.arrays(), save=True)
     assert not out[6:8].any() and (lse[:, 6:8] == -math.inf).all()
-    q = ch.Paged([(6, 9), (3, 3)], 4, 2, 64, 16, DTYPES[dt], 7)
+    q = ch.Paged([(6, 9), (3, 3)], 16, 2, 64, 16, DTYPES[dt], 7)
     q.seqs = [(6, 9), (1, 1)]
     q.q = torch.cat([p.q[:6], p.q[8:9]])
     q.tokens = 7
@@ -100,9 +136,10 @@ def test_rows_without_a_key(eng, dt):
         {(int(p.table[0, 0]), i) for i in range(3, 9)} | {(last, 0)}
 
 
+@pytest.mark.parametrize("columns", [0, WIDE // 16])
 @pytest.mark.parametrize("dt", sorted(DTYPES))
-def test_bad_pages_hold_no_keys(eng, dt):
-    p = ch.Paged([(4, 150), (1, 64), (1, 5)], 8, 2, 64, 16, DTYPES[dt], 8)
+def test_bad_pages_hold_no_keys(eng, dt, columns):
+    p = ch.Paged([(4, 150), (1, 64), (1, 5)], 16, 2, 64, 16, DTYPES[dt], 8, columns=columns)
     bad = {(0, 2): -1, (0, 9): p.n_pages, (1, 0): 2 ** 31 - 1, (2, 0): -2 ** 31}
     hidden = [(b, i) for (b, pg) in bad for i in range(16 * pg, min(16 * pg + 16, p.seqs[b][1]))]
     for (b, pg), to in bad.items():
