@@ -451,41 +451,48 @@ def cache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, m
     [n_pages, Hkv, page_size, D] of one dtype, each page contiguous and the
     pages any one stride apart; cu_tokens [n + 1], kv_lens [n] and page_table
     [n, max_pages] int32, the table's rows any stride apart."""
-    i32 = _torch().int32
-    if k_pages.dim() != 4:
+    shape, dtype, i32 = k_pages.shape, k_pages.dtype, _torch().int32
+    if len(shape) != 4:
         raise TypeError("k_pages must be [n_pages, n_heads_kv, page_size, head_dim]")
-    n_pages, hkv, page, d = k_pages.shape
-    strides = []
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if t.shape != k_pages.shape or t.dtype is not k_pages.dtype:
-            raise TypeError(f"{name} must be {k_pages.dtype} of shape {tuple(k_pages.shape)}, got "
-                            f"{t.dtype} of {tuple(t.shape)}")
-        if n_pages < 2 or t.is_contiguous():
-            strides.append(hkv * page * d)
-        else:
-            strides.append(t.stride(0))
-        if not (t.is_contiguous() or (n_pages > 0 and t[0].is_contiguous())):
-            raise TypeError(f"{name}: each page must be contiguous")
-        if t.get_device() != device:
-            raise TypeError(f"{name} must be on cuda:{device}, got {t.device}")
-    if strides[0] != strides[1]:
-        raise TypeError(f"k_pages and v_pages must have one page stride, got {strides[0]} and {strides[1]}")
-    if page_table.dim() != 2 or page_table.dtype is not i32:
+    if v_pages.shape != shape or v_pages.dtype is not dtype:
+        raise TypeError(f"v_pages must be {dtype} of shape {tuple(shape)}, got {v_pages.dtype} of "
+                        f"{tuple(v_pages.shape)}")
+    n_pages, hkv, page, d = shape
+    if k_pages.is_contiguous() and v_pages.is_contiguous():
+        stride = hkv * page * d
+    else:
+        stride = _page_stride(k_pages, v_pages)
+    if len(page_table.shape) != 2 or page_table.dtype is not i32:
         raise TypeError("page_table must be an int32 [n_seqs, max_pages] tensor")
     n, most = page_table.shape
-    if most > 1 and page_table.stride(1) != 1:
-        raise TypeError("page_table's rows must be contiguous")
-    if page_table.get_device() != device:
-        raise TypeError(f"page_table must be on cuda:{device}, got {page_table.device}")
-    row = page_table.stride(0) if n > 1 else most
-    if row < most:
-        raise TypeError("page_table's rows must not overlap")
-    cache = KvCache(k_pages.data_ptr(), v_pages.data_ptr(), strides[0], n_pages, page, hkv, d,
-                    GpuAttentionEngine._io_of(k_pages))
-    batch = CacheBatch(_address(cu_tokens, "cu_tokens", (n + 1,), i32, device),
+    if page_table.is_contiguous():
+        row = most
+    else:
+        row = page_table.stride(0) if n > 1 else most
+        if most > 1 and page_table.stride(1) != 1:
+            raise TypeError("page_table's rows must be contiguous")
+        if row < most:
+            raise TypeError("page_table's rows must not overlap")
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages"), (page_table, "page_table")):
+        if t.get_device() != device:
+            raise TypeError(f"{name} must be on cuda:{device}, got {t.device}")
+    return (KvCache(k_pages.data_ptr(), v_pages.data_ptr(), stride, n_pages, page, hkv, d,
+                    GpuAttentionEngine._io_of(k_pages)),
+            CacheBatch(_address(cu_tokens, "cu_tokens", (n + 1,), i32, device),
                        _address(kv_lens, "kv_lens", (n,), i32, device), page_table.data_ptr(), row, n,
-                       total_tokens, most, int(max_new), int(max_kv))
-    return cache, batch
+                       total_tokens, most, int(max_new), int(max_kv)))
+
+
+def _page_stride(k_pages, v_pages):
+    """The one stride of pages that are not one contiguous tensor each."""
+    strides = []
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if not t[0].is_contiguous():
+            raise TypeError(f"{name}: each page must be contiguous")
+        strides.append(t.stride(0) if len(t) > 1 else t[0].numel())
+    if strides[0] != strides[1]:
+        raise TypeError(f"k_pages and v_pages must have one page stride, got {strides[0]} and {strides[1]}")
+    return strides[0]
 
 
 class GpuAttentionEngine:
@@ -823,32 +830,29 @@ class GpuAttentionEngine:
     # ---- per-head norms of queries and keys (glacier_norm.h) ---------------
     def _bind_device_stream(self):
         """torch's current stream of this engine's device, whichever device is current."""
-        raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
-        dev = self.device_ordinal
+        raw, dev = getattr(_torch()._C, "_cuda_getCurrentRawStream", None), self.device_ordinal
         stream = _torch_mod.cuda.current_stream(dev).cuda_stream if raw is None else raw(dev)
-        rc = load().glacier_attn_set_stream(self._h, stream)
+        rc = _lib.glacier_attn_set_stream(self._h, stream)
         if rc != OK:
             _check(rc)
 
     def _workspace(self, size):
         """`size` bytes of torch's allocator on the current stream of the engine's
         device (inside a capture: the graph's own memory)."""
-        if size == 0:
-            return None
         return _torch().empty(size, dtype=_torch_mod.uint8, device=self.device_ordinal)
 
     def _qk_args(self, q, k, q_weight, k_weight, eps, rope_freq_base, positions):
-        if q.dim() != 3 or k.dim() != 3:
+        shape, dtype = q.shape, q.dtype
+        if len(shape) != 3 or k.dim() != 3:
             raise TypeError("q must be [T, Hq, D] and k [T, Hkv, D]")
         torch, dev = _torch(), self.device_ordinal
-        T, hq, d = q.shape
-        hkv = k.shape[1]
-        desc = QkNormDesc(T, hq, hkv, d, self._io_of(q), eps, rope_freq_base or 0.0)
-        return desc, (_address(q, "q", (T, hq, d), q.dtype, dev),
-                      _address(k, "k", (T, hkv, d), q.dtype, dev),
-                      _address(q_weight, "q_weight", (d,), torch.float32, dev),
-                      _address(k_weight, "k_weight", (d,), torch.float32, dev),
-                      _optional(positions, "positions", (T,), torch.int32, dev))
+        T, hq, d = shape
+        hkv, f32 = k.shape[1], torch.float32
+        desc = QkNormDesc(T, hq, hkv, d, self._io_of(q), float(eps), float(rope_freq_base or 0.0))
+        return desc, (_address(q, "q", shape, dtype, dev), _address(k, "k", (T, hkv, d), dtype, dev),
+                      _address(q_weight, "q_weight", (d,), f32, dev),
+                      _address(k_weight, "k_weight", (d,), f32, dev),
+                      None if positions is None else _address(positions, "positions", (T,), torch.int32, dev))
 
     def qk_norm_forward(self, q, k, q_weight, k_weight, eps, rope_freq_base=None, positions=None,
                         q_out=None, k_out=None):
@@ -863,7 +867,9 @@ class GpuAttentionEngine:
         outs = (_address(q_out, "q_out", q.shape, q.dtype, dev),
                 _address(k_out, "k_out", k.shape, q.dtype, dev))
         self._bind_device_stream()
-        _check(load().glacier_rmsnorm_qk_forward(self._h, ctypes.byref(desc), *args, *outs))
+        rc = _lib.glacier_rmsnorm_qk_forward(self._h, ctypes.byref(desc), *args, *outs)
+        if rc != OK:
+            _check(rc)
         return q_out, k_out
 
     def qk_norm_backward(self, dq_out, dk_out, q, k, q_weight, k_weight, eps, rope_freq_base=None,
@@ -881,13 +887,15 @@ class GpuAttentionEngine:
         outs = (_address(dq, "dq", q.shape, q.dtype, dev), _address(dk, "dk", k.shape, q.dtype, dev),
                 _optional(dq_weight, "dq_weight", (d,), torch.float32, dev),
                 _optional(dk_weight, "dk_weight", (d,), torch.float32, dev))
-        L, size, work = load(), 0, None
+        L, size, work = _lib, 0, None
         if dq_weight is not None or dk_weight is not None:
             size = L.glacier_rmsnorm_qk_workspace(ctypes.byref(desc))
             work = self._workspace(size)
         self._bind_device_stream()
-        _check(L.glacier_rmsnorm_qk_backward(self._h, ctypes.byref(desc), *grads, *args, *outs,
-                                             self._ptr(work), size))
+        rc = L.glacier_rmsnorm_qk_backward(self._h, ctypes.byref(desc), *grads, *args, *outs,
+                                           self._ptr(work), size)
+        if rc != OK:
+            _check(rc)
         return dq, dk
 
     # ---- paged key/value cache (glacier_cache.h) ---------------------------
@@ -914,8 +922,10 @@ class GpuAttentionEngine:
             qp = _address(q, "q", (T, hq, cache.head_dim), dt, dev)
             rp = _address(q_rot, "q_rot", (T, hq, cache.head_dim), dt, dev)
         self._bind_device_stream()
-        _check(load().glacier_attn_cache_append(self._h, ctypes.byref(cache), ctypes.byref(batch), kp,
-                                                vp, rope_freq_base or 0.0, hq, qp, rp))
+        rc = _lib.glacier_attn_cache_append(self._h, ctypes.byref(cache), ctypes.byref(batch), kp, vp,
+                                            float(rope_freq_base or 0.0), hq, qp, rp)
+        if rc != OK:
+            _check(rc)
         return q_rot if q is not None else None
 
     def cache_forward(self, q, k_pages, v_pages, cu_tokens, kv_lens, page_table, max_new=0, max_kv=0,
@@ -941,11 +951,13 @@ class GpuAttentionEngine:
             lse = torch.empty((hq, T), dtype=torch.float32, device=q.device)
         op = _address(out, "out", shape, dt, dev)
         lp = _optional(lse, "lse", (hq, T), torch.float32, dev)
-        L, cp, bp = load(), ctypes.byref(cache), ctypes.byref(batch)
+        L, cp, bp = _lib, ctypes.byref(cache), ctypes.byref(batch)
         size = L.glacier_attn_cache_workspace(self._h, cp, bp, hq)
-        work = self._workspace(size)
+        work = None if size == 0 else self._workspace(size)
         self._bind_device_stream()
-        _check(L.glacier_attn_cache_forward(self._h, cp, bp, hq, qp, op, lp, self._ptr(work), size))
+        rc = L.glacier_attn_cache_forward(self._h, cp, bp, hq, qp, op, lp, self._ptr(work), size)
+        if rc != OK:
+            _check(rc)
         return out, lse
 
     # ---- LM-head cross-entropy (glacier_lmhead.h) -------------------------
