@@ -235,28 +235,27 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[mb][db][r] *= alpha;
     }
-    // O^T += V^T P^T
+    // O^T += V^T P^T; in bf16 each weight in two terms, which leaves 16 bits of
+    // it: reading V bounds these calls, and one term would add as much error as
+    // the result's own rounding
     if constexpr (sizeof(T) == 2) {
-      bf16x8 pf[MB];
+      bf16x8 hi[MB], lo[MB];
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          pf[mb][r] = (bf16)st[mb][0][r];
-          pf[mb][4 + r] = (bf16)st[mb][NS - 1][r];
+        for (int e = 0; e < 8; ++e) {
+          const float p = st[mb][e < 4 ? 0 : NS - 1][e % 4];
+          hi[mb][e] = (bf16)p;
+          lo[mb][e] = (bf16)(p - (float)hi[mb][e]);
         }
 #pragma unroll
       for (int db = 0; db < DP / 16; ++db) {
-        const bf16x4 lo = read_tr<L::S>(vt, 0, 16 * db, lane);
-        const bf16x4 hi = read_tr<L::S>(vt, 16, 16 * db, lane);
-        bf16x8 vf;
+        const bf16x8 vf = join8(read_tr<L::S>(vt, 0, 16 * db, lane), read_tr<L::S>(vt, 16, 16 * db, lane));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          vf[r] = lo[r];
-          vf[4 + r] = hi[r];
+        for (int mb = 0; mb < MB; ++mb) {
+          acc[mb][db] = M::mma(vf, lo[mb], acc[mb][db]);
+          acc[mb][db] = M::mma(vf, hi[mb], acc[mb][db]);
         }
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) acc[mb][db] = M::mma(vf, pf[mb], acc[mb][db]);
       }
     } else {
       // V in wide reads: row i of the four blocks 4 x .. 4 x + 3 is column
