@@ -472,9 +472,11 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   // up to 4 over up to 2048 (17e6) 13.7, 18.3; 16 tokens over 8192 (29e6) 28.7,
   // 20.2; 32 sequences of up to 8 over up to 2048 (134e6) 46, 30; 14/2 heads of
   // 64, 8 sequences of up to 16 over up to 2048 (15e6) 12.9, 14.4; of up to 32
-  // (29e6) 18.4, 16.6.
-  const bool wide = c.io_bf16 && c.D <= 128 && longest * group > 16 &&
-                    (double)tiles_of(16) * c.hkv * keys * c.D > 25e6;
+  // (29e6) 18.4, 16.6.  Above 128 columns one workgroup of wide tiles fills a CU:
+  // 8/2 heads of 256, 8 sequences of up to 32 over up to 2048 (67e6) 30.7, 36.8;
+  // 512 tokens over 2048 (134e6) 40.4, 41.7; 1024 over 8192 (1e9) 260, 121.
+  const bool wide = c.io_bf16 && longest * group > 16 &&
+                    (double)tiles_of(16) * c.hkv * keys * c.D > (c.D <= 128 ? 25e6 : 100e6);
   p.rows = wide ? kCacheWideRows : 16;
   const long groups = tiles_of(p.rows) * c.hkv;
   // Splits of 512 keys or more, as many as fill the workgroups the CUs hold at
@@ -495,7 +497,7 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   // 57, 52, 67; 512 over 512 19, 22; 2048 over 8192 (448) 232, 248, 260, 299;
   // 16 chunks of up to 128 over up to 2048 (320) 55, 69; 8 of up to 256 over up
   // to 4096 (320) 98, 87, 98, 119.
-  const long per_cu = wide ? 2 : !c.io_bf16 ? 1 : c.D <= 64 ? 4 : c.D <= 128 ? 2 : 1;
+  const long per_cu = wide ? (c.D <= 128 ? 2 : 1) : !c.io_bf16 ? 1 : c.D <= 64 ? 4 : c.D <= 128 ? 2 : 1;
   // (rounded up from the half where chunks differ and the estimate is high)
   const long want = (per_cu * n_cu + (wide && c.n_seqs > 1 ? groups / 2 : 0)) / groups;
   const long least = !wide ? 512 : groups < 64 ? 256 : groups < 256 ? 512 : 2048;

@@ -1,23 +1,37 @@
 // cache_attn_wide.hip -- attention of chunks of new tokens over the paged
-// cache on 32x32x16 MFMAs: bf16, head sizes up to 128, many rows.
+// cache on 32x32x16 MFMAs (bf16).
 //
 // A workgroup takes 128 rows (token, head of the group) of one KV head, 32 a
-// wave, and walks the keys 64 at a time; two workgroups share a CU, so one's
-// softmax runs beside the other's products.  K and V tiles come page by page
-// through registers into two LDS buffers, the next tile's loads in flight
-// during a tile's products, with one barrier a tile.  Rows of 16-byte pieces
-// are swizzled (lds_sw, lds_mfma.hpp), which keeps both reads free of bank
-// conflicts.
+// wave, and walks the keys 64 at a time; up to 128 columns two workgroups share
+// a CU.  K and V tiles come page by page by LDS DMA, two slots each, one barrier
+// a tile: while a tile's weights meet V, its successor's scores are formed from
+// the K tile that came a step earlier, so matrix and vector instructions of one
+// wave have no order between them.  Rows of 16-byte pieces are swizzled (lds_sw,
+// lds_mfma.hpp), which keeps both reads free of bank conflicts.
 //
 // Scores are formed transposed: S^T = K Q^T leaves a lane with 16 keys of one
 // row in each accumulator block, and elements 8 s .. 8 s + 7 are the k-slots of
 // step s of O^T += V^T P^T, whose V operand comes from two transposing LDS
-// reads (the accumulator layout is described in attn_bwd3.hip).
+// reads (the accumulator layout is described in attn_bwd3.hip).  Each weight is
+// rounded to bf16 (a second term, as in the 16-row kernel, would cost a quarter
+// of the products here); the sum takes them unrounded.
 //
 // The running maximum is only followed where it has grown by more than 8 (in
 // log2): until then weights are taken against the old one, at most 2^8 large,
 // and the sums need no rescaling.  The result is the same: any reference value
 // cancels in out and lse.
+//
+// KV heads alternate over the workgroups, so that an XCD's L2 serves few of
+// them, and long tiles start first.
+//
+// Measured: 2048 tokens over 8192 keys, 28/4 heads of 128: 221-231 us (950-910
+// TFLOP/s; a library product of 8192^3 reaches 1205 on the card).  MFMAs are
+// busy 54% of the time of a CU with two workgroups, vector instructions nearly
+// all of the rest; tiles of 448 workgroups on 256 CUs leave an eighth of them
+// idle.  Tried and slower: tiles through registers (278 us), 256 rows on eight
+// waves (295), equal shares of all tiles' steps for every workgroup with
+// fragments joined afterwards (278: the workgroups lose each other's L2 lines),
+// scheduling hints of the compiler (235-281).
 #include "cache_tiles.hpp"
 
 namespace glacier {
@@ -127,7 +141,7 @@ __device__ __forceinline__ void wide_step(WideState<DP>& w, f32x16 (&st)[2], f32
 }
 
 template <int DP>
-__global__ __launch_bounds__(64 * kWavesWide, 2) void cache_attn_wide_kernel(CacheAttn a) {
+__global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn_wide_kernel(CacheAttn a) {
   using W = Wide<DP>;
   extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
@@ -322,7 +336,7 @@ __global__ __launch_bounds__(256) void cache_join_tiles_kernel(CacheAttn a) {
   if (tile < 0 || r0 >= n_rows) return;
   const TileKeys tk = tile_keys(a, s, tile);
   if (tk.active <= 1) return;
-  const int lanes = c.D <= 64 ? 16 : 32, d = 4 * (threadIdx.x % lanes);
+  const int lanes = c.D <= 64 ? 16 : c.D <= 128 ? 32 : 64, d = 4 * (threadIdx.x % lanes);
   const long step = (long)c.T * a.hq;
   for (int r = r0 + threadIdx.x / lanes; r < min(n_rows, r0 + kJoinRows); r += 256 / lanes) {
     const int tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
@@ -377,7 +391,7 @@ hipError_t attend(const CacheAttn& a, hipStream_t st) {
 
 hipError_t launch_cache_attn_wide(const CacheAttn& a, hipStream_t st) {
   static_assert(kRowsWide == kCacheWideRows, "rows of a wide tile");
-  GL_CHECK(a.c.D <= 64 ? attend<64>(a, st) : attend<128>(a, st));
+  GL_CHECK(a.c.D <= 64 ? attend<64>(a, st) : a.c.D <= 128 ? attend<128>(a, st) : attend<256>(a, st));
   if (a.n_splits == 1 || a.n_splits > kCacheTileJoin) return hipSuccess;
   hipLaunchKernelGGL(cache_join_tiles_kernel, dim3(tile_numbers(a) * a.c.hkv, kRowsWide / kJoinRows),
                      dim3(256), 0, st, a);

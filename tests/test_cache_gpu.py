@@ -80,6 +80,9 @@ CHUNKS = {  # more than 16 rows a KV head: 128-row tiles where the table is wide
     "d128_one_head_groups": ([(128, 128), (129, 130), (127, 1000)], 4, 4, 128, 16, 7),
     "d128_group_of_40": ([(9, 3000), (5, 5)], 40, 1, 128, 128, 0),
     "d128_many": ([(3 + i, 40 + 13 * i) for i in range(70)], 16, 2, 128, 16, 2),
+    "d256": ([(60, 61), (129, 700), (1, 90)], 8, 2, 256, 16, 3),
+    "d136": ([(50, 900)], 6, 3, 136, 32, 0),
+    "d248_group_of_16": ([(17, 400), (40, 41)], 16, 1, 248, 64, 0),
     "d120_long": ([(20, 6000)], 10, 2, 120, 512, 0),
 }
 
