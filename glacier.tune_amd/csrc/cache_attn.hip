@@ -43,7 +43,8 @@ struct CaLayout {
   static constexpr int OS = DP + 4;  // row stride (floats) of a wave's sums in the join
   static constexpr int WAVE = 16 * MB * (OS + 2);  // sums, maxima, totals
   static constexpr int JOIN = WAVES * WAVE * 4;
-  static constexpr int BYTES = TILES > JOIN ? TILES : JOIN;
+  static constexpr int NOTES = TILES > JOIN ? TILES : JOIN;  // then the noted blocks of each wave
+  static constexpr int BYTES = NOTES + WAVES * kNotedBlocks / 8;
   static_assert(BYTES <= 160 * 1024, "exceeds the LDS of a CU");
 };
 
@@ -134,13 +135,6 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
 
   f32x4 acc[MB][DP / 16];
   float m[MB], l[MB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    m[mb] = kNegBig;
-    l[mb] = 0.0f;
-#pragma unroll
-    for (int db = 0; db < DP / 16; ++db) acc[mb][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
 
   T* const kt = reinterpret_cast<T*>(smem) + w * 2 * KB * L::S;
   T* const vt = kt + KB * L::S;
@@ -165,119 +159,193 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
     vr.load(vb, rows, rowb, off);
   };
   const int first_limit = s.pos0 + r0 / a.group;  // the tile's first row sees keys up to here
-  int j = k0 + w * KB;
-  if (j < k1) fetch(j);
-  for (; j < k1; j += WAVES * KB) {
-    wave_lds_fence();
-    kr.store(kt, lane);
-    vr.store(vt, lane);
-    wave_lds_fence();
-    int here[NS];
-    bool whole = j + KB - 1 <= first_limit;
-#pragma unroll
-    for (int p = 0; p < NS; ++p) {
-      here[p] = rows[p];
-      whole = whole && rows[p] == 16;
-    }
-    if (j + WAVES * KB < k1) fetch(j + WAVES * KB);
-    // S^T: keys 16 p + 4 g + r of this block, row col of each 16-row block
-    f32x4 st[MB][NS];
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-      for (int p = 0; p < NS; ++p) st[mb][p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int p = 0; p < NS; ++p)
-#pragma unroll
-      for (int x = 0; x < NW; ++x) {
-        const i32x4 kw = *reinterpret_cast<const i32x4*>(kt + (16 * p + col) * L::S + first_col(x));
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          if constexpr (sizeof(T) == 2) {
-            st[mb][p] = M::mma(__builtin_bit_cast(bf16x8, kw), __builtin_bit_cast(bf16x8, qw[mb][x]), st[mb][p]);
-          } else {
-            const f32x4 kf = __builtin_bit_cast(f32x4, kw), qf = __builtin_bit_cast(f32x4, qw[mb][x]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) st[mb][p] = M::mma(kf[e], qf[e], st[mb][p]);
-          }
-        }
-      }
+  unsigned* const notes = reinterpret_cast<unsigned*>(smem + L::NOTES) + w * (kNotedBlocks / 32);
+  auto note_of = [&](int j) { return (j - k0) / (WAVES * KB) % kNotedBlocks; };
+  auto walk = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
-      float top = kNegBig;
+      m[mb] = kNegBig;
+      l[mb] = 0.0f;
 #pragma unroll
-      for (int p = 0; p < NS; ++p)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = st[mb][p][r] * a.scale_log2;
-          if (!whole) {
-            const int at = 4 * g + r;
-            x = at < here[p] && j + 16 * p + at <= limit[mb] ? x : -INFINITY;
-          }
-          st[mb][p][r] = x;
-          top = fmaxf(top, x);
-        }
-      const float mn = fmaxf(m[mb], col_max_swap(top));
-      const float alpha = weight(m[mb] - mn);
-      m[mb] = mn;
-      float sum = 0.0f;
-#pragma unroll
-      for (int p = 0; p < NS; ++p)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float e = weight(st[mb][p][r] - mn);
-          st[mb][p][r] = e;
-          sum += e;
-        }
-      l[mb] = l[mb] * alpha + sum;
-#pragma unroll
-      for (int db = 0; db < DP / 16; ++db)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[mb][db][r] *= alpha;
+      for (int db = 0; db < DP / 16; ++db) acc[mb][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // O^T += V^T P^T; in bf16 each weight in two terms, which leaves 16 bits of
-    // it: reading V bounds these calls, and one term would add as much error as
-    // the result's own rounding
-    if constexpr (sizeof(T) == 2) {
-      bf16x8 hi[MB], lo[MB];
+    int j = k0 + w * KB;
+    if (j < k1) fetch(j);
+    for (; j < k1; j += WAVES * KB) {
+      int here[NS];
+      bool whole = j + KB - 1 <= first_limit;
+#pragma unroll
+      for (int p = 0; p < NS; ++p) {
+        here[p] = rows[p];
+        whole = whole && rows[p] == 16;
+      }
+      if constexpr (careful()) {
+        unsigned found = 0;
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) found |= clear_not_finite<T>(vr.w[i]);
+        if (__any(found != 0) && lane == 0) notes[note_of(j) / 32] |= 1u << note_of(j) % 32;
+      }
+      wave_lds_fence();
+      kr.store(kt, lane);
+      vr.store(vt, lane);
+      wave_lds_fence();
+      if (j + WAVES * KB < k1) fetch(j + WAVES * KB);
+      // S^T: keys 16 p + 4 g + r of this block, row col of each 16-row block
+      f32x4 st[MB][NS];
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = st[mb][e < 4 ? 0 : NS - 1][e % 4];
-          hi[mb][e] = (bf16)p;
-          lo[mb][e] = (bf16)(p - (float)hi[mb][e]);
-        }
+        for (int p = 0; p < NS; ++p) st[mb][p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int db = 0; db < DP / 16; ++db) {
-        const bf16x8 vf = join8(read_tr<L::S>(vt, 0, 16 * db, lane), read_tr<L::S>(vt, 16, 16 * db, lane));
+      for (int p = 0; p < NS; ++p)
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          acc[mb][db] = M::mma(vf, lo[mb], acc[mb][db]);
-          acc[mb][db] = M::mma(vf, hi[mb], acc[mb][db]);
-        }
-      }
-    } else {
-      // V in wide reads: row i of the four blocks 4 x .. 4 x + 3 is column
-      // 64 x + 4 i + their number, and of a last pair 64 x + 2 i + its number
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float* const vrow = vt + (4 * g + r) * L::S;
-#pragma unroll
-        for (int x = 0; x < DP / 64; ++x) {
-          const f32x4 vf = *reinterpret_cast<const f32x4*>(vrow + 64 * x + 4 * col);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
-              acc[mb][4 * x + e] = M::mma(vf[e], st[mb][0][r], acc[mb][4 * x + e]);
-        }
-        if constexpr (DP % 64 != 0) {
-          const float2 vf = *reinterpret_cast<const float2*>(vrow + DP / 64 * 64 + 2 * col);
+        for (int x = 0; x < NW; ++x) {
+          const i32x4 kw = *reinterpret_cast<const i32x4*>(kt + (16 * p + col) * L::S + first_col(x));
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) {
-            acc[mb][DP / 16 - 2] = M::mma(vf.x, st[mb][0][r], acc[mb][DP / 16 - 2]);
-            acc[mb][DP / 16 - 1] = M::mma(vf.y, st[mb][0][r], acc[mb][DP / 16 - 1]);
+            if constexpr (sizeof(T) == 2) {
+              st[mb][p] = M::mma(__builtin_bit_cast(bf16x8, kw), __builtin_bit_cast(bf16x8, qw[mb][x]), st[mb][p]);
+            } else {
+              const f32x4 kf = __builtin_bit_cast(f32x4, kw), qf = __builtin_bit_cast(f32x4, qw[mb][x]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) st[mb][p] = M::mma(kf[e], qf[e], st[mb][p]);
+            }
+          }
+        }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        float top = kNegBig;
+#pragma unroll
+        for (int p = 0; p < NS; ++p)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float x = st[mb][p][r] * a.scale_log2;
+            if (!whole) {
+              const int at = 4 * g + r;
+              x = at < here[p] && j + 16 * p + at <= limit[mb] ? x : -INFINITY;
+            }
+            st[mb][p][r] = x;
+            top = fmaxf(top, x);
+          }
+        const float mn = fmaxf(m[mb], col_max_swap(top));
+        const float alpha = weight(m[mb] - mn);
+        m[mb] = mn;
+        float sum = 0.0f;
+#pragma unroll
+        for (int p = 0; p < NS; ++p)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float e = weight(st[mb][p][r] - mn);
+            st[mb][p][r] = e;
+            sum += e;
+          }
+        l[mb] = l[mb] * alpha + sum;
+#pragma unroll
+        for (int db = 0; db < DP / 16; ++db)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[mb][db][r] *= alpha;
+      }
+      // O^T += V^T P^T; in bf16 each weight in two terms, which leaves 16 bits of
+      // it: reading V bounds these calls, and one term would add as much error as
+      // the result's own rounding
+      if constexpr (sizeof(T) == 2) {
+        bf16x8 hi[MB], lo[MB];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float p = st[mb][e < 4 ? 0 : NS - 1][e % 4];
+            hi[mb][e] = (bf16)p;
+            lo[mb][e] = (bf16)(p - (float)hi[mb][e]);
+          }
+#pragma unroll
+        for (int db = 0; db < DP / 16; ++db) {
+          const bf16x8 vf = join8(read_tr<L::S>(vt, 0, 16 * db, lane), read_tr<L::S>(vt, 16, 16 * db, lane));
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) {
+            acc[mb][db] = M::mma(vf, lo[mb], acc[mb][db]);
+            acc[mb][db] = M::mma(vf, hi[mb], acc[mb][db]);
+          }
+        }
+      } else {
+        // V in wide reads: row i of the four blocks 4 x .. 4 x + 3 is column
+        // 64 x + 4 i + their number, and of a last pair 64 x + 2 i + its number
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float* const vrow = vt + (4 * g + r) * L::S;
+#pragma unroll
+          for (int x = 0; x < DP / 64; ++x) {
+            const f32x4 vf = *reinterpret_cast<const f32x4*>(vrow + 64 * x + 4 * col);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int mb = 0; mb < MB; ++mb)
+                acc[mb][4 * x + e] = M::mma(vf[e], st[mb][0][r], acc[mb][4 * x + e]);
+          }
+          if constexpr (DP % 64 != 0) {
+            const float2 vf = *reinterpret_cast<const float2*>(vrow + DP / 64 * 64 + 2 * col);
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+              acc[mb][DP / 16 - 2] = M::mma(vf.x, st[mb][0][r], acc[mb][DP / 16 - 2]);
+              acc[mb][DP / 16 - 1] = M::mma(vf.y, st[mb][0][r], acc[mb][DP / 16 - 1]);
+            }
+          }
+        }
+      }
+    }
+  };
+  walk(std::false_type{});
+  unsigned odd = 0;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int db = 0; db < DP / 16; ++db)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) odd |= limit[mb] >= 0 ? not_finite(acc[mb][db][r]) : 0;
+  if (__any(odd != 0)) {
+    if (lane < kNotedBlocks / 32) notes[lane] = 0;
+    wave_lds_fence();
+    walk(std::true_type{});
+    wave_lds_fence();
+    for (int j = k0 + w * KB; j < k1; j += WAVES * KB) {
+      if (!(notes[note_of(j) / 32] >> note_of(j) % 32 & 1)) continue;
+      for (int key = j; key < min(k1, j + KB); ++key) {
+        const int page = cache_page(c, b, key);
+        if (page < 0) continue;
+        const char* const v = static_cast<const char*>(c.v_pages) + page * strideb + head +
+                              (key & ((1 << c.page_shift) - 1)) * rowb;
+        unsigned sees[MB];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) sees[mb] = key <= limit[mb] ? ~0u : 0u;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int db = 0; db < DP / 16; ++db) {
+            const bf16x4 x = __builtin_bit_cast(bf16x4, load8_within(v, rowb, 2 * (16 * db + 4 * g)));
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int mb = 0; mb < MB; ++mb) acc[mb][db][r] += given_back((float)x[r], sees[mb]);
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int x = 0; x < DP / 64; ++x) {
+              const f32x4 f = __builtin_bit_cast(f32x4, load_within(v, rowb, 4 * (64 * x + 16 * g + 4 * r)));
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb) acc[mb][4 * x + e][r] += given_back(f[e], sees[mb]);
+            }
+            if constexpr (DP % 64 != 0) {
+              const float2 f =
+                  __builtin_bit_cast(float2, load8_within(v, rowb, 4 * (DP / 64 * 64 + 8 * g + 2 * r)));
+#pragma unroll
+              for (int mb = 0; mb < MB; ++mb) {
+                acc[mb][DP / 16 - 2][r] += given_back(f.x, sees[mb]);
+                acc[mb][DP / 16 - 1][r] += given_back(f.y, sees[mb]);
+              }
+            }
           }
         }
       }

@@ -47,7 +47,8 @@ struct Wide {
   static constexpr int RB = 2 * DP;   // bytes of an LDS row
   static constexpr int PPR = DP / 8;  // 16-byte pieces of a row
   static constexpr int TILE = kKeysWide * RB;
-  static constexpr int BYTES = 4 * TILE;  // K and V, two slots each
+  static constexpr int NOTES = 4 * TILE;  // after K and V, two slots each: the noted tiles
+  static constexpr int BYTES = NOTES + kNotedBlocks / 8;
   static constexpr int NKK = DP / 16, NDB = DP / 32;
   static constexpr int ND = 16 * RB / 1024;  // DMA instructions of a page piece
 };
@@ -229,8 +230,22 @@ __global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn
     for (int n = 0; n < W::ND; ++n)
       dma16(static_cast<const char*>(pages) + off, bytes, doff[n], to + w * 16 * W::RB + 1024 * n);
   };
-  unsigned char* const ks[2] = {smem, smem + W::TILE};
-  unsigned char* const vs[2] = {smem + 2 * W::TILE, smem + 3 * W::TILE};
+  auto k_slot = [&](int i) { return smem + i * W::TILE; };
+  auto v_slot = [&](int i) { return smem + (2 + i) * W::TILE; };
+  unsigned* const notes = reinterpret_cast<unsigned*>(smem + W::NOTES);
+  // (second walk) clears what is not finite in this wave's piece of V
+  auto look_through = [&](unsigned char* v, int j) {
+    unsigned found = 0;
+#pragma unroll
+    for (int n = 0; n < W::ND; ++n) {
+      i32x4* const at = reinterpret_cast<i32x4*>(v + w * 16 * W::RB + 1024 * n + 16 * lane);
+      i32x4 x = *at;
+      found |= clear_not_finite<bf16>(x);
+      *at = x;
+    }
+    const int block = (j - k0) / kKeysWide % kNotedBlocks;
+    if (__any(found != 0) && lane == 0) atomicOr(&notes[block / 32], 1u << block % 32);
+  };
   // whether every piece of the keys has a page (if not, each tile is looked at)
   bool clean = true;
   for (int p = (k0 >> c.page_shift) + lane; p <= (k1 - 1) >> c.page_shift; p += 64)
@@ -238,32 +253,11 @@ __global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn
   clean = __all(clean);
 
   WideState<DP> ws;
-#pragma unroll
-  for (int db = 0; db < W::NDB; ++db)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) ws.o[db][e] = 0.0f;
-  ws.m = kNegBig;
-  ws.l = 0.0f;
-  ws.top = kNegBig;
   f32x16 sa[2], sb[2];
   int v_page = -1, k_page = -1;  // of the next V tile and of the K tile after it
-  if (k0 < k1) {
-    const int first = look_up(k0);
-    v_page = look_up(k0 + kKeysWide);
-    k_page = look_up(k0 + 2 * kKeysWide);
-    bring(c.k_pages, ks[0], k0, first);
-    bring(c.v_pages, vs[0], k0, first);
-    bring(c.k_pages, ks[1], k0 + kKeysWide, v_page);
-    vmw<0>();
-    wg_barrier();
-    wide_scores<DP>(sa, ks[0], koff, qf);
-    ws.top = wide_largest(sa);
-    lgkm<0>();
-    wg_barrier();
-  }
-  auto tile_step = [&](f32x16 (&st)[2], f32x16 (&sn)[2], int j, int odd) {
-    bring(c.k_pages, ks[odd], j + 2 * kKeysWide, k_page);
-    bring(c.v_pages, vs[odd ^ 1], j + kKeysWide, v_page);
+  auto tile_step = [&](f32x16 (&st)[2], f32x16 (&sn)[2], int j, int odd, auto careful) __attribute__((always_inline)) {
+    bring(c.k_pages, k_slot(odd), j + 2 * kKeysWide, k_page);
+    bring(c.v_pages, v_slot(odd ^ 1), j + kKeysWide, v_page);
     v_page = k_page;
     k_page = look_up(j + 3 * kKeysWide);
     __builtin_amdgcn_sched_barrier(0);
@@ -280,15 +274,71 @@ __global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn
           }
         ws.top = wide_largest(st);
       }
-      wide_step<DP>(ws, st, sn, ks[odd ^ 1], vs[odd], koff, voff, qf, a.scale_log2);
+      wide_step<DP>(ws, st, sn, k_slot(odd ^ 1), v_slot(odd), koff, voff, qf, a.scale_log2);
     }
     vmw<0>();
+    if constexpr (careful()) look_through(v_slot(odd ^ 1), j + kKeysWide);
     lgkm<0>();
     wg_barrier();
   };
-  for (int j = k0; j < k1; j += 2 * kKeysWide) {
-    tile_step(sa, sb, j, 0);
-    if (j + kKeysWide < k1) tile_step(sb, sa, j + kKeysWide, 1);
+  auto walk = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+    for (int db = 0; db < W::NDB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ws.o[db][e] = 0.0f;
+    ws.m = kNegBig;
+    ws.l = 0.0f;
+    ws.top = kNegBig;
+    if (k0 < k1) {
+      const int first = look_up(k0);
+      v_page = look_up(k0 + kKeysWide);
+      k_page = look_up(k0 + 2 * kKeysWide);
+      bring(c.k_pages, k_slot(0), k0, first);
+      bring(c.v_pages, v_slot(0), k0, first);
+      bring(c.k_pages, k_slot(1), k0 + kKeysWide, v_page);
+      vmw<0>();
+      if constexpr (careful()) look_through(v_slot(0), k0);
+      lgkm<0>();
+      wg_barrier();
+      wide_scores<DP>(sa, k_slot(0), koff, qf);
+      ws.top = wide_largest(sa);
+      lgkm<0>();
+      wg_barrier();
+    }
+    for (int j = k0; j < k1; j += 2 * kKeysWide) {
+      tile_step(sa, sb, j, 0, careful);
+      if (j + kKeysWide < k1) tile_step(sb, sa, j + kKeysWide, 1, careful);
+    }
+  };
+  walk(std::false_type{});
+  unsigned odd = 0;
+#pragma unroll
+  for (int db = 0; db < W::NDB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) odd |= not_finite(ws.o[db][e]);
+  if (__syncthreads_or(odd != 0 && live)) {
+    if (threadIdx.x < kNotedBlocks / 32) notes[threadIdx.x] = 0;
+    __syncthreads();
+    walk(std::true_type{});
+    __syncthreads();
+    for (int j = k0; j < k1; j += kKeysWide) {
+      const int block = (j - k0) / kKeysWide % kNotedBlocks;
+      if (!(notes[block / 32] >> block % 32 & 1)) continue;
+      for (int key = j; key < min(k1, j + kKeysWide); ++key) {
+        const int page = cache_page(c, b, key);
+        if (page < 0) continue;
+        const char* const v = static_cast<const char*>(c.v_pages) + page * strideb + head + (key & in_page) * rowb;
+        const unsigned sees = key <= limit ? ~0u : 0u;
+#pragma unroll
+        for (int db = 0; db < W::NDB; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const bf16x4 x = __builtin_bit_cast(bf16x4, load8_within(v, rowb, 2 * (32 * db + 8 * q + 4 * h)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ws.o[db][4 * q + e] += given_back((float)x[e], sees);
+          }
+      }
+    }
   }
   f32x16 (&o)[W::NDB] = ws.o;
   const float m = ws.m;

@@ -44,9 +44,54 @@ __device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int 
   return k;
 }
 
+// A masked weight is zero, but zero times an infinity or a NaN is not.  The
+// kernels find out at the end: where a sum is not finite they walk the keys once
+// more, clear what is not finite in V before the products, note which key blocks
+// had any, and give those values to the rows that see their keys afterwards.
+constexpr int kNotedBlocks = 1024;  // blocks share a note past so many
+// All ones where an element of the word (one fp32 or two bf16) is not finite: an
+// exponent of all ones carries into the sign's place when one is added.  (No
+// comparisons: their results would crowd the scalar registers of the main loop.)
+template <typename T>
+__device__ inline unsigned not_finite_mask(unsigned u) {
+  if constexpr (sizeof(T) == 2)
+    return ((((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu;
+  else
+    return static_cast<unsigned>(static_cast<int>((u & 0x7f800000u) + 0x00800000u) >> 31);
+}
+// Clears the elements of a 16-byte word that are not finite; their places.
+template <typename T>
+__device__ inline unsigned clear_not_finite(i32x4& w) {
+  unsigned found = 0;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const unsigned m = not_finite_mask<T>(static_cast<unsigned>(w[x]));
+    w[x] &= static_cast<int>(~m);
+    found |= m;
+  }
+  return found;
+}
+// x if it is not finite and the lane's row sees its key (all ones), else zero
+__device__ inline float given_back(float x, unsigned sees) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  return __builtin_bit_cast(float, u & not_finite_mask<float>(u) & sees);
+}
+// Accumulates whether any of the values is not finite (nonzero then).
+__device__ inline unsigned not_finite(float x) { return not_finite_mask<float>(__builtin_bit_cast(unsigned, x)); }
+
 // exp2 of the weights: the instruction itself, whose results below 2^-126 are
 // zero (exp2f spends four more instructions to keep them).
 __device__ inline float weight(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 8 bytes at `off` of the wave's [base, base + bytes); zeros past its end.
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+__device__ inline i32x2 load8_within(const void* base, int bytes, int off) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_raw_buffer_load_b64(wave_rsrc(base, bytes), off, 0, 0);
+#else
+  return i32x2{0, 0};
+#endif
+}
 
 // 16 bytes at `off` of the wave's [base, base + bytes); zeros past its end.
 __device__ inline i32x4 load_within(const void* base, int bytes, int off) {

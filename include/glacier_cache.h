@@ -40,9 +40,10 @@
  * (glacier_attn_forward forms its angles in fp32 as the reference does, which
  * puts them off by up to pos * 2^-23 at far positions.)
  *
- * bf16 tensors: bf16 operands, fp32 sums and softmax; each weight is rounded
- * to bf16 before it multiplies V.  fp32 tensors: fp32 throughout.  Results are
- * bitwise repeatable.  Contexts, status codes and dtypes are those of
+ * bf16 tensors: bf16 operands, fp32 sums and softmax; weights multiply V as two
+ * bf16 terms (one in large chunks).  fp32 tensors: fp32 throughout.  Results are
+ * bitwise repeatable for one layout of the work (below: max_new, max_kv).  NaN
+ * and infinities in a token's K or V reach only the rows that see the token.  Contexts, status codes and dtypes are those of
  * glacier_attn.h; calls enqueue on the context's stream.  Tensors are 16-byte
  * aligned, q, k, v and out contiguous; head_dim is a multiple of 8 up to 256.
  */

@@ -160,6 +160,41 @@ def test_bad_pages_hold_no_keys(eng, dt, columns):
     assert changed == {(int(p.table[1, 3]), 15)}
 
 
+@pytest.mark.parametrize("columns", [0, WIDE // 16])
+@pytest.mark.parametrize("hq,d", [(8, 64), (16, 128), (4, 96), (6, 256)])
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_not_finite_keys_reach_only_rows_that_see_them(eng, dt, hq, d, columns):
+    # NaN and infinities in K and V of late tokens of a chunk: rows before them are
+    # those of the same chunk without them, rows from them on are not finite
+    seqs, bad = [(90, 130), (20, 20), (1, 70)], {0: (100, 117), 1: (9, 9)}
+    p = ch.Paged(seqs, hq, 2, d, 16, DTYPES[dt], 16, columns=columns)
+    ref = ch.attend_ref(p)
+    for what in (math.nan, math.inf, -math.inf):
+        for side in (0, 1):
+            both = p.both.clone()
+            for b, (first, last) in bad.items():
+                for pos in (first, last):
+                    both[p.table[b, pos // 16], side, :, pos % 16, 3::7] = what
+            arrays = (both[:, 0], both[:, 1], p.cu, p.kv_lens, p.table)
+            out, lse = eng.cache_forward(p.q.cuda(), *arrays, save=True)
+            clean = torch.ones(p.tokens, dtype=torch.bool)
+            clean[100 - 40:90] = False  # positions 100 .. 129 of the first sequence
+            clean[90 + 9:90 + 20] = False
+            ch.check("out", out[clean.cuda()], ref[0][clean], ref[1][clean])
+            ch.check("lse", lse[:, clean.cuda()], ref[2][:, clean], ref[3][:, clean])
+            rest = out[~clean.cuda()].float().cpu()
+            if side == 1:  # V: its columns, in every row that sees it
+                assert not torch.isfinite(rest[..., 3::7]).any()
+                others = torch.ones(d, dtype=torch.bool)
+                others[3::7] = False
+                want, bound = ref[0].clone(), ref[1]
+                ch.check("out", rest[..., others], want[~clean][..., others], bound[~clean][..., others])
+                if what != what or what > 0:
+                    assert (rest[..., 3::7] == what).all() or what != what
+            elif what != what:
+                assert rest.isnan().all()
+
+
 def test_lengths_past_the_table(eng):
     # positions the table has no column for hold no key
     p = ch.Paged([(1, 64)], 4, 1, 64, 16, torch.bfloat16, 9)
