@@ -143,20 +143,33 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   const int rowb = D * static_cast<int>(sizeof(T));
   const int off = lane % R::LPR * R::CE < D ? lane / R::LPR * rowb + lane % R::LPR * 16 : 1 << 20;
   const long head = ((long)kvh << c.page_shift) * rowb, strideb = c.page_stride * sizeof(T);
+  // The pages of a block are looked up a block before its rows are requested, by
+  // scalar loads (a vector load would wait for the rows in flight).
+  const auto* const table = (const __attribute__((address_space(4))) int32_t*)(
+      reinterpret_cast<uintptr_t>(c.table + (long)b * c.table_stride));
+  int page[NS];  // of the block to be fetched next
+  auto look_up = [&](int j) {
+#pragma unroll
+    for (int p = 0; p < NS; ++p) {
+      const int key = j + 16 * p;
+      const int at = table[min(key >> c.page_shift, c.max_pages - 1)];
+      page[p] = key < k1 && static_cast<unsigned>(at) < static_cast<unsigned>(c.n_pages) ? at : -1;
+    }
+  };
   int rows[NS];  // keys of the fetched block's pieces
   auto fetch = [&](int j) {
     const char *kb[NS], *vb[NS];
 #pragma unroll
     for (int p = 0; p < NS; ++p) {
       const int key = j + 16 * p;
-      const int page = key < k1 ? __builtin_amdgcn_readfirstlane(cache_page(c, b, key)) : -1;
-      rows[p] = page < 0 ? 0 : min(16, k1 - key);
-      const long at = (page < 0 ? 0 : page) * strideb + head + (key & ((1 << c.page_shift) - 1)) * rowb;
+      rows[p] = page[p] < 0 ? 0 : min(16, k1 - key);
+      const long at = (page[p] < 0 ? 0 : page[p]) * strideb + head + (key & ((1 << c.page_shift) - 1)) * rowb;
       kb[p] = static_cast<const char*>(c.k_pages) + at;
       vb[p] = static_cast<const char*>(c.v_pages) + at;
     }
     kr.load(kb, rows, rowb, off);
     vr.load(vb, rows, rowb, off);
+    look_up(j + WAVES * KB);
   };
   const int first_limit = s.pos0 + r0 / a.group;  // the tile's first row sees keys up to here
   unsigned* const notes = reinterpret_cast<unsigned*>(smem + L::NOTES) + w * (kNotedBlocks / 32);
@@ -170,7 +183,10 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
       for (int db = 0; db < DP / 16; ++db) acc[mb][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     int j = k0 + w * KB;
-    if (j < k1) fetch(j);
+    if (j < k1) {
+      look_up(j);
+      fetch(j);
+    }
     for (; j < k1; j += WAVES * KB) {
       int here[NS];
       bool whole = j + KB - 1 <= first_limit;
