@@ -274,13 +274,19 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
             hi[mb][e] = (bf16)p;
             lo[mb][e] = (bf16)(p - (float)hi[mb][e]);
           }
+        // (two blocks at a time: a product waits for the one before it on its sums)
 #pragma unroll
-        for (int db = 0; db < DP / 16; ++db) {
-          const bf16x8 vf = join8(read_tr<L::S>(vt, 0, 16 * db, lane), read_tr<L::S>(vt, 16, 16 * db, lane));
+        for (int db = 0; db < DP / 16; db += 2) {
+          bf16x8 vf[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            vf[x] = join8(read_tr<L::S>(vt, 0, 16 * (db + x), lane), read_tr<L::S>(vt, 16, 16 * (db + x), lane));
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) {
-            acc[mb][db] = M::mma(vf, lo[mb], acc[mb][db]);
-            acc[mb][db] = M::mma(vf, hi[mb], acc[mb][db]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) acc[mb][db + x] = M::mma(vf[x], lo[mb], acc[mb][db + x]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) acc[mb][db + x] = M::mma(vf[x], hi[mb], acc[mb][db + x]);
           }
         }
       } else {
