@@ -584,12 +584,11 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   // more (512 from 64 workgroups on, 2048 from 256 on), none up to 512 keys.  us
   // a call, 28/4 heads of 128, whole and in 2, 4, 8 splits: 32 tokens over 8192
   // keys (8 workgroups) 146, 83, 49, 35, and 25 in 32; 512 over 4096 (112) 80,
-  // 57, 52, 67; 512 over 512 19, 22; 2048 over 8192 (448) 232, 248, 260, 299;
-  // 16 chunks of up to 128 over up to 2048 (320) 55, 69; 8 of up to 256 over up
-  // to 4096 (320) 98, 87, 98, 119.
+  // 57, 52, 67; 512 over 512 19, 22; 2048 over 8192 (448) 231, 246, 258, 299;
+  // 16 chunks of up to 128 over up to 2048 (320) 55, 66; 8 of up to 256 over up
+  // to 4096 (320) 90, 88, 100; 3 of up to 300 over up to 5000 (132) 94, 80, 69.
   const long per_cu = wide ? (c.D <= 128 ? 2 : 1) : !c.io_bf16 ? 1 : c.D <= 64 ? 4 : c.D <= 128 ? 2 : 1;
-  // (rounded up from the half where chunks differ and the estimate is high)
-  const long want = (per_cu * n_cu + (wide && c.n_seqs > 1 ? groups / 2 : 0)) / groups;
+  const long want = per_cu * n_cu / groups;
   const long least = !wide ? 512 : groups < 64 ? 256 : groups < 256 ? 512 : 2048;
   const long most = keys <= (wide ? 512 : 1024) ? 1 : keys / least;
   const long cap_splits = wide && (long)c.T * hq > kCacheJoinRows ? kCacheTileJoin : kMaxSplits;

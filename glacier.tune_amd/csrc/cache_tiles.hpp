@@ -19,6 +19,40 @@ __device__ inline CacheSeq seq_of_tile(const CacheAttn& a, int lane, int number)
   return find_seq(a.c, lane, number, [&](int b, int to) { return first_tile(a, b, to); });
 }
 
+// The sequence of tile `number` and the tile's place in it when tiles are numbered
+// from the longest sequence to the shortest and from a sequence's last tile to
+// its first (batches of at most 64 sequences; others from the last to the first),
+// so that long tiles start first and short ones fill in beside them.  tile: -1 if
+// there is no such tile.
+__device__ inline CacheSeq seq_of_long_tile(const CacheAttn& a, int lane, int number, int numbers, int& tile) {
+  const CacheView& c = a.c;
+  tile = -1;
+  if (c.n_seqs > 64) {
+    number = numbers - 1 - number;
+    const CacheSeq s = seq_of_tile(a, lane, number);
+    if (s.b < c.n_seqs) tile = number - first_tile(a, s.b, s.tok0);
+    return s;
+  }
+  const int i = lane < c.n_seqs ? lane : c.n_seqs - 1;
+  const int from = clamp_row(c.cu[i], c.T), len = c.kv_lens[i];
+  const int n = lane < c.n_seqs ? max(0, clamp_row(c.cu[i + 1], c.T) - from) : 0;
+  const int tiles = (n * a.group + a.rows - 1) / a.rows;
+  int before = 0;  // tiles of the sequences that go first
+  for (int u = 0; u < c.n_seqs; ++u) {
+    const int other = __builtin_amdgcn_readlane(len, u);
+    if (other > len || (other == len && u < lane)) before += __builtin_amdgcn_readlane(tiles, u);
+  }
+  const unsigned long long mine = __ballot(number >= before && number < before + tiles);
+  CacheSeq s{c.n_seqs, 0, 0, 0};
+  if (mine == 0) return s;
+  s.b = __ffsll(mine) - 1;
+  s.tok0 = __builtin_amdgcn_readlane(from, s.b);
+  s.n = __builtin_amdgcn_readlane(n, s.b);
+  s.pos0 = __builtin_amdgcn_readlane(len, s.b) - s.n;
+  tile = __builtin_amdgcn_readlane(before + tiles, s.b) - 1 - number;
+  return s;
+}
+
 // How many tile numbers a batch of the call's size can use at most.
 inline unsigned tile_numbers(const CacheAttn& a) {
   return static_cast<unsigned>((long)a.c.T * a.group / a.rows + a.c.n_seqs);
