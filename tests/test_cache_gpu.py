@@ -359,3 +359,69 @@ def test_another_stream(eng):
         got = eng.cache_forward(q, *p.arrays())[0]
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_offsets_past_32_bits(eng, dt):
+    # pages whose elements lie past 2^31 (and bytes past 2^32) of one allocation
+    d, page, hkv, hq = 128, 256, 8, 16
+    size = hkv * page * d
+    n = 2 ** 31 // size + 40
+    p = ch.Paged([(3, 700), (1, 300)], hq, hkv, d, page, DTYPES[dt], 17, spare=0)
+    far = torch.arange(n - p.n_pages, n, device="cuda")
+    pages = []
+    for x in (p.k_pages, p.v_pages):
+        big = torch.empty(n, hkv, page, d, device="cuda", dtype=DTYPES[dt])
+        big[far] = x
+        pages.append(big)
+    table = torch.where(p.table >= 0, p.table + n - p.n_pages, p.table)
+    ref = ch.attend_ref(p)
+    out, lse = eng.cache_forward(p.q.cuda(), *pages, p.cu, p.kv_lens, table, save=True)
+    ch.check("out", out, ref[0], ref[1])
+    ch.check("lse", lse, ref[2], ref[3])
+    k = torch.randn(4, hkv, d, device="cuda").to(DTYPES[dt])
+    eng.cache_append(k, 2 * k, *pages, p.cu, p.kv_lens, table)
+    for t, (b, pos) in enumerate([(0, 697), (0, 698), (0, 699), (1, 299)]):
+        at = int(table[b, pos // page])
+        assert torch.equal(pages[0][at, :, pos % page], k[t])
+        assert torch.equal(pages[1][at, :, pos % page], 2 * k[t])
+
+
+def test_two_graphs_of_one_engine_run_side_by_side(eng):
+    # each captured call has a workspace of its own, so graphs of one engine may
+    # run at the same time; every replay is checked against the eager result
+    g = torch.Generator(device="cuda").manual_seed(5)
+    runs = []
+    for seqs, hq, hkv, d in (([(1, 6000), (1, 3000)], 28, 4, 128), ([(150, 5000)], 16, 4, 128)):
+        p = ch.Paged(seqs, hq, hkv, d, 64, torch.bfloat16, 18)
+        q = p.q.cuda()
+        w = torch.ones(d, device="cuda")
+        dw = torch.zeros(2, d, device="cuda")
+        out, lse = torch.empty_like(q), torch.empty(hq, p.tokens, device="cuda")
+        x = torch.randn(400, hq, d, device="cuda", generator=g).bfloat16()
+        dx = torch.empty_like(x), torch.empty_like(x)
+
+        def step(p=p, q=q, w=w, dw=dw, out=out, lse=lse, x=x, dx=dx):
+            dw.zero_()
+            eng.cache_forward(q, *p.arrays(), out=out, lse=lse)
+            eng.qk_norm_backward(x, x, x, x, w, w, 1e-6, rope_freq_base=1e6, dq=dx[0], dk=dx[1],
+                                 dq_weight=dw[0], dk_weight=dw[1])
+
+        step()
+        torch.cuda.synchronize()
+        want = [t.clone() for t in (out, lse, dw, *dx)]
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph):
+            step()
+        runs.append((graph, stream, (out, lse, dw, *dx), want, p, q, w, x))
+    for _ in range(4):
+        for _, _, got, _, *_ in runs:
+            for t in got:
+                t.fill_(5.0)
+        torch.cuda.synchronize()
+        for graph, stream, *_ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, _, got, want, *_ in runs:
+            assert all(torch.equal(x, y) for x, y in zip(got, want))

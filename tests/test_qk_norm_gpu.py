@@ -151,3 +151,27 @@ def test_repeatable_and_captured(eng):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(want, (yq, yk, dq, dk, dwq, dwk)))
+
+
+def test_offsets_past_32_bits(eng):
+    # rows past 2^31 elements: the first and last tokens of one call
+    T, hq, hkv, d = 2 ** 31 // (30 * 128) + 100, 30, 2, 128
+    q = torch.zeros(T, hq, d, device="cuda", dtype=torch.bfloat16)
+    k = torch.zeros(T, hkv, d, device="cuda", dtype=torch.bfloat16)
+    ends = torch.tensor([0, 1, T - 2, T - 1])
+    sq, sk, gq, gk, wq, wk, _ = _inputs(4, hq, hkv, d, torch.bfloat16, 6, 9)
+    q[ends.cuda()], k[ends.cuda()] = sq, sk
+    eng.qk_norm_forward(q, k, wq, wk, EPS, rope_freq_base=1e6, q_out=q, k_out=k)
+    for name, x, w, y in (("q", sq, wq, q), ("k", sk, wk, k)):
+        ch.check(name, y[ends.cuda()], *ch.norm_ref(x, w, ends, 1e6, EPS, torch.bfloat16))
+    dy, dyk = torch.zeros_like(q), torch.zeros_like(k)
+    q.zero_()
+    k.zero_()
+    q[ends.cuda()], k[ends.cuda()], dy[ends.cuda()], dyk[ends.cuda()] = sq, sk, gq, gk
+    dwq, dwk = torch.zeros(d, device="cuda"), torch.zeros(d, device="cuda")
+    eng.qk_norm_backward(dy, dyk, q, k, wq, wk, EPS, rope_freq_base=1e6, dq=dy, dk=dyk, dq_weight=dwq,
+                         dk_weight=dwk)
+    for name, g, x, w, dx, dw in (("q", gq, sq, wq, dy, dwq), ("k", gk, sk, wk, dyk, dwk)):
+        rx, bx, rw, bw = ch.norm_grad_ref(g, x, w, ends, 1e6, EPS, torch.bfloat16)
+        ch.check(f"d{name}", dx[ends.cuda()], rx, bx)
+        ch.check(f"d{name}_weight", dw, rw, bw)
