@@ -1399,7 +1399,9 @@ QkNorm qk_norm_of(const glacier_rmsnorm_qk_desc* desc) {
     fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
   need_base(d.rope_freq_base);
   need_head_dim(d.head_dim);
-  if ((long long)d.total_tokens * ((long long)d.n_heads_q + d.n_heads_kv) >= (1LL << 31))
+  // (a launch has fewer than 2^32 threads, and 64 of them or more to a token)
+  if ((long long)d.total_tokens * ((long long)d.n_heads_q + d.n_heads_kv) >= (1LL << 30) ||
+      d.total_tokens >= (1 << 26))
     fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
   QkNorm a{};
   a.T = d.total_tokens;
@@ -1480,10 +1482,13 @@ void need_heads_q(const CacheView& c, int hq) {
     fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT,
          "n_heads_q (" + std::to_string(hq) + ") must be a multiple of n_heads_kv (" + std::to_string(c.hkv) + ")");
 }
-void need_cache_size(const CacheView& c, int heads) {
-  if ((long long)c.T * heads >= (1LL << 31) || c.n_seqs >= (1 << 30) ||
-      (long long)c.T * heads * c.D >= (1LL << 40))
-    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
+// A launch has fewer than 2^32 threads: 64 to a token at most (append), 512 to 16
+// rows of a KV head and to each sequence, 256 to 128 rows and to each sequence and
+// KV head (attention).
+void need_cache_size(const CacheView& c, long long heads) {
+  if (c.T * heads >= (1LL << 26)) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
+  if (c.n_seqs >= (1 << 21) || (long long)c.n_seqs * c.hkv >= (1LL << 23))
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "too many sequences");
   if (c.hkv > 65535) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "more than 65535 KV heads");
 }
 
@@ -1854,7 +1859,7 @@ int glacier_attn_cache_append(glacier_attn_ctx* ctx, const glacier_kv_cache* cac
         fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "q is given, but there is no rotation (rope_freq_base is 0)");
       glacier::need_row_tensor(q_rot, "q_rot", rows);
     }
-    glacier::need_cache_size(a.c, a.hq + 2 * a.c.hkv);
+    glacier::need_cache_size(a.c, a.hq + 2LL * a.c.hkv);
     glacier::need_cache_arrays(a.c);
     glacier::need_row_tensor(k, "k", rows);
     glacier::need_row_tensor(v, "v", rows);

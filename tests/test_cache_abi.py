@@ -172,3 +172,23 @@ def test_front_end_checks_tensors_before_the_abi():
                    dict(k_pages=kp.half(), v_pages=kp.half()), dict(device=0)):
         with pytest.raises(TypeError):
             ga.cache_args(**dict(good, **change))
+
+
+@pytest.mark.parametrize("call", [_append, _forward])
+@pytest.mark.parametrize("change,word", [
+    (dict(total_tokens=1 << 26), "tensor too large"), (dict(n_seqs=1 << 21), "too many sequences"),
+    (dict(n_seqs=1 << 20, n_heads_kv=8, hq=8, page_stride=8 * 16 * 64), "too many sequences"),
+    (dict(hq=2 ** 31 - 2), "tensor too large"),
+    (dict(n_heads_kv=2 ** 30, hq=2 ** 30, page_stride=2 ** 39, page_size=16, head_dim=8, n_pages=1),
+     "tensor too large")])
+def test_more_threads_than_a_launch_has(call, change, word):
+    # (and head counts whose sum passes 32 bits)
+    rc, msg = call(**change)
+    assert rc == UNSUPPORTED and word in msg, msg
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("change", [dict(T=1 << 26, hq=1, hkv=1), dict(T=1, hq=2 ** 30), dict(T=2, hq=2 ** 29)])
+def test_more_rows_than_a_norm_counts(backward, change):
+    rc, msg = _norm(backward=backward, **change)
+    assert rc == UNSUPPORTED and "too large" in msg, msg
