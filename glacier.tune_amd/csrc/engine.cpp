@@ -1475,6 +1475,32 @@ void need_cache_arrays(const CacheView& c) {
   need_row_tensor(c.v_pages, "v_pages", c.n_pages > 0);
 }
 
+// A tensor that shares memory with one of the pages at `pages`.
+void need_off_pages(const CacheView& c, const void* pages, const char* pages_name, const void* p, size_t bytes,
+                    const char* name) {
+  if (pages == nullptr || p == nullptr || bytes == 0) return;
+  const long long esz = c.io_bf16 ? 2 : 4, stride = esz * c.page_stride;
+  const long long page = esz * ((long long)c.hkv << c.page_shift) * c.D;
+  const long long at = static_cast<long long>(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(pages));
+  // the first page that ends behind the tensor's begin
+  const long long first = at < page ? 0 : (at - page) / stride + 1;
+  if (first < c.n_pages && first * stride < at + static_cast<long long>(bytes))
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, std::string(name) + " overlaps " + pages_name);
+}
+void need_off_both(const CacheView& c, const void* p, size_t bytes, const char* name) {
+  need_off_pages(c, c.k_pages, "k_pages", p, bytes, name);
+  need_off_pages(c, c.v_pages, "v_pages", p, bytes, name);
+}
+// K and V pages that share memory.  (Whichever begin later: where their first page
+// lies in a gap of the others, their i-th one lies i gaps further.)
+void need_pages_apart(const CacheView& c) {
+  const size_t page = (c.io_bf16 ? 2 : 4) * ((size_t)c.hkv << c.page_shift) * c.D;
+  if (reinterpret_cast<uintptr_t>(c.k_pages) <= reinterpret_cast<uintptr_t>(c.v_pages))
+    need_off_pages(c, c.k_pages, "k_pages", c.v_pages, page, "v_pages");
+  else
+    need_off_pages(c, c.v_pages, "v_pages", c.k_pages, page, "k_pages");
+}
+
 // Query heads of a call over the cache.
 void need_heads_q(const CacheView& c, int hq) {
   if (hq <= 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "head counts must be positive");
@@ -1833,6 +1859,14 @@ int glacier_rmsnorm_qk_backward(glacier_attn_ctx* ctx, const glacier_rmsnorm_qk_
     const bool dw = dq_weight != nullptr || dk_weight != nullptr;
     if (dw && dq_weight == dk_weight)
       fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "dq_weight and dk_weight are the same array");
+    const size_t wb = sizeof(float) * a.D;
+    glacier::need_apart(dq_weight, wb, "dq_weight", dk_weight, wb, "dk_weight", false);
+    for (const auto& [w, name] : {std::pair{dq_weight, "dq_weight"}, std::pair{dk_weight, "dk_weight"}}) {
+      glacier::need_apart(w, wb, name, q_weight, wb, "q_weight", false);
+      glacier::need_apart(w, wb, name, k_weight, wb, "k_weight", false);
+      glacier::need_apart(w, wb, name, dq, qb, "dq", false);
+      glacier::need_apart(w, wb, name, dk, kb, "dk", false);
+    }
     if (dw && rows) glacier::need_workspace(workspace, workspace_bytes, glacier::qk_norm_workspace(a));
     need(ctx, "ctx");
     a.dq_out = dq_out; a.dk_out = dk_out; a.q = q; a.k = k; a.wq = q_weight; a.wk = k_weight;
@@ -1866,6 +1900,13 @@ int glacier_attn_cache_append(glacier_attn_ctx* ctx, const glacier_kv_cache* cac
     glacier::need_row_tensor(q, "q", false);
     const size_t esz = a.c.io_bf16 ? 2 : 4;
     const size_t qb = esz * a.c.T * a.hq * a.c.D, kb = esz * a.c.T * a.c.hkv * a.c.D;
+    if (rows) {
+      glacier::need_pages_apart(a.c);
+      glacier::need_off_both(a.c, k, kb, "k");
+      glacier::need_off_both(a.c, v, kb, "v");
+      if (q != nullptr) glacier::need_off_both(a.c, q, qb, "q");
+      if (q != nullptr) glacier::need_off_both(a.c, q_rot, qb, "q_rot");
+    }
     if (q != nullptr) {
       glacier::need_apart(q_rot, qb, "q_rot", q, qb, "q", true);
       glacier::need_apart(q_rot, qb, "q_rot", k, kb, "k", false);
@@ -1906,7 +1947,14 @@ int glacier_attn_cache_forward(glacier_attn_ctx* ctx, const glacier_kv_cache* ca
     glacier::need_row_tensor(q, "q", rows);
     glacier::need_row_tensor(out, "out", rows);
     const size_t qb = (a.c.io_bf16 ? 2 : 4) * (size_t)a.c.T * n_heads_q * a.c.D;
+    const size_t lb = sizeof(float) * a.c.T * n_heads_q;
     glacier::need_apart(out, qb, "out", q, qb, "q", true);
+    glacier::need_apart(lse, lb, "lse", q, qb, "q", false);
+    glacier::need_apart(lse, lb, "lse", out, qb, "out", false);
+    if (rows) {
+      glacier::need_off_both(a.c, out, qb, "out");
+      glacier::need_off_both(a.c, lse, lb, "lse");
+    }
     need(ctx, "ctx");
     const glacier::CachePlan p = ctx->eng->PlanCacheAttention(a.c, n_heads_q, batch->max_new, batch->max_kv);
     glacier::need_workspace(workspace, workspace_bytes, p.bytes);

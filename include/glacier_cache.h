@@ -29,7 +29,7 @@
  * the new tokens of sequence b, and kv_lens[b] is its length with them, so its
  * i-th new token is at position kv_lens[b] - (cu_tokens[b+1] - cu_tokens[b])
  * + i.  A sequence may have no new token.  Rows at or past cu_tokens[n_seqs]
- * (a batch padded to a fixed size) are neither read nor written.  cu_tokens,
+ * (a batch padded to a fixed size) change nothing and are not written.  cu_tokens,
  * kv_lens and page_table are device arrays, so a captured graph replays with
  * whatever they hold then; both calls are safe to capture: they allocate
  * nothing and do not wait.  K and V rows past a sequence's end may hold
@@ -85,7 +85,9 @@ typedef struct glacier_cache_batch {
  * rotated already) and v, [total_tokens][n_heads_kv][head_dim], into the pages.
  * q [total_tokens][n_heads_q][head_dim], when not NULL, is rotated into q_rot,
  * which may be q; it needs rope_freq_base > 0.  n_heads_q is read only then.
- * Two tokens of one call never share a place: their positions differ. */
+ * Sequences may share pages that they only read; a page that takes new tokens
+ * belongs to one of them.  K pages, V pages, k, v, q and q_rot share no memory
+ * (but q_rot and q); pages of K and V may alternate. */
 int glacier_attn_cache_append(glacier_attn_ctx *ctx, const glacier_kv_cache *cache,
                               const glacier_cache_batch *batch, const void *k, const void *v,
                               float rope_freq_base, int32_t n_heads_q, const void *q, void *q_rot);
@@ -101,7 +103,7 @@ size_t glacier_attn_cache_workspace(glacier_attn_ctx *ctx, const glacier_kv_cach
  * [total_tokens] fp32, the natural log-sum-exp of the scores.  A row without a
  * key gets 0 and -inf.  workspace: at least glacier_attn_cache_workspace bytes,
  * 256-byte aligned, the call's own until it has run (calls that overlap need
- * one each).  out may be q. */
+ * one each).  out may be q; out and lse lie outside the pages. */
 int glacier_attn_cache_forward(glacier_attn_ctx *ctx, const glacier_kv_cache *cache,
                                const glacier_cache_batch *batch, int32_t n_heads_q, const void *q,
                                void *out, float *lse, void *workspace, size_t workspace_bytes);

@@ -192,3 +192,44 @@ def test_more_threads_than_a_launch_has(call, change, word):
 def test_more_rows_than_a_norm_counts(backward, change):
     rc, msg = _norm(backward=backward, **change)
     assert rc == UNSUPPORTED and "too large" in msg, msg
+
+
+PAGE = 2 * 2 * 16 * 64  # bytes of a page of _cache()
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(v_pages=MB), "v_pages overlaps k_pages"), (dict(v_pages=MB + PAGE), "v_pages overlaps k_pages"),
+    (dict(v_pages=MB - PAGE + 16), "k_pages overlaps v_pages"), (dict(v_pages=MB + 9 * PAGE), "ctx"),
+    (dict(v_pages=MB - 9 * PAGE), "ctx"), (dict(v_pages=MB + 9 * PAGE - 16), "v_pages overlaps"),
+    # interleaved pages: the others' lie in the gaps
+    (dict(v_pages=MB + PAGE, page_stride=PAGE), "ctx"), (dict(v_pages=MB + 3 * PAGE, page_stride=PAGE), "ctx"),
+    (dict(v_pages=MB + 2 * PAGE, page_stride=PAGE), "v_pages overlaps"),
+    (dict(v_pages=MB + PAGE - 16, page_stride=PAGE), "v_pages overlaps"),
+    (dict(v_pages=MB + PAGE + 16, page_stride=PAGE), "v_pages overlaps"),
+    (dict(k=MB + 16), "k overlaps k_pages"), (dict(v=2 * MB + 8 * PAGE), "v overlaps v_pages"),
+    (dict(q=MB + PAGE), "q overlaps k_pages"), (dict(q_rot=2 * MB - 16), "q_rot overlaps v_pages"),
+    (dict(k=MB + 9 * PAGE), "ctx"), (dict(k=MB - 8 * 2 * 64 * 2), "ctx"),
+    (dict(k=MB + PAGE, page_stride=PAGE), "ctx"), (dict(k=MB + PAGE + 16, page_stride=2 * PAGE, v_pages=4 * MB), "ctx"),
+    (dict(v_pages=MB, n_pages=0), "ctx")])
+def test_append_keeps_off_the_pages(change, word):
+    rc, msg = _append(**change)
+    assert rc == INVALID and word in msg, msg
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(out=MB), "out overlaps k_pages"), (dict(lse=2 * MB + 4), "lse overlaps v_pages"),
+    (dict(lse=8 * MB), "lse overlaps q"), (dict(lse=9 * MB + 64), "lse overlaps out"),
+    (dict(v_pages=MB), "ctx"), (dict(q=MB), "ctx")])
+def test_forward_keeps_off_the_pages(change, word):
+    # (reading may share memory: one set of pages as K and V is fine)
+    rc, msg = _forward(**change)
+    assert rc == INVALID and word in msg, msg
+
+
+@pytest.mark.parametrize("at,word", [
+    ({"dk_weight": 10 * MB}, "same array"), ({"dk_weight": 10 * MB + 16}, "dq_weight overlaps dk_weight"),
+    ({"dq_weight": 5 * MB}, "dq_weight overlaps q_weight"), ({"dk_weight": 6 * MB + 4}, "dk_weight overlaps k_weight"),
+    ({"dk_weight": 8 * MB + 64}, "dk_weight overlaps dq"), ({"dq_weight": 10 * MB + 256}, "ctx")])
+def test_weight_gradients_share_no_memory(at, word):
+    rc, msg = _norm(backward=True, at=at)
+    assert rc == INVALID and word in msg, msg
