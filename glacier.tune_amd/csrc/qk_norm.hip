@@ -175,14 +175,16 @@ __global__ __launch_bounds__(64 * kWavesQkBwd) void qk_norm_bwd_kernel(QkNorm a,
     c = lanes_sum<L>(c);
     if (ok) {
       const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
-      const float kx = r * r * r / (float)a.D * c;
+      // (by n = x r, whose size is that of 1: r^3 leaves fp32 for rows below 1e-13)
+      const float cn = c * r / (float)a.D;
       float o0[E], o1[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        o0[e] = r * (w0[e] * g0[e]) - kx * x0[e];
-        o1[e] = r * (w1[e] * g1[e]) - kx * x1[e];
+        const float n0 = x0[e] * r, n1 = x1[e] * r;
+        o0[e] = r * (w0[e] * g0[e] - n0 * cn);
+        o1[e] = r * (w1[e] * g1[e] - n1 * cn);
         if constexpr (DW) {
-          const float v0 = g0[e] * (x0[e] * r), v1 = g1[e] * (x1[e] * r);
+          const float v0 = g0[e] * n0, v1 = g1[e] * n1;
           dq0[e] += is_q ? v0 : 0.0f;
           dq1[e] += is_q ? v1 : 0.0f;
           dk0[e] += is_q ? 0.0f : v0;

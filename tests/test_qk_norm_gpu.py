@@ -122,6 +122,22 @@ def test_zero_rows_and_zero_tokens(eng):
     assert yq.shape == (0, 4, 64) and yk.shape == (0, 1, 64)
 
 
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_tiny_rows_without_eps(eng, dt):
+    # 1 / sqrt(mean x^2) is 1e14: its cube leaves fp32, the gradients do not
+    q, k, gq, gk, wq, wk, pos = _inputs(5, 6, 2, 64, DTYPES[dt], 8, 100)
+    q, k = q * 1e-14, k * 1e-14
+    yq, yk = eng.qk_norm_forward(q, k, wq, wk, 0.0, rope_freq_base=1e4, positions=pos.cuda())
+    dwq, dwk = torch.zeros_like(wq), torch.zeros_like(wk)
+    dq, dk = eng.qk_norm_backward(gq, gk, q, k, wq, wk, 0.0, rope_freq_base=1e4, positions=pos.cuda(),
+                                  dq_weight=dwq, dk_weight=dwk)
+    for name, x, w, y, g, dx, dw in (("q", q, wq, yq, gq, dq, dwq), ("k", k, wk, yk, gk, dk, dwk)):
+        ch.check(name, y, *ch.norm_ref(x, w, pos, 1e4, 0.0, DTYPES[dt]))
+        rx, bx, rw, bw = ch.norm_grad_ref(g, x, w, pos, 1e4, 0.0, DTYPES[dt])
+        ch.check(f"d{name}", dx, rx, bx)
+        ch.check(f"d{name}_weight", dw, rw, bw)
+
+
 def test_repeatable_and_captured(eng):
     q, k, gq, gk, wq, wk, pos = _inputs(700, 28, 4, 128, torch.bfloat16, 4, 4096)
     pos = pos.cuda()
