@@ -411,6 +411,14 @@ __device__ inline float swap_sum(float x, bool rows16) {
   const unsigned a = r[0], b = r[1];
   return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
 }
+// Orders this wave's LDS accesses before and after it (LDS serves a wave in
+// order, so only the compiler has to be told).
+__device__ inline void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 __device__ inline float col_max_swap(float x) { return swap_max(swap_max(x, false), true); }
 __device__ inline float col_sum_swap(float x) { return swap_sum(swap_sum(x, false), true); }
 

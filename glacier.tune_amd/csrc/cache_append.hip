@@ -92,7 +92,7 @@ hipError_t append(CacheAppend& a, const TurnRates& r, int n_cu, hipStream_t st) 
 }  // namespace
 
 hipError_t launch_cache_append(CacheAppend a, const TurnRates& r, int n_cu, hipStream_t st) {
-  GL_BY_HEAD(append, a.c.io_bf16, a.c.D, piece_elems(a.c.io_bf16, a.c.D), a, r, n_cu, st);
+  GL_BY_HEAD(append, a.c.io_bf16, a.c.D, a, r, n_cu, st);
 }
 
 }  // namespace glacier

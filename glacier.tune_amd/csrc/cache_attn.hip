@@ -5,10 +5,11 @@
 // token r / group, head r % group.  One new token of 7 heads and a long chunk
 // are then the same product, and K and V are read once per tile, not per head.
 //
-// A workgroup takes one tile of one KV head, and one split of the keys the
-// tile sees.  Its four waves take keys in turn, KB at a time, each with its own
-// LDS tiles and its own running maximum and sum of the softmax, so the loop
-// has no barrier; the waves are joined through LDS at the end.  Scores are
+// A workgroup takes one tile of 16 rows of one KV head, and one split of the
+// keys the tile sees.  Its waves (four; eight in fp32 up to 128 columns) take keys
+// in turn, KB at a time, each with its own LDS tiles and its own running maximum
+// and sum of the softmax, so the loop has no barrier; the waves are joined
+// through LDS at the end.  Scores are
 // formed transposed (S^T = K Q^T, attn_common.hpp), which leaves a lane with
 // one row's weights and feeds them to O^T += V^T P^T as they are.
 //
@@ -23,7 +24,6 @@
 namespace glacier {
 namespace {
 
-
 template <typename T>
 struct KeyBlock;
 template <>
@@ -35,13 +35,14 @@ struct KeyBlock<float> {
   static constexpr int KB = 16;  // two blocks of 256 columns and their copies fit the LDS
 };
 
-template <typename T, int DP, int MB, int WAVES>
+template <typename T, int DP, int WAVES>
 struct CaLayout {
   static constexpr int KB = KeyBlock<T>::KB;
   static constexpr int S = Lds<T, DP>::STRIDE;
   static constexpr int TILES = WAVES * 2 * KB * S * static_cast<int>(sizeof(T));
   static constexpr int OS = DP + 4;  // row stride (floats) of a wave's sums in the join
-  static constexpr int WAVE = 16 * MB * (OS + 2);  // sums, maxima, totals
+  static constexpr int ROWS = 16;
+  static constexpr int WAVE = ROWS * (OS + 2);  // sums, maxima, totals
   static constexpr int JOIN = WAVES * WAVE * 4;
   static constexpr int NOTES = TILES > JOIN ? TILES : JOIN;  // then the noted blocks of each wave
   static constexpr int BYTES = NOTES + WAVES * kNotedBlocks / 8;
@@ -78,17 +79,11 @@ struct BlockRegs {
   }
 };
 
-__device__ inline void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-template <typename T, int DP, int MB, int WAVES>
+template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   using M = Mfma<T>;
-  using L = CaLayout<T, DP, MB, WAVES>;
-  constexpr int KB = L::KB, NS = KB / 16, ROWS = 16 * MB;
+  using L = CaLayout<T, DP, WAVES>;
+  constexpr int KB = L::KB, NS = KB / 16, ROWS = L::ROWS;
   constexpr int NW = DP * sizeof(T) / 64;  // 16-byte words a lane holds of a row
   extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
@@ -105,36 +100,29 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   if (split >= tk.active) return;
   const int k0 = split * tk.per, k1 = min(tk.kend, k0 + tk.per);
 
-  // this lane's rows (one per 16-row block): operand fragments and last key
-  i32x4 qw[MB][NW];
-  int limit[MB];
+  // this lane's row: operand fragments and last key
+  i32x4 qw[NW];
   // the first of the 16 bytes of columns that this lane holds in word x of a
   // row of Q or K: one k-step's 8 columns in bf16; in fp32, where a k-step takes
   // one column a lane, those of four steps (step 4 x + e takes column
   // 16 x + 4 g + e: a dot product may take its terms in any order)
   auto first_col = [&](int x) { return sizeof(T) == 2 ? 32 * x + 8 * g : 16 * x + 4 * g; };
+  const int r = r0 + col, tok = r / a.group;
+  const int limit = r < n_rows ? s.pos0 + tok : -1;
+  // (loaded from the tile's first row where there is none, and cleared after
+  // all loads are under way)
+  const T* const q = static_cast<const T*>(a.q) +
+                     (r < n_rows ? (long)(s.tok0 + tok) * a.hq + kvh * a.group + (r - tok * a.group)
+                                 : (long)(s.tok0 + r0 / a.group) * a.hq) * D;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const int r = r0 + 16 * mb + col;
-    const int i = r / a.group, h = kvh * a.group + (r - i * a.group);
-    const bool ok = r < n_rows;
-    limit[mb] = ok ? s.pos0 + i : -1;
-    // (loaded from the tile's first row where there is none, and cleared after
-    // all loads are under way)
-    const T* q = static_cast<const T*>(a.q) +
-                 (ok ? (long)(s.tok0 + i) * a.hq + h : (long)(s.tok0 + r0 / a.group) * a.hq) * D;
+  for (int x = 0; x < NW; ++x)
+    qw[x] = *reinterpret_cast<const i32x4*>(q + (first_col(x) < D ? first_col(x) : 0));
 #pragma unroll
-    for (int x = 0; x < NW; ++x)
-      qw[mb][x] = *reinterpret_cast<const i32x4*>(q + (first_col(x) < D ? first_col(x) : 0));
-  }
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-    for (int x = 0; x < NW; ++x)
-      if (limit[mb] < 0 || first_col(x) >= D) qw[mb][x] = i32x4{0, 0, 0, 0};
+  for (int x = 0; x < NW; ++x)
+    if (limit < 0 || first_col(x) >= D) qw[x] = i32x4{0, 0, 0, 0};
 
-  f32x4 acc[MB][DP / 16];
-  float m[MB], l[MB];
+  f32x4 acc[DP / 16];
+  float m, l;
 
   T* const kt = reinterpret_cast<T*>(smem) + w * 2 * KB * L::S;
   T* const vt = kt + KB * L::S;
@@ -175,13 +163,10 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   unsigned* const notes = reinterpret_cast<unsigned*>(smem + L::NOTES) + w * (kNotedBlocks / 32);
   auto note_of = [&](int j) { return (j - k0) / (WAVES * KB) % kNotedBlocks; };
   auto walk = [&](auto careful) __attribute__((always_inline)) {
+    m = kNegBig;
+    l = 0.0f;
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      m[mb] = kNegBig;
-      l[mb] = 0.0f;
-#pragma unroll
-      for (int db = 0; db < DP / 16; ++db) acc[mb][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int db = 0; db < DP / 16; ++db) acc[db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     int j = k0 + w * KB;
     if (j < k1) {
       look_up(j);
@@ -201,79 +186,69 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
         for (int i = 0; i < R::N; ++i) found |= clear_not_finite<T>(vr.w[i]);
         if (__any(found != 0) && lane == 0) notes[note_of(j) / 32] |= 1u << note_of(j) % 32;
       }
-      wave_lds_fence();
+      wave_lds_order();
       kr.store(kt, lane);
       vr.store(vt, lane);
-      wave_lds_fence();
+      wave_lds_order();
       if (j + WAVES * KB < k1) fetch(j + WAVES * KB);
       // S^T: keys 16 p + 4 g + r of this block, row col of each 16-row block
-      f32x4 st[MB][NS];
+      f32x4 st[NS];
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int p = 0; p < NS; ++p) st[mb][p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int p = 0; p < NS; ++p) st[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int p = 0; p < NS; ++p)
 #pragma unroll
         for (int x = 0; x < NW; ++x) {
           const i32x4 kw = *reinterpret_cast<const i32x4*>(kt + (16 * p + col) * L::S + first_col(x));
+          if constexpr (sizeof(T) == 2) {
+            st[p] = M::mma(__builtin_bit_cast(bf16x8, kw), __builtin_bit_cast(bf16x8, qw[x]), st[p]);
+          } else {
+            const f32x4 kf = __builtin_bit_cast(f32x4, kw), qf = __builtin_bit_cast(f32x4, qw[x]);
 #pragma unroll
-          for (int mb = 0; mb < MB; ++mb) {
-            if constexpr (sizeof(T) == 2) {
-              st[mb][p] = M::mma(__builtin_bit_cast(bf16x8, kw), __builtin_bit_cast(bf16x8, qw[mb][x]), st[mb][p]);
-            } else {
-              const f32x4 kf = __builtin_bit_cast(f32x4, kw), qf = __builtin_bit_cast(f32x4, qw[mb][x]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) st[mb][p] = M::mma(kf[e], qf[e], st[mb][p]);
-            }
+            for (int e = 0; e < 4; ++e) st[p] = M::mma(kf[e], qf[e], st[p]);
           }
         }
+      float top = kNegBig;
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        float top = kNegBig;
+      for (int p = 0; p < NS; ++p)
 #pragma unroll
-        for (int p = 0; p < NS; ++p)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float x = st[mb][p][r] * a.scale_log2;
-            if (!whole) {
-              const int at = 4 * g + r;
-              x = at < here[p] && j + 16 * p + at <= limit[mb] ? x : -INFINITY;
-            }
-            st[mb][p][r] = x;
-            top = fmaxf(top, x);
+        for (int r = 0; r < 4; ++r) {
+          float x = st[p][r] * a.scale_log2;
+          if (!whole) {
+            const int at = 4 * g + r;
+            x = at < here[p] && j + 16 * p + at <= limit ? x : -INFINITY;
           }
-        const float mn = fmaxf(m[mb], col_max_swap(top));
-        const float alpha = weight(m[mb] - mn);
-        m[mb] = mn;
-        float sum = 0.0f;
+          st[p][r] = x;
+          top = fmaxf(top, x);
+        }
+      const float mn = fmaxf(m, col_max_swap(top));
+      const float alpha = weight(m - mn);
+      m = mn;
+      float sum = 0.0f;
 #pragma unroll
-        for (int p = 0; p < NS; ++p)
+      for (int p = 0; p < NS; ++p)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float e = weight(st[mb][p][r] - mn);
-            st[mb][p][r] = e;
-            sum += e;
-          }
-        l[mb] = l[mb] * alpha + sum;
+        for (int r = 0; r < 4; ++r) {
+          const float e = weight(st[p][r] - mn);
+          st[p][r] = e;
+          sum += e;
+        }
+      l = l * alpha + sum;
 #pragma unroll
-        for (int db = 0; db < DP / 16; ++db)
+      for (int db = 0; db < DP / 16; ++db)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[mb][db][r] *= alpha;
-      }
+        for (int r = 0; r < 4; ++r) acc[db][r] *= alpha;
       // O^T += V^T P^T; in bf16 each weight in two terms, which leaves 16 bits of
       // it: reading V bounds these calls, and one term would add as much error as
       // the result's own rounding
       if constexpr (sizeof(T) == 2) {
-        bf16x8 hi[MB], lo[MB];
+        bf16x8 hi, lo;
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float p = st[mb][e < 4 ? 0 : NS - 1][e % 4];
-            hi[mb][e] = (bf16)p;
-            lo[mb][e] = (bf16)(p - (float)hi[mb][e]);
-          }
+        for (int e = 0; e < 8; ++e) {
+          const float p = st[e < 4 ? 0 : NS - 1][e % 4];
+          hi[e] = (bf16)p;
+          lo[e] = (bf16)(p - (float)hi[e]);
+        }
         // (two blocks at a time: a product waits for the one before it on its sums)
 #pragma unroll
         for (int db = 0; db < DP / 16; db += 2) {
@@ -282,12 +257,9 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
           for (int x = 0; x < 2; ++x)
             vf[x] = join8(read_tr<L::S>(vt, 0, 16 * (db + x), lane), read_tr<L::S>(vt, 16, 16 * (db + x), lane));
 #pragma unroll
-          for (int mb = 0; mb < MB; ++mb) {
+          for (int x = 0; x < 2; ++x) acc[db + x] = M::mma(vf[x], lo, acc[db + x]);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) acc[mb][db + x] = M::mma(vf[x], lo[mb], acc[mb][db + x]);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) acc[mb][db + x] = M::mma(vf[x], hi[mb], acc[mb][db + x]);
-          }
+          for (int x = 0; x < 2; ++x) acc[db + x] = M::mma(vf[x], hi, acc[db + x]);
         }
       } else {
         // V in wide reads: row i of the four blocks 4 x .. 4 x + 3 is column
@@ -299,18 +271,12 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
           for (int x = 0; x < DP / 64; ++x) {
             const f32x4 vf = *reinterpret_cast<const f32x4*>(vrow + 64 * x + 4 * col);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int mb = 0; mb < MB; ++mb)
-                acc[mb][4 * x + e] = M::mma(vf[e], st[mb][0][r], acc[mb][4 * x + e]);
+            for (int e = 0; e < 4; ++e) acc[4 * x + e] = M::mma(vf[e], st[0][r], acc[4 * x + e]);
           }
           if constexpr (DP % 64 != 0) {
             const float2 vf = *reinterpret_cast<const float2*>(vrow + DP / 64 * 64 + 2 * col);
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb) {
-              acc[mb][DP / 16 - 2] = M::mma(vf.x, st[mb][0][r], acc[mb][DP / 16 - 2]);
-              acc[mb][DP / 16 - 1] = M::mma(vf.y, st[mb][0][r], acc[mb][DP / 16 - 1]);
-            }
+            acc[DP / 16 - 2] = M::mma(vf.x, st[0][r], acc[DP / 16 - 2]);
+            acc[DP / 16 - 1] = M::mma(vf.y, st[0][r], acc[DP / 16 - 1]);
           }
         }
       }
@@ -319,16 +285,14 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   walk(std::false_type{});
   unsigned odd = 0;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
+  for (int db = 0; db < DP / 16; ++db)
 #pragma unroll
-    for (int db = 0; db < DP / 16; ++db)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) odd |= limit[mb] >= 0 ? not_finite(acc[mb][db][r]) : 0;
+    for (int r = 0; r < 4; ++r) odd |= limit >= 0 ? not_finite(acc[db][r]) : 0;
   if (__any(odd != 0)) {
     if (lane < kNotedBlocks / 32) notes[lane] = 0;
-    wave_lds_fence();
+    wave_lds_order();
     walk(std::true_type{});
-    wave_lds_fence();
+    wave_lds_order();
     for (int j = k0 + w * KB; j < k1; j += WAVES * KB) {
       if (!(notes[note_of(j) / 32] >> note_of(j) % 32 & 1)) continue;
       for (int key = j; key < min(k1, j + KB); ++key) {
@@ -336,17 +300,13 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
         if (page < 0) continue;
         const char* const v = static_cast<const char*>(c.v_pages) + page * strideb + head +
                               (key & ((1 << c.page_shift) - 1)) * rowb;
-        unsigned sees[MB];
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) sees[mb] = key <= limit[mb] ? ~0u : 0u;
+        const unsigned sees = key <= limit ? ~0u : 0u;
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
           for (int db = 0; db < DP / 16; ++db) {
             const bf16x4 x = __builtin_bit_cast(bf16x4, load8_within(v, rowb, 2 * (16 * db + 4 * g)));
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int mb = 0; mb < MB; ++mb) acc[mb][db][r] += given_back((float)x[r], sees[mb]);
+            for (int r = 0; r < 4; ++r) acc[db][r] += given_back((float)x[r], sees);
           }
         } else {
 #pragma unroll
@@ -355,18 +315,13 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
             for (int x = 0; x < DP / 64; ++x) {
               const f32x4 f = __builtin_bit_cast(f32x4, load_within(v, rowb, 4 * (64 * x + 16 * g + 4 * r)));
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int mb = 0; mb < MB; ++mb) acc[mb][4 * x + e][r] += given_back(f[e], sees[mb]);
+              for (int e = 0; e < 4; ++e) acc[4 * x + e][r] += given_back(f[e], sees);
             }
             if constexpr (DP % 64 != 0) {
               const float2 f =
                   __builtin_bit_cast(float2, load8_within(v, rowb, 4 * (DP / 64 * 64 + 8 * g + 2 * r)));
-#pragma unroll
-              for (int mb = 0; mb < MB; ++mb) {
-                acc[mb][DP / 16 - 2][r] += given_back(f.x, sees[mb]);
-                acc[mb][DP / 16 - 1][r] += given_back(f.y, sees[mb]);
-              }
+              acc[DP / 16 - 2][r] += given_back(f.x, sees);
+              acc[DP / 16 - 1][r] += given_back(f.y, sees);
             }
           }
         }
@@ -377,33 +332,29 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   // join the waves: region of wave u: sums [ROWS][OS], maxima [ROWS], totals [ROWS]
   __syncthreads();
   float* const mine = reinterpret_cast<float*>(smem) + w * L::WAVE;
+  const float total = col_sum_swap(l);
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const float total = col_sum_swap(l[mb]);
-    const int row = 16 * mb + col;
-    if constexpr (sizeof(T) == 2) {
+    for (int db = 0; db < DP / 16; ++db)
+      store4(mine + col * L::OS + 16 * db + 4 * g, acc[db]);
+  } else {
 #pragma unroll
-      for (int db = 0; db < DP / 16; ++db)
-        store4(mine + row * L::OS + 16 * db + 4 * g, acc[mb][db]);
-    } else {
+    for (int r = 0; r < 4; ++r) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int x = 0; x < DP / 64; ++x) {
+        f32x4 v;
 #pragma unroll
-        for (int x = 0; x < DP / 64; ++x) {
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[mb][4 * x + e][r];
-          store4(mine + row * L::OS + 64 * x + 16 * g + 4 * r, v);
-        }
-        if constexpr (DP % 64 != 0)
-          *reinterpret_cast<float2*>(mine + row * L::OS + DP / 64 * 64 + 8 * g + 2 * r) =
-              make_float2(acc[mb][DP / 16 - 2][r], acc[mb][DP / 16 - 1][r]);
+        for (int e = 0; e < 4; ++e) v[e] = acc[4 * x + e][r];
+        store4(mine + col * L::OS + 64 * x + 16 * g + 4 * r, v);
       }
+      if constexpr (DP % 64 != 0)
+        *reinterpret_cast<float2*>(mine + col * L::OS + DP / 64 * 64 + 8 * g + 2 * r) =
+            make_float2(acc[DP / 16 - 2][r], acc[DP / 16 - 1][r]);
     }
-    if (g == 0) {
-      mine[ROWS * L::OS + row] = m[mb];
-      mine[ROWS * (L::OS + 1) + row] = total;
-    }
+  }
+  if (g == 0) {
+    mine[ROWS * L::OS + col] = m;
+    mine[ROWS * (L::OS + 1) + col] = total;
   }
   __syncthreads();
   const float* const all = reinterpret_cast<const float*>(smem);
@@ -513,12 +464,12 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttn a) {
     a.lse[(long)h * c.T + t] = total == 0.0f ? -INFINITY : (mx + log2f(total)) * kLn2;
 }
 
-template <typename T, int DP, int MB, int WAVES>
+template <typename T, int DP, int WAVES>
 hipError_t attend(const CacheAttn& a, hipStream_t st) {
-  using L = CaLayout<T, DP, MB, WAVES>;
-  auto* fn = &cache_attn_kernel<T, DP, MB, WAVES>;
+  using L = CaLayout<T, DP, WAVES>;
+  auto* fn = &cache_attn_kernel<T, DP, WAVES>;
   GL_CHECK(allow_lds(fn, L::BYTES));
-  hipLaunchKernelGGL((cache_attn_kernel<T, DP, MB, WAVES>), dim3(tile_numbers(a), a.c.hkv, a.n_splits),
+  hipLaunchKernelGGL((cache_attn_kernel<T, DP, WAVES>), dim3(tile_numbers(a), a.c.hkv, a.n_splits),
                      dim3(64 * WAVES), L::BYTES, st, a);
   return hipGetLastError();
 }
@@ -538,11 +489,11 @@ template <typename T>
 hipError_t by_head(const CacheAttn& a, hipStream_t st) {
   constexpr int WAVES = sizeof(T) == 2 ? 4 : 8;
   const int d = a.c.D;
-  if (d <= 32) return attend<T, 32, 1, WAVES>(a, st);
-  if (d <= 64) return attend<T, 64, 1, WAVES>(a, st);
-  if (d <= 96) return attend<T, 96, 1, WAVES>(a, st);
-  if (d <= 128) return attend<T, 128, 1, WAVES>(a, st);
-  return attend<T, 256, 1, 4>(a, st);  // eight waves' fp32 tiles exceed the LDS
+  if (d <= 32) return attend<T, 32, WAVES>(a, st);
+  if (d <= 64) return attend<T, 64, WAVES>(a, st);
+  if (d <= 96) return attend<T, 96, WAVES>(a, st);
+  if (d <= 128) return attend<T, 128, WAVES>(a, st);
+  return attend<T, 256, 4>(a, st);  // eight waves' fp32 tiles exceed the LDS
 }
 
 }  // namespace

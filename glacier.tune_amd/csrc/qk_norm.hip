@@ -279,11 +279,11 @@ hipError_t bwd(QkNorm& a, const TurnRates& r, int n_cu, hipStream_t st) {
 }  // namespace
 
 hipError_t launch_qk_norm_forward(QkNorm a, const TurnRates& r, int n_cu, hipStream_t st) {
-  GL_BY_HEAD(fwd, a.io_bf16, a.D, piece_elems(a.io_bf16, a.D), a, r, n_cu, st);
+  GL_BY_HEAD(fwd, a.io_bf16, a.D, a, r, n_cu, st);
 }
 
 hipError_t launch_qk_norm_backward(QkNorm a, const TurnRates& r, int n_cu, hipStream_t st) {
-  GL_BY_HEAD(bwd, a.io_bf16, a.D, 4, a, r, n_cu, st);
+  GL_BY_HEAD4(bwd, a.io_bf16, a.D, a, r, n_cu, st);
 }
 
 }  // namespace glacier

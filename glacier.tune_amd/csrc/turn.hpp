@@ -42,14 +42,6 @@ __device__ inline float2 turn_of(double rev, int pos) {
   return make_float2(c, s);
 }
 
-// Orders this wave's LDS accesses before and after it (LDS serves a wave in
-// order, so only the compiler has to be told).
-__device__ inline void wave_lds_order() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // The rates of the pairs whose angles this lane forms.
 struct LaneRates {
   double lo, hi;
@@ -75,35 +67,42 @@ inline int turn_parts(int tokens, int steps, int n_cu) {
   return static_cast<int>(parts < 1 ? 1 : parts > steps ? steps : parts);
 }
 
-// Elements a lane takes of each half: 16 bytes where D allows.
-inline int piece_elems(bool io_bf16, int D) { return io_bf16 && D % 16 == 0 ? 8 : 4; }
-// Lanes of one head: a power of two, at least 4.
+// Lanes of one head whose lanes take E elements of each half: a power of two, at
+// least 4.
 inline int lanes_of(int D, int E) {
   int l = 4;
   while (l * E < D / 2) l *= 2;
   return l;
 }
 
-// F<IO, E, L> for the call's dtype, head size and piece.
-#define GL_BY_HEAD(F, io_bf16, D, piece, ...)                 \
-  do {                                                        \
-    const int e_ = piece;                                     \
-    const int l_ = lanes_of(D, e_);                           \
-    if ((io_bf16) && e_ == 8) {                               \
-      if (l_ == 4) return F<bf16, 8, 4>(__VA_ARGS__);         \
-      if (l_ == 8) return F<bf16, 8, 8>(__VA_ARGS__);         \
-      return F<bf16, 8, 16>(__VA_ARGS__);                     \
-    }                                                         \
-    if (io_bf16) {                                            \
-      if (l_ == 4) return F<bf16, 4, 4>(__VA_ARGS__);         \
-      if (l_ == 8) return F<bf16, 4, 8>(__VA_ARGS__);         \
-      if (l_ == 16) return F<bf16, 4, 16>(__VA_ARGS__);       \
-      return F<bf16, 4, 32>(__VA_ARGS__);                     \
-    }                                                         \
-    if (l_ == 4) return F<float, 4, 4>(__VA_ARGS__);          \
-    if (l_ == 8) return F<float, 4, 8>(__VA_ARGS__);          \
-    if (l_ == 16) return F<float, 4, 16>(__VA_ARGS__);        \
-    return F<float, 4, 32>(__VA_ARGS__);                      \
+// F<IO, 4, L> for the call's dtype and head size, from pieces of 4 elements.
+#define GL_BY_HEAD4(F, io_bf16, D, ...)                                 \
+  do {                                                                  \
+    const int l_ = lanes_of(D, 4);                                      \
+    if (l_ == 4) {                                                      \
+      if (io_bf16) return F<bf16, 4, 4>(__VA_ARGS__);                   \
+      return F<float, 4, 4>(__VA_ARGS__);                               \
+    }                                                                   \
+    if (l_ == 8) {                                                      \
+      if (io_bf16) return F<bf16, 4, 8>(__VA_ARGS__);                   \
+      return F<float, 4, 8>(__VA_ARGS__);                               \
+    }                                                                   \
+    if (l_ == 16) {                                                     \
+      if (io_bf16) return F<bf16, 4, 16>(__VA_ARGS__);                  \
+      return F<float, 4, 16>(__VA_ARGS__);                              \
+    }                                                                   \
+    if (io_bf16) return F<bf16, 4, 32>(__VA_ARGS__);                    \
+    return F<float, 4, 32>(__VA_ARGS__);                                \
+  } while (0)
+
+// F<IO, E, L>: pieces of 8 elements (16 bytes) of bf16 where D allows.
+#define GL_BY_HEAD(F, io_bf16, D, ...)                                  \
+  do {                                                                  \
+    if (!(io_bf16) || (D) % 16 != 0) GL_BY_HEAD4(F, io_bf16, D, __VA_ARGS__); \
+    const int l8_ = lanes_of(D, 8);                                     \
+    if (l8_ == 4) return F<bf16, 8, 4>(__VA_ARGS__);                    \
+    if (l8_ == 8) return F<bf16, 8, 8>(__VA_ARGS__);                    \
+    return F<bf16, 8, 16>(__VA_ARGS__);                                 \
   } while (0)
 
 }  // namespace glacier
