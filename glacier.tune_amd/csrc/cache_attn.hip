@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   unsigned* const notes = reinterpret_cast<unsigned*>(smem + L::NOTES) + w * (kNotedBlocks / 32);
   auto note_of = [&](int j) { return (j - k0) / (WAVES * KB) % kNotedBlocks; };
   auto walk = [&](auto careful) __attribute__((always_inline)) {
-    m = kNegBig;
+    m = kLeast;
     l = 0.0f;
 #pragma unroll
     for (int db = 0; db < DP / 16; ++db) acc[db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
             for (int e = 0; e < 4; ++e) st[p] = M::mma(kf[e], qf[e], st[p]);
           }
         }
-      float top = kNegBig;
+      float top = kLeast;
 #pragma unroll
       for (int p = 0; p < NS; ++p)
 #pragma unroll
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   for (int idx = threadIdx.x; idx < ROWS * CPR; idx += 64 * WAVES) {
     const int row = idx / CPR, d = 4 * (idx % CPR), r = r0 + row;
     if (r >= n_rows || d >= D) continue;
-    float mx = kNegBig;
+    float mx = kLeast;
 #pragma unroll
     for (int u = 0; u < WAVES; ++u) mx = fmaxf(mx, all[u * L::WAVE + ROWS * L::OS + row]);
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttn a) {
   const TileKeys tk = tile_keys(a, s, ((t - s.tok0) * a.group + h % a.group) / a.rows);
   if (tk.active <= 1) return;
   const long step = (long)c.T * a.hq;
-  float2 ml = make_float2(kNegBig, 0.0f);
+  float2 ml = make_float2(kLeast, 0.0f);
   if (lane < tk.active) ml = a.part_ml[lane * step + at];
   // lanes of a split: a power of two that holds D / 4
   const int lanes = c.D <= 32 ? 8 : c.D <= 64 ? 16 : c.D <= 128 ? 32 : 64;

@@ -94,9 +94,23 @@ __device__ __forceinline__ float wide_largest(const f32x16 (&st)[2]) {
   return top;
 }
 
+// The weight of a score.  The fused form keeps what rounding the product would
+// take off, which is the better value until scores of 2^30 and more leave so much
+// of it that a row's largest weight is far from 1, and leaves fp32: the second walk
+// rounds the product as the reference was rounded.
+template <bool EXACT>
+__device__ __forceinline__ float weight_of(float score, float scale_log2, float reference) {
+  if constexpr (EXACT) {
+#pragma clang fp contract(off)
+    const float scaled = score * scale_log2;
+    return weight(scaled - reference);
+  }
+  return weight(fmaf(score, scale_log2, -reference));
+}
+
 // One tile: its scores st (formed a tile earlier) become weights and meet V,
-// while the next tile's scores are formed into sn.
-template <int DP>
+// while the next tile's scores are formed into sn.  EXACT (second walk): see weight_of.
+template <int DP, bool EXACT>
 __device__ __forceinline__ void wide_step(WideState<DP>& w, f32x16 (&st)[2], f32x16 (&sn)[2],
                                           const unsigned char* __restrict__ kt,
                                           const unsigned char* __restrict__ vt, const int (&koff)[DP / 16],
@@ -119,7 +133,7 @@ __device__ __forceinline__ void wide_step(WideState<DP>& w, f32x16 (&st)[2], f32
   for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      st[kb][e] = weight(fmaf(st[kb][e], scale_log2, -w.m));
+      st[kb][e] = weight_of<EXACT>(st[kb][e], scale_log2, w.m);
       pf[2 * kb + e / 8][e % 8] = (bf16)st[kb][e];
     }
 #pragma unroll
@@ -273,7 +287,7 @@ __global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn
           }
         ws.top = wide_largest(st);
       }
-      wide_step<DP>(ws, st, sn, k_slot(odd ^ 1), v_slot(odd), koff, voff, qf, a.scale_log2);
+      wide_step<DP, careful()>(ws, st, sn, k_slot(odd ^ 1), v_slot(odd), koff, voff, qf, a.scale_log2);
     }
     vmw<0>();
     if constexpr (careful()) look_through(v_slot(odd ^ 1), j + kKeysWide);
@@ -285,9 +299,9 @@ __global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn
     for (int db = 0; db < W::NDB; ++db)
 #pragma unroll
       for (int e = 0; e < 16; ++e) ws.o[db][e] = 0.0f;
-    ws.m = kNegBig;
+    ws.m = kLeast;
     ws.l = 0.0f;
-    ws.top = kNegBig;
+    ws.top = kLeast;
     if (k0 < k1) {
       const int first = look_up(k0);
       v_page = look_up(k0 + kKeysWide);
@@ -310,12 +324,15 @@ __global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn
     }
   };
   walk(std::false_type{});
-  unsigned odd = 0;
+  // not finite, or no weight although the row sees keys (a tile's last row sees
+  // them all, so that nothing in V escapes it)
+  const float first_sum = swap_sum(ws.l, false);
+  unsigned odd = not_finite(first_sum) | not_finite(__builtin_amdgcn_rcpf(first_sum));
 #pragma unroll
   for (int db = 0; db < W::NDB; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) odd |= not_finite(ws.o[db][e]);
-  if (__syncthreads_or(odd != 0 && live)) {
+  if (__syncthreads_or(odd != 0 && limit >= k0)) {
     if (threadIdx.x < kNotedBlocks / 32) notes[threadIdx.x] = 0;
     __syncthreads();
     walk(std::true_type{});
@@ -390,7 +407,7 @@ __global__ __launch_bounds__(256) void cache_join_tiles_kernel(CacheAttn a) {
   for (int r = r0 + threadIdx.x / lanes; r < min(n_rows, r0 + kJoinRows); r += 256 / lanes) {
     const int tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
     const long t = s.tok0 + tok, at = t * a.hq + h;
-    float mx = kNegBig, total = 0.0f;
+    float mx = kLeast, total = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int u0 = 0; u0 < tk.active; u0 += 4) {
       float2 ml[4];

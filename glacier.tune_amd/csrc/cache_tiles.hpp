@@ -11,6 +11,8 @@ namespace glacier {
 constexpr int kMaxSplits = 64;   // one lane each in the join
 constexpr int kSplitUnit = 128;  // splits begin at multiples of it
 
+constexpr float kLeast = -3.402823466e38f;  // where running maxima begin: below every score
+
 // Tiles are numbered through all sequences: sequence b's first one is
 // first_tile(a, b, cu[b]), which leaves room for every tile it can have.
 __device__ inline int first_tile(const CacheAttn& a, int b, int cu) { return cu * a.group / a.rows + b; }

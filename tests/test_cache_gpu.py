@@ -195,6 +195,40 @@ def test_not_finite_keys_reach_only_rows_that_see_them(eng, dt, hq, d, columns):
                 assert rest.isnan().all()
 
 
+@pytest.mark.parametrize("columns", [0, WIDE // 16])
+@pytest.mark.parametrize("power", [0, 12, 17, 54])
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_scores_far_from_zero(eng, dt, power, columns):
+    # q and k times 2^power: but for near ties a row is its best key's value
+    seqs, hq, hkv, d = [(40, 300), (3, 900), (1, 50), (60, 60)], 8, 2, 128
+    p = ch.Paged(seqs, hq, hkv, d, 16, DTYPES[dt], 21, columns=columns)
+    p.k_pages.mul_(2.0 ** power)
+    out, lse = eng.cache_forward((p.q * 2.0 ** power).cuda(), *p.arrays(), save=True)
+    if power == 0:
+        ref = ch.attend_ref(p)
+        ch.check("out", out, ref[0], ref[1])
+        ch.check("lse", lse, ref[2], ref[3])
+        return
+    at, sure = 0, 0
+    for b, (n, kv) in enumerate(seqs):
+        for h in range(hq):
+            q, k = p.q[at:at + n, h].double() * 2.0 ** power, p.k[b][:, h // (hq // hkv)].double() * 2.0 ** power
+            hidden = torch.arange(kv)[None, :] > torch.arange(kv - n, kv)[:, None]
+            score = ((q @ k.T) / math.sqrt(d)).masked_fill(hidden, -math.inf)
+            # an fp32 sum of d products and its scaling, at their largest
+            off = ((q.abs() @ k.abs().T) / math.sqrt(d) * (d + 4) * ch.F).masked_fill(hidden, 0).amax(-1)
+            top = torch.cat([score, torch.full((n, 1), -math.inf)], -1).topk(2, -1)
+            ok = top.values[:, 0] - top.values[:, 1] > 2 * off + 40
+            best = p.v[b][top.indices[:, 0], h // (hq // hkv)].double()
+            # the weight's rounding and the result's
+            ch.check("out", out[at:at + n, h][ok.cuda()], best[ok],
+                     (2 if dt == "bf16" else 4) * ch.half_step(DTYPES[dt]) * best[ok].abs())
+            ch.check("lse", lse[h, at:at + n], top.values[:, 0], off + 4 * ch.F * top.values[:, 0].abs() + 40)
+            sure += int(ok.sum())
+        at += n
+    assert sure >= 0.9 * at * hq
+
+
 def test_lengths_past_the_table(eng):
     # positions the table has no column for hold no key
     p = ch.Paged([(1, 64)], 4, 1, 64, 16, torch.bfloat16, 9)
