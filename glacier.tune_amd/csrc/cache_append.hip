@@ -7,6 +7,10 @@
 // sequence is found by all lanes at once (one load deep: a binary search would
 // chain one per halving), and the first rows are requested before it, since
 // only where they go depends on it.
+//
+// Measured: 16 chunks of up to 512 tokens, 32/8 heads of 128, bf16, 23.1 us (5.7
+// TB/s: the rows were written shortly before and are partly in the last-level
+// cache); 64 sequences of one token 3.4 us in a replayed graph, the launch.
 #include "cache_view.hpp"
 #include "turn.hpp"
 

@@ -9,12 +9,17 @@
 // HBM-bound: each row is read once and written once, a head's sums are one
 // fixed-order reduction over the lanes that hold it (turn.hpp), and queries and
 // keys share the launch.  Each lane reads its pieces before it writes them, so
-// outputs may lie on inputs.
+// outputs may lie on inputs.  Measured: 4096 tokens of 32/8 heads of 128, bf16,
+// 16.3 us (5.1 TB/s: part of it stays in the last-level cache; a 4 GiB copy
+// reaches 4.77); 8 tokens of 28/4 heads 3.9 us in a replayed graph, the launch.
 //
 // Weight gradients: a lane meets the same columns in every head and token, so
 // it sums them in registers; a workgroup's sums go to the workspace and a second
 // launch adds the workgroups in order.  No atomics: results are bitwise
-// repeatable.
+// repeatable.  The backward holds four rows' pieces and four columns' sums a lane,
+// so its pieces are 8 bytes in bf16: with 16 it has registers for half the waves
+// (4096 tokens of 28/4 heads of 128, bf16, with weight gradients: 35 us against
+// 30.8, 3.3 TB/s, of them 4 in the second launch).
 #include "turn.hpp"
 
 namespace glacier {
