@@ -1,6 +1,7 @@
 """The paged key/value cache (glacier_attn_cache_*), through the Python front
 end, against its definition in 64 bits."""
 import math
+import threading
 
 import pytest
 
@@ -84,6 +85,7 @@ CHUNKS = {  # more than 16 rows a KV head: 128-row tiles where the table is wide
     "d136": ([(50, 900)], 6, 3, 136, 32, 0),
     "d248_group_of_16": ([(17, 400), (40, 41)], 16, 1, 248, 64, 0),
     "d120_long": ([(20, 6000)], 10, 2, 120, 512, 0),
+    "d64_group_of_130": ([(3, 700), (1, 40)], 130, 1, 64, 16, 2),  # a token's heads in two tiles
 }
 
 
@@ -459,3 +461,67 @@ def test_two_graphs_of_one_engine_run_side_by_side(eng):
         torch.cuda.synchronize()
         for _, _, got, want, *_ in runs:
             assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("columns", [0, WIDE // 16])
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_sequences_that_share_a_prefix(eng, dt, columns):
+    # the first 64 tokens of both are one set of pages
+    p = ch.Paged([(9, 100), (20, 130)], 8, 2, 64, 16, DTYPES[dt], 23, columns=columns)
+    p.table[1, :4] = p.table[0, :4]
+    for x in (p.k, p.v):
+        x[1][:64] = x[0][:64]
+    ref = ch.attend_ref(p)
+    out, lse = eng.cache_forward(p.q.cuda(), *p.arrays(), save=True)
+    ch.check("out", out, ref[0], ref[1])
+    ch.check("lse", lse, ref[2], ref[3])
+
+
+@pytest.mark.parametrize("columns", [0, WIDE // 16])
+@pytest.mark.parametrize("cu", [[0, 9, 200], [0, 60, 20], [-7, 9, 29], [29, 29, 29], [5, 4, 3]])
+def test_wrong_offsets_stay_in_their_rows(eng, cu, columns):
+    # cu_tokens that no batch has: wrong rows at most, none outside the tensors
+    p = ch.Paged([(9, 100), (20, 130)], 8, 2, 64, 16, torch.bfloat16, 24, columns=columns)
+    bad = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    args = (p.k_pages, p.v_pages, bad, p.kv_lens, p.table)
+    rows = torch.full((3 * p.tokens, 8, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+    lse = torch.full((3, 8, p.tokens), 7.0, device="cuda")
+    own = slice(p.tokens, 2 * p.tokens)
+    q, used = p.q.cuda(), p.both.clone()
+    eng.cache_forward(q, *args, out=rows[own], lse=lse[1])
+    eng.cache_append(q[:, :2].contiguous(), q[:, 2:4].contiguous(), *args, rope_freq_base=1e4, q=q,
+                     q_rot=rows[own])
+    assert (rows[:p.tokens] == 7.0).all() and (rows[2 * p.tokens:] == 7.0).all()
+    assert (lse[0] == 7.0).all() and (lse[2] == 7.0).all()
+    # appended rows lie in the sequences' pages
+    free = torch.ones(p.n_pages, dtype=torch.bool, device="cuda")
+    free[p.table[p.table >= 0].long()] = False
+    assert torch.equal(p.both[free].view(torch.int16), used[free].view(torch.int16))
+
+
+def test_two_engines_from_two_threads():
+    runs, failed = [], []
+    for seed, (seqs, hq, hkv, d) in enumerate((([(1, 4000), (1, 900)], 28, 4, 128), ([(100, 900)], 8, 2, 64))):
+        p = ch.Paged(seqs, hq, hkv, d, 16, torch.bfloat16, 25 + seed)
+        runs.append((ga.GpuAttentionEngine(0, ga.PREC_BF16), torch.cuda.Stream(), p, p.q.cuda()))
+    want = [e.cache_forward(q, *p.arrays())[0] for e, _, p, q in runs]
+    torch.cuda.synchronize()
+
+    def work(i):
+        e, stream, p, q = runs[i]
+        try:
+            with torch.cuda.stream(stream):
+                got = [e.cache_forward(q, *p.arrays())[0] for _ in range(20)]
+                stream.synchronize()
+            assert all(torch.equal(x, want[i]) for x in got)
+        except BaseException as x:  # noqa: BLE001
+            failed.append(x)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for e, *_ in runs:
+        e.close()
+    assert not failed, failed

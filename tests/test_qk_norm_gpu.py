@@ -43,6 +43,7 @@ SHAPES = [  # T, hq, hkv, D, theta, positions below
     (257, 7, 1, 96, None, 9),
     (1, 130, 1, 32, 1e4, 77),
     (9000, 2, 1, 16, 1e4, 9000),
+    (6, 2, 5, 48, 1e4, 300),
 ]
 
 
