@@ -32,14 +32,18 @@ struct Piece {
 };
 
 // cos and sin of pos times pair i's angle.  The number of revolutions is
-// formed and reduced to [-1/2, 1/2] in 64 bits, so the angle is right to fp32
-// rounding wherever pos lies (in fp32 it would be off by pos 2^-24 radians).
+// formed and reduced to [-1/2, 1/2] in 64 bits, so the angle is right wherever
+// pos lies (in fp32 it would be off by pos 2^-24 radians); what rounding it to 32
+// bits leaves turns the result by one more step (fp32 gradients of 333 tokens: off by
+// 8.1e-8, now 7.4e-8; the weights' 1.78e-7, now 1.28e-7).
 __device__ inline float2 turn_of(double rev, int pos) {
   double a = rev * (double)pos;
   a -= rint(a);
+  const float near = (float)a;
+  const float rest = (float)(a - near) * 6.2831853f;
   float s, c;
-  sincospif(2.0f * (float)a, &s, &c);
-  return make_float2(c, s);
+  sincospif(2.0f * near, &s, &c);
+  return make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
 }
 
 // The rates of the pairs whose angles this lane forms.
