@@ -44,8 +44,9 @@
  * bf16 terms (one in large chunks).  fp32 tensors: fp32 throughout.  Results are
  * bitwise repeatable for one layout of the work (below: max_new, max_kv).  NaN
  * and infinities in a token's K or V reach only the rows that see the token.
- * Contexts, status codes and dtypes are those of glacier_attn.h; calls enqueue on the context's stream.  Tensors are 16-byte
- * aligned, q, k, v and out contiguous; head_dim is a multiple of 8 up to 256.
+ * Contexts, status codes and dtypes are those of glacier_attn.h; calls enqueue on
+ * the context's stream.  Tensors are 16-byte aligned, q, k, v and out contiguous;
+ * head_dim is a multiple of 8 up to 256.
  * One call takes fewer than 2^26 rows (tokens times its heads) and 2^21 sequences.
  */
 #ifndef GLACIER_CACHE_H
