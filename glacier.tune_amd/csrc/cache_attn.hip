@@ -20,6 +20,11 @@
 // are bound by the fp32 MFMAs (three of up to 120 tokens over up to 1001 keys, 8/2
 // heads of 96: 23 us, 35 TFLOP/s on 138 of the 256 CUs).
 //
+// KV heads alternate over the workgroups, so that an XCD's L2 serves few of them
+// (fp32, 16 sequences of up to 8000 keys, one token each: 93 -> 70 us; 512 tokens
+// over 4096 keys 375 -> 365; 2 of up to 900 over up to 3000, 8/8 heads of 64: 100 ->
+// 81).
+//
 // A tile's splits write sums and (maximum, sum) to the workspace, and a second
 // launch joins them; a tile with one split writes its result itself.
 //
@@ -95,12 +100,13 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
   const int w = wave_id(), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-  const int kvh = blockIdx.y, split = blockIdx.z, D = c.D;
+  const int kvh = blockIdx.x % c.hkv, split = blockIdx.y, D = c.D;
 
-  const CacheSeq s = seq_of_tile(a, lane, static_cast<int>(blockIdx.x));
+  const int number = static_cast<int>(blockIdx.x / c.hkv);
+  const CacheSeq s = seq_of_tile(a, lane, number);
   const int b = s.b;
   if (b >= c.n_seqs) return;
-  const int tile = static_cast<int>(blockIdx.x) - first_tile(a, b, s.tok0);
+  const int tile = number - first_tile(a, b, s.tok0);
   const int r0 = tile * ROWS, n_rows = s.n * a.group;
   if (tile < 0 || r0 >= n_rows) return;
   const TileKeys tk = tile_keys(a, s, tile);
@@ -476,7 +482,7 @@ hipError_t attend(const CacheAttn& a, hipStream_t st) {
   using L = CaLayout<T, DP, WAVES>;
   auto* fn = &cache_attn_kernel<T, DP, WAVES>;
   GL_CHECK(allow_lds(fn, L::BYTES));
-  hipLaunchKernelGGL((cache_attn_kernel<T, DP, WAVES>), dim3(tile_numbers(a), a.c.hkv, a.n_splits),
+  hipLaunchKernelGGL((cache_attn_kernel<T, DP, WAVES>), dim3(tile_numbers(a) * a.c.hkv, a.n_splits),
                      dim3(64 * WAVES), L::BYTES, st, a);
   return hipGetLastError();
 }

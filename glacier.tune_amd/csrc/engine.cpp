@@ -1509,13 +1509,11 @@ void need_heads_q(const CacheView& c, int hq) {
          "n_heads_q (" + std::to_string(hq) + ") must be a multiple of n_heads_kv (" + std::to_string(c.hkv) + ")");
 }
 // A launch has fewer than 2^32 threads: 64 to a token at most (append), 512 to 16
-// rows of a KV head and to each sequence, 256 to 128 rows and to each sequence and
-// KV head (attention).
+// rows of a KV head and to each sequence and KV head (attention).
 void need_cache_size(const CacheView& c, long long heads) {
   if (c.T * heads >= (1LL << 26)) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
-  if (c.n_seqs >= (1 << 21) || (long long)c.n_seqs * c.hkv >= (1LL << 23))
+  if ((long long)c.n_seqs * c.hkv >= (1LL << 22))
     fail(GLACIER_ATTN_ERR_UNSUPPORTED, "too many sequences");
-  if (c.hkv > 65535) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "more than 65535 KV heads");
 }
 
 void need(const void* p, const char* name) {

@@ -47,7 +47,8 @@
  * Contexts, status codes and dtypes are those of glacier_attn.h; calls enqueue on
  * the context's stream.  Tensors are 16-byte aligned, q, k, v and out contiguous;
  * head_dim is a multiple of 8 up to 256.
- * One call takes fewer than 2^26 rows (tokens times its heads) and 2^21 sequences.
+ * One call takes fewer than 2^26 rows (tokens times its heads) and 2^22
+ * sequences times KV heads.
  */
 #ifndef GLACIER_CACHE_H
 #define GLACIER_CACHE_H
