@@ -5,20 +5,21 @@
 // token r / group, head r % group.  One new token of 7 heads and a long chunk
 // are then the same product, and K and V are read once per tile, not per head.
 //
-// A workgroup takes one tile of 16 rows of one KV head, and one split of the
+// A workgroup takes one tile of 16 or 32 rows of one KV head, and one split of the
 // keys the tile sees.  Its waves (four; eight in fp32 up to 128 columns) take keys
 // in turn, KB at a time, each with its own LDS tiles and its own running maximum
 // and sum of the softmax, so the loop has no barrier; the waves are joined
-// through LDS at the end.  Scores are
-// formed transposed (S^T = K Q^T, attn_common.hpp), which leaves a lane with
+// through LDS at the end.  Scores are formed
+// transposed (S^T = K Q^T, attn_common.hpp), which leaves a lane with
 // one row's weights and feeds them to O^T += V^T P^T as they are.
 //
 // Bound by reading K and V for single tokens: one over 65536 keys, 32/8 heads of
 // 128, bf16, 57.4 us (4.67 TB/s of the 4.77 of a large copy); 32 sequences of up to
 // 8192 keys, 28/4 heads, 65-67 us (4.1 TB/s, uneven splits); one over 512 keys, 14/2
 // heads of 64, 6.8 us: four dependent loads and four blocks of keys.  fp32 chunks
-// are bound by the fp32 MFMAs (three of up to 120 tokens over up to 1001 keys, 8/2
-// heads of 96: 23 us, 35 TFLOP/s on 138 of the 256 CUs).
+// are bound by the fp32 MFMAs and by tiles of uneven length (1024 tokens over 8192 keys,
+// 8/2 heads of 96: 225 us, 107 TFLOP/s of the 154 of a large library product; three of
+// up to 120 over up to 1001: 23 us, on 138 of the 256 CUs).
 //
 // KV heads alternate over the workgroups, so that an XCD's L2 serves few of them
 // (fp32, 16 sequences of up to 8000 keys, one token each: 93 -> 70 us; 512 tokens
@@ -47,14 +48,13 @@ struct KeyBlock<float> {
   static constexpr int KB = 16;  // two blocks of 256 columns and their copies fit the LDS
 };
 
-template <typename T, int DP, int WAVES>
+template <typename T, int DP, int MB, int WAVES>
 struct CaLayout {
   static constexpr int KB = KeyBlock<T>::KB;
   static constexpr int S = Lds<T, DP>::STRIDE;
   static constexpr int TILES = WAVES * 2 * KB * S * static_cast<int>(sizeof(T));
   static constexpr int OS = DP + 4;  // row stride (floats) of a wave's sums in the join
-  static constexpr int ROWS = 16;
-  static constexpr int WAVE = ROWS * (OS + 2);  // sums, maxima, totals
+  static constexpr int WAVE = 16 * MB * (OS + 2);  // sums, maxima, totals
   static constexpr int JOIN = WAVES * WAVE * 4;
   static constexpr int NOTES = TILES > JOIN ? TILES : JOIN;  // then the noted blocks of each wave
   static constexpr int BYTES = NOTES + WAVES * kNotedBlocks / 8;
@@ -91,51 +91,63 @@ struct BlockRegs {
   }
 };
 
-template <typename T, int DP, int WAVES>
+template <typename T, int DP, int MB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   using M = Mfma<T>;
-  using L = CaLayout<T, DP, WAVES>;
-  constexpr int KB = L::KB, NS = KB / 16, ROWS = L::ROWS;
+  using L = CaLayout<T, DP, MB, WAVES>;
+  constexpr int KB = L::KB, NS = KB / 16, ROWS = 16 * MB;
   constexpr int NW = DP * sizeof(T) / 64;  // 16-byte words a lane holds of a row
   extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
   const int w = wave_id(), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int kvh = blockIdx.x % c.hkv, split = blockIdx.y, D = c.D;
-
   const int number = static_cast<int>(blockIdx.x / c.hkv);
-  const CacheSeq s = seq_of_tile(a, lane, number);
+  int tile;
+  CacheSeq s;
+  if (a.long_first) {
+    s = seq_of_long_tile(a, lane, number, static_cast<int>(gridDim.x / c.hkv), tile);
+  } else {
+    s = seq_of_tile(a, lane, number);
+    tile = number - first_tile(a, s.b, s.tok0);
+  }
   const int b = s.b;
   if (b >= c.n_seqs) return;
-  const int tile = number - first_tile(a, b, s.tok0);
   const int r0 = tile * ROWS, n_rows = s.n * a.group;
   if (tile < 0 || r0 >= n_rows) return;
   const TileKeys tk = tile_keys(a, s, tile);
   if (split >= tk.active) return;
   const int k0 = split * tk.per, k1 = min(tk.kend, k0 + tk.per);
 
-  // this lane's row: operand fragments and last key
-  i32x4 qw[NW];
+  // this lane's rows (one per 16-row block): operand fragments and last key
+  i32x4 qw[MB][NW];
+  int limit[MB];
   // the first of the 16 bytes of columns that this lane holds in word x of a
   // row of Q or K: one k-step's 8 columns in bf16; in fp32, where a k-step takes
   // one column a lane, those of four steps (step 4 x + e takes column
   // 16 x + 4 g + e: a dot product may take its terms in any order)
   auto first_col = [&](int x) { return sizeof(T) == 2 ? 32 * x + 8 * g : 16 * x + 4 * g; };
-  const int r = r0 + col, tok = r / a.group;
-  const int limit = r < n_rows ? s.pos0 + tok : -1;
-  // (loaded from the tile's first row where there is none, and cleared after
-  // all loads are under way)
-  const T* const q = static_cast<const T*>(a.q) +
-                     (r < n_rows ? (long)(s.tok0 + tok) * a.hq + kvh * a.group + (r - tok * a.group)
-                                 : (long)(s.tok0 + r0 / a.group) * a.hq) * D;
 #pragma unroll
-  for (int x = 0; x < NW; ++x)
-    qw[x] = *reinterpret_cast<const i32x4*>(q + (first_col(x) < D ? first_col(x) : 0));
+  for (int mb = 0; mb < MB; ++mb) {
+    const int r = r0 + 16 * mb + col;
+    const int i = r / a.group, h = kvh * a.group + (r - i * a.group);
+    const bool ok = r < n_rows;
+    limit[mb] = ok ? s.pos0 + i : -1;
+    // (loaded from the tile's first row where there is none, and cleared after
+    // all loads are under way)
+    const T* q = static_cast<const T*>(a.q) +
+                 (ok ? (long)(s.tok0 + i) * a.hq + h : (long)(s.tok0 + r0 / a.group) * a.hq) * D;
 #pragma unroll
-  for (int x = 0; x < NW; ++x)
-    if (limit < 0 || first_col(x) >= D) qw[x] = i32x4{0, 0, 0, 0};
+    for (int x = 0; x < NW; ++x)
+      qw[mb][x] = *reinterpret_cast<const i32x4*>(q + (first_col(x) < D ? first_col(x) : 0));
+  }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int x = 0; x < NW; ++x)
+      if (limit[mb] < 0 || first_col(x) >= D) qw[mb][x] = i32x4{0, 0, 0, 0};
 
-  f32x4 acc[DP / 16];
-  float m, l;
+  f32x4 acc[MB][DP / 16];
+  float m[MB], l[MB];
 
   T* const kt = reinterpret_cast<T*>(smem) + w * 2 * KB * L::S;
   T* const vt = kt + KB * L::S;
@@ -176,10 +188,13 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   unsigned* const notes = reinterpret_cast<unsigned*>(smem + L::NOTES) + w * (kNotedBlocks / 32);
   auto note_of = [&](int j) { return (j - k0) / (WAVES * KB) % kNotedBlocks; };
   auto walk = [&](auto careful) __attribute__((always_inline)) {
-    m = kLeast;
-    l = 0.0f;
 #pragma unroll
-    for (int db = 0; db < DP / 16; ++db) acc[db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int mb = 0; mb < MB; ++mb) {
+      m[mb] = kLeast;
+      l[mb] = 0.0f;
+#pragma unroll
+      for (int db = 0; db < DP / 16; ++db) acc[mb][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     int j = k0 + w * KB;
     if (j < k1) {
       look_up(j);
@@ -205,63 +220,73 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
       wave_lds_order();
       if (j + WAVES * KB < k1) fetch(j + WAVES * KB);
       // S^T: keys 16 p + 4 g + r of this block, row col of each 16-row block
-      f32x4 st[NS];
+      f32x4 st[MB][NS];
 #pragma unroll
-      for (int p = 0; p < NS; ++p) st[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int p = 0; p < NS; ++p) st[mb][p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int p = 0; p < NS; ++p)
 #pragma unroll
         for (int x = 0; x < NW; ++x) {
           const i32x4 kw = *reinterpret_cast<const i32x4*>(kt + (16 * p + col) * L::S + first_col(x));
-          if constexpr (sizeof(T) == 2) {
-            st[p] = M::mma(__builtin_bit_cast(bf16x8, kw), __builtin_bit_cast(bf16x8, qw[x]), st[p]);
-          } else {
-            const f32x4 kf = __builtin_bit_cast(f32x4, kw), qf = __builtin_bit_cast(f32x4, qw[x]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st[p] = M::mma(kf[e], qf[e], st[p]);
+          for (int mb = 0; mb < MB; ++mb) {
+            if constexpr (sizeof(T) == 2) {
+              st[mb][p] = M::mma(__builtin_bit_cast(bf16x8, kw), __builtin_bit_cast(bf16x8, qw[mb][x]), st[mb][p]);
+            } else {
+              const f32x4 kf = __builtin_bit_cast(f32x4, kw), qf = __builtin_bit_cast(f32x4, qw[mb][x]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) st[mb][p] = M::mma(kf[e], qf[e], st[mb][p]);
+            }
           }
         }
-      float top = kLeast;
 #pragma unroll
-      for (int p = 0; p < NS; ++p)
+      for (int mb = 0; mb < MB; ++mb) {
+        float top = kLeast;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = st[p][r] * a.scale_log2;
-          if (!whole) {
-            const int at = 4 * g + r;
-            x = at < here[p] && j + 16 * p + at <= limit ? x : -INFINITY;
+        for (int p = 0; p < NS; ++p)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float x = st[mb][p][r] * a.scale_log2;
+            if (!whole) {
+              const int at = 4 * g + r;
+              x = at < here[p] && j + 16 * p + at <= limit[mb] ? x : -INFINITY;
+            }
+            st[mb][p][r] = x;
+            top = fmaxf(top, x);
           }
-          st[p][r] = x;
-          top = fmaxf(top, x);
-        }
-      const float mn = fmaxf(m, col_max_swap(top));
-      const float alpha = weight(m - mn);
-      m = mn;
-      float sum = 0.0f;
+        const float mn = fmaxf(m[mb], col_max_swap(top));
+        const float alpha = weight(m[mb] - mn);
+        m[mb] = mn;
+        float sum = 0.0f;
 #pragma unroll
-      for (int p = 0; p < NS; ++p)
+        for (int p = 0; p < NS; ++p)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float e = weight(st[p][r] - mn);
-          st[p][r] = e;
-          sum += e;
-        }
-      l = l * alpha + sum;
+          for (int r = 0; r < 4; ++r) {
+            const float e = weight(st[mb][p][r] - mn);
+            st[mb][p][r] = e;
+            sum += e;
+          }
+        l[mb] = l[mb] * alpha + sum;
 #pragma unroll
-      for (int db = 0; db < DP / 16; ++db)
+        for (int db = 0; db < DP / 16; ++db)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[db][r] *= alpha;
+          for (int r = 0; r < 4; ++r) acc[mb][db][r] *= alpha;
+      }
       // O^T += V^T P^T; in bf16 each weight in two terms, which leaves 16 bits of
       // it: reading V bounds these calls, and one term would add as much error as
       // the result's own rounding
       if constexpr (sizeof(T) == 2) {
-        bf16x8 hi, lo;
+        bf16x8 hi[MB], lo[MB];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = st[e < 4 ? 0 : NS - 1][e % 4];
-          hi[e] = (bf16)p;
-          lo[e] = (bf16)(p - (float)hi[e]);
-        }
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float p = st[mb][e < 4 ? 0 : NS - 1][e % 4];
+            hi[mb][e] = (bf16)p;
+            lo[mb][e] = (bf16)(p - (float)hi[mb][e]);
+          }
         // (two blocks at a time: a product waits for the one before it on its sums)
 #pragma unroll
         for (int db = 0; db < DP / 16; db += 2) {
@@ -270,9 +295,12 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
           for (int x = 0; x < 2; ++x)
             vf[x] = join8(read_tr<L::S>(vt, 0, 16 * (db + x), lane), read_tr<L::S>(vt, 16, 16 * (db + x), lane));
 #pragma unroll
-          for (int x = 0; x < 2; ++x) acc[db + x] = M::mma(vf[x], lo, acc[db + x]);
+          for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) acc[db + x] = M::mma(vf[x], hi, acc[db + x]);
+            for (int x = 0; x < 2; ++x) acc[mb][db + x] = M::mma(vf[x], lo[mb], acc[mb][db + x]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) acc[mb][db + x] = M::mma(vf[x], hi[mb], acc[mb][db + x]);
+          }
         }
       } else {
         // V in wide reads: row i of the four blocks 4 x .. 4 x + 3 is column
@@ -284,12 +312,18 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
           for (int x = 0; x < DP / 64; ++x) {
             const f32x4 vf = *reinterpret_cast<const f32x4*>(vrow + 64 * x + 4 * col);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[4 * x + e] = M::mma(vf[e], st[0][r], acc[4 * x + e]);
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int mb = 0; mb < MB; ++mb)
+                acc[mb][4 * x + e] = M::mma(vf[e], st[mb][0][r], acc[mb][4 * x + e]);
           }
           if constexpr (DP % 64 != 0) {
             const float2 vf = *reinterpret_cast<const float2*>(vrow + DP / 64 * 64 + 2 * col);
-            acc[DP / 16 - 2] = M::mma(vf.x, st[0][r], acc[DP / 16 - 2]);
-            acc[DP / 16 - 1] = M::mma(vf.y, st[0][r], acc[DP / 16 - 1]);
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+              acc[mb][DP / 16 - 2] = M::mma(vf.x, st[mb][0][r], acc[mb][DP / 16 - 2]);
+              acc[mb][DP / 16 - 1] = M::mma(vf.y, st[mb][0][r], acc[mb][DP / 16 - 1]);
+            }
           }
         }
       }
@@ -298,9 +332,11 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   walk(std::false_type{});
   unsigned odd = 0;
 #pragma unroll
-  for (int db = 0; db < DP / 16; ++db)
+  for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) odd |= limit >= 0 ? not_finite(acc[db][r]) : 0;
+    for (int db = 0; db < DP / 16; ++db)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) odd |= limit[mb] >= 0 ? not_finite(acc[mb][db][r]) : 0;
   if (__any(odd != 0)) {
     if (lane < kNotedBlocks / 32) notes[lane] = 0;
     wave_lds_order();
@@ -313,13 +349,17 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
         if (page < 0) continue;
         const char* const v = static_cast<const char*>(c.v_pages) + page * strideb + head +
                               (key & ((1 << c.page_shift) - 1)) * rowb;
-        const unsigned sees = key <= limit ? ~0u : 0u;
+        unsigned sees[MB];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) sees[mb] = key <= limit[mb] ? ~0u : 0u;
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
           for (int db = 0; db < DP / 16; ++db) {
             const bf16x4 x = __builtin_bit_cast(bf16x4, load8_within(v, rowb, 2 * (16 * db + 4 * g)));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[db][r] += given_back((float)x[r], sees);
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int mb = 0; mb < MB; ++mb) acc[mb][db][r] += given_back((float)x[r], sees[mb]);
           }
         } else {
 #pragma unroll
@@ -328,13 +368,18 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
             for (int x = 0; x < DP / 64; ++x) {
               const f32x4 f = __builtin_bit_cast(f32x4, load_within(v, rowb, 4 * (64 * x + 16 * g + 4 * r)));
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[4 * x + e][r] += given_back(f[e], sees);
+              for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb) acc[mb][4 * x + e][r] += given_back(f[e], sees[mb]);
             }
             if constexpr (DP % 64 != 0) {
               const float2 f =
                   __builtin_bit_cast(float2, load8_within(v, rowb, 4 * (DP / 64 * 64 + 8 * g + 2 * r)));
-              acc[DP / 16 - 2][r] += given_back(f.x, sees);
-              acc[DP / 16 - 1][r] += given_back(f.y, sees);
+#pragma unroll
+              for (int mb = 0; mb < MB; ++mb) {
+                acc[mb][DP / 16 - 2][r] += given_back(f.x, sees[mb]);
+                acc[mb][DP / 16 - 1][r] += given_back(f.y, sees[mb]);
+              }
             }
           }
         }
@@ -345,29 +390,33 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   // join the waves: region of wave u: sums [ROWS][OS], maxima [ROWS], totals [ROWS]
   __syncthreads();
   float* const mine = reinterpret_cast<float*>(smem) + w * L::WAVE;
-  const float total = col_sum_swap(l);
-  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int db = 0; db < DP / 16; ++db)
-      store4(mine + col * L::OS + 16 * db + 4 * g, acc[db]);
-  } else {
+  for (int mb = 0; mb < MB; ++mb) {
+    const float total = col_sum_swap(l[mb]);
+    const int row = 16 * mb + col;
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+      for (int db = 0; db < DP / 16; ++db)
+        store4(mine + row * L::OS + 16 * db + 4 * g, acc[mb][db]);
+    } else {
 #pragma unroll
-      for (int x = 0; x < DP / 64; ++x) {
-        f32x4 v;
+      for (int r = 0; r < 4; ++r) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[4 * x + e][r];
-        store4(mine + col * L::OS + 64 * x + 16 * g + 4 * r, v);
+        for (int x = 0; x < DP / 64; ++x) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[mb][4 * x + e][r];
+          store4(mine + row * L::OS + 64 * x + 16 * g + 4 * r, v);
+        }
+        if constexpr (DP % 64 != 0)
+          *reinterpret_cast<float2*>(mine + row * L::OS + DP / 64 * 64 + 8 * g + 2 * r) =
+              make_float2(acc[mb][DP / 16 - 2][r], acc[mb][DP / 16 - 1][r]);
       }
-      if constexpr (DP % 64 != 0)
-        *reinterpret_cast<float2*>(mine + col * L::OS + DP / 64 * 64 + 8 * g + 2 * r) =
-            make_float2(acc[DP / 16 - 2][r], acc[DP / 16 - 1][r]);
     }
-  }
-  if (g == 0) {
-    mine[ROWS * L::OS + col] = m;
-    mine[ROWS * (L::OS + 1) + col] = total;
+    if (g == 0) {
+      mine[ROWS * L::OS + row] = m[mb];
+      mine[ROWS * (L::OS + 1) + row] = total;
+    }
   }
   __syncthreads();
   const float* const all = reinterpret_cast<const float*>(smem);
@@ -477,12 +526,12 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttn a) {
     a.lse[(long)h * c.T + t] = total == 0.0f ? -INFINITY : (mx + log2f(total)) * kLn2;
 }
 
-template <typename T, int DP, int WAVES>
+template <typename T, int DP, int MB, int WAVES>
 hipError_t attend(const CacheAttn& a, hipStream_t st) {
-  using L = CaLayout<T, DP, WAVES>;
-  auto* fn = &cache_attn_kernel<T, DP, WAVES>;
+  using L = CaLayout<T, DP, MB, WAVES>;
+  auto* fn = &cache_attn_kernel<T, DP, MB, WAVES>;
   GL_CHECK(allow_lds(fn, L::BYTES));
-  hipLaunchKernelGGL((cache_attn_kernel<T, DP, WAVES>), dim3(tile_numbers(a) * a.c.hkv, a.n_splits),
+  hipLaunchKernelGGL((cache_attn_kernel<T, DP, MB, WAVES>), dim3(tile_numbers(a) * a.c.hkv, a.n_splits),
                      dim3(64 * WAVES), L::BYTES, st, a);
   return hipGetLastError();
 }
@@ -498,15 +547,22 @@ hipError_t join(const CacheAttn& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// 32 rows a tile: fp32 chunks of heads of 65 .. 128 (cache_attn_plan)
+constexpr int kRowsMid = 32;
+
 template <typename T>
 hipError_t by_head(const CacheAttn& a, hipStream_t st) {
   constexpr int WAVES = sizeof(T) == 2 ? 4 : 8;
   const int d = a.c.D;
-  if (d <= 32) return attend<T, 32, WAVES>(a, st);
-  if (d <= 64) return attend<T, 64, WAVES>(a, st);
-  if (d <= 96) return attend<T, 96, WAVES>(a, st);
-  if (d <= 128) return attend<T, 128, WAVES>(a, st);
-  return attend<T, 256, 4>(a, st);  // eight waves' fp32 tiles exceed the LDS
+  if constexpr (sizeof(T) == 4) {
+    if (a.rows == kRowsMid && d <= 96) return attend<T, 96, 2, WAVES>(a, st);
+    if (a.rows == kRowsMid) return attend<T, 128, 2, WAVES>(a, st);
+  }
+  if (d <= 32) return attend<T, 32, 1, WAVES>(a, st);
+  if (d <= 64) return attend<T, 64, 1, WAVES>(a, st);
+  if (d <= 96) return attend<T, 96, 1, WAVES>(a, st);
+  if (d <= 128) return attend<T, 128, 1, WAVES>(a, st);
+  return attend<T, 256, 1, 4>(a, st);  // eight waves' fp32 tiles exceed the LDS
 }
 
 }  // namespace
@@ -531,7 +587,22 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   // 512 tokens over 2048 (134e6) 40.4, 41.7; 1024 over 8192 (1e9) 260, 121.
   const bool wide = c.io_bf16 && longest * group > 16 &&
                     (double)tiles_of(16) * c.hkv * keys * c.D > (c.D <= 128 ? 25e6 : 100e6);
-  p.rows = wide ? kCacheWideRows : 16;
+  // fp32 chunks: tiles of 32 rows read K and V half as often, from 65 columns on (fewer
+  // leave too few tiles), up to 128 (their sums fill the registers).  us a call, 16
+  // and 32 rows: 512 tokens over 4096 keys, 28/4 heads of 128, 362, 303; 1024 over
+  // 8192, 8/2 of 96, 256, 225; 8 chunks of up to 64 over up to 4000, 32/8 of 128, 229,
+  // 212; 6 of up to 30 over up to 4000, 12/2 of 128, 55, 50; 4 of up to 300 over up to
+  // 4000, 14/2 of 64, 98, 112; 2 of up to 900 over up to 3000, 8/8 of 64, 81, 90; 4 of
+  // up to 300 over up to 4000, 8/2 of 256, 352, 391.  Not where they leave CUs idle
+  // even in splits: 3 of up to 120 over up to 1001, 8/2 of 96 (54 tiles) 23, 36.
+  const bool chunk = !c.io_bf16 && longest * group > 16;
+  const long narrow_splits = keys <= 1024 ? 1 : keys / 512;
+  const bool mid = chunk && c.D > 64 && c.D <= 128 && tiles_of(kRowsMid) * c.hkv * narrow_splits >= n_cu;
+  p.rows = wide ? kCacheWideRows : mid ? kRowsMid : 16;
+  // and their long tiles first: 1000 tokens as they come, 40/8 heads of 128, 148 -> 136
+  // us; 8 chunks of up to 64 as above 229 -> 212; 4 of up to 300, 14/2 of 64, 105 -> 98
+  // (2 of up to 900, 8/8 of 64, 81 -> 85); bf16 single tokens lose 1 of 67.
+  p.long_first = chunk;
   const long groups = tiles_of(p.rows) * c.hkv;
   // Splits of 512 keys or more, as many as fill the workgroups the CUs hold at
   // once (by their LDS); none up to 1024 keys, where the second launch costs
@@ -553,8 +624,8 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   // to 4096 (320) 90, 88, 100; 3 of up to 300 over up to 5000 (132) 94, 80, 69.
   const long per_cu = wide ? (c.D <= 128 ? 2 : 1) : !c.io_bf16 ? 1 : c.D <= 64 ? 4 : c.D <= 128 ? 2 : 1;
   const long want = per_cu * n_cu / groups;
-  const long least = !wide ? 512 : groups < 64 ? 256 : groups < 256 ? 512 : 2048;
-  const long most = keys <= (wide ? 512 : 1024) ? 1 : keys / least;
+  const long least = groups < 64 ? 256 : groups < 256 ? 512 : 2048;
+  const long most = !wide ? narrow_splits : keys <= 512 ? 1 : keys / least;
   const long cap_splits = wide && (long)c.T * hq > kCacheJoinRows ? kCacheTileJoin : kMaxSplits;
   p.n_splits = static_cast<int>(std::max(1L, std::min({want, most, cap_splits})));
   const long even = (keys + p.n_splits - 1) / p.n_splits;

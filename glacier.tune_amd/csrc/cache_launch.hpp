@@ -66,6 +66,7 @@ struct CacheAttn {
   void* out;
   float* lse;     // or null
   int rows;       // rows of a tile: the kernel variant
+  bool long_first;  // tiles of long sequences come first
   int n_splits;   // key splits a tile may take (1: no workspace)
   int split_keys;  // keys of a split, unless a sequence needs more for n_splits of them
   float* part_o;  // [n_splits][T hq][D]
@@ -74,6 +75,7 @@ struct CacheAttn {
 // How a call is laid out, from what the host knows (cache_attn.hip).
 struct CachePlan {
   int rows, n_splits, split_keys;
+  bool long_first;
   size_t bytes;  // workspace
 };
 CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, int n_cu);

@@ -1961,6 +1961,7 @@ int glacier_attn_cache_forward(glacier_attn_ctx* ctx, const glacier_kv_cache* ca
     a.scale_log2 = glacier::kLog2e / std::sqrt(static_cast<float>(a.c.D));
     a.q = q; a.out = out; a.lse = lse;
     a.rows = p.rows;
+    a.long_first = p.long_first;
     a.n_splits = p.n_splits;
     a.split_keys = p.split_keys;
     if (p.n_splits > 1) {

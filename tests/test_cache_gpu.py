@@ -104,6 +104,21 @@ def test_chunks_in_every_layout(eng, name, keys):
     assert not pad or ((out[-pad:] == 7.0).all() and (lse[:, -pad:] == 7.0).all())
 
 
+@pytest.mark.parametrize("keys", [800, 1500, WIDE])
+@pytest.mark.parametrize("name", sorted(CHUNKS))
+def test_fp32_chunks_in_every_layout(eng, name, keys):
+    # tiles of 16 and of 32 rows, whole and in splits, in order and longest first
+    seqs, hq, hkv, d, page, pad = CHUNKS[name]
+    p = ch.Paged(seqs, hq, hkv, d, page, torch.float32, 16, pad, columns=WIDE // page)
+    out = torch.full((p.tokens, hq, d), 7.0, device="cuda")
+    lse = torch.full((hq, p.tokens), 7.0, device="cuda")
+    ref = ch.attend_ref(p)
+    eng.cache_forward(p.q.cuda(), *p.arrays(), max_kv=keys, out=out, lse=lse)
+    ch.check("out", out, ref[0], ref[1])
+    ch.check("lse", lse, ref[2], ref[3])
+    assert not pad or ((out[-pad:] == 7.0).all() and (lse[:, -pad:] == 7.0).all())
+
+
 @pytest.mark.parametrize("dt", sorted(DTYPES))
 def test_wrong_hints_change_nothing_but_the_layout(eng, dt):
     p = ch.Paged([(70, 400), (1, 2500)], 8, 2, 128, 16, DTYPES[dt], 6)
