@@ -24,7 +24,12 @@
 // KV heads alternate over the workgroups, so that an XCD's L2 serves few of them
 // (fp32, 16 sequences of up to 8000 keys, one token each: 93 -> 70 us; 512 tokens
 // over 4096 keys 375 -> 365; 2 of up to 900 over up to 3000, 8/8 heads of 64: 100 ->
-// 81).
+// 81).  In bf16 the splits of a tile alternate first, each tile's from another one
+// on: an XCD then gets long and short tiles, first and last splits alike (single
+// tokens: 24 sequences of up to 8000 keys, 32/8 heads of 128, 100 -> 93; 32 of up to
+// 8192, 28/4, 67.7 -> 65.1).  fp32, with one workgroup a CU, loses by it where an XCD
+// gets one more than it has CUs (6 chunks of up to 30 over up to 4000, 12/2 heads of
+// 128: 50 -> 71).
 //
 // A tile's splits write sums and (maximum, sum) to the workspace, and a second
 // launch joins them; a tile with one split writes its result itself.
@@ -100,12 +105,21 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
   const int w = wave_id(), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-  const int kvh = blockIdx.x % c.hkv, split = blockIdx.y, D = c.D;
-  const int number = static_cast<int>(blockIdx.x / c.hkv);
+  const int D = c.D, numbers = static_cast<int>(gridDim.x / (a.n_splits * c.hkv));
+  int kvh, split, number;
+  if constexpr (sizeof(T) == 2) {
+    kvh = blockIdx.x / a.n_splits % c.hkv;
+    number = blockIdx.x / (a.n_splits * c.hkv);
+    split = (blockIdx.x + number) % a.n_splits;
+  } else {
+    kvh = blockIdx.x % c.hkv;
+    number = blockIdx.x / c.hkv % numbers;
+    split = blockIdx.x / (c.hkv * numbers);
+  }
   int tile;
   CacheSeq s;
   if (a.long_first) {
-    s = seq_of_long_tile(a, lane, number, static_cast<int>(gridDim.x / c.hkv), tile);
+    s = seq_of_long_tile(a, lane, number, numbers, tile);
   } else {
     s = seq_of_tile(a, lane, number);
     tile = number - first_tile(a, s.b, s.tok0);
@@ -531,7 +545,7 @@ hipError_t attend(const CacheAttn& a, hipStream_t st) {
   using L = CaLayout<T, DP, MB, WAVES>;
   auto* fn = &cache_attn_kernel<T, DP, MB, WAVES>;
   GL_CHECK(allow_lds(fn, L::BYTES));
-  hipLaunchKernelGGL((cache_attn_kernel<T, DP, MB, WAVES>), dim3(tile_numbers(a) * a.c.hkv, a.n_splits),
+  hipLaunchKernelGGL((cache_attn_kernel<T, DP, MB, WAVES>), dim3(tile_numbers(a) * a.c.hkv * a.n_splits),
                      dim3(64 * WAVES), L::BYTES, st, a);
   return hipGetLastError();
 }
@@ -627,7 +641,8 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   const long least = groups < 64 ? 256 : groups < 256 ? 512 : 2048;
   const long most = !wide ? narrow_splits : keys <= 512 ? 1 : keys / least;
   const long cap_splits = wide && (long)c.T * hq > kCacheJoinRows ? kCacheTileJoin : kMaxSplits;
-  p.n_splits = static_cast<int>(std::max(1L, std::min({want, most, cap_splits})));
+  const long launch = (1L << 22) / ((long)c.n_seqs * c.hkv);  // threads of a launch, with idle sequences
+  p.n_splits = static_cast<int>(std::max(1L, std::min({want, most, cap_splits, launch})));
   const long even = (keys + p.n_splits - 1) / p.n_splits;
   p.split_keys = static_cast<int>((even + kSplitUnit - 1) / kSplitUnit * kSplitUnit);
   if (p.n_splits > 1) {
