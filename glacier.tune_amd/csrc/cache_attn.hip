@@ -15,7 +15,7 @@
 //
 // Bound by reading K and V for single tokens: one over 65536 keys, 32/8 heads of
 // 128, bf16, 57.4 us (4.67 TB/s of the 4.77 of a large copy); 32 sequences of up to
-// 8192 keys, 28/4 heads, 65-67 us (4.1 TB/s, uneven splits); one over 512 keys, 14/2
+// 8192 keys, 28/4 heads, 64-65 us (4.3 TB/s, uneven splits); one over 512 keys, 14/2
 // heads of 64, 6.8 us: four dependent loads and four blocks of keys.  fp32 chunks
 // are bound by the fp32 MFMAs and by tiles of uneven length (1024 tokens over 8192 keys,
 // 8/2 heads of 96: 225 us, 107 TFLOP/s of the 154 of a large library product; three of
