@@ -12,9 +12,11 @@
 // Scores are formed transposed: S^T = K Q^T leaves a lane with 16 keys of one
 // row in each accumulator block, and elements 8 s .. 8 s + 7 are the k-slots of
 // step s of O^T += V^T P^T, whose V operand comes from two transposing LDS
-// reads (the accumulator layout is described in attn_bwd3.hip).  Each weight is
-// rounded to bf16 (a second term, as in the 16-row kernel, would cost a quarter
-// of the products here); the sum takes them unrounded.
+// reads (the accumulator layout is described in attn_bwd3.hip).  Each weight
+// multiplies V as two bf16 terms, as in the 16-row kernel: a token's result is as
+// good beside a long chunk as alone (2048 tokens as below, off from 64 bits by
+// 0.0017 of the result, the rounding of bf16 itself; one term leaves 0.0024 in
+// 223-231 us, two 0.0017 in 304-314).  The sum takes the weights unrounded.
 //
 // The running maximum is only followed where it has grown by more than 8 (in
 // log2): until then weights are taken against the old one, at most 2^8 large,
@@ -25,11 +27,12 @@
 // them, and the tiles of long sequences start first (eight ragged chunks: 117 ->
 // 94 us).
 //
-// Measured: 2048 tokens over 8192 keys, 28/4 heads of 128: 221-231 us (950-910
-// TFLOP/s; a library product of 8192^3 reaches 1205 on the card).  MFMAs are
-// busy 54% of the time of a CU with two workgroups, vector instructions nearly
-// all of the rest; tiles of 448 workgroups on 256 CUs leave an eighth of them
-// idle.  Tried and slower: tiles through registers (278 us), 256 rows on eight
+// Measured: 2048 tokens over 8192 keys, 28/4 heads of 128: 304-314 us (690-670
+// TFLOP/s, 1035 with the second terms' products; a library product of 8192^3
+// reaches 1205 on the card).  Counters, in 1.95 GHz cycles: MFMAs busy 48%, vector
+// instructions issuing 37%, waves that could issue and wait for the other's
+// instruction 42% of their cycles; tiles of 448 workgroups on 512 places leave an
+// eighth of the card idle.  Tried and slower (with one term, then at 221-231): tiles through registers (278 us), 256 rows on eight
 // waves (295), lines asked for two tiles ahead (245), equal shares of all tiles' steps for every workgroup with
 // fragments joined afterwards (278: the workgroups lose each other's L2 lines),
 // scheduling hints of the compiler (235-281).
@@ -74,7 +77,7 @@ struct WideState {
 };
 
 template <int DP>
-__device__ __forceinline__ void wide_scores(f32x16 (&st)[2], const unsigned char* kt, const int (&koff)[DP / 16],
+__device__ __forceinline__ void wide_scores(f32x16 (&st)[2], const unsigned char* kt, int koff,
                                             const bf16x8 (&qf)[DP / 16]) {
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb)
@@ -84,7 +87,7 @@ __device__ __forceinline__ void wide_scores(f32x16 (&st)[2], const unsigned char
   for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
-      st[kb] = mma16(*reinterpret_cast<const bf16x8*>(kt + koff[kk] + kb * 32 * 2 * DP), qf[kk], st[kb]);
+      st[kb] = mma16(*reinterpret_cast<const bf16x8*>(kt + (koff ^ 32 * kk) + kb * 32 * 2 * DP), qf[kk], st[kb]);
 }
 
 __device__ __forceinline__ float wide_largest(const f32x16 (&st)[2]) {
@@ -108,14 +111,27 @@ __device__ __forceinline__ float weight_of(float score, float scale_log2, float 
   return weight(fmaf(score, scale_log2, -reference));
 }
 
+// Two values rounded to bf16, the first in the lower half.
+__device__ __forceinline__ unsigned pair16(float a, float b) {
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, bf16x2{(bf16)a, (bf16)b});
+}
+// Only scalar instructions are moved past it.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(4); }
+
 // One tile: its scores st (formed a tile earlier) become weights and meet V,
 // while the next tile's scores are formed into sn.  EXACT (second walk): see weight_of.
+// Products and weights alternate, two or four products to two or four weights, and a
+// product's K or V is read one such group ahead (324 -> 304 us for 2048 tokens as
+// above; left to the compiler, all weights come before all of V's products).  The
+// blocks of a row differ by an exclusive or of the address, formed again for each
+// tile: kept, they are 14 registers that the kernel has not got.
 template <int DP, bool EXACT>
 __device__ __forceinline__ void wide_step(WideState<DP>& w, f32x16 (&st)[2], f32x16 (&sn)[2],
                                           const unsigned char* __restrict__ kt,
-                                          const unsigned char* __restrict__ vt, const int (&koff)[DP / 16],
-                                          const int (&voff)[DP / 32][2], const bf16x8 (&qf)[DP / 16],
-                                          float scale_log2) {
+                                          const unsigned char* __restrict__ vt, int koff, int voff0, int voff1,
+                                          const bf16x8 (&qf)[DP / 16], float scale_log2) {
+  asm volatile("" : "+v"(koff), "+v"(voff0), "+v"(voff1));  // (not kept from the tile before)
   w.top = swap_max(w.top, false) * scale_log2;
   if (__any(w.top > w.m + kGrowth)) {
     const float mn = fmaxf(w.m, w.top);
@@ -127,33 +143,74 @@ __device__ __forceinline__ void wide_step(WideState<DP>& w, f32x16 (&st)[2], f32
 #pragma unroll
       for (int e = 0; e < 16; ++e) w.o[db][e] *= f;
   }
-  wide_scores<DP>(sn, kt, koff, qf);
-  bf16x8 pf[4];
-#pragma unroll
-  for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      st[kb][e] = weight_of<EXACT>(st[kb][e], scale_log2, w.m);
-      pf[2 * kb + e / 8][e % 8] = (bf16)st[kb][e];
-    }
-#pragma unroll
-  for (int sp = 0; sp < 4; ++sp)
-#pragma unroll
-    for (int db = 0; db < DP / 32; ++db) {
-      const unsigned char* const p = vt + sp * 16 * 2 * DP;
-      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-          (bf16x4 GLACIER_LDS*)(const_cast<unsigned char*>(p + voff[db][0])));
-      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-          (bf16x4 GLACIER_LDS*)(const_cast<unsigned char*>(p + voff[db][1])));
-      w.o[db] = mma16(join8(lo, hi), pf[sp], w.o[db]);
-    }
   float sum = 0.0f;
+  i32x4 hi[4], lo[4];  // the weights' two terms, 16 keys each
+  auto weights = [&](int from, int to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = from; i < to; i += 2) {
+      const float p0 = weight_of<EXACT>(st[i / 16][i % 16], scale_log2, w.m);
+      const float p1 = weight_of<EXACT>(st[i / 16][i % 16 + 1], scale_log2, w.m);
+      const unsigned h = pair16(p0, p1);
+      hi[i / 8][i % 8 / 2] = static_cast<int>(h);
+      lo[i / 8][i % 8 / 2] = static_cast<int>(
+          pair16(p0 - __builtin_bit_cast(float, h << 16), p1 - __builtin_bit_cast(float, h & 0xffff0000u)));
+      sum += p0 + p1;
+      asm volatile("" : "+v"(sum));  // (here, or the compiler keeps every weight to the end)
+    }
+  };
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sum += st[kb][e];
+    for (int e = 0; e < 16; ++e) sn[kb][e] = 0.0f;
+  constexpr int NKK = DP / 16, NPAIR = DP / 64;
+  struct Pair {
+    bf16x8 x[2];
+  };
+  // (of both 32-key halves; of 16 keys, two blocks of columns)
+  auto keys = [&](int kk) __attribute__((always_inline)) {
+    return Pair{*reinterpret_cast<const bf16x8*>(kt + (koff ^ 32 * kk)),
+                *reinterpret_cast<const bf16x8*>(kt + (koff ^ 32 * kk) + 32 * 2 * DP)};
+  };
+  auto values = [&](int i) __attribute__((always_inline)) {
+    const unsigned char* const from = vt + i / NPAIR * 16 * 2 * DP;
+    Pair v;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int db = 2 * (i % NPAIR) + x;
+      v.x[x] = join8(__builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                         (bf16x4 GLACIER_LDS*)(const_cast<unsigned char*>(from + (voff0 ^ 64 * db)))),
+                     __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                         (bf16x4 GLACIER_LDS*)(const_cast<unsigned char*>(from + (voff1 ^ 64 * db)))));
+    }
+    return v;
+  };
+  Pair f = keys(0);
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) {
+    const Pair next = kk + 1 < NKK ? keys(kk + 1) : values(0);
+    keep_order();
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) sn[kb] = mma16(f.x[kb], qf[kk], sn[kb]);
+    weights(2 * (8 * kk / NKK), 2 * (8 * (kk + 1) / NKK));
+    keep_order();
+    f = next;
+  }
+#pragma unroll
+  for (int i = 0; i < 4 * NPAIR; ++i) {
+    const int sp = i / NPAIR, db = 2 * (i % NPAIR);
+    Pair next;
+    if (i + 1 < 4 * NPAIR) next = values(i + 1);
+    keep_order();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) w.o[db + x] = mma16(f.x[x], __builtin_bit_cast(bf16x8, lo[sp]), w.o[db + x]);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) w.o[db + x] = mma16(f.x[x], __builtin_bit_cast(bf16x8, hi[sp]), w.o[db + x]);
+    if (sp < 2) weights(16 + 8 * i / NPAIR, 16 + 8 * (i + 1) / NPAIR);
+    if (i == 2 * NPAIR) w.top = wide_largest(sn);
+    keep_order();
+    f = next;
+  }
   w.l += sum;
-  w.top = wide_largest(sn);
 }
 
 template <int DP>
@@ -197,21 +254,16 @@ __global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn
   const int first_limit = s.pos0 + wr / a.group;
   const int last_limit = wr < n_rows ? s.pos0 + min(s.n - 1, (wr + 31) / a.group) : -1;
 
-  // LDS offsets of this lane's reads: K pieces of row col; V pieces of rows
-  // 4 h + 8 u + (lane % 16) / 4 at columns 32 db + 16 (lane / 16 % 2) + 4 (lane % 4)
-  int koff[W::NKK], voff[W::NDB][2];
-#pragma unroll
-  for (int kk = 0; kk < W::NKK; ++kk) koff[kk] = col * W::RB + 16 * ((2 * kk + h) ^ lds_sw<DP>(col));
-  {
+  // LDS offsets of this lane's reads in block 0 (block kk of K is 32 kk away by an
+  // exclusive or, block db of V 64 db): K pieces of row col; V pieces of rows
+  // 4 h + 8 u + (lane % 16) / 4 at columns 16 (lane / 16 % 2) + 4 (lane % 4)
+  const int koff = col * W::RB + 16 * (h ^ lds_sw<DP>(col));
+  auto v_off = [&](int u) {
     const int gr = lane >> 4, ra = (lane & 15) >> 2, cb = lane & 3;
-#pragma unroll
-    for (int db = 0; db < W::NDB; ++db)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int row = 8 * u + 4 * h + ra, piece = 4 * db + 2 * (gr & 1) + (cb >> 1);
-        voff[db][u] = row * W::RB + 16 * (piece ^ lds_sw<DP>(row)) + 8 * (cb & 1);
-      }
-  }
+    const int row = 8 * u + 4 * h + ra, piece = 2 * (gr & 1) + (cb >> 1);
+    return row * W::RB + 16 * (piece ^ lds_sw<DP>(row)) + 8 * (cb & 1);
+  };
+  const int voff0 = v_off(0), voff1 = v_off(1);
 
   // A tile is four page pieces of 16 keys; a wave brings one of them, of K and
   // of V.  The piece is read through a buffer resource that
@@ -287,7 +339,7 @@ __global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn
           }
         ws.top = wide_largest(st);
       }
-      wide_step<DP, careful()>(ws, st, sn, k_slot(odd ^ 1), v_slot(odd), koff, voff, qf, a.scale_log2);
+      wide_step<DP, careful()>(ws, st, sn, k_slot(odd ^ 1), v_slot(odd), koff, voff0, voff1, qf, a.scale_log2);
     }
     vmw<0>();
     if constexpr (careful()) look_through(v_slot(odd ^ 1), j + kKeysWide);

@@ -41,7 +41,7 @@
  * puts them off by up to pos * 2^-23 at far positions.)
  *
  * bf16 tensors: bf16 operands, fp32 sums and softmax; weights multiply V as two
- * bf16 terms (one in large chunks).  fp32 tensors: fp32 throughout.  Results are
+ * bf16 terms, 16 bits of them.  fp32 tensors: fp32 throughout.  Results are
  * bitwise repeatable for one layout of the work (below: max_new, max_kv).  NaN
  * and infinities in a token's K or V reach only the rows that see the token.
  * Contexts, status codes and dtypes are those of glacier_attn.h; calls enqueue on
