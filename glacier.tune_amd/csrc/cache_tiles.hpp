@@ -3,13 +3,11 @@
 // exist and how their keys are split follows from device data.
 #pragma once
 
+#include "cache_split.hpp"
 #include "cache_view.hpp"
 #include "lds_mfma.hpp"
 
 namespace glacier {
-
-constexpr int kMaxSplits = 64;   // one lane each in the join
-constexpr int kSplitUnit = 128;  // splits begin at multiples of it
 
 constexpr float kLeast = -3.402823466e38f;  // where running maxima begin: below every score
 
@@ -71,12 +69,9 @@ __device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int 
   const long cap = (long)a.c.max_pages << a.c.page_shift;
   const long end = (long)s.pos0 + last + 1;
   k.kend = static_cast<int>(end < 0 ? 0 : end < cap ? end : cap);
-  const int even = (k.kend + a.n_splits - 1) / a.n_splits;
-  k.per = max(a.split_keys, (even + kSplitUnit - 1) / kSplitUnit * kSplitUnit);
-  k.active = max(1, (k.kend + k.per - 1) / k.per);
-  // as many splits as that, evenly
-  k.per = ((k.kend + k.active - 1) / k.active + kSplitUnit - 1) / kSplitUnit * kSplitUnit;
-  k.active = max(1, (k.kend + k.per - 1) / k.per);
+  const KeySplit split = split_of(k.kend, a.n_splits, a.split_keys);
+  k.per = split.per;
+  k.active = split.active;
   return k;
 }
 

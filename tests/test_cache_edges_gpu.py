@@ -14,7 +14,7 @@ from test_cache_gpu import CHUNKS, WIDE  # noqa: E402
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
 DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
-LAYOUTS = [512, 3000, WIDE]  # max_kv: 16-row tiles, 128-row tiles whole, in splits
+LAYOUTS = [512, 3000, WIDE]  # max_kv: 16-row tiles, 128-row tiles in few and in many splits
 
 
 @pytest.fixture(scope="module")
@@ -62,3 +62,57 @@ def test_weights_that_all_round_one_way(eng, d, keys):
     q[..., :2] = 1.0
     out = eng.cache_forward(q, *p.arrays(), max_kv=keys)[0]
     assert (out == 1.0).all(), (out.min(), out.max())
+
+
+# layouts: dtype, hq, hkv, D, max_kv
+NO_KEY_LAYOUTS = {
+    "bf16 16 rows": ("bf16", 8, 2, 64, 300), "bf16 16 rows, splits": ("bf16", 8, 2, 64, 2000),
+    "bf16 128 rows": ("bf16", 64, 4, 128, 512), "bf16 128 rows, splits": ("bf16", 8, 2, 64, WIDE),
+    "bf16 128 rows, wide heads": ("bf16", 8, 2, 256, WIDE), "fp32 16 rows": ("fp32", 8, 2, 96, 800),
+    "fp32 16 rows, splits": ("fp32", 8, 2, 64, WIDE), "fp32 32 rows": ("fp32", 128, 8, 96, 1000),
+    "fp32 32 rows, splits": ("fp32", 8, 2, 96, WIDE)}
+
+
+@pytest.mark.parametrize("layout", sorted(NO_KEY_LAYOUTS))
+def test_tiles_without_a_key(eng, layout):
+    # new tokens of sequences without a key (length zero and below), a sequence
+    # with keys and idle ones beside them, rows behind the last sequence
+    dt, hq, hkv, d, keys = NO_KEY_LAYOUTS[layout]
+    seqs, pad = [(20, 20), (0, 50), (33, 33), (40, 300), (0, 0), (9, 9)], 3
+    p = ch.Paged(seqs, hq, hkv, d, 16, DTYPES[dt], 33, pad, columns=WIDE // 16)
+    p.kv_lens.copy_(torch.tensor([0, 50, -7, 300, 0, -2 ** 31 + 9], dtype=torch.int32))
+    live = torch.zeros(p.tokens, dtype=torch.bool)
+    live[53:93] = True
+    none = ~live
+    none[-pad:] = False
+    out = torch.full((p.tokens, hq, d), 7.0, device="cuda", dtype=DTYPES[dt])
+    lse = torch.full((hq, p.tokens), 7.0, device="cuda")
+    ref = ch.attend_ref(p)
+    eng.cache_forward(p.q.cuda(), *p.arrays(), max_kv=keys, out=out, lse=lse)
+    ch.check("out", out[live.cuda()], ref[0][live], ref[1][live])
+    ch.check("lse", lse[:, live.cuda()], ref[2][:, live], ref[3][:, live])
+    assert not out[none.cuda()].any() and (lse[:, none.cuda()] == -math.inf).all()
+    assert (out[-pad:] == 7.0).all() and (lse[:, -pad:] == 7.0).all()
+    before = p.both.clone()
+    k = torch.ones(p.tokens, hkv, d, device="cuda", dtype=DTYPES[dt])
+    eng.cache_append(k, 2 * k, *p.arrays())
+    changed = (~(torch.eq(before, p.both) | (before.isnan() & p.both.isnan()))).any(-1).nonzero()
+    want = {(int(p.table[3, pos // 16]), pos % 16) for pos in range(260, 300)}
+    assert {(int(r[0]), int(r[3])) for r in changed} == want
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_a_page_table_without_columns(eng, dt):
+    p = ch.Paged([(40, 300), (1, 5)], 16, 2, 96, 16, DTYPES[dt], 34, pad=1)
+    table = p.table[:, :0].contiguous()
+    args = (p.k_pages, p.v_pages, p.cu, p.kv_lens, table)
+    out = torch.full((p.tokens, 16, 96), 7.0, device="cuda", dtype=DTYPES[dt])
+    lse = torch.full((16, p.tokens), 7.0, device="cuda")
+    for hints in ({}, dict(max_new=40, max_kv=300)):
+        eng.cache_forward(p.q.cuda(), *args, out=out, lse=lse, **hints)
+        assert not out[:-1].any() and (lse[:, :-1] == -math.inf).all()
+        assert (out[-1] == 7.0).all() and (lse[:, -1] == 7.0).all()
+    before = p.both.clone()
+    k = torch.ones(p.tokens, 2, 96, device="cuda", dtype=DTYPES[dt])
+    eng.cache_append(k, k, *args)
+    assert torch.equal(before.nan_to_num(9.0), p.both.nan_to_num(9.0))
