@@ -21,7 +21,8 @@
 // The running maximum is only followed where it has grown by more than 8 (in
 // log2): until then weights are taken against the old one, at most 2^8 large,
 // and the sums need no rescaling.  The result is the same: any reference value
-// cancels in out and lse.
+// cancels in out and lse.  (The second walk, which also takes the sums that leave
+// fp32, follows it always: with V from 2^120 on it is those 2^8 that count.)
 //
 // KV heads alternate over the workgroups, so that an XCD's L2 serves few of
 // them, and the tiles of long sequences start first (eight ragged chunks: 117 ->
@@ -133,7 +134,7 @@ __device__ __forceinline__ void wide_step(WideState<DP>& w, f32x16 (&st)[2], f32
                                           const bf16x8 (&qf)[DP / 16], float scale_log2) {
   asm volatile("" : "+v"(koff), "+v"(voff0), "+v"(voff1));  // (not kept from the tile before)
   w.top = swap_max(w.top, false) * scale_log2;
-  if (__any(w.top > w.m + kGrowth)) {
+  if (__any(w.top > w.m + (EXACT ? 0.0f : kGrowth))) {
     const float mn = fmaxf(w.m, w.top);
     const float f = weight(w.m - mn);
     w.m = mn;

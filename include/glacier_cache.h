@@ -43,7 +43,9 @@
  * bf16 tensors: bf16 operands, fp32 sums and softmax; weights multiply V as two
  * bf16 terms, 16 bits of them.  fp32 tensors: fp32 throughout.  Results are
  * bitwise repeatable for one layout of the work (below: max_new, max_kv).  NaN
- * and infinities in a token's K or V reach only the rows that see the token.
+ * and infinities in a token's K or V reach only the rows that see the token.  Sums
+ * of up to as many terms of V as there are keys stay within fp32 (|V| below 2^127
+ * divided by their number).
  * Contexts, status codes and dtypes are those of glacier_attn.h; calls enqueue on
  * the context's stream.  Tensors are 16-byte aligned, q, k, v and out contiguous;
  * head_dim is a multiple of 8 up to 256.

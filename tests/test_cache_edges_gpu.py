@@ -116,3 +116,34 @@ def test_a_page_table_without_columns(eng, dt):
     k = torch.ones(p.tokens, 2, 96, device="cuda", dtype=DTYPES[dt])
     eng.cache_append(k, k, *args)
     assert torch.equal(before.nan_to_num(9.0), p.both.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("keys", LAYOUTS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_large_values_under_growing_scores(eng, dt, d, keys):
+    # V between 2^121 and 2^122; of every 64 keys one counts, whose weight grows
+    # from 1 to 2^7.5: against the first one as reference the sum would leave
+    # fp32, against the largest it is below 2^126.  (The others' scores fall, so
+    # that no part of the keys has many weights near its own largest.)
+    n, kv, hq, hkv = 40, 700, 8, 2
+    p = ch.Paged([(n, kv)], hq, hkv, d, 16, DTYPES[dt], 35, columns=WIDE // 16)
+    score = -100.0 - 2.0 * torch.arange(kv)
+    score[5::64] = torch.arange(len(score[5::64])).mul(1.5).clamp(max=7.5)
+    k = torch.zeros(kv, hkv, d)
+    k[..., 0] = (score * math.log(2) * math.sqrt(d))[:, None]
+    g = torch.Generator().manual_seed(36)
+    v = (1 + torch.rand(kv, hkv, d, generator=g)) * 2.0 ** 121
+    p.k[0], p.v[0] = k.to(DTYPES[dt]), v.to(DTYPES[dt])
+    p.q = torch.zeros(n, hq, d, dtype=DTYPES[dt])
+    p.q[..., 0] = 1.0
+    pages = p.table[0, :-(-kv // 16)].long().cpu()
+    for to, x in ((p.k_pages, p.k[0]), (p.v_pages, p.v[0])):
+        rows = torch.zeros(len(pages) * 16, hkv, d, dtype=DTYPES[dt])
+        rows[:kv] = x
+        to[pages.cuda()] = rows.view(-1, 16, hkv, d).transpose(1, 2).contiguous().cuda()
+    out, lse = eng.cache_forward(p.q.cuda(), *p.arrays(), max_kv=keys, save=True)
+    ref = ch.attend_ref(p)
+    assert torch.isfinite(out).all()
+    ch.check("out", out, ref[0], ref[1])
+    ch.check("lse", lse, ref[2], ref[3])
