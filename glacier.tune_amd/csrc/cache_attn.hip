@@ -586,9 +586,13 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   const long group = hq / c.hkv;
   const long cap = (long)c.max_pages << c.page_shift;
   const long keys = max_kv > 0 && max_kv < cap ? max_kv : cap;
-  const long longest = max_new > 0 && max_new < c.T ? max_new : c.T;  // chunk
-  // tiles of so many rows, if the new tokens are spread evenly over the sequences
+  // where the caller does not say, the new tokens are taken to be spread evenly over
+  // the sequences, rounded down (a padded batch of single tokens).  us a call as one
+  // chunk of them all and like that: 64 sequences of one token, 14/2 heads of 64, over
+  // up to 4096 keys, 32 and 21; 32 of 28/4 heads of 128 over up to 8192, 61 and 53.
   const long seqs = std::min(c.T, c.n_seqs);
+  const long longest = max_new > 0 && max_new < c.T ? max_new : max_new > 0 ? c.T : c.T / seqs;
+  // tiles of so many rows, spread like that
   auto tiles_of = [&](long rows) { return seqs * ((c.T * group + seqs * rows - 1) / (seqs * rows)); };
   // Tiles of 128 rows for chunks that need more than one of 16, where tiles of 16
   // would read enough keys (tiles x keys x D).  us a call, tiles of 16 and of 128:

@@ -80,9 +80,10 @@ typedef struct glacier_cache_batch {
   int32_t n_seqs;
   int32_t total_tokens;       /* rows of q, k, v and out */
   int32_t max_pages;
-  int32_t max_new;            /* new tokens of the longest chunk, or 0 if not known: */
-  int32_t max_kv;             /* and the longest kv_lens, or 0.  Both only steer how the work is
-                                 laid out; results are right whatever they say */
+  int32_t max_new;            /* new tokens of the longest chunk, or 0 if not known (the tokens
+                                 are then taken to be spread evenly over the sequences) */
+  int32_t max_kv;             /* the longest kv_lens, or 0 (then what max_pages allows).  Both only
+                                 steer how the work is laid out; results are right whatever they say */
 } glacier_cache_batch;
 
 /* Writes k (rotated when rope_freq_base > 0; 0: as it is, for keys that are

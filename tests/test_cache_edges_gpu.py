@@ -147,3 +147,26 @@ def test_large_values_under_growing_scores(eng, dt, d, keys):
     assert torch.isfinite(out).all()
     ch.check("out", out, ref[0], ref[1])
     ch.check("lse", lse, ref[2], ref[3])
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("n,hq,hkv,d,pad", [(32, 28, 4, 128, 0), (8, 32, 8, 128, 3), (64, 14, 2, 64, 0),
+                                            (12, 40, 1, 64, 5), (5, 8, 2, 256, 0)])
+def test_single_tokens_without_hints(eng, n, hq, hkv, d, pad, dt):
+    # a call that does not know its longest chunk takes a batch of single tokens for
+    # what it is: the layout, and so every bit, of a call that says so
+    p = ch.Paged([(1, 1 + 37 * i % 900) for i in range(n)], hq, hkv, d, 16, DTYPES[dt], 37, pad, columns=2 ** 14 // 16)
+    q = p.q.cuda()
+    hints = dict(max_kv=8192)
+    want = eng.cache_forward(q, *p.arrays(), max_new=1, save=True, **hints)
+    got = eng.cache_forward(q, *p.arrays(), save=True, **hints)
+    live = slice(0, p.tokens - pad)
+    assert torch.equal(got[0][live], want[0][live]) and torch.equal(got[1][:, live], want[1][:, live])
+    size = []
+    for max_new in (0, 1):
+        cache, batch = ga.cache_args(*p.arrays(), p.tokens, max_new, 8192, 0)
+        size.append(ga.load().glacier_attn_cache_workspace(eng._h, cache, batch, hq))
+    assert size[0] == size[1]
+    ref = ch.attend_ref(p)
+    ch.check("out", got[0], ref[0], ref[1])
+    ch.check("lse", got[1], ref[2], ref[3])
