@@ -1399,9 +1399,10 @@ QkNorm qk_norm_of(const glacier_rmsnorm_qk_desc* desc) {
     fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
   need_base(d.rope_freq_base);
   need_head_dim(d.head_dim);
-  // (a launch has fewer than 2^32 threads, and 64 of them or more to a token)
+  // (a launch has fewer than 2^32 threads: 64 of them or more to a token, in workgroups
+  // of four tokens)
   if ((long long)d.total_tokens * ((long long)d.n_heads_q + d.n_heads_kv) >= (1LL << 30) ||
-      d.total_tokens >= (1 << 26))
+      d.total_tokens > (1 << 26) - 4)
     fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
   QkNorm a{};
   a.T = d.total_tokens;

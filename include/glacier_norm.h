@@ -75,7 +75,7 @@ int glacier_rmsnorm_backward(glacier_attn_ctx *ctx, const glacier_norm_desc *des
  * glacier_attn_forward, which rotates by itself).  The sums are fp32, and every
  * result is rounded once. */
 typedef struct glacier_rmsnorm_qk_desc {
-  int32_t total_tokens;  /* T (may be 0), below 2^26 */
+  int32_t total_tokens;  /* T (may be 0), at most 2^26 - 4 */
   int32_t n_heads_q;     /* q [T][n_heads_q][D] */
   int32_t n_heads_kv;    /* k [T][n_heads_kv][D] */
   int32_t head_dim;      /* D: a multiple of 8, at most 256 */

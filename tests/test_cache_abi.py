@@ -233,3 +233,16 @@ def test_forward_keeps_off_the_pages(change, word):
 def test_weight_gradients_share_no_memory(at, word):
     rc, msg = _norm(backward=True, at=at)
     assert rc == INVALID and word in msg, msg
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("short,code,word", [(4, INVALID, "ctx"), (3, UNSUPPORTED, "too large"),
+                                             (1, UNSUPPORTED, "too large")])
+def test_the_longest_norm(backward, short, code, word):
+    # four tokens to a workgroup of 256 threads: one more than 2^26 - 4 tokens
+    # rounds up to the 2^32 threads that a launch does not have
+    names = (["dq_out", "dk_out"] if backward else []) + ["q", "k", "q_weight", "k_weight", "positions"] + (
+        ["dq", "dk", "dq_weight", "dk_weight"] if backward else ["q_out", "k_out"])
+    rc, msg = _norm(backward=backward, T=2 ** 26 - short, hq=1, hkv=1, d=8,
+                    at={n: (i + 1) << 34 for i, n in enumerate(names)})
+    assert rc == code and word in msg, msg
