@@ -439,6 +439,10 @@ __global__ __launch_bounds__(64 * kWavesWide, DP <= 128 ? 2 : 1) void cache_attn
     a.lse[(at % a.hq) * c.T + at / a.hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
+__device__ inline float masked(float x, unsigned kept) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & kept);
+}
+
 // Joins the splits of a tile's rows, 32 of them a workgroup: D / 4 lanes to a
 // row, four splits' sums in flight.  (A wave for each row, as after the 16-row
 // kernel, spends more on finding the row's sequence than on joining it: 84 us
@@ -481,10 +485,14 @@ __global__ __launch_bounds__(256) void cache_join_tiles_kernel(CacheAttn a) {
       for (int e = 0; e < 4; ++e) o[e] *= f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float g = u0 + i < tk.active ? weight(ml[i].x - mx) : 0.0f;
+        // (a weight of zero is not enough where the sums are infinite; by a mask, as a
+        // choice becomes a branch with the load in it)
+        unsigned kept = u0 + i < tk.active ? ~0u : 0u;
+        asm volatile("" : "+v"(kept));
+        const float g = masked(weight(ml[i].x - mx), kept);
         total += g * ml[i].y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += g * v[i][e];
+        for (int e = 0; e < 4; ++e) o[e] += g * masked(v[i][e], kept);
       }
     }
     if (d >= c.D) continue;

@@ -170,3 +170,27 @@ def test_single_tokens_without_hints(eng, n, hq, hkv, d, pad, dt):
     ref = ch.attend_ref(p)
     ch.check("out", got[0], ref[0], ref[1])
     ch.check("lse", got[1], ref[2], ref[3])
+
+
+@pytest.mark.parametrize("seqs,hq,hkv,d,keys", [
+    ([(200, 900)], 14, 2, 64, 3000), ([(130, 700), (60, 60)], 32, 8, 128, 2500), ([(150, 1500)], 8, 2, 256, 6000),
+    ([(30, 700)], 8, 2, 128, WIDE), ([(1, 1500)], 28, 4, 128, 3000)])
+def test_an_infinite_value_in_the_last_split(eng, seqs, hq, hkv, d, keys):
+    # an infinity in V makes its columns infinite in every row that sees it (not NaN),
+    # whichever split of the keys it lies in and however many there are
+    p = ch.Paged(seqs, hq, hkv, d, 16, BF16, 38, columns=WIDE // 16)
+    ref = ch.attend_ref(p)
+    n, kv = seqs[0]
+    sees = torch.zeros(p.tokens, dtype=torch.bool)
+    for pos in (kv - 1, kv - n, kv // 2, 0):
+        for what in (math.inf, -math.inf):
+            both = p.both.clone()
+            both[p.table[0, pos // 16], 1, :, pos % 16, 3::7] = what
+            out, lse = eng.cache_forward(p.q.cuda(), both[:, 0], both[:, 1], p.cu, p.kv_lens, p.table, max_kv=keys,
+                                         save=True)
+            sees[:n] = torch.arange(kv - n, kv) >= pos
+            assert (out[sees.cuda()][..., 3::7] == what).all()
+            rest = ref[0].clone()
+            rest[sees, :, 3::7] = math.nan
+            ch.check("out", torch.where(rest.isnan().cuda(), 0.0, out.double()), rest, ref[1])
+            ch.check("lse", lse, ref[2], ref[3])
