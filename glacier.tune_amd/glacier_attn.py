@@ -445,6 +445,14 @@ def _optional(t, name, shape, dtype, device):
     return None if t is None else _address(t, name, shape, dtype, device)
 
 
+_LARGEST = 2 ** 31 - 1  # of a descriptor's 32-bit sizes: ctypes would wrap larger ones
+
+
+def _need_32_bits(*sizes):
+    if max(sizes) > _LARGEST:
+        raise Unsupported(ERR_UNSUPPORTED, "tensor too large")
+
+
 def cache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, max_new, max_kv,
                device):
     """(glacier_kv_cache, glacier_cache_batch) of a cache and batch: pages
@@ -465,6 +473,7 @@ def cache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, m
     if len(page_table.shape) != 2 or page_table.dtype is not i32:
         raise TypeError("page_table must be an int32 [n_seqs, max_pages] tensor")
     n, most = page_table.shape
+    _need_32_bits(total_tokens, n_pages, hkv, page, d, n, most)
     if page_table.is_contiguous():
         row = most
     else:
@@ -480,7 +489,7 @@ def cache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, m
                     GpuAttentionEngine._io_of(k_pages)),
             CacheBatch(_address(cu_tokens, "cu_tokens", (n + 1,), i32, device),
                        _address(kv_lens, "kv_lens", (n,), i32, device), page_table.data_ptr(), row, n,
-                       total_tokens, most, int(max_new), int(max_kv)))
+                       total_tokens, most, min(int(max_new), _LARGEST), min(int(max_kv), _LARGEST)))
 
 
 def _page_stride(k_pages, v_pages):
@@ -848,6 +857,7 @@ class GpuAttentionEngine:
         torch, dev = _torch(), self.device_ordinal
         T, hq, d = shape
         hkv, f32 = k.shape[1], torch.float32
+        _need_32_bits(T, hq, hkv, d)
         desc = QkNormDesc(T, hq, hkv, d, self._io_of(q), float(eps), float(rope_freq_base or 0.0))
         return desc, (_address(q, "q", shape, dtype, dev), _address(k, "k", (T, hkv, d), dtype, dev),
                       _address(q_weight, "q_weight", (d,), f32, dev),

@@ -246,3 +246,30 @@ def test_the_longest_norm(backward, short, code, word):
     rc, msg = _norm(backward=backward, T=2 ** 26 - short, hq=1, hkv=1, d=8,
                     at={n: (i + 1) << 34 for i, n in enumerate(names)})
     assert rc == code and word in msg, msg
+
+
+def test_sizes_past_32_bits_are_refused_not_wrapped():
+    # (descriptors hold 32-bit sizes; tensors without memory stand for the large ones)
+    torch = pytest.importorskip("torch")
+    import types
+
+    bf16, i32, big = torch.bfloat16, torch.int32, 2 ** 32 + 5
+    eng = types.SimpleNamespace(device_ordinal=-1, _io_of=ga.GpuAttentionEngine._io_of)
+    q = torch.empty(big, 1, 8, dtype=bf16, device="meta")
+    w = torch.zeros(8)
+    with pytest.raises(ga.Unsupported, match="too large"):
+        ga.GpuAttentionEngine._qk_args(eng, q, q, w, w, 1e-6, None, None)
+    heads = torch.empty(1, big, 8, dtype=bf16, device="meta")
+    with pytest.raises(ga.Unsupported, match="too large"):
+        ga.GpuAttentionEngine._qk_args(eng, heads, heads, w, w, 1e-6, None, None)
+    kp = torch.zeros(4, 2, 16, 64, dtype=bf16)
+    good = dict(k_pages=kp, v_pages=kp.clone(), cu_tokens=torch.zeros(2, dtype=i32), kv_lens=torch.zeros(1, dtype=i32),
+                page_table=torch.zeros(1, 3, dtype=i32), total_tokens=1, max_new=0, max_kv=0, device=-1)
+    pages = torch.empty(big, 2, 16, 64, dtype=bf16, device="meta")
+    for change in (dict(total_tokens=big), dict(total_tokens=2 ** 31),
+                   dict(page_table=torch.empty(1, big, dtype=i32, device="meta")),
+                   dict(k_pages=pages, v_pages=pages)):
+        with pytest.raises(ga.Unsupported, match="too large"):
+            ga.cache_args(**dict(good, **change))
+    _, batch = ga.cache_args(**dict(good, max_new=big, max_kv=2 ** 40))  # (hints: any size is fine)
+    assert batch.max_new == batch.max_kv == 2 ** 31 - 1
