@@ -1016,6 +1016,8 @@ class GpuAttentionEngine:
 
     # ---- instrumentation ---------------------------------------------------
     def set_kernel_timing(self, enable: bool) -> None:
+        """Per-kernel timing of attention and RMSNorm (the projections, the per-head norms and
+        the key/value cache are not timed)."""
         _check(load().glacier_attn_set_kernel_timing(self._h, 1 if enable else 0))
 
     def kernel_times(self) -> dict:

@@ -213,7 +213,10 @@ int glacier_attn_synchronize(glacier_attn_ctx *ctx);
  * phases with Stopwatch, TransformerBlock.cs:311-321) ---------------------- */
 
 /* Enables (1) or disables (0) per-kernel hipEvent timing on the context's
- * stream; enabling clears the counters. */
+ * stream; enabling clears the counters.  Timed are the kernels of glacier_attn_forward
+ * and _backward (host and device forms) and of glacier_rmsnorm_forward and _backward;
+ * the projections, the per-head norms of queries and keys (glacier_rmsnorm_qk_*) and
+ * the key/value cache (glacier_attn_cache_*) are not. */
 int glacier_attn_set_kernel_timing(glacier_attn_ctx *ctx, int enable);
 
 /* Number of kernel kinds the library launches. */
