@@ -595,16 +595,23 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   // tiles of so many rows, spread like that
   auto tiles_of = [&](long rows) { return seqs * ((c.T * group + seqs * rows - 1) / (seqs * rows)); };
   // Tiles of 128 rows for chunks that need more than one of 16, where tiles of 16
-  // would read enough keys (tiles x keys x D).  us a call, tiles of 16 and of 128:
-  // 28/4 heads of 128, 32 tokens over 1024 keys (7e6) 12.6, 18.3; 8 sequences of
-  // up to 4 over up to 2048 (17e6) 13.7, 18.3; 16 tokens over 8192 (29e6) 28.7,
-  // 20.2; 32 sequences of up to 8 over up to 2048 (134e6) 46, 30; 14/2 heads of
-  // 64, 8 sequences of up to 16 over up to 2048 (15e6) 12.9, 14.4; of up to 32
-  // (29e6) 18.4, 16.6.  Above 128 columns one workgroup of wide tiles fills a CU:
-  // 8/2 heads of 256, 8 sequences of up to 32 over up to 2048 (67e6) 30.7, 36.8;
-  // 512 tokens over 2048 (134e6) 40.4, 41.7; 1024 over 8192 (1e9) 260, 121.
-  const bool wide = c.io_bf16 && longest * group > 16 &&
-                    (double)tiles_of(16) * c.hkv * keys * c.D > (c.D <= 128 ? 25e6 : 100e6);
+  // would read enough keys (tiles x keys x D).  us a call, tiles of 16 and of 128,
+  // 28/4 heads of 128 where nothing else is said.  Up to 2048 keys, where the wide
+  // tiles find few splits: 64 tokens over 1024 (15e6) 14, 22; 512 over 512 (59e6) 18,
+  // 21; 16 chunks of up to 32 over up to 1024 (76e6) 27, 31; 8 of up to 128 over up to
+  // 512, 32/8 (109e6) 33, 23; 512 over 1024 (117e6) 31, 32; 512 over 2048 (235e6) 53,
+  // 42; 14/2 heads of 64: 1000 over 1000 (56e6) 15, 24; 8 of up to 200 over up to 2048
+  // (109e6) 26, 28.  Over more: 16 over 8192 (29e6) 28, 22; 4 of up to 12 over up to
+  // 4096 (34e6) 25, 24; 2 of up to 40 over up to 4096 (59e6) 26, 29; 16 of up to 6 over
+  // up to 8192 (201e6) 71, 53; 40 over 4096, 12/2 (16e6) 15, 20; 14/2 heads of 64: 4 of
+  // up to 100 over up to 4000 (61e6) 25, 24.  Above 128 columns one workgroup of wide
+  // tiles fills a CU; 8/2 heads of 256: 256 over 2048 (67e6) 30, 41; 512 over 2048
+  // (134e6) 40, 42; 600 over 1000, 16/4 (154e6) 54, 55; 1024 over 2048 (268e6) 70, 48;
+  // 200 over 4096 (105e6) 46, 37; 128 over 8192 (134e6) 46, 58; 512 over 4096 (268e6)
+  // 72, 52; 1024 over 8192 (1e9) 259, 120.
+  const double enough = c.D <= 128 ? (keys <= 2048 ? 110e6 : 25e6) : keys <= 2048 ? 160e6 : 100e6;
+  const bool wide =
+      c.io_bf16 && longest * group > 16 && (double)tiles_of(16) * c.hkv * keys * c.D > enough;
   // fp32 chunks: tiles of 32 rows read K and V half as often, from 65 columns on (fewer
   // leave too few tiles), up to 128 (their sums fill the registers).  us a call, 16
   // and 32 rows: 512 tokens over 4096 keys, 28/4 heads of 128, 362, 303; 1024 over
@@ -617,9 +624,9 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   const long narrow_splits = keys <= 1024 ? 1 : keys / 512;
   const bool mid = chunk && c.D > 64 && c.D <= 128 && tiles_of(kRowsMid) * c.hkv * narrow_splits >= n_cu;
   p.rows = wide ? kCacheWideRows : mid ? kRowsMid : 16;
-  // and their long tiles first: 1000 tokens as they come, 40/8 heads of 128, 148 -> 136
-  // us; 8 chunks of up to 64 as above 229 -> 212; 4 of up to 300, 14/2 of 64, 105 -> 98
-  // (2 of up to 900, 8/8 of 64, 81 -> 85); bf16 single tokens lose 1 of 67.
+  // and their long tiles first: 1000 tokens as they come, 40/8 heads of 128, 159 -> 137
+  // us; 8 chunks of up to 64 as above 248 -> 205; 4 of up to 300, 14/2 of 64, 97 -> 61;
+  // 2 of up to 900, 8/8 of 64, 100 -> 96; bf16 single tokens lose 1 of 67.
   p.long_first = chunk;
   const long groups = tiles_of(p.rows) * c.hkv;
   // Splits of 512 keys or more, as many as fill the workgroups the CUs hold at
@@ -636,10 +643,11 @@ CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, i
   // Tiles of 128 rows, two to a CU: as many splits as fill it, of 256 keys or
   // more (512 from 64 workgroups on, 2048 from 256 on), none up to 512 keys.  us
   // a call, 28/4 heads of 128, whole and in 2, 4, 8 splits: 32 tokens over 8192
-  // keys (8 workgroups) 146, 83, 49, 35, and 25 in 32; 512 over 4096 (112) 80,
-  // 57, 52, 67; 512 over 512 19, 22; 2048 over 8192 (448) 231, 246, 258, 299;
-  // 16 chunks of up to 128 over up to 2048 (320) 55, 66; 8 of up to 256 over up
-  // to 4096 (320) 90, 88, 100; 3 of up to 300 over up to 5000 (132) 94, 80, 69.
+  // keys (8 workgroups) 189, 106, 61, 41, and 26 in 32; 512 over 4096 (112) 103,
+  // 68, 63, 73; 512 over 512 21, 24, 25, 25; 2048 over 8192 (448) 322, 321, 329,
+  // 356; 16 chunks of up to 128 over up to 2048 (320) 62, 60, 68, 86; 8 of up to 256
+  // over up to 4096 (320) 108, 96, 105, 112; 3 of up to 300 over up to 5000 (132) 122,
+  // 77, 69, 78; 8/2 heads of 256, 1024 over 8192 (64) 353, 195, 117, 137.
   const long per_cu = wide ? (c.D <= 128 ? 2 : 1) : !c.io_bf16 ? 1 : c.D <= 64 ? 4 : c.D <= 128 ? 2 : 1;
   const long want = per_cu * n_cu / groups;
   const long least = groups < 64 ? 256 : groups < 256 ? 512 : 2048;

@@ -67,7 +67,7 @@ def test_weights_that_all_round_one_way(eng, d, keys):
 # layouts: dtype, hq, hkv, D, max_kv
 NO_KEY_LAYOUTS = {
     "bf16 16 rows": ("bf16", 8, 2, 64, 300), "bf16 16 rows, splits": ("bf16", 8, 2, 64, 2000),
-    "bf16 128 rows": ("bf16", 64, 4, 128, 512), "bf16 128 rows, splits": ("bf16", 8, 2, 64, WIDE),
+    "bf16 128 rows": ("bf16", 320, 20, 128, 512), "bf16 128 rows, splits": ("bf16", 8, 2, 64, WIDE),
     "bf16 128 rows, wide heads": ("bf16", 8, 2, 256, WIDE), "fp32 16 rows": ("fp32", 8, 2, 96, 800),
     "fp32 16 rows, splits": ("fp32", 8, 2, 64, WIDE), "fp32 32 rows": ("fp32", 128, 8, 96, 1000),
     "fp32 32 rows, splits": ("fp32", 8, 2, 96, WIDE)}
