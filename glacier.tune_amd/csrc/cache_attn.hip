@@ -15,11 +15,15 @@
 //
 // Bound by reading K and V for single tokens: one over 65536 keys, 32/8 heads of
 // 128, bf16, 57.4 us (4.67 TB/s of the 4.77 of a large copy); 32 sequences of up to
-// 8192 keys, 28/4 heads, 64-65 us (4.3 TB/s, uneven splits); one over 512 keys, 14/2
-// heads of 64, 6.8 us: four dependent loads and four blocks of keys.  fp32 chunks
-// are bound by the fp32 MFMAs and by tiles of uneven length (1024 tokens over 8192 keys,
-// 8/2 heads of 96: 225 us, 107 TFLOP/s of the 154 of a large library product; three of
-// up to 120 over up to 1001: 23 us, on 138 of the 256 CUs).
+// 8192 keys, 28/4 heads, 64-65 us (4.3 TB/s, uneven splits); heads of 64 and 256 less
+// (8 sequences of up to 16000 keys, 14/2 of 64, 16 us, 2.2 TB/s; 6 of up to 9000, 8/2 of
+// 256, 24 us, 3.6); one over 512 keys, 14/2 heads of 64, 6.8 us: four dependent loads
+// and four blocks of keys.  Long fp32 chunks are bound by the fp32 MFMAs (1024 tokens
+// over 8192 keys, 8/2 heads of 96: 226 us, 107 TFLOP/s of the 154 of a large library
+// product; MFMAs busy 66% of the card's cycles), short ones by one workgroup a CU that
+// waits for its own loads and LDS (three of up to 120 over up to 1001: 22-23 us on 138
+// of the 256 CUs, MFMAs busy 23 thousand cycles there of about 57 thousand; 18% of the
+// LDS cycles are bank conflicts).
 //
 // KV heads alternate over the workgroups, so that an XCD's L2 serves few of them
 // (fp32, 16 sequences of up to 8000 keys, one token each: 93 -> 70 us; 512 tokens

@@ -25,15 +25,16 @@
 // fp32, follows it always: with V from 2^120 on it is those 2^8 that count.)
 //
 // KV heads alternate over the workgroups, so that an XCD's L2 serves few of
-// them, and the tiles of long sequences start first (eight ragged chunks: 117 ->
-// 94 us).
+// them, and the tiles of long sequences start first (eight ragged chunks, with one
+// term: 117 -> 94 us; now 116-125).
 //
 // Measured: 2048 tokens over 8192 keys, 28/4 heads of 128: 304-314 us (690-670
 // TFLOP/s, 1035 with the second terms' products; a library product of 8192^3
-// reaches 1205 on the card).  Counters, in 1.95 GHz cycles: MFMAs busy 48%, vector
-// instructions issuing 37%, waves that could issue and wait for the other's
-// instruction 42% of their cycles; tiles of 448 workgroups on 512 places leave an
-// eighth of the card idle.  Tried and slower (with one term, then at 221-231): tiles through registers (278 us), 256 rows on eight
+// reaches 1205 on the card).  Of the cycles that the card counts as active (1.95 GHz)
+// MFMAs are busy 47% and vector instructions issue 37%; waves spend 42% of theirs ready
+// and waiting for the other's instruction; tiles of 448 workgroups on 512 places leave
+// an eighth of the card idle.  1024 tokens over 8192 keys, 8/2 heads of 256, one wave a
+// SIMD: 116-121 us (550-530 TFLOP/s), MFMAs busy 36%.  Tried and slower (with one term, then at 221-231): tiles through registers (278 us), 256 rows on eight
 // waves (295), lines asked for two tiles ahead (245), equal shares of all tiles' steps for every workgroup with
 // fragments joined afterwards (278: the workgroups lose each other's L2 lines),
 // scheduling hints of the compiler (235-281).

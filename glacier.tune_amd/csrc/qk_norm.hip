@@ -10,8 +10,9 @@
 // fixed-order reduction over the lanes that hold it (turn.hpp), and queries and
 // keys share the launch.  Each lane reads its pieces before it writes them, so
 // outputs may lie on inputs.  Measured: 4096 tokens of 32/8 heads of 128, bf16,
-// 16.3 us (5.1 TB/s: part of it stays in the last-level cache; a 4 GiB copy
-// reaches 4.77); 8 tokens of 28/4 heads 3.9 us in a replayed graph, the launch.
+// 15.3-17 us (5.5-4.9 TB/s: part of it stays in the last-level cache; a 4 GiB copy
+// reaches 4.77), 15.2 without the rotation; fp32 30.8 and 28.2 (5.4, 6.0 TB/s); 8
+// tokens of 28/4 heads 3.6 us in a replayed graph, the launch (2.9 without).
 //
 // Weight gradients: a lane meets the same columns in every head and token, so
 // it sums them in registers; a workgroup's sums go to the workspace and a second
@@ -19,7 +20,9 @@
 // repeatable.  The backward holds four rows' pieces and four columns' sums a lane,
 // so its pieces are 8 bytes in bf16: with 16 it has registers for half the waves
 // (4096 tokens of 28/4 heads of 128, bf16, with weight gradients: 35 us against
-// 30.8, 3.3 TB/s, of them 4 in the second launch).
+// 30.8).  Now, in a replayed graph: 27.6 us (3.7 TB/s, of them 4 in the second
+// launch), 21.5 without weight gradients; as training calls it, without the rotation,
+// 25.7 and 20.1; fp32 37.8 and 32.7 with it, 36.8 and 32.0 without.
 #include "turn.hpp"
 
 namespace glacier {

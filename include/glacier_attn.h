@@ -219,7 +219,7 @@ int glacier_attn_synchronize(glacier_attn_ctx *ctx);
  * the key/value cache (glacier_attn_cache_*) are not. */
 int glacier_attn_set_kernel_timing(glacier_attn_ctx *ctx, int enable);
 
-/* Number of kernel kinds the library launches. */
+/* Number of kernel kinds that are timed. */
 int glacier_attn_kernel_count(void);
 
 /* Name of kernel kind `id`, or NULL. */

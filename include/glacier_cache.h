@@ -41,7 +41,8 @@
  * puts them off by up to pos * 2^-23 at far positions.)
  *
  * bf16 tensors: bf16 operands, fp32 sums and softmax; weights multiply V as two
- * bf16 terms, 16 bits of them.  fp32 tensors: fp32 throughout.  Results are
+ * bf16 terms, 16 bits of them.  fp32 tensors: fp32 throughout, whatever the
+ * context's precision.  Results are
  * bitwise repeatable for one layout of the work (below: max_new, max_kv).  NaN
  * and infinities in a token's K or V reach only the rows that see the token.  Sums
  * of up to as many terms of V as there are keys stay within fp32 (|V| below 2^127
