@@ -4,7 +4,7 @@
 // HBM-bound: each row is read once and written once, whole.  A wave takes one
 // token, or a share of its heads when there are few tokens; queries, keys and
 // values follow each other as heads of that token (turn.hpp).  The token's
-// sequence is found by all lanes at once (one load deep: a binary search would
+// sequence is found by all lanes at once (one load deep up to 64: a binary search would
 // chain one per halving), and the first rows are requested before it, since
 // only where they go depends on it.
 //

@@ -19,25 +19,30 @@ struct CacheSeq {
 __device__ inline int clamp_row(int r, int T) { return r < 0 ? 0 : r > T ? T : r; }
 
 // The sequence b with start(b, cu[b]) <= x < start(b + 1, cu[b + 1]), start
-// growing with b; b = n_seqs if there is none.  Every lane reads one sequence's
-// entries, 64 sequences at a time, and the lane that holds the sequence hands
-// them out: the search and the sequence's lengths are one load deep together.
+// growing with b; b = n_seqs if there is none.  Up to 64 sequences every lane reads
+// one's entries, and the lane that holds the sequence hands them out: the search
+// and the sequence's lengths are one load deep together.  More are narrowed down to
+// 64 first, 64 parts at a time.
 template <typename F>
 __device__ inline CacheSeq find_seq(const CacheView& c, int lane, int x, F start) {
   CacheSeq s{c.n_seqs, 0, 0, 0};
-  for (int b0 = 0; b0 < c.n_seqs; b0 += 64) {
-    const int b = b0 + lane, i = b < c.n_seqs ? b : c.n_seqs - 1;
-    const int from = clamp_row(c.cu[i], c.T), to = clamp_row(c.cu[i + 1], c.T), len = c.kv_lens[i];
-    const int before = __popcll(__ballot(b < c.n_seqs && start(i + 1, to) <= x));
-    if (before == 64) continue;
-    if (b0 + before >= c.n_seqs) break;
-    s.b = b0 + before;
-    s.tok0 = __builtin_amdgcn_readlane(from, before);
-    const int end = __builtin_amdgcn_readlane(to, before);
-    s.n = end > s.tok0 ? end - s.tok0 : 0;
-    s.pos0 = __builtin_amdgcn_readlane(len, before) - s.n;
-    break;
+  int b0 = 0, end = c.n_seqs;  // the sequence is in here, if anywhere
+  while (end - b0 > 64) {
+    const int part = (end - b0 + 63) / 64, last = min(end, b0 + (lane + 1) * part) - 1;
+    const int before = __popcll(__ballot(b0 + lane * part < end && start(last + 1, clamp_row(c.cu[last + 1], c.T)) <= x));
+    b0 += before * part;
+    if (b0 >= end) return s;
+    end = min(end, b0 + part);
   }
+  const int b = b0 + lane, i = b < end ? b : end - 1;
+  const int from = clamp_row(c.cu[i], c.T), to = clamp_row(c.cu[i + 1], c.T), len = c.kv_lens[i];
+  const int before = __popcll(__ballot(b < end && start(i + 1, to) <= x));
+  if (b0 + before >= end) return s;
+  s.b = b0 + before;
+  s.tok0 = __builtin_amdgcn_readlane(from, before);
+  const int to_row = __builtin_amdgcn_readlane(to, before);
+  s.n = to_row > s.tok0 ? to_row - s.tok0 : 0;
+  s.pos0 = __builtin_amdgcn_readlane(len, before) - s.n;
   return s;
 }
 // The sequence that token row t belongs to.

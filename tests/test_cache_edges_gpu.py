@@ -194,3 +194,53 @@ def test_an_infinite_value_in_the_last_split(eng, seqs, hq, hkv, d, keys):
             rest[sees, :, 3::7] = math.nan
             ch.check("out", torch.where(rest.isnan().cuda(), 0.0, out.double()), rest, ref[1])
             ch.check("lse", lse, ref[2], ref[3])
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("count", [65, 4096, 4097, 20000])
+def test_many_sequences_most_of_them_idle(eng, dt, count):
+    # chunks and single tokens at both ends of a long batch and within it
+    busy = {0: (40, 90), 1: (1, 7), count // 3: (1, 200), count // 2: (70, 70), count - 2: (3, 30), count - 1: (1, 65)}
+    seqs = [busy.get(b, (0, 0)) for b in range(count)]
+    p = ch.Paged(seqs, 8, 2, 64, 16, DTYPES[dt], 40, pad=2)
+    out = torch.full((p.tokens, 8, 64), 7.0, device="cuda", dtype=DTYPES[dt])
+    lse = torch.full((8, p.tokens), 7.0, device="cuda")
+    ref = ch.attend_ref(p)
+    for hints in ({}, dict(max_new=70, max_kv=200), dict(max_new=70, max_kv=90000)):
+        eng.cache_forward(p.q.cuda(), *p.arrays(), out=out, lse=lse, **hints)
+        ch.check("out", out, ref[0], ref[1])
+        ch.check("lse", lse, ref[2], ref[3])
+        assert (out[-2:] == 7.0).all() and (lse[:, -2:] == 7.0).all()
+    k = torch.randn(p.tokens, 2, 64, device="cuda").to(DTYPES[dt])
+    eng.cache_append(k, 2 * k, *p.arrays())
+    t = 0
+    for b, (n, kv) in sorted(busy.items()):
+        for pos in range(kv - n, kv):
+            page = int(p.table[b, pos // 16])
+            assert torch.equal(p.k_pages[page, :, pos % 16], k[t]) and torch.equal(p.v_pages[page, :, pos % 16], 2 * k[t])
+            t += 1
+
+
+def test_the_search_for_a_sequence_does_not_grow_with_the_batch(eng):
+    # 2^19 sequences, all but two idle: a search that looks at all of them in turn in
+    # each of as many workgroups takes half a second here, a narrowing one some ms
+    n, page = 2 ** 19, 16
+    p = ch.Paged([(1, 40), (5, 33)], 8, 1, 64, page, BF16, 41)
+    cu = torch.full((n + 1,), 6, device="cuda", dtype=torch.int32)
+    cu[:n // 2 + 1] = 0
+    cu[n // 2 + 1:n] = 1
+    lens = torch.zeros(n, device="cuda", dtype=torch.int32)
+    lens[n // 2], lens[n - 1] = 40, 33
+    table = torch.full((n, p.table.shape[1]), -1, device="cuda", dtype=torch.int32)
+    table[n // 2], table[n - 1] = p.table[0], p.table[1]
+    args = (p.q.cuda(), p.k_pages, p.v_pages, cu, lens, table)
+    ref = ch.attend_ref(p)
+    out, lse = eng.cache_forward(*args, save=True)
+    ch.check("out", out, ref[0], ref[1])
+    ch.check("lse", lse, ref[2], ref[3])
+    start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    eng.cache_forward(*args, save=True)
+    stop.record()
+    torch.cuda.synchronize()
+    assert start.elapsed_time(stop) < 100.0, f"{start.elapsed_time(stop)} ms"
