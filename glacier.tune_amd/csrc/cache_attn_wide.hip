@@ -34,10 +34,12 @@
 // MFMAs are busy 47% and vector instructions issue 37%; waves spend 42% of theirs ready
 // and waiting for the other's instruction; tiles of 448 workgroups on 512 places leave
 // an eighth of the card idle.  1024 tokens over 8192 keys, 8/2 heads of 256, one wave a
-// SIMD: 116-121 us (550-530 TFLOP/s), MFMAs busy 36%.  Tried and slower (with one term, then at 221-231): tiles through registers (278 us), 256 rows on eight
-// waves (295), lines asked for two tiles ahead (245), equal shares of all tiles' steps for every workgroup with
-// fragments joined afterwards (278: the workgroups lose each other's L2 lines),
-// scheduling hints of the compiler (235-281).
+// SIMD: 116-121 us (550-530 TFLOP/s), MFMAs busy 36%.
+//
+// Tried and slower (with one term, then at 221-231): tiles through registers (278 us),
+// 256 rows on eight waves (295), lines asked for two tiles ahead (245), equal shares of
+// all tiles' steps for every workgroup with fragments joined afterwards (278: the
+// workgroups lose each other's L2 lines), scheduling hints of the compiler (235-281).
 #include "cache_tiles.hpp"
 
 namespace glacier {
