@@ -18,8 +18,9 @@ columns 32 i + 8 c .., scale row G + i is group i's.  Values: word (row / 4 4 G 
 4 + row % 4 holds columns 8 r .., scale (row / 4 G + i) 4 + row % 4 is group i's.
 
 Weights.  [out / 16][in / 128][64] times four words: word i of entry 16 c + r holds
-row r's columns 32 i + 8 c .. of the block; then the scales [out / 16][in / group][16]
-in fp16, then, where there are any, the offsets alike: a weight is (n - 8) s + offset.
+row r's columns 32 i + 8 c .. of the block; then the scales [out / 16][in / 128][16]
+[128 / group] in fp16, then, where there are any, the offsets alike: a weight is
+(n - 8) s + offset.
 Rows and columns are padded with zeros.
 """
 import math
@@ -32,7 +33,7 @@ import torch
 own = False
 
 DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
-LARGEST = 7936.0  # of the cache's scales
+LARGEST = 2688.0  # of the cache's scales
 _engine = None
 
 
@@ -227,7 +228,8 @@ def _packed(n, scales, mins, group):
     for t in (scales, mins):
         if t is not None:
             t = torch.nn.functional.pad(t, (0, n.shape[1] // group - t.shape[1], 0, -rows % 16))
-            found.append(t.unflatten(0, (-1, 16)).transpose(1, 2).reshape(-1).view(torch.uint8))
+            t = t.unflatten(1, (-1, 128 // group)).unflatten(0, (-1, 16)).transpose(1, 2)
+            found.append(t.reshape(-1).view(torch.uint8))
     return torch.cat(found)
 
 
@@ -237,7 +239,8 @@ def _weights(packed, rows, cols, group, mins):
     size, groups = tiles * blocks * 1024, blocks * 128 // group
     n = _numbers(packed[:size].view(torch.int32).view(tiles, blocks, 4, 16, 4).permute(0, 3, 1, 4, 2))
     n = n.reshape(tiles * 16, groups, group)
-    rest = packed[size:].view(torch.float16).view(-1, tiles, groups, 16).transpose(2, 3).reshape(-1, tiles * 16, groups)
+    rest = packed[size:].view(torch.float16).view(-1, tiles, blocks, 16, 128 // group)
+    rest = rest.transpose(2, 3).reshape(-1, tiles * 16, groups)
     w = n * rest[0].float()[..., None]
     if mins:
         w += rest[1].float()[..., None]
@@ -476,15 +479,15 @@ def exact(case, seed):
         col = torch.arange(case["width"], device="cuda")
         for p in s["projs"]:
             y = torch.empty(x.shape[0], p["out"], device="cuda", dtype=torch.float64)
-            tiles, groups = -(-p["out"] // 16), blocks * 128 // group
+            tiles = -(-p["out"] // 16)
             for r0 in range(0, p["out"], 2048):
                 row = torch.arange(r0, min(p["out"], r0 + 2048), device="cuda")[:, None]
                 word = (((row // 16) * blocks + col // 128) * 64 + col % 32 // 8 * 16 + row % 16) * 4 + col % 128 // 32
-                at = ((row // 16) * groups + col // group) * 16 + row % 16
+                at = (((row // 16) * blocks + col // 128) * 16 + row % 16) * (128 // group) + col % 128 // group
                 scales = p["w"][tiles * blocks * 1024:]
                 w = (_nibble(p["w"], word, col) - 8).double() * _half(scales, at)
                 if case["mins"]:
-                    w += _half(scales[tiles * groups * 32:], at)
+                    w += _half(scales[tiles * blocks * 4096 // group:], at)
                 y[:, r0:r0 + 2048] = x @ w.t()
             if case["rank"]:
                 y += p["scaling"] * ((x @ p["a"].double()) @ p["b"].double())
