@@ -55,6 +55,9 @@ SOURCES = {
     "cache_append.hip": (),
     "cache_attn.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
     "cache_attn_wide.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
+    "qcache_append.hip": (),
+    "qcache_attn.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
+    "proj_quant.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
     "lmhead.hip": (),
     "lora_file.cpp": (),
     "engine.cpp": (),

@@ -675,6 +675,10 @@ hipError_t launch_cache_attn(const CacheAttn& a, hipStream_t st) {
     GL_CHECK(a.c.io_bf16 ? by_head<bf16>(a, st) : by_head<float>(a, st));
   // few splits of wide tiles are joined by tiles (launch_cache_attn_wide)
   if (a.n_splits == 1 || (a.rows == kCacheWideRows && a.n_splits <= kCacheTileJoin)) return hipSuccess;
+  return launch_cache_join(a, st);
+}
+
+hipError_t launch_cache_join(const CacheAttn& a, hipStream_t st) {
   return a.c.io_bf16 ? join<bf16>(a, st) : join<float>(a, st);
 }
 

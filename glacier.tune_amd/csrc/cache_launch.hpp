@@ -80,6 +80,8 @@ struct CachePlan {
 };
 CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, int n_cu);
 hipError_t launch_cache_attn(const CacheAttn& a, hipStream_t st);
+// Joins the splits' sums of tiles of at most 32 rows (a.n_splits > 1).
+hipError_t launch_cache_join(const CacheAttn& a, hipStream_t st);
 
 constexpr int kCacheWideRows = 128;  // rows of a tile of cache_attn_wide.hip
 constexpr int kCacheTileJoin = 8;     // up to so many splits it joins them itself, tile by tile;

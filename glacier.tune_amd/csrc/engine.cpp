@@ -23,6 +23,7 @@
 
 #include "../../include/glacier_attn.h"
 #include "../../include/glacier_cache.h"
+#include "../../include/glacier_quant.h"
 #include "../../include/glacier_lmhead.h"
 #include "../../include/glacier_norm.h"
 #include "../../include/glacier_qkv.h"
@@ -34,6 +35,7 @@
 #include "noalloc.hpp"
 #include "norm_launch.hpp"
 #include "proj_launch.hpp"
+#include "quant_launch.hpp"
 
 namespace glacier {
 
@@ -851,6 +853,31 @@ class GpuAttentionEngine {
     check_hip(launch_cache_attn(a, stream()), "cache attention launch");
   }
 
+  // ---- answering in 4 bits (glacier_quant.h) ------------------------------
+  void AppendToQuantCache(const CacheAppend& a, float base) {
+    if (a.c.T == 0 || a.c.n_seqs == 0) return;
+    check_hip(launch_qcache_append(a, turn_rates(base, a.c.D), n_cu_, stream()), "4-bit cache append launch");
+  }
+  void ReadQuantCache(const QCacheRead& a) {
+    if (a.c.T == 0 || a.c.n_seqs == 0) return;
+    check_hip(launch_qcache_read(a, n_cu_, stream()), "4-bit cache read launch");
+  }
+  QCachePlan PlanQuantCacheAttention(const CacheView& c, int hq, int max_new, int max_kv) const {
+    if (c.T == 0 || c.n_seqs == 0) return QCachePlan{};
+    return qcache_attn_plan(c, hq, max_new, max_kv, n_cu_);
+  }
+  void AttendToQuantCache(const CacheAttn& a, const QCachePlan& plan, void* workspace) {
+    if (a.c.T == 0 || a.c.n_seqs == 0) return;
+    check_hip(launch_qcache_attn(a, plan, workspace, stream()), "4-bit cache attention launch");
+  }
+  void PackQuantWeights(const QuantPack& a) {
+    check_hip(launch_quant_pack(a, stream()), "4-bit weights layout launch");
+  }
+  void QuantProjForward(const QuantProj& q) {
+    if (q.a.T == 0) return;
+    check_hip(launch_quant_proj(q, n_cu_, stream()), "4-bit projection launch");
+  }
+
   // ---- LM-head cross-entropy (glacier_lmhead.h) -------------------------
   // FusedCrossEntropyLoss.ComputeLoss / ComputeLossAndGradients
   // (FusedCrossEntropyLoss.cs:38-364): the kept rows are found on the host
@@ -1419,7 +1446,8 @@ size_t qk_norm_workspace(const QkNorm& a) { return sizeof(float) * kQkMaxGroups 
 
 // Checks a cache and a batch (not the device arrays' contents, which the
 // kernels bound) and fills their part of a launch.
-CacheView cache_view_of(const glacier_kv_cache* cache, const glacier_cache_batch* batch) {
+// quant: the pages of glacier_quant.h, whose strides count bytes.
+CacheView cache_view_of(const glacier_kv_cache* cache, const glacier_cache_batch* batch, bool quant = false) {
   if (cache == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "cache is NULL");
   if (batch == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "batch is NULL");
   const glacier_kv_cache& k = *cache;
@@ -1432,10 +1460,14 @@ CacheView cache_view_of(const glacier_kv_cache* cache, const glacier_cache_batch
   if (k.page_size < 16 || k.page_size > 1024 || (k.page_size & (k.page_size - 1)) != 0)
     fail(GLACIER_ATTN_ERR_UNSUPPORTED, "page_size must be a power of two from 16 to 1024, not " +
                                            std::to_string(k.page_size));
-  const long long page = (long long)k.n_heads_kv * k.page_size * k.head_dim;
+  const long long page =
+      (long long)k.n_heads_kv * k.page_size * (quant ? quant_row_bytes(k.head_dim) : k.head_dim);
   if (k.page_stride < page)
-    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "page_stride must be at least n_heads_kv page_size head_dim");
-  if (k.page_stride % 8 != 0) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "page_stride must be a multiple of 8");
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, quant ? "page_stride must be at least a page's bytes"
+                                                  : "page_stride must be at least n_heads_kv page_size head_dim");
+  const int unit = quant ? 16 : 8;
+  if (k.page_stride % unit != 0)
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "page_stride must be a multiple of " + std::to_string(unit));
   if (k.page_stride >= (1LL << 40) || (long long)k.n_pages * k.page_stride >= (1LL << 46))
     fail(GLACIER_ATTN_ERR_UNSUPPORTED, "cache too large");
   if (b.n_seqs < 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "n_seqs must be >= 0");
@@ -1476,30 +1508,37 @@ void need_cache_arrays(const CacheView& c) {
   need_row_tensor(c.v_pages, "v_pages", c.n_pages > 0);
 }
 
+// Bytes of a page, and from one to the next.
+struct PageBytes {
+  long long page, stride;
+};
+PageBytes page_bytes(const CacheView& c, bool quant) {
+  if (quant) return {((long long)c.hkv << c.page_shift) * quant_row_bytes(c.D), c.page_stride};
+  const long long esz = c.io_bf16 ? 2 : 4;
+  return {esz * ((long long)c.hkv << c.page_shift) * c.D, esz * c.page_stride};
+}
 // A tensor that shares memory with one of the pages at `pages`.
-void need_off_pages(const CacheView& c, const void* pages, const char* pages_name, const void* p, size_t bytes,
-                    const char* name) {
+void need_off_pages(const CacheView& c, PageBytes b, const void* pages, const char* pages_name, const void* p,
+                    size_t bytes, const char* name) {
   if (pages == nullptr || p == nullptr || bytes == 0) return;
-  const long long esz = c.io_bf16 ? 2 : 4, stride = esz * c.page_stride;
-  const long long page = esz * ((long long)c.hkv << c.page_shift) * c.D;
   const long long at = static_cast<long long>(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(pages));
   // the first page that ends behind the tensor's begin
-  const long long first = at < page ? 0 : (at - page) / stride + 1;
-  if (first < c.n_pages && first * stride < at + static_cast<long long>(bytes))
+  const long long first = at < b.page ? 0 : (at - b.page) / b.stride + 1;
+  if (first < c.n_pages && first * b.stride < at + static_cast<long long>(bytes))
     fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, std::string(name) + " overlaps " + pages_name);
 }
-void need_off_both(const CacheView& c, const void* p, size_t bytes, const char* name) {
-  need_off_pages(c, c.k_pages, "k_pages", p, bytes, name);
-  need_off_pages(c, c.v_pages, "v_pages", p, bytes, name);
+void need_off_both(const CacheView& c, const void* p, size_t bytes, const char* name, bool quant = false) {
+  need_off_pages(c, page_bytes(c, quant), c.k_pages, "k_pages", p, bytes, name);
+  need_off_pages(c, page_bytes(c, quant), c.v_pages, "v_pages", p, bytes, name);
 }
 // K and V pages that share memory.  (Whichever begin later: where their first page
 // lies in a gap of the others, their i-th one lies i gaps further.)
-void need_pages_apart(const CacheView& c) {
-  const size_t page = (c.io_bf16 ? 2 : 4) * ((size_t)c.hkv << c.page_shift) * c.D;
+void need_pages_apart(const CacheView& c, bool quant = false) {
+  const PageBytes b = page_bytes(c, quant);
   if (reinterpret_cast<uintptr_t>(c.k_pages) <= reinterpret_cast<uintptr_t>(c.v_pages))
-    need_off_pages(c, c.k_pages, "k_pages", c.v_pages, page, "v_pages");
+    need_off_pages(c, b, c.k_pages, "k_pages", c.v_pages, b.page, "v_pages");
   else
-    need_off_pages(c, c.v_pages, "v_pages", c.k_pages, page, "k_pages");
+    need_off_pages(c, b, c.v_pages, "v_pages", c.k_pages, b.page, "k_pages");
 }
 
 // Query heads of a call over the cache.
@@ -1515,6 +1554,100 @@ void need_cache_size(const CacheView& c, long long heads) {
   if (c.T * heads >= (1LL << 26)) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
   if ((long long)c.n_seqs * c.hkv >= (1LL << 22))
     fail(GLACIER_ATTN_ERR_UNSUPPORTED, "too many sequences");
+}
+
+// Weights in 4 bits: checked, and where their parts begin.
+QuantLayout quant_layout_of(long long out, long long in, int group, int offsets) {
+  if (out <= 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "out_features must be positive");
+  if (in <= 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "in_features must be positive");
+  if (group != 32 && group != 64 && group != 128)
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "group must be 32, 64 or 128, not " + std::to_string(group));
+  if (offsets != 0 && offsets != 1) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "offsets must be 0 or 1");
+  if (out % 4 != 0) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "out_features must be a multiple of 4");
+  if (in % 32 != 0 || in % group != 0)
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "in_features must be a multiple of 32 and of group");
+  if (out * in >= (1LL << 31)) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
+  return quant_layout(out, in, group, offsets != 0);
+}
+QuantLayout quant_layout_of(const glacier_quant_weights* w) {
+  if (w == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "w is NULL");
+  return quant_layout_of(w->out_features, w->in_features, w->group, w->offsets);
+}
+
+// The sizes of a call with 4-bit weights, checked; its pointers as they are.
+QuantProj quant_proj_of(const glacier_quant_proj_desc* desc, const glacier_lora_proj* proj, int n_proj) {
+  if (desc == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "desc is NULL");
+  const glacier_quant_proj_desc& d = *desc;
+  if (d.total_tokens < 0) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "total_tokens must be >= 0");
+  if (d.io_dtype != GLACIER_ATTN_IO_F32 && d.io_dtype != GLACIER_ATTN_IO_BF16)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "unknown io dtype " + std::to_string(d.io_dtype));
+  if (proj == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "proj is NULL");
+  if (n_proj < 1 || n_proj > GLACIER_PROJ_MAX_PROJ)
+    fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "n_proj must be 1.." + std::to_string(GLACIER_PROJ_MAX_PROJ));
+  QuantProj q{};
+  q.a.T = d.total_tokens;
+  q.a.in = d.in_features;
+  q.a.rank = d.rank;
+  q.a.io_bf16 = d.io_dtype == GLACIER_ATTN_IO_BF16;
+  q.a.n_proj = n_proj;
+  q.group = d.group;
+  q.offsets = d.offsets != 0;
+  if ((long long)d.total_tokens * std::max(d.in_features, 1) >= (1LL << 31))
+    fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
+  for (int p = 0; p < n_proj; ++p) {
+    const glacier_lora_proj& g = proj[p];
+    const std::string at = "proj[" + std::to_string(p) + "]";
+    (void)quant_layout_of(g.out_features, d.in_features, d.group, d.offsets);
+    if ((long long)d.total_tokens * g.out_features >= (1LL << 31))
+      fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
+    if (g.lora_a != nullptr) {
+      if (g.lora_b == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, at + ".lora_b is NULL");
+      if (!std::isfinite(g.scaling)) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, at + ".scaling is not finite");
+      if (d.rank < 1 || d.rank > GLACIER_PROJ_MAX_RANK)
+        fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT,
+             "rank must be 1.." + std::to_string(GLACIER_PROJ_MAX_RANK) + " when an adapter is given");
+    }
+    q.a.p[p] = ProjSpec{g.w, g.bias, g.lora_a, g.lora_b, g.scaling, g.out_features, g.y, nullptr, nullptr, nullptr};
+  }
+  return q;
+}
+// x A_p of every projection (in its place also without an adapter).
+size_t quant_proj_workspace(const QuantProj& q) {
+  bool any = false;
+  for (int p = 0; p < q.a.n_proj; ++p) any = any || q.a.p[p].a != nullptr;
+  return any ? sizeof(float) * q.a.n_proj * (size_t)q.a.T * q.a.rank : 0;
+}
+void need_quant_tensors(const QuantProj& q, const void* x) {
+  const ProjLaunch& a = q.a;
+  const size_t esz = a.io_bf16 ? 2 : 4, xb = esz * a.T * a.in;
+  const bool rows = a.T > 0;
+  need_row_tensor(x, "x", rows);
+  for (int p = 0; p < a.n_proj; ++p) {
+    const ProjSpec& s = a.p[p];
+    const std::string at = "proj[" + std::to_string(p) + "]";
+    need_row_tensor(s.w, (at + ".w").c_str(), rows);
+    need_row_tensor(s.y, (at + ".y").c_str(), rows);
+    need_row_tensor(s.a, (at + ".lora_a").c_str(), false);
+    need_row_tensor(s.b, (at + ".lora_b").c_str(), false);
+  }
+  if (!rows) return;
+  for (int p = 0; p < a.n_proj; ++p) {
+    const ProjSpec& s = a.p[p];
+    const std::string name = "proj[" + std::to_string(p) + "].y";
+    const size_t yb = esz * a.T * s.out;
+    need_apart(s.y, yb, name.c_str(), x, xb, "x", false);
+    for (int i = 0; i < a.n_proj; ++i) {
+      const ProjSpec& o = a.p[i];
+      const std::string at = "proj[" + std::to_string(i) + "]";
+      if (i != p) need_apart(s.y, yb, name.c_str(), o.y, esz * a.T * o.out, (at + ".y").c_str(), false);
+      need_apart(s.y, yb, name.c_str(), o.w, quant_layout(o.out, a.in, q.group, q.offsets).bytes,
+                 (at + ".w").c_str(), false);
+      need_apart(s.y, yb, name.c_str(), o.bias, sizeof(float) * o.out, (at + ".bias").c_str(), false);
+      need_apart(s.y, yb, name.c_str(), o.a, sizeof(float) * a.in * a.rank, (at + ".lora_a").c_str(), false);
+      need_apart(s.y, yb, name.c_str(), o.a != nullptr ? o.b : nullptr, sizeof(float) * a.rank * o.out,
+                 (at + ".lora_b").c_str(), false);
+    }
+  }
 }
 
 void need(const void* p, const char* name) {
@@ -1877,12 +2010,15 @@ int glacier_rmsnorm_qk_backward(glacier_attn_ctx* ctx, const glacier_rmsnorm_qk_
   });
 }
 
-int glacier_attn_cache_append(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
-                              const glacier_cache_batch* batch, const void* k, const void* v,
-                              float rope_freq_base, int32_t n_heads_q, const void* q, void* q_rot) {
+namespace {
+
+// glacier_attn_cache_append, or (quant) glacier_attn_qcache_append
+int append_call(glacier_attn_ctx* ctx, const glacier_kv_cache* cache, const glacier_cache_batch* batch,
+                const void* k, const void* v, float rope_freq_base, int32_t n_heads_q, const void* q, void* q_rot,
+                bool quant) {
   return guarded([&] {
     glacier::CacheAppend a{};
-    a.c = glacier::cache_view_of(cache, batch);
+    a.c = glacier::cache_view_of(cache, batch, quant);
     glacier::need_base(rope_freq_base);
     const bool rows = a.c.T > 0 && a.c.n_seqs > 0;
     if (q != nullptr) {
@@ -1900,11 +2036,11 @@ int glacier_attn_cache_append(glacier_attn_ctx* ctx, const glacier_kv_cache* cac
     const size_t esz = a.c.io_bf16 ? 2 : 4;
     const size_t qb = esz * a.c.T * a.hq * a.c.D, kb = esz * a.c.T * a.c.hkv * a.c.D;
     if (rows) {
-      glacier::need_pages_apart(a.c);
-      glacier::need_off_both(a.c, k, kb, "k");
-      glacier::need_off_both(a.c, v, kb, "v");
-      if (q != nullptr) glacier::need_off_both(a.c, q, qb, "q");
-      if (q != nullptr) glacier::need_off_both(a.c, q_rot, qb, "q_rot");
+      glacier::need_pages_apart(a.c, quant);
+      glacier::need_off_both(a.c, k, kb, "k", quant);
+      glacier::need_off_both(a.c, v, kb, "v", quant);
+      if (q != nullptr) glacier::need_off_both(a.c, q, qb, "q", quant);
+      if (q != nullptr) glacier::need_off_both(a.c, q_rot, qb, "q_rot", quant);
     }
     if (q != nullptr) {
       glacier::need_apart(q_rot, qb, "q_rot", q, qb, "q", true);
@@ -1916,9 +2052,64 @@ int glacier_attn_cache_append(glacier_attn_ctx* ctx, const glacier_kv_cache* cac
     a.k = k; a.v = v; a.q = q; a.q_rot = q_rot;
     std::lock_guard<std::mutex> g(ctx->eng->lock());
     glacier::DeviceScope on(ctx->eng->device());
-    ctx->eng->AppendToCache(a, rope_freq_base);
+    if (quant)
+      ctx->eng->AppendToQuantCache(a, rope_freq_base);
+    else
+      ctx->eng->AppendToCache(a, rope_freq_base);
   });
 }
+
+}  // namespace
+
+int glacier_attn_cache_append(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
+                              const glacier_cache_batch* batch, const void* k, const void* v,
+                              float rope_freq_base, int32_t n_heads_q, const void* q, void* q_rot) {
+  return append_call(ctx, cache, batch, k, v, rope_freq_base, n_heads_q, q, q_rot, false);
+}
+
+int glacier_attn_qcache_append(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
+                               const glacier_cache_batch* batch, const void* k, const void* v,
+                               float rope_freq_base, int32_t n_heads_q, const void* q, void* q_rot) {
+  return append_call(ctx, cache, batch, k, v, rope_freq_base, n_heads_q, q, q_rot, true);
+}
+
+size_t glacier_attn_qcache_page_bytes(const glacier_kv_cache* cache) {
+  size_t bytes = 0;
+  (void)guarded([&] {
+    if (cache == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "cache is NULL");
+    glacier_kv_cache k = *cache;
+    k.page_stride = 1LL << 39;  // any that holds a page
+    k.n_pages = 0;
+    const glacier_cache_batch none{};
+    bytes = glacier::page_bytes(glacier::cache_view_of(&k, &none, true), true).page;
+  });
+  return bytes;
+}
+
+int glacier_attn_qcache_read(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
+                             const glacier_cache_batch* batch, void* k, void* v) {
+  return guarded([&] {
+    glacier::QCacheRead a{};
+    a.c = glacier::cache_view_of(cache, batch, true);
+    glacier::need_cache_size(a.c, 2LL * a.c.hkv);
+    glacier::need_cache_arrays(a.c);
+    const bool rows = a.c.T > 0 && a.c.n_seqs > 0;
+    glacier::need_row_tensor(k, "k", rows);
+    glacier::need_row_tensor(v, "v", rows);
+    const size_t kb = (a.c.io_bf16 ? 2 : 4) * (size_t)a.c.T * a.c.hkv * a.c.D;
+    glacier::need_apart(k, kb, "k", v, kb, "v", false);
+    if (rows) {
+      glacier::need_off_both(a.c, k, kb, "k", true);
+      glacier::need_off_both(a.c, v, kb, "v", true);
+    }
+    need(ctx, "ctx");
+    a.k = k; a.v = v;
+    std::lock_guard<std::mutex> g(ctx->eng->lock());
+    glacier::DeviceScope on(ctx->eng->device());
+    ctx->eng->ReadQuantCache(a);
+  });
+}
+
 
 size_t glacier_attn_cache_workspace(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
                                     const glacier_cache_batch* batch, int32_t n_heads_q) {
@@ -1933,38 +2124,52 @@ size_t glacier_attn_cache_workspace(glacier_attn_ctx* ctx, const glacier_kv_cach
   return bytes;
 }
 
+namespace {
+
+// The arguments of an attention call over the cache, checked, but for its layout.
+glacier::CacheAttn attention_of(const glacier_kv_cache* cache, const glacier_cache_batch* batch, int32_t n_heads_q,
+                                const void* q, void* out, float* lse, bool quant) {
+  glacier::CacheAttn a{};
+  a.c = glacier::cache_view_of(cache, batch, quant);
+  glacier::need_heads_q(a.c, n_heads_q);
+  glacier::need_cache_size(a.c, n_heads_q);
+  glacier::need_cache_arrays(a.c);
+  const bool rows = a.c.T > 0 && a.c.n_seqs > 0;
+  glacier::need_row_tensor(q, "q", rows);
+  glacier::need_row_tensor(out, "out", rows);
+  const size_t qb = (a.c.io_bf16 ? 2 : 4) * (size_t)a.c.T * n_heads_q * a.c.D;
+  const size_t lb = sizeof(float) * a.c.T * n_heads_q;
+  glacier::need_apart(out, qb, "out", q, qb, "q", true);
+  glacier::need_apart(lse, lb, "lse", q, qb, "q", false);
+  glacier::need_apart(lse, lb, "lse", out, qb, "out", false);
+  if (rows) {
+    glacier::need_off_both(a.c, out, qb, "out", quant);
+    glacier::need_off_both(a.c, lse, lb, "lse", quant);
+  }
+  a.hq = n_heads_q;
+  a.group = n_heads_q / a.c.hkv;
+  a.scale_log2 = glacier::kLog2e / std::sqrt(static_cast<float>(a.c.D));
+  a.q = q; a.out = out; a.lse = lse;
+  return a;
+}
+void lay_out(glacier::CacheAttn& a, const glacier::CachePlan& p) {
+  a.rows = p.rows;
+  a.long_first = p.long_first;
+  a.n_splits = p.n_splits;
+  a.split_keys = p.split_keys;
+}
+
+}  // namespace
+
 int glacier_attn_cache_forward(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
                                const glacier_cache_batch* batch, int32_t n_heads_q, const void* q, void* out,
                                float* lse, void* workspace, size_t workspace_bytes) {
   return guarded([&] {
-    glacier::CacheAttn a{};
-    a.c = glacier::cache_view_of(cache, batch);
-    glacier::need_heads_q(a.c, n_heads_q);
-    glacier::need_cache_size(a.c, n_heads_q);
-    glacier::need_cache_arrays(a.c);
-    const bool rows = a.c.T > 0 && a.c.n_seqs > 0;
-    glacier::need_row_tensor(q, "q", rows);
-    glacier::need_row_tensor(out, "out", rows);
-    const size_t qb = (a.c.io_bf16 ? 2 : 4) * (size_t)a.c.T * n_heads_q * a.c.D;
-    const size_t lb = sizeof(float) * a.c.T * n_heads_q;
-    glacier::need_apart(out, qb, "out", q, qb, "q", true);
-    glacier::need_apart(lse, lb, "lse", q, qb, "q", false);
-    glacier::need_apart(lse, lb, "lse", out, qb, "out", false);
-    if (rows) {
-      glacier::need_off_both(a.c, out, qb, "out");
-      glacier::need_off_both(a.c, lse, lb, "lse");
-    }
+    glacier::CacheAttn a = attention_of(cache, batch, n_heads_q, q, out, lse, false);
     need(ctx, "ctx");
     const glacier::CachePlan p = ctx->eng->PlanCacheAttention(a.c, n_heads_q, batch->max_new, batch->max_kv);
     glacier::need_workspace(workspace, workspace_bytes, p.bytes);
-    a.hq = n_heads_q;
-    a.group = n_heads_q / a.c.hkv;
-    a.scale_log2 = glacier::kLog2e / std::sqrt(static_cast<float>(a.c.D));
-    a.q = q; a.out = out; a.lse = lse;
-    a.rows = p.rows;
-    a.long_first = p.long_first;
-    a.n_splits = p.n_splits;
-    a.split_keys = p.split_keys;
+    lay_out(a, p);
     if (p.n_splits > 1) {
       const size_t sums = p.n_splits * (size_t)a.c.T * n_heads_q * a.c.D;
       a.part_o = static_cast<float*>(workspace);
@@ -1973,6 +2178,83 @@ int glacier_attn_cache_forward(glacier_attn_ctx* ctx, const glacier_kv_cache* ca
     std::lock_guard<std::mutex> g(ctx->eng->lock());
     glacier::DeviceScope on(ctx->eng->device());
     ctx->eng->AttendToCache(a);
+  });
+}
+
+size_t glacier_attn_qcache_workspace(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
+                                     const glacier_cache_batch* batch, int32_t n_heads_q) {
+  size_t bytes = 0;
+  (void)guarded([&] {
+    const glacier::CacheView c = glacier::cache_view_of(cache, batch, true);
+    glacier::need_heads_q(c, n_heads_q);
+    glacier::need_cache_size(c, n_heads_q);
+    need(ctx, "ctx");
+    bytes = ctx->eng->PlanQuantCacheAttention(c, n_heads_q, batch->max_new, batch->max_kv).bytes;
+  });
+  return bytes;
+}
+
+int glacier_attn_qcache_forward(glacier_attn_ctx* ctx, const glacier_kv_cache* cache,
+                                const glacier_cache_batch* batch, int32_t n_heads_q, const void* q, void* out,
+                                float* lse, void* workspace, size_t workspace_bytes) {
+  return guarded([&] {
+    glacier::CacheAttn a = attention_of(cache, batch, n_heads_q, q, out, lse, true);
+    need(ctx, "ctx");
+    const glacier::QCachePlan p = ctx->eng->PlanQuantCacheAttention(a.c, n_heads_q, batch->max_new, batch->max_kv);
+    glacier::need_workspace(workspace, workspace_bytes, p.bytes);
+    lay_out(a, p.attn);
+    std::lock_guard<std::mutex> g(ctx->eng->lock());
+    glacier::DeviceScope on(ctx->eng->device());
+    ctx->eng->AttendToQuantCache(a, p, workspace);
+  });
+}
+
+size_t glacier_proj_quant_bytes(const glacier_quant_weights* w) {
+  size_t bytes = 0;
+  (void)guarded([&] { bytes = glacier::quant_layout_of(w).bytes; });
+  return bytes;
+}
+
+int glacier_proj_quant_pack(glacier_attn_ctx* ctx, const glacier_quant_weights* w, const void* numbers,
+                            const void* scales, const void* offsets, void* packed) {
+  return guarded([&] {
+    const glacier::QuantLayout l = glacier::quant_layout_of(w);
+    need(numbers, "numbers"); need(scales, "scales"); need(packed, "packed");
+    if ((offsets != nullptr) != (w->offsets != 0))
+      fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, w->offsets ? "offsets is NULL" : "offsets are given for weights without them");
+    if (!glacier::aligned16(packed)) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "packed must be 16-byte aligned");
+    if (((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(offsets)) & 1) != 0)
+      fail(GLACIER_ATTN_ERR_UNSUPPORTED, "scales and offsets must be 2-byte aligned");
+    const size_t nb = (size_t)w->out_features * w->in_features / 2;
+    const size_t sb = (size_t)w->out_features * (w->in_features / w->group) * 2;
+    glacier::need_apart(packed, l.bytes, "packed", numbers, nb, "numbers", false);
+    glacier::need_apart(packed, l.bytes, "packed", scales, sb, "scales", false);
+    glacier::need_apart(packed, l.bytes, "packed", offsets, sb, "offsets", false);
+    need(ctx, "ctx");
+    std::lock_guard<std::mutex> g(ctx->eng->lock());
+    glacier::DeviceScope on(ctx->eng->device());
+    ctx->eng->PackQuantWeights({w->out_features, w->in_features, w->group, numbers, scales, offsets, packed});
+  });
+}
+
+size_t glacier_proj_quant_workspace(const glacier_quant_proj_desc* desc, const glacier_lora_proj* proj, int n_proj) {
+  size_t bytes = 0;
+  (void)guarded([&] { bytes = glacier::quant_proj_workspace(glacier::quant_proj_of(desc, proj, n_proj)); });
+  return bytes;
+}
+
+int glacier_proj_quant_forward(glacier_attn_ctx* ctx, const glacier_quant_proj_desc* desc, const void* x,
+                               const glacier_lora_proj* proj, int n_proj, void* workspace, size_t workspace_bytes) {
+  return guarded([&] {
+    glacier::QuantProj q = glacier::quant_proj_of(desc, proj, n_proj);
+    glacier::need_quant_tensors(q, x);
+    need(ctx, "ctx");
+    q.a.x = x;
+    glacier::need_workspace(workspace, workspace_bytes, glacier::quant_proj_workspace(q));
+    q.low = static_cast<float*>(workspace);
+    std::lock_guard<std::mutex> g(ctx->eng->lock());
+    glacier::DeviceScope on(ctx->eng->device());
+    ctx->eng->QuantProjForward(q);
   });
 }
 

@@ -82,6 +82,10 @@ struct ProjScratchNeed {
 };
 ProjScratchNeed proj_scratch_need(const ProjLaunch& a, bool backward);
 
+// L_p = X A_p into l[p] [T][rank] for the projections with an adapter, nothing else
+// (of a: x, T, in, rank, io_bf16, n_proj and every p[].a).
+hipError_t launch_lowrank_forward(const ProjLaunch& a, float* const (&l)[kMaxProj], hipStream_t st);
+
 // Enqueue on st.
 hipError_t launch_proj_forward(const ProjLaunch& a, hipStream_t st);
 hipError_t launch_proj_backward(const ProjLaunch& a, hipStream_t st);

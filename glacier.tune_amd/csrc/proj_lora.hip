@@ -703,6 +703,14 @@ ProjScratchNeed proj_scratch_need(const ProjLaunch& a, bool backward) {
   return need;
 }
 
+hipError_t launch_lowrank_forward(const ProjLaunch& a, float* const (&l)[kMaxProj], hipStream_t st) {
+  SplitCall c{};
+  for (int p = 0; p < a.n_proj; ++p)
+    if (a.p[p].a != nullptr) c.j[c.n++] = SplitJob{a.x, a.p[p].a, l[p], nullptr, 0.0f, a.in, 0};
+  if (c.n == 0) return hipSuccess;
+  return a.io_bf16 ? launch_lowrank<bf16, true>(a, c, st) : launch_lowrank<float, false>(a, c, st);
+}
+
 hipError_t launch_proj_forward(const ProjLaunch& a, hipStream_t st) { return run_call(a, false, st); }
 
 hipError_t launch_proj_backward(const ProjLaunch& a, hipStream_t st) { return run_call(a, true, st); }

@@ -1,0 +1,111 @@
+// quant_page.hpp -- device side of the 4-bit formats: a cache's groups of 32
+// columns as they are quantised and read, and words of eight numbers unpacked for
+// the matrix cores.
+//
+// A number n (0 .. 15) stands for (n - 8) s.  s has five significant bits and n - 8
+// three, so a held value is exact in bf16 and in fp16, and no kernel rounds it.  A
+// word's eight numbers lie so that (word >> 4 j) & 0x000f000f are neighbouring
+// columns 2 j and 2 j + 1 in the two halves of a register: one more OR makes them
+// floats 128 + n (bf16) or 16 + n (fp16, shifted), exact, without a conversion.
+#pragma once
+
+#include "attn_common.hpp"
+#include "quant_launch.hpp"
+
+namespace glacier {
+
+constexpr float kQuantScaleMax = 2688.0f;  // five bits; 24 times it is an fp16 value
+constexpr unsigned kQuantNan = 0x7e00u;    // scale of a group that is not finite
+constexpr unsigned kQuantZero = 0x88888888u;  // a word of zeros
+
+typedef _Float16 f16;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ inline float half_at(unsigned w, int hi) {  // fp16 in a register's half
+  return (float)__builtin_bit_cast(f16x2, w)[hi];
+}
+
+// s (fp32) at five significant bits, ties to even, within +-kQuantScaleMax, as fp16.
+__device__ inline f16 quant_scale(float s) {
+  unsigned u = __builtin_bit_cast(unsigned, s);
+  u = (u + 0x3ffffu + ((u >> 19) & 1u)) & ~0x7ffffu;
+  return (f16)fminf(fmaxf(__builtin_bit_cast(float, u), -kQuantScaleMax), kQuantScaleMax);
+}
+
+// The number of x: floor(x / s + 1/2) + 8 within 0 .. 15.  inv: about 1 / s; the
+// product may land on the wrong side of a border, which the remainder tells (it is
+// exact there: x and n s agree in their leading bits).
+__device__ inline unsigned quant_number(float x, float s, float inv) {
+  const float t = fminf(fmaxf(x * inv, -9.0f), 8.0f);
+  float n = floorf(t + 0.5f);
+  const float r = fmaf(-n, s, x), half = 0.5f * fabsf(s);
+  const float over = s < 0.0f ? -r : r;  // (x / s - n) |s|
+  n += over >= half ? 1.0f : 0.0f;
+  n -= over < -half ? 1.0f : 0.0f;
+  return static_cast<unsigned>(fminf(fmaxf(n + 8.0f, 0.0f), 15.0f));
+}
+
+// Eight columns (of a group of 32 that four neighbouring lanes hold) as a word and
+// the group's scale.
+__device__ inline unsigned quantise8(const float (&x)[8], f16& scale) {
+  float top = x[0], low = x[0];
+  unsigned odd = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    top = fmaxf(top, x[e]);
+    low = fminf(low, x[e]);
+    odd |= (__builtin_bit_cast(unsigned, x[e]) & 0x7f800000u) == 0x7f800000u ? 1u : 0u;
+  }
+#pragma unroll
+  for (int d = 1; d < 4; d *= 2) {
+    top = fmaxf(top, __shfl_xor(top, d));
+    low = fminf(low, __shfl_xor(low, d));
+    odd |= __shfl_xor(odd, d);
+  }
+  scale = odd ? __builtin_bit_cast(f16, static_cast<unsigned short>(kQuantNan))
+              : quant_scale((top >= -low ? top : low) * -0.125f);
+  const float s = (float)scale;
+  if (odd || s == 0.0f) return kQuantZero;
+  const float inv = 1.0f / s;
+  unsigned w = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w |= quant_number(x[e], s, inv) << (4 * (e / 2) + 16 * (e % 2));
+  return w;
+}
+
+// A word's columns as floats (n - 8) s.
+__device__ inline void dequantise8(unsigned w, float s, float (&x)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    x[e] = (float)(static_cast<int>((w >> (4 * (e / 2) + 16 * (e % 2))) & 15u) - 8) * s;
+}
+
+// Where a token's head lies in a page's head part of 18 G P bytes: `row` the token's
+// place in the page.  Words in units of 4 bytes, scales in units of 2 behind them.
+__device__ inline int k_word(int row, int G, int col8) { return (row * 4 + col8 % 4) * G + col8 / 4; }
+__device__ inline int k_scale(int row, int G, int i) { return row * G + i; }
+__device__ inline int v_word(int row, int G, int col8) { return ((row >> 2) * 4 * G + col8) * 4 + (row & 3); }
+__device__ inline int v_scale(int row, int G, int i) { return ((row >> 2) * G + i) * 4 + (row & 3); }
+
+// Two numbers n, n' (in bits 0-3 and 16-19 of w >> shift) as bf16 128 + n, 128 + n'.
+__device__ inline unsigned pair_bf16(unsigned w, int shift) { return ((w >> shift) & 0x000f000fu) | 0x43004300u; }
+// A word's columns as a bf16 operand of 128 + n.
+__device__ inline bf16x8 raw8_bf16(unsigned w) {
+  return __builtin_bit_cast(bf16x8, u32x4{pair_bf16(w, 0), pair_bf16(w, 4), pair_bf16(w, 8), pair_bf16(w, 12)});
+}
+// Upper halves of two floats (bf16 values) as a pair.
+__device__ inline unsigned upper_pair(float lo, float hi) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, hi), __builtin_bit_cast(unsigned, lo), 0x07060302u);
+}
+// A word's columns as a bf16 operand of n - 8.
+__device__ inline unsigned exact_pair(unsigned w, int shift) {
+  const unsigned p = pair_bf16(w, shift);
+  return upper_pair(__builtin_bit_cast(float, p << 16) - 136.0f, __builtin_bit_cast(float, p & 0xffff0000u) - 136.0f);
+}
+__device__ inline bf16x8 exact8_bf16(unsigned w) {
+  return __builtin_bit_cast(bf16x8, u32x4{exact_pair(w, 0), exact_pair(w, 4), exact_pair(w, 8), exact_pair(w, 12)});
+}
+
+}  // namespace glacier

@@ -33,7 +33,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libglacier_attn.so")
 HEADERS = [os.path.join(os.path.dirname(HERE), "include", h)
            for h in ("glacier_attn.h", "glacier_qkv.h", "glacier_norm.h", "glacier_cache.h",
-                     "glacier_lmhead.h", "glacier_lora_file.h")]
+                     "glacier_quant.h", "glacier_lmhead.h", "glacier_lora_file.h")]
 
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_DEVICE, ERR_OUT_OF_MEMORY = 0, 1, 2, 3, 4
 PREC_FP32, PREC_BF16 = 0, 1
@@ -143,6 +143,28 @@ class CacheBatch(ctypes.Structure):
         ("max_pages", ctypes.c_int32),
         ("max_new", ctypes.c_int32),
         ("max_kv", ctypes.c_int32),
+    ]
+
+
+class QuantWeights(ctypes.Structure):
+    """glacier_quant_weights (include/glacier_quant.h)."""
+    _fields_ = [
+        ("out_features", ctypes.c_int32),
+        ("in_features", ctypes.c_int32),
+        ("group", ctypes.c_int32),
+        ("offsets", ctypes.c_int32),
+    ]
+
+
+class QuantProjDesc(ctypes.Structure):
+    """glacier_quant_proj_desc (include/glacier_quant.h)."""
+    _fields_ = [
+        ("total_tokens", ctypes.c_int32),
+        ("in_features", ctypes.c_int32),
+        ("group", ctypes.c_int32),
+        ("offsets", ctypes.c_int32),
+        ("rank", ctypes.c_int32),
+        ("io_dtype", ctypes.c_int32),
     ]
 
 
@@ -276,6 +298,20 @@ def load():
     L.glacier_attn_cache_workspace.restype = ctypes.c_size_t
     L.glacier_attn_cache_forward.argtypes = [vp, kp, bp, ctypes.c_int32, vp, vp, vp, vp,
                                              ctypes.c_size_t]
+    L.glacier_attn_qcache_page_bytes.argtypes = [kp]
+    L.glacier_attn_qcache_page_bytes.restype = ctypes.c_size_t
+    L.glacier_attn_qcache_append.argtypes = L.glacier_attn_cache_append.argtypes
+    L.glacier_attn_qcache_read.argtypes = [vp, kp, bp, vp, vp]
+    L.glacier_attn_qcache_workspace.argtypes = [vp, kp, bp, ctypes.c_int32]
+    L.glacier_attn_qcache_workspace.restype = ctypes.c_size_t
+    L.glacier_attn_qcache_forward.argtypes = L.glacier_attn_cache_forward.argtypes
+    wp, dp, lp = ctypes.POINTER(QuantWeights), ctypes.POINTER(QuantProjDesc), ctypes.POINTER(LoraProj)
+    L.glacier_proj_quant_bytes.argtypes = [wp]
+    L.glacier_proj_quant_bytes.restype = ctypes.c_size_t
+    L.glacier_proj_quant_pack.argtypes = [vp, wp, vp, vp, vp, vp]
+    L.glacier_proj_quant_workspace.argtypes = [dp, lp, c_int]
+    L.glacier_proj_quant_workspace.restype = ctypes.c_size_t
+    L.glacier_proj_quant_forward.argtypes = [vp, dp, vp, lp, c_int, vp, ctypes.c_size_t]
     L.glacier_proj_backward.argtypes = [vp, ctypes.POINTER(ProjDesc), vp,
                                         ctypes.POINTER(LoraProj), c_int, vp]
     _lib = L
@@ -437,7 +473,7 @@ def _address(t, name, shape, dtype, device):
     if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
         _need(t, name, shape, dtype=dtype)
     if t.get_device() != device:
-        raise TypeError(f"{name} must be on cuda:{device}, got {t.device}")
+        raise TypeError(f"{_label(name)} must be on cuda:{device}, got {t.device}")
     return t.data_ptr()
 
 
@@ -459,21 +495,41 @@ def cache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, m
     [n_pages, Hkv, page_size, D] of one dtype, each page contiguous and the
     pages any one stride apart; cu_tokens [n + 1], kv_lens [n] and page_table
     [n, max_pages] int32, the table's rows any stride apart."""
-    shape, dtype, i32 = k_pages.shape, k_pages.dtype, _torch().int32
+    shape = k_pages.shape
     if len(shape) != 4:
         raise TypeError("k_pages must be [n_pages, n_heads_kv, page_size, head_dim]")
+    stride = _pages(k_pages, v_pages, device)
+    n_pages, hkv, page, d = shape
+    batch = _batch_args(cu_tokens, kv_lens, page_table, total_tokens, max_new, max_kv, device)
+    _need_32_bits(n_pages, hkv, page, d)
+    return (KvCache(k_pages.data_ptr(), v_pages.data_ptr(), stride, n_pages, page, hkv, d,
+                    GpuAttentionEngine._io_of(k_pages)), batch)
+
+
+def _pages(k_pages, v_pages, device):
+    """The stride of K's and V's pages, alike in shape and dtype."""
+    shape, dtype = k_pages.shape, k_pages.dtype
     if v_pages.shape != shape or v_pages.dtype is not dtype:
         raise TypeError(f"v_pages must be {dtype} of shape {tuple(shape)}, got {v_pages.dtype} of "
                         f"{tuple(v_pages.shape)}")
-    n_pages, hkv, page, d = shape
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if t.get_device() != device:
+            raise TypeError(f"{name} must be on cuda:{device}, got {t.device}")
     if k_pages.is_contiguous() and v_pages.is_contiguous():
-        stride = hkv * page * d
-    else:
-        stride = _page_stride(k_pages, v_pages)
+        size = 1
+        for n in shape[1:]:
+            size *= n
+        return size
+    return _page_stride(k_pages, v_pages)
+
+
+def _batch_args(cu_tokens, kv_lens, page_table, total_tokens, max_new, max_kv, device):
+    """glacier_cache_batch (see cache_args)."""
+    i32 = _torch().int32
     if len(page_table.shape) != 2 or page_table.dtype is not i32:
         raise TypeError("page_table must be an int32 [n_seqs, max_pages] tensor")
     n, most = page_table.shape
-    _need_32_bits(total_tokens, n_pages, hkv, page, d, n, most)
+    _need_32_bits(total_tokens, n, most)
     if page_table.is_contiguous():
         row = most
     else:
@@ -482,14 +538,58 @@ def cache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, m
             raise TypeError("page_table's rows must be contiguous")
         if row < most:
             raise TypeError("page_table's rows must not overlap")
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages"), (page_table, "page_table")):
-        if t.get_device() != device:
-            raise TypeError(f"{name} must be on cuda:{device}, got {t.device}")
-    return (KvCache(k_pages.data_ptr(), v_pages.data_ptr(), stride, n_pages, page, hkv, d,
-                    GpuAttentionEngine._io_of(k_pages)),
-            CacheBatch(_address(cu_tokens, "cu_tokens", (n + 1,), i32, device),
-                       _address(kv_lens, "kv_lens", (n,), i32, device), page_table.data_ptr(), row, n,
-                       total_tokens, most, min(int(max_new), _LARGEST), min(int(max_kv), _LARGEST)))
+    if page_table.get_device() != device:
+        raise TypeError(f"page_table must be on cuda:{device}, got {page_table.device}")
+    return CacheBatch(_address(cu_tokens, "cu_tokens", (n + 1,), i32, device),
+                      _address(kv_lens, "kv_lens", (n,), i32, device), page_table.data_ptr(), row, n,
+                      total_tokens, most, min(int(max_new), _LARGEST), min(int(max_kv), _LARGEST))
+
+
+def quant_groups(head_dim):
+    """Groups of 32 columns that a head takes in a 4-bit cache."""
+    g = -(-head_dim // 32)
+    return g + (g in (5, 7))
+
+
+def quant_page_bytes(page_size, head_dim):
+    """Bytes of one KV head's part of a 4-bit page: a cache's pages are uint8
+    [n_pages, Hkv, quant_page_bytes(page_size, head_dim)]."""
+    return 18 * quant_groups(head_dim) * page_size
+
+
+def qcache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, max_new, max_kv, device,
+                head_dim, dtype):
+    """As cache_args, for the 4-bit pages of heads of head_dim columns and tensors
+    of dtype."""
+    torch, shape = _torch(), k_pages.shape
+    if len(shape) != 3 or k_pages.dtype is not torch.uint8:
+        raise TypeError("k_pages must be uint8 [n_pages, n_heads_kv, quant_page_bytes(page_size, head_dim)]")
+    n_pages, hkv, size = shape
+    if head_dim <= 0 or size % quant_page_bytes(1, head_dim) != 0:
+        raise TypeError(f"a page's head of {size} bytes holds no whole tokens of {head_dim} columns")
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"unsupported tensor dtype {dtype}")
+    stride = _pages(k_pages, v_pages, device)
+    batch = _batch_args(cu_tokens, kv_lens, page_table, total_tokens, max_new, max_kv, device)
+    _need_32_bits(n_pages, hkv, size, head_dim)
+    return (KvCache(k_pages.data_ptr(), v_pages.data_ptr(), stride, n_pages,
+                    size // quant_page_bytes(1, head_dim), hkv, head_dim,
+                    IO_F32 if dtype is torch.float32 else IO_BF16), batch)
+
+
+def quantise_rows(w, group=32):
+    """w [out, in] in 4 bits: (numbers uint8 [out, in / 2], scales float16 [out,
+    in / group]) as quant_pack takes them, w ~ (n - 8) s.  s brings the element of
+    largest magnitude of each group to n = 0."""
+    torch = _torch()
+
+    g = w.float().unflatten(1, (-1, group))
+    top, low = g.amax(-1), g.amin(-1)
+    s = (torch.where(top >= -low, top, low) / -8.0).half()
+    unit = s.float()[..., None]
+    n = torch.where(unit == 0, torch.zeros_like(g), torch.round(g / unit)).clamp(-8, 7).flatten(1)
+    n = (n + 8).to(torch.uint8)
+    return n[:, 0::2] | (n[:, 1::2] << 4), s
 
 
 def _page_stride(k_pages, v_pages):
@@ -969,6 +1069,148 @@ class GpuAttentionEngine:
         if rc != OK:
             _check(rc)
         return out, lse
+
+    # ---- answering in 4 bits (glacier_quant.h) ------------------------------
+    def qcache_append(self, k, v, k_pages, v_pages, cu_tokens, kv_lens, page_table,
+                      rope_freq_base=None, q=None, q_rot=None):
+        """As cache_append, into pages that hold keys and values in 4 bits: uint8
+        [n_pages, Hkv, quant_page_bytes(page_size, D)]."""
+        if k.dim() != 3:
+            raise TypeError("k must be [T, Hkv, D]")
+        dev, dt, (T, hkv, d) = self.device_ordinal, k.dtype, k.shape
+        cache, batch = qcache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, T, 0, 0, dev, d, dt)
+        shape = (T, cache.n_heads_kv, d)
+        kp, vp = _address(k, "k", shape, dt, dev), _address(v, "v", shape, dt, dev)
+        hq, qp, rp = 0, None, None
+        if q is not None:
+            if q.dim() != 3:
+                raise TypeError("q must be [T, Hq, D]")
+            hq = q.shape[1]
+            q_rot = _torch_mod.empty_like(q) if q_rot is None else q_rot
+            qp = _address(q, "q", (T, hq, d), dt, dev)
+            rp = _address(q_rot, "q_rot", (T, hq, d), dt, dev)
+        self._bind_device_stream()
+        rc = _lib.glacier_attn_qcache_append(self._h, ctypes.byref(cache), ctypes.byref(batch), kp, vp,
+                                             float(rope_freq_base or 0.0), hq, qp, rp)
+        if rc != OK:
+            _check(rc)
+        return q_rot if q is not None else None
+
+    def qcache_read(self, k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, head_dim, dtype,
+                    k=None, v=None):
+        """The tokens that a qcache_append of this batch wrote (sequence b's last
+        cu_tokens[b + 1] - cu_tokens[b]; all of every sequence with the running sum of
+        kv_lens) from the pages: (k, v) [total_tokens, Hkv, head_dim] of dtype.  Rows at
+        or past cu_tokens[-1] are not written."""
+        dev, T = self.device_ordinal, int(total_tokens)
+        cache, batch = qcache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, T, 0, 0, dev,
+                                   int(head_dim), dtype)
+        shape, torch = (T, cache.n_heads_kv, cache.head_dim), _torch_mod
+        k = torch.empty(shape, dtype=dtype, device=dev) if k is None else k
+        v = torch.empty(shape, dtype=dtype, device=dev) if v is None else v
+        kp, vp = _address(k, "k", shape, dtype, dev), _address(v, "v", shape, dtype, dev)
+        self._bind_device_stream()
+        rc = _lib.glacier_attn_qcache_read(self._h, ctypes.byref(cache), ctypes.byref(batch), kp, vp)
+        if rc != OK:
+            _check(rc)
+        return k, v
+
+    def qcache_forward(self, q, k_pages, v_pages, cu_tokens, kv_lens, page_table, max_new=0, max_kv=0,
+                       out=None, lse=None, save=False):
+        """As cache_forward, over 4-bit pages (see qcache_append)."""
+        if q.dim() != 3:
+            raise TypeError("q must be [T, Hq, D]")
+        dev, dt, (T, hq, d) = self.device_ordinal, q.dtype, q.shape
+        cache, batch = qcache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, T, max_new, max_kv,
+                                   dev, d, dt)
+        shape = (T, hq, d)
+        qp = _address(q, "q", shape, dt, dev)
+        torch = _torch_mod
+        out = torch.empty_like(q) if out is None else out
+        if lse is None and save:
+            lse = torch.empty((hq, T), dtype=torch.float32, device=q.device)
+        op = _address(out, "out", shape, dt, dev)
+        lp = _optional(lse, "lse", (hq, T), torch.float32, dev)
+        L, cp, bp = _lib, ctypes.byref(cache), ctypes.byref(batch)
+        size = L.glacier_attn_qcache_workspace(self._h, cp, bp, hq)
+        work = None if size == 0 else self._workspace(size)
+        self._bind_device_stream()
+        rc = L.glacier_attn_qcache_forward(self._h, cp, bp, hq, qp, op, lp, self._ptr(work), size)
+        if rc != OK:
+            _check(rc)
+        return out, lse
+
+    @staticmethod
+    def quant_bytes(out_features, in_features, group=32, offsets=False):
+        """Bytes of packed 4-bit weights (0: not a size that is taken)."""
+        _need_32_bits(out_features, in_features)
+        return load().glacier_proj_quant_bytes(
+            ctypes.byref(QuantWeights(int(out_features), int(in_features), int(group), int(bool(offsets)))))
+
+    def quant_pack(self, numbers, scales, offsets=None, packed=None):
+        """4-bit weights laid out for proj_quant_forward: numbers uint8 [out, in / 2]
+        (two to a byte, the even column in the low half), scales and offsets float16
+        [out, in / group], a weight being (n - 8) scale + offset (quantise_rows makes
+        them).  Returns the packed weights (uint8)."""
+        torch, dev = _torch(), self.device_ordinal
+        if numbers.dim() != 2 or scales.dim() != 2:
+            raise TypeError("numbers must be [out, in / 2] and scales [out, in / group]")
+        rows, cols = numbers.shape[0], 2 * numbers.shape[1]
+        if scales.shape[1] == 0 or cols % scales.shape[1] != 0:
+            raise TypeError(f"scales must be [{rows}, {cols} / group]")
+        _need_32_bits(rows, cols)
+        w = QuantWeights(rows, cols, cols // scales.shape[1], int(offsets is not None))
+        size = load().glacier_proj_quant_bytes(ctypes.byref(w))
+        if size == 0:
+            _check(ERR_UNSUPPORTED)
+        packed = torch.empty(size, dtype=torch.uint8, device=dev) if packed is None else packed
+        args = (_address(numbers, "numbers", (rows, cols // 2), torch.uint8, dev),
+                _address(scales, "scales", scales.shape if len(scales) == rows else (rows, scales.shape[1]),
+                         torch.float16, dev),
+                _optional(offsets, "offsets", scales.shape, torch.float16, dev),
+                _address(packed, "packed", (size,), torch.uint8, dev))
+        self._bind_device_stream()
+        rc = _lib.glacier_proj_quant_pack(self._h, ctypes.byref(w), *args)
+        if rc != OK:
+            _check(rc)
+        return packed
+
+    def proj_quant_forward(self, x, projs, rank=0, group=32, mins=False):
+        """proj_forward with base weights in 4 bits.  x [T, in] (float32 or
+        bfloat16).  projs: dicts with w (quant_pack's, of weights [out, in] in groups
+        of `group` columns, with offsets if mins), out, optional bias [out], a [in,
+        rank], b [rank, out] (float32), scaling, and optionally y [T, out] to write.
+        Returns the list of y."""
+        if x.dim() != 2:
+            raise TypeError("x must be [T, in]")
+        torch, dev = _torch(), self.device_ordinal
+        (T, n_in), dt, f32 = x.shape, x.dtype, torch.float32
+        _need_32_bits(T, n_in, rank)
+        desc = QuantProjDesc(T, n_in, int(group), int(bool(mins)), int(rank), self._io_of(x))
+        xp = _address(x, "x", (T, n_in), dt, dev)
+        L, ys, arr = load(), [], (LoraProj * len(projs))()
+        for i, pr in enumerate(projs):
+            get = pr.get
+            n_out, y = int(pr["out"]), get("y")
+            _need_32_bits(n_out)
+            if y is None:
+                y = torch.empty((T, n_out), dtype=dt, device=dev)
+            ys.append(y)
+            size = L.glacier_proj_quant_bytes(ctypes.byref(QuantWeights(n_out, n_in, desc.group, desc.offsets)))
+            if size == 0:
+                _check(ERR_UNSUPPORTED)
+            arr[i] = (_address(pr["w"], (i, "w"), (size,), torch.uint8, dev),
+                      _optional(get("bias"), (i, "bias"), (n_out,), f32, dev),
+                      _optional(get("a"), (i, "a"), (n_in, rank), f32, dev),
+                      _optional(get("b"), (i, "b"), (rank, n_out), f32, dev), float(get("scaling", 0.0)), n_out,
+                      _address(y, (i, "y"), (T, n_out), dt, dev), None, None, None)
+        size = L.glacier_proj_quant_workspace(ctypes.byref(desc), arr, len(projs))
+        work = None if size == 0 else self._workspace(size)
+        self._bind_device_stream()
+        rc = L.glacier_proj_quant_forward(self._h, ctypes.byref(desc), xp, arr, len(projs), self._ptr(work), size)
+        if rc != OK:
+            _check(rc)
+        return ys
 
     # ---- LM-head cross-entropy (glacier_lmhead.h) -------------------------
     def _lmhead(self, hidden, targets, weight, d_hidden, grad, precision):
