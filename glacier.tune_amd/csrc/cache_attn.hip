@@ -473,6 +473,17 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(CacheAttn a) {
   }
 }
 
+// Sum and maximum over a wave's lanes, pair by pair (lanes_sum, swap_sum): no LDS.
+__device__ inline float lanes_total(float x) { return col_sum_swap(lanes_sum<16>(x)); }
+__device__ inline float lanes_most(float x) {
+  auto of = [](float y, float z) { return fmaxf(y, z); };
+  x = of(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xB1, 0xF, 0xF, false)));
+  x = of(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4E, 0xF, 0xF, false)));
+  x = of(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x141, 0xF, 0xF, false)));
+  x = of(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x140, 0xF, 0xF, false)));
+  return col_max_swap(x);
+}
+
 // Joins the splits of a row.  A split's sums take ceil(D / 4) lanes of 4
 // columns, so a wave reads several splits at once where D <= 128, and up to
 // eight such loads are in flight.  WAVES waves share a row (1: few splits; 4:
@@ -485,41 +496,43 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttn a) {
   const int lane = threadIdx.x & 63, w = wave_id();
   const long at = WAVES == 1 ? (long)blockIdx.x * 4 + w : blockIdx.x;
   if (at >= (long)c.T * a.hq) return;
+  const long step = (long)c.T * a.hq;
+  // lanes of a split: a power of two that holds D / 4
+  const int lanes = c.D <= 32 ? 8 : c.D <= 64 ? 16 : c.D <= 128 ? 32 : 64;
+  const int per_load = 64 / lanes, d = 4 * (lane % lanes);
+  const int first = (WAVES == 1 ? 0 : w * per_load) + lane / lanes, stride = WAVES * per_load;
+  // What the splits may have left is requested before it is known how many of them
+  // there are (the workspace holds every one, whatever is in it): one load deep less.
+  f32x4 v[8], o = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto fetch = [&](int u0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int u = u0 + i * stride + first;
+      v[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (u < a.n_splits && d < c.D) v[i] = *reinterpret_cast<const f32x4*>(a.part_o + (u * step + at) * c.D + d);
+    }
+  };
+  float2 ml = make_float2(kLeast, 0.0f);
+  if (lane < a.n_splits) ml = a.part_ml[lane * step + at];
+  fetch(0);
   const int t = static_cast<int>(at / a.hq), h = static_cast<int>(at % a.hq);
   const CacheSeq s = seq_of_token(c, lane, t);
   if (s.b >= c.n_seqs) return;
   if (t < s.tok0) return;
   const TileKeys tk = tile_keys(a, s, ((t - s.tok0) * a.group + h % a.group) / a.rows);
   if (tk.active <= 1) return;
-  const long step = (long)c.T * a.hq;
-  float2 ml = make_float2(kLeast, 0.0f);
-  if (lane < tk.active) ml = a.part_ml[lane * step + at];
-  // lanes of a split: a power of two that holds D / 4
-  const int lanes = c.D <= 32 ? 8 : c.D <= 64 ? 16 : c.D <= 128 ? 32 : 64;
-  const int per_load = 64 / lanes, d = 4 * (lane % lanes);
-  const int first = (WAVES == 1 ? 0 : w * per_load) + lane / lanes, stride = WAVES * per_load;
-  f32x4 v[8], o = {0.0f, 0.0f, 0.0f, 0.0f};
-  float mx = ml.x;
-#pragma unroll
-  for (int x = 1; x < 64; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x));
+  if (lane >= tk.active) ml = make_float2(kLeast, 0.0f);
+  const float mx = lanes_most(ml.x);
   const float f = weight(ml.x - mx);
-  float total = f * ml.y;
-#pragma unroll
-  for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
+  const float total = lanes_total(f * ml.y);
   for (int u0 = 0; u0 < tk.active; u0 += 8 * stride) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int u = u0 + i * stride + first;
-      v[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (u < tk.active && d < c.D)
-        v[i] = *reinterpret_cast<const f32x4*>(a.part_o + (u * step + at) * c.D + d);
-    }
+    if (u0 > 0) fetch(u0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int u = u0 + i * stride + first;
       const float fu = __shfl(f, u & 63);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += (u < tk.active ? fu : 0.0f) * v[i][e];
+      for (int e = 0; e < 4; ++e) o[e] = u < tk.active ? o[e] + fu * v[i][e] : o[e];
     }
   }
   for (int x = lanes; x < 64; x *= 2)

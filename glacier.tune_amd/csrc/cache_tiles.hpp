@@ -63,9 +63,8 @@ struct TileKeys {
   int kend;  // keys 0 .. kend - 1
   int per, active;  // keys of a split, and how many splits have any
 };
-__device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int tile) {
+__device__ inline TileKeys keys_up_to(const CacheAttn& a, const CacheSeq& s, int last) {
   TileKeys k;
-  const int last = min(s.n - 1, (tile * a.rows + a.rows - 1) / a.group);
   const long cap = (long)a.c.max_pages << a.c.page_shift;
   const long end = (long)s.pos0 + last + 1;
   k.kend = static_cast<int>(end < 0 ? 0 : end < cap ? end : cap);
@@ -73,6 +72,9 @@ __device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int 
   k.per = split.per;
   k.active = split.active;
   return k;
+}
+__device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int tile) {
+  return keys_up_to(a, s, min(s.n - 1, (tile * a.rows + a.rows - 1) / a.group));
 }
 
 // A masked weight is zero, but zero times an infinity or a NaN is not.  The

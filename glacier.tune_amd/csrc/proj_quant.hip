@@ -96,6 +96,7 @@ __global__ __launch_bounds__(64 * KS) void quant_proj_kernel(QuantCall a) {
       }
     }
   };
+  const QuantMagic magic;
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
   f32x4 y[NT];
 #pragma unroll
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(64 * KS) void quant_proj_kernel(QuantCall a) {
         for (int n = 0; n < NT; ++n) d[n] = d0[n] = zero;
 #pragma unroll
         for (int i = q * 4 / GP; i < (q + 1) * 4 / GP; ++i) {
-          const bf16x8 wf = exact8_bf16(from.w[i]);
+          const bf16x8 wf = exact8_bf16(from.w[i], magic);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             bf16x8 h, m, l;
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(64 * KS) void quant_proj_kernel(QuantCall a) {
         for (int n = 0; n < NT; ++n) d[n] = d0[n];
 #pragma unroll
         for (int i = q * 4 / GP; i < (q + 1) * 4 / GP; ++i) {
-          const bf16x8 wf = raw8_bf16(from.w[i]);
+          const bf16x8 wf = raw8_bf16(from.w[i], magic);
 #pragma unroll
           for (int n = 0; n < NT; ++n) d[n] = Mfma<bf16>::mma(wf, from.x[n][i], d[n]);
         }

@@ -16,9 +16,9 @@
 // eight columns of both: a lane's words are the operands of eight products (columns 8 x
 // + one of 0 .. 7), of four where a head has at most 64 columns (then two lanes take a
 // word's halves).
-//   V as bf16 (n - 8) s, exact (five bits by three): (16 + n) s - 24 s, where 16 + n is
-//   an fp16 value by one OR, formed by fp32 operations that take fp16 operands, of
-//   whose results the upper halves are kept.  The weights in two bf16 terms (16 bits of
+//   V as bf16 (n - 8) s, exact (five bits by three): (1024 + n) s - 1032 s, or (64 + n) s
+//   - 72 s, where the sum in brackets is an fp16 value by one OR, formed by fp32
+//   operations that take fp16 operands, of whose results the upper halves are kept.  The weights in two bf16 terms (16 bits of
 //   them; fp32: three).
 //
 // A held value is NaN only by its scale (it is never infinite).  Where a sum is not
@@ -33,48 +33,93 @@
 namespace glacier {
 namespace {
 
-constexpr int kWavesQ = 4;
+#ifndef GL_QW
+#define GL_QW 4
+#endif
+constexpr int kWavesQ = GL_QW;
 [[maybe_unused]] constexpr int kKeysQ = 32;  // keys of a wave's block: one k-step of the second product
+#ifndef GL_QSTAGES
+#define GL_QSTAGES 2
+#endif
+#ifndef GL_QOCC
+#define GL_QOCC (G <= 4 ? 2 : 1)
+#endif
 
+// A wave's blocks in LDS, a ring of STAGES: for each tile of 16 keys the words and then
+// the scales of K and of V, as they lie in the page.
 template <int G>
 struct QaLayout {
   static constexpr int NV = (G + 3) / 4;    // blocks of 16 words of a token of V
   static constexpr bool HALF = G <= 2;      // two lanes share a word
   static constexpr int NB = HALF ? 4 : 8 * NV;  // 16-column products
   static constexpr int DP = 32 * G;
+  static constexpr int WORDS = 256 * G, SCALES = 32 * G;  // bytes, of 16 keys
+  static constexpr int KS = WORDS, V = KS + SCALES, VS = V + WORDS;  // behind K's words
+  static constexpr int TILE = VS + SCALES, BLOCK = 2 * TILE;
+  static constexpr int ND = (WORDS + 1023) / 1024;  // DMA instructions of a tile's words
+  static constexpr int LOADS = 4 * (ND + 1);        // of a block
+  static constexpr int STAGES = GL_QSTAGES;
   static constexpr int OS = DP + 4;         // row stride (floats) of a wave's sums in the join
   static constexpr int WAVE = 16 * (OS + 2);
-};
-
-// What a wave loads of 32 keys: two tiles of 16.
-template <int G>
-struct QBlock {
-  static constexpr int NV = QaLayout<G>::NV;
-  unsigned k[2][G];      // lane (key l % 16, columns 8 (l / 16) .. of each group)
-  unsigned ks[2][2 * G];  // scales of keys 4 (l / 16) ..: halves key G + i
-  unsigned v[2][NV][4];   // lane (word l % 16 or its pair, tokens 4 (l / 16) ..)
-  unsigned vs[2][NV][2];  // their scales
+  static constexpr int RING = kWavesQ * STAGES * BLOCK, JOIN = kWavesQ * WAVE * 4;
+  static constexpr int BYTES = RING > JOIN ? RING : JOIN;
+  static_assert(BYTES <= 160 * 1024, "exceeds the LDS of a CU");
+  static_assert((STAGES - 1) * LOADS < 64, "more loads in flight than are counted");
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
-template <int N>
-__device__ inline void load_words(__amdgpu_buffer_rsrc_t rs, int voff, int soff, unsigned* to) {
-  if constexpr (N >= 4) {
-    const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, voff, soff, 0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) to[e] = static_cast<unsigned>(w[e]);
-    if constexpr (N > 4) load_words<N - 4>(rs, voff + 16, soff, to + 4);
-  } else if constexpr (N == 3) {
-    const auto w = __builtin_amdgcn_raw_buffer_load_b96(rs, voff, soff, 0);
-#pragma unroll
-    for (int e = 0; e < 3; ++e) to[e] = static_cast<unsigned>(w[e]);
-  } else if constexpr (N == 2) {
-    const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, voff, soff, 0);
-    to[0] = static_cast<unsigned>(w[0]), to[1] = static_cast<unsigned>(w[1]);
-  } else {
-    to[0] = static_cast<unsigned>(__builtin_amdgcn_raw_buffer_load_b32(rs, voff, soff, 0));
+// N words at an LDS address plus OFF, issued only: see settled.
+template <int N, int OFF>
+struct LdsWords {
+  LdsWords<N - 4, OFF + 16> rest;
+  u32x4 w;
+  __device__ inline void issue(unsigned at) {
+    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(w) : "v"(at), "i"(OFF));
+    rest.issue(at);
   }
-}
+  __device__ inline void settled() {
+    asm volatile("" : "+v"(w));
+    rest.settled();
+  }
+  __device__ inline unsigned operator[](int i) const { return i < 4 ? w[i] : rest[i - 4]; }
+  __device__ inline void keep(int i, unsigned mask) { i < 4 ? (void)(w[i] &= mask) : rest.keep(i - 4, mask); }
+};
+template <int OFF>
+struct LdsWords<3, OFF> {
+  typedef unsigned u32x3 __attribute__((ext_vector_type(3)));
+  u32x3 w;
+  __device__ inline void issue(unsigned at) {
+    asm volatile("ds_read_b96 %0, %1 offset:%2" : "=v"(w) : "v"(at), "i"(OFF));
+  }
+  __device__ inline void settled() { asm volatile("" : "+v"(w)); }
+  __device__ inline unsigned operator[](int i) const { return w[i]; }
+};
+template <int OFF>
+struct LdsWords<2, OFF> {
+  u32x2 w;
+  __device__ inline void issue(unsigned at) {
+    asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(w) : "v"(at), "i"(OFF));
+  }
+  __device__ inline void settled() { asm volatile("" : "+v"(w)); }
+  __device__ inline unsigned operator[](int i) const { return w[i]; }
+  __device__ inline void keep(int i, unsigned mask) { w[i] &= mask; }
+};
+template <int OFF>
+struct LdsWords<1, OFF> {
+  unsigned w;
+  __device__ inline void issue(unsigned at) {
+    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(w) : "v"(at), "i"(OFF));
+  }
+  __device__ inline void settled() { asm volatile("" : "+v"(w)); }
+  __device__ inline unsigned operator[](int) const { return w; }
+};
+template <int OFF>
+struct LdsWords<0, OFF> {
+  __device__ inline void issue(unsigned) {}
+  __device__ inline void settled() {}
+  __device__ inline unsigned operator[](int) const { return 0; }
+  __device__ inline void keep(int, unsigned) {}
+};
 #endif
 
 // Halves of a register that are NaN, as a mask (scales are never infinite).
@@ -82,122 +127,187 @@ __device__ inline void load_words(__amdgpu_buffer_rsrc_t rs, int voff, int soff,
   return ((((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u) >> 15) * 0xffffu;
 }
 
+// Division of x by a number known before the launch: one multiplication while x d is
+// below 2^32 for every x of the call (the product's error, below x d / 2^32, stays
+// under one step then), else a division.  A dozen divisions of 30 instructions each
+// were a third of what a workgroup of four short blocks executes.
+struct FixedDiv {
+  unsigned d, m;
+  static FixedDiv by(unsigned d, unsigned long long most) {
+    return {d, d > 1 && most * d < (1ull << 32) ? static_cast<unsigned>(((1ull << 32) + d - 1) / d) : 0u};
+  }
+  __device__ inline int of(int x) const {
+    return d == 1 ? x : m != 0 ? static_cast<int>(__umulhi(static_cast<unsigned>(x), m)) : x / static_cast<int>(d);
+  }
+};
+struct TileDivs {
+  FixedDiv splits, heads, group;
+  unsigned few;  // 2^16 / group, rounded up
+  // x / group for x < group + 15
+  __device__ inline int few_of(int x, int of) const {
+    return of >= 16 ? (x >= of ? 1 : 0) : static_cast<int>(static_cast<unsigned>(x) * few >> 16);
+  }
+};
+
 template <typename T, int G>
-__global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kernel(CacheAttn a) {
+__global__ __launch_bounds__(64 * kWavesQ, GL_QOCC) void qcache_attn_kernel(CacheAttn a, TileDivs f) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using L = QaLayout<G>;
-  using B = QBlock<G>;
   constexpr int NV = L::NV, NB = L::NB;
   constexpr bool F32 = sizeof(T) == 4, HALF = L::HALF;
-  __shared__ __align__(16) float all[kWavesQ * L::WAVE];
+  extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
-  const int w = wave_id(), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-  const int D = c.D, numbers = static_cast<int>(gridDim.x / (a.n_splits * c.hkv));
-  const int kvh = blockIdx.x / a.n_splits % c.hkv;
-  const int number = blockIdx.x / (a.n_splits * c.hkv);
-  const int split = (blockIdx.x + number) % a.n_splits;
-  int tile;
-  CacheSeq s;
-  if (a.long_first) {
-    s = seq_of_long_tile(a, lane, number, numbers, tile);
-  } else {
-    s = seq_of_tile(a, lane, number);
-    tile = number - first_tile(a, s.b, s.tok0);
-  }
+  const int w = wave_id(), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15, D = c.D;
+  const int rest = f.splits.of(blockIdx.x), number = f.heads.of(rest);
+  const int kvh = rest - number * c.hkv;
+  int split = blockIdx.x - rest * a.n_splits + number;  // (a tile's splits from another one on)
+  split -= f.splits.of(split) * a.n_splits;
+  const CacheSeq s = find_seq(c, lane, number, [&](int b, int to) { return (to * a.group >> 4) + b; });
   const int b = s.b;
   if (b >= c.n_seqs) return;
-  const int r0 = tile * 16, n_rows = s.n * a.group;
-  if (tile < 0 || r0 >= n_rows) return;
-  const TileKeys tk = tile_keys(a, s, tile);
+  const int r0 = 16 * (number - (s.tok0 * a.group >> 4) - b), n_rows = s.n * a.group;
+  if (r0 < 0 || r0 >= n_rows) return;
+  const int tok0 = f.group.of(r0), head0 = r0 - tok0 * a.group;  // the tile's first row
+  const int last = min(s.n - 1, tok0 + f.few_of(head0 + 15, a.group));
+  const TileKeys tk = keys_up_to(a, s, last);
   if (split >= tk.active) return;
   const int k0 = split * tk.per, k1 = min(tk.kend, k0 + tk.per);
 
-  // this lane's row: its last key and its query, columns 32 i + 8 g .. of each group
-  const int row = r0 + col, tok = row / a.group, head = kvh * a.group + (row - tok * a.group);
-  const bool has_row = row < n_rows;
-  const int limit = has_row ? s.pos0 + tok : -1;
-  const T* const q = static_cast<const T*>(a.q) +
-                     (has_row ? (long)(s.tok0 + tok) * a.hq + head : (long)(s.tok0 + r0 / a.group) * a.hq) * D;
-  constexpr int TERMS = F32 ? 3 : 1;
-  bf16x8 qf[TERMS][G];
-  f32x4 base[F32 ? 1 : G];  // -136 sum(q) of each group
-#pragma unroll
-  for (int i = 0; i < G; ++i) {
-    const int at = 32 * i + 8 * g;
-    const bool ok = has_row && at < D;
-    float x[8];
-    load8(q + (at < D ? at : 0), x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = ok ? x[e] : 0.0f;
-    if constexpr (F32) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        qf[0][i][e] = (bf16)x[e];
-        const float r1 = x[e] - (float)qf[0][i][e];
-        qf[1][i][e] = (bf16)r1;
-        qf[2][i][e] = (bf16)(r1 - (float)qf[1][i][e]);
-      }
-    } else {
-      float sum = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        qf[0][i][e] = (bf16)x[e];
-        sum += x[e];
-      }
-      sum = -136.0f * col_sum_swap(sum);
-      base[i] = f32x4{sum, sum, sum, sum};
-    }
-  }
-
   const int part_bytes = quant_row_bytes(D) << c.page_shift, words_bytes = (16 * G) << c.page_shift;
   const long head_at = (long)kvh * part_bytes;
-  // this lane's places in 16 keys (bytes): words and scales of K and V
-  const int k_at = (col * 4 + g) * G * 4, ks_at = 8 * G * g;
-  int v_at[NV], vs_at[NV];
+  // this lane's places in a tile of its ring (bytes): words and scales of K and V
+  unsigned char* const ring = smem + w * L::STAGES * L::BLOCK;
+  const unsigned ring_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>((GLACIER_LDS unsigned char*)ring));
+  const unsigned k_at = ring_at + (col * 4 + g) * G * 4, ks_at = ring_at + L::KS + 8 * G * g;
+  unsigned v_at[NV], vs_at[NV];
 #pragma unroll
   for (int x = 0; x < NV; ++x) {
     const int word = min(HALF ? col >> 1 : 16 * x + col, 4 * G - 1);
-    v_at[x] = (g * 4 * G + word) * 16;
-    vs_at[x] = (g * G + word / 4) * 8;
+    v_at[x] = ring_at + L::V + (g * 4 * G + word) * 16;
+    vs_at[x] = ring_at + L::VS + (g * G + word / 4) * 8;
   }
   const unsigned pick = HALF && (col & 1) ? 0x07060302u : 0x05040100u;  // which halves of a pair of words
   const auto* const table = (const __attribute__((address_space(4))) int32_t*)(
       reinterpret_cast<uintptr_t>(c.table + (long)b * c.table_stride));
-  int page[2];  // of the block to be loaded next
+  // The table's entries of the block to be requested next.  They are looked up a block
+  // ahead, by scalar loads, and not looked at before they are needed: any wait for LDS
+  // is one for them too.
+  int entry[2];
   auto look_up = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       const int key = j + 16 * p;
-      const int at = table[min(key >> c.page_shift, c.max_pages - 1)];
-      page[p] = key < k1 && static_cast<unsigned>(at) < static_cast<unsigned>(c.n_pages) ? at : -1;
+      entry[p] = -1;
+      if (key < k1) entry[p] = table[min(key >> c.page_shift, c.max_pages - 1)];
     }
   };
-  // loads block j and looks up the wave's next one
-  auto load = [&](B& x, int (&here)[2], int j) __attribute__((always_inline)) {
+  // requests block j into slot `to` of the ring (zeros for a tile without a page);
+  // which of its tiles have a page
+  auto load = [&](int to, int j) __attribute__((always_inline)) {
+    unsigned found = 0;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int key = j + 16 * p, in_page = key & ((1 << c.page_shift) - 1);
-      here[p] = page[p] < 0 ? 0 : min(16, k1 - key);
-      const long at = (page[p] < 0 ? 0 : page[p]) * c.page_stride + head_at;
-      const int bytes = page[p] < 0 ? 0 : part_bytes;
-      const auto kr = wave_rsrc(static_cast<const char*>(c.k_pages) + at, bytes);
-      const auto vr = wave_rsrc(static_cast<const char*>(c.v_pages) + at, bytes);
-      const int rows = in_page * 16 * G, scales = words_bytes + in_page * 2 * G;
-      load_words<G>(kr, k_at, rows, x.k[p]);
-      load_words<2 * G>(kr, ks_at, scales, x.ks[p]);
+      const int in_page = (j + 16 * p) & ((1 << c.page_shift) - 1);
+      const bool held = static_cast<unsigned>(entry[p]) < static_cast<unsigned>(c.n_pages);
+      const long at = (held ? entry[p] : 0) * c.page_stride + head_at;
+      const int bytes = held ? part_bytes : 0;
+      found |= held ? 1u << p : 0u;
+      unsigned char* const slot = ring + to * L::BLOCK + p * L::TILE;
 #pragma unroll
-      for (int y = 0; y < NV; ++y) {
-        load_words<4>(vr, v_at[y], rows, x.v[p][y]);
-        load_words<2>(vr, vs_at[y], scales, x.vs[p][y]);
+      for (int side = 0; side < 2; ++side) {
+        const auto rs = wave_rsrc(static_cast<const char*>(side ? c.v_pages : c.k_pages) + at, bytes);
+        unsigned char* const dst = slot + (side ? L::V : 0);
+#pragma unroll
+        for (int n = 0; n < L::ND; ++n)
+          if (L::WORDS % 1024 == 0 || lane < (L::WORDS - 1024 * n) / 16)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (GLACIER_LDS void*)(dst + 1024 * n), 16,
+                                                     16 * lane + 1024 * n, in_page * 16 * G, 0, 0);
+        if (lane < L::SCALES / 16)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (GLACIER_LDS void*)(dst + L::WORDS), 16, 16 * lane,
+                                                   words_bytes + in_page * 2 * G, 0, 0);
       }
     }
-    look_up(j + kWavesQ * kKeysQ);
+    return found;
   };
 
+  constexpr int STEP = kWavesQ * kKeysQ, AHEAD = L::STAGES - 1;
+  const int first = k0 + w * kKeysQ, blocks = first < k1 ? (k1 - first + STEP - 1) / STEP : 0;
+  unsigned there;  // two bits a block: its tiles that have a page, this block's lowest
+  auto request = [&](int i) __attribute__((always_inline)) {
+    there |= load(i % L::STAGES, first + i * STEP) << 2 * AHEAD;
+  };
+  // the first blocks of a walk (past its end: loads of nothing, so that the compiler
+  // sees how many are under way when it waits for the queries)
+  auto start = [&]() __attribute__((always_inline)) {
+    there = 0;
+    look_up(first);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      request(i);
+      look_up(first + (i + 1) * STEP);
+      there >>= 2;
+    }
+  };
+
+  // this lane's row: its last key and its query, columns 32 i + 8 g .. of each group
+  const int over = f.few_of(head0 + col, a.group), tok = tok0 + over, head = kvh * a.group + head0 + col - over * a.group;
+  const bool has_row = r0 + col < n_rows;
+  const int limit = has_row ? s.pos0 + tok : -1;
+  const T* const q = static_cast<const T*>(a.q) +
+                     (has_row ? (long)(s.tok0 + tok) * a.hq + head : (long)(s.tok0 + tok0) * a.hq) * D;
+  constexpr int TERMS = F32 ? 3 : 1;
+  bf16x8 qf[TERMS][G];
+  f32x4 base[F32 ? 1 : G];  // -136 sum(q) of each group, by a product of its own
+  i32x4 raw[G][F32 ? 2 : 1];
+#pragma unroll
+  for (int i = 0; i < G; ++i)
+#pragma unroll
+    for (int x = 0; x < (F32 ? 2 : 1); ++x)
+      raw[i][x] = *reinterpret_cast<const i32x4*>(q + (32 * i + 8 * g < D ? 32 * i + 8 * g + 4 * x : 0));
+  __builtin_amdgcn_sched_barrier(0);  // (requested before the keys, or its wait is for them too)
+  start();
+  bf16x8 minus;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) minus[e] = (bf16)-136.0f;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    const bool ok = has_row && 32 * i + 8 * g < D;
+#pragma unroll
+    for (int x = 0; x < (F32 ? 2 : 1); ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw[i][x][e] = ok ? raw[i][x][e] : 0;
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_bit_cast(f32x4, raw[i][e / 4])[e % 4];
+        qf[0][i][e] = (bf16)x;
+        const float r1 = x - (float)qf[0][i][e];
+        qf[1][i][e] = (bf16)r1;
+        qf[2][i][e] = (bf16)(r1 - (float)qf[1][i][e]);
+      }
+    } else {
+      qf[0][i] = __builtin_bit_cast(bf16x8, raw[i][0]);
+      base[i] = Mfma<bf16>::mma(minus, qf[0][i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    }
+  }
+
+  const QuantMagic magic;
   f32x4 acc[NB];
   float m, l;
-  const int first_limit = s.pos0 + r0 / a.group;  // the tile's first row sees keys up to here
-  auto take = [&](B& x, const int (&here)[2], int j, auto careful) __attribute__((always_inline)) {
+  const int first_limit = s.pos0 + tok0;  // the tile's first row sees keys up to here
+  auto take = [&](int slot, const int (&here)[2], int j, auto careful) __attribute__((always_inline)) {
+    const unsigned base_at = slot * L::BLOCK;
+    LdsWords<G, 0> kw[2];
+    LdsWords<2 * G, 0> ks[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      kw[p].issue(k_at + base_at + p * L::TILE);
+      ks[p].issue(ks_at + base_at + p * L::TILE);
+    }
+    lgkm<0>();
+#pragma unroll
+    for (int p = 0; p < 2; ++p) kw[p].settled(), ks[p].settled();
+    look_up(j + L::STAGES * kWavesQ * kKeysQ);
     const bool whole = j + kKeysQ - 1 <= first_limit && here[0] == 16 && here[1] == 16;
     // S^T: keys 16 p + 4 g + r of this block, row col
     f32x4 st[2];
@@ -208,30 +318,44 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
       for (int i = 0; i < G; ++i) {
         f32x4 d;
         if constexpr (F32) {
-          const bf16x8 kf = exact8_bf16(x.k[p][i]);
+          const bf16x8 kf = exact8_bf16(kw[p][i], magic);
           d = Mfma<bf16>::mma(kf, qf[2][i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
           d = Mfma<bf16>::mma(kf, qf[1][i], d);
           d = Mfma<bf16>::mma(kf, qf[0][i], d);
         } else {
-          d = Mfma<bf16>::mma(raw8_bf16(x.k[p][i]), qf[0][i], base[i]);
+          d = Mfma<bf16>::mma(raw8_bf16(kw[p][i], magic), qf[0][i], base[i]);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) st[p][r] = fmaf(half_at(x.ks[p][(r * G + i) / 2], (r * G + i) % 2), d[r], st[p][r]);
+        for (int r = 0; r < 4; ++r) st[p][r] = fmaf(half_at(ks[p][(r * G + i) / 2], (r * G + i) % 2), d[r], st[p][r]);
       }
+    }
+    LdsWords<4, 0> vw[2][NV];
+    LdsWords<2, 0> vs[2][NV];
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int y = 0; y < NV; ++y) {
+        vw[p][y].issue(v_at[y] + base_at + p * L::TILE);
+        vs[p][y].issue(vs_at[y] + base_at + p * L::TILE);
+      }
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[p][r] *= a.scale_log2;
+    if (!whole) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int at = 4 * g + r;
+          st[p][r] = at < here[p] && j + 16 * p + at <= limit ? st[p][r] : -INFINITY;
+        }
     }
     float top = kLeast;
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float y = st[p][r] * a.scale_log2;
-        if (!whole) {
-          const int at = 4 * g + r;
-          y = at < here[p] && j + 16 * p + at <= limit ? y : -INFINITY;
-        }
-        st[p][r] = y;
-        top = fmaxf(top, y);
-      }
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, st[p][r]);
     const float mn = fmaxf(m, col_max_swap(top));
     if (__any(mn != m)) {
       const float alpha = weight(m - mn);
@@ -249,6 +373,11 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
         st[p][r] = weight(st[p][r] - mn);
         l += st[p][r];
       }
+    lgkm<0>();
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int y = 0; y < NV; ++y) vw[p][y].settled(), vs[p][y].settled();
     // scales of V that count: not those of keys that are not there
     if (!whole) {
 #pragma unroll
@@ -256,7 +385,7 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
         const int n = here[p] - 4 * g;  // of this lane's four tokens
         const unsigned keep0 = n <= 0 ? 0u : n == 1 ? 0xffffu : ~0u, keep1 = n <= 2 ? 0u : n == 3 ? 0xffffu : ~0u;
 #pragma unroll
-        for (int y = 0; y < NV; ++y) x.vs[p][y][0] &= keep0, x.vs[p][y][1] &= keep1;
+        for (int y = 0; y < NV; ++y) vs[p][y].keep(0, keep0), vs[p][y].keep(1, keep1);
       }
     }
     if constexpr (careful()) {
@@ -265,7 +394,7 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
 #pragma unroll
         for (int y = 0; y < NV; ++y)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) x.vs[p][y][u] &= ~nan_halves(x.vs[p][y][u]);
+          for (int u = 0; u < 2; ++u) vs[p][y].keep(u, ~nan_halves(vs[p][y][u]));
     }
     // O^T += V^T P^T
     constexpr int PT = F32 ? 3 : 2;
@@ -279,16 +408,16 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
         rest -= (float)pf[z][e];
       }
     }
-    const f16x2 k24 = {(f16)-24.0f, (f16)-24.0f};
 #pragma unroll
     for (int y = 0; y < NV; ++y) {
-      f16x2 sc[2][2], off[2][2];
+      float off[2][4][2];  // of a token: -1032 s and -72 s
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          sc[p][u] = __builtin_bit_cast(f16x2, x.vs[p][y][u]);
-          off[p][u] = sc[p][u] * k24;
+        for (int u = 0; u < 4; ++u) {
+          const float sc = half_at(vs[p][y][u / 2], u % 2);
+          off[p][u][0] = -1032.0f * sc;
+          off[p][u][1] = -72.0f * sc;
         }
 #pragma unroll
       for (int z = 0; z < (HALF ? 1 : 2); ++z) {
@@ -297,7 +426,7 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) both[p][u] = __builtin_amdgcn_perm(x.v[p][y][2 * u + 1], x.v[p][y][2 * u], sel);
+          for (int u = 0; u < 2; ++u) both[p][u] = __builtin_amdgcn_perm(vw[p][y][2 * u + 1], vw[p][y][2 * u], sel);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           u32x4 vf;
@@ -305,12 +434,12 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
           for (int p = 0; p < 2; ++p)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              // 16 + n: the number in the four bits above 2^-7 of 16
-              const unsigned n = both[p][u];
-              const unsigned at = e == 0 ? n << 6 : e == 1 ? n << 2 : e == 2 ? n >> 2 : n >> 6;
-              const f16x2 h = __builtin_bit_cast(f16x2, (at & 0x03c003c0u) | 0x4c004c00u);
-              vf[2 * p + u] = upper_pair(fmaf((float)h[0], (float)sc[p][u][0], (float)off[p][u][0]),
-                                         fmaf((float)h[1], (float)sc[p][u][1], (float)off[p][u][1]));
+              // 1024 + n from bits 0-3 of a half, 64 + n from bits 4-7
+              const unsigned n = e < 2 ? both[p][u] : both[p][u] >> 8;
+              const f16x2 h = __builtin_bit_cast(
+                  f16x2, e % 2 == 0 ? (n & 0x000f000fu) | magic.h1024 : (n & 0x00f000f0u) | magic.h64);
+              vf[2 * p + u] = upper_pair(fmaf((float)h[0], half_at(vs[p][y][u], 0), off[p][2 * u][e % 2]),
+                                         fmaf((float)h[1], half_at(vs[p][y][u], 1), off[p][2 * u + 1][e % 2]));
             }
           const int n = 8 * y + 4 * z + e;
 #pragma unroll
@@ -324,20 +453,17 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
     l = 0.0f;
 #pragma unroll
     for (int n = 0; n < NB; ++n) acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int STEP = kWavesQ * kKeysQ;
-    B x, y;
-    int here_x[2], here_y[2];
-    int j = k0 + w * kKeysQ;
-    if (j < k1) {
-      look_up(j);
-      load(x, here_x, j);
-    }
-    for (; j < k1; j += 2 * STEP) {  // two blocks a turn, each loaded while the other is worked on
-      if (j + STEP < k1) load(y, here_y, j + STEP);
-      take(x, here_x, j, careful);
-      if (j + STEP >= k1) break;
-      if (j + 2 * STEP < k1) load(x, here_x, j + 2 * STEP);
-      take(y, here_y, j + STEP, careful);
+    for (int i = 0; i < blocks; ++i) {
+      if (i + AHEAD < blocks) {
+        request(i + AHEAD);
+        vmw<AHEAD * L::LOADS>();
+      } else {
+        vm_wait_v((blocks - 1 - i) * L::LOADS);
+      }
+      const int j = first + i * STEP;
+      const int here[2] = {there & 1 ? min(16, k1 - j) : 0, there & 2 ? max(0, min(16, k1 - j - 16)) : 0};
+      take(i % L::STAGES, here, j, careful);
+      there >>= 2;
     }
   };
   walk(std::false_type{});
@@ -347,6 +473,7 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
 #pragma unroll
     for (int r = 0; r < 4; ++r) odd |= has_row ? not_finite(acc[n][r]) : 0;
   if (__any(odd != 0)) {
+    start();
     walk(std::true_type{});
     // a lane's sums of one block belong to one group of columns
     for (int j = k0 + w * kKeysQ; j < k1; j += kWavesQ * kKeysQ)
@@ -369,6 +496,9 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
   }
 
   // join the waves: region of wave u: sums [16][OS], maxima [16], totals [16]
+  vmw<0>();
+  __syncthreads();
+  float* const all = reinterpret_cast<float*>(smem);
   float* const mine = all + w * L::WAVE;
   const float total_w = col_sum_swap(l);
 #pragma unroll
@@ -407,14 +537,14 @@ __global__ __launch_bounds__(64 * kWavesQ, G <= 4 ? 2 : 1) void qcache_attn_kern
 #pragma unroll
     for (int u = 0; u < kWavesQ; ++u) {
       const float* reg = all + u * L::WAVE;
-      const float f = weight(reg[16 * L::OS + at_row] - mx);
-      total += f * reg[16 * (L::OS + 1) + at_row];
+      const float part = weight(reg[16 * L::OS + at_row] - mx);
+      total += part * reg[16 * (L::OS + 1) + at_row];
       const f32x4 v = *reinterpret_cast<const f32x4*>(reg + at_row * L::OS + d);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += f * v[e];
+      for (int e = 0; e < 4; ++e) o[e] += part * v[e];
     }
-    const int i = r / a.group, h = kvh * a.group + (r - i * a.group);
-    const long t = s.tok0 + i, at = t * a.hq + h;
+    const int i = f.few_of(head0 + at_row, a.group), h = kvh * a.group + head0 + at_row - i * a.group;
+    const long t = s.tok0 + tok0 + i, at = t * a.hq + h;
     if (tk.active > 1) {
       const long slot = (long)split * c.T * a.hq + at;
       store4(a.part_o + slot * D + d, o);
@@ -465,8 +595,12 @@ __global__ __launch_bounds__(kExpandThreads) void qcache_expand_kernel(CacheView
 
 template <typename T, int G>
 hipError_t attend(const CacheAttn& a, hipStream_t st) {
-  hipLaunchKernelGGL((qcache_attn_kernel<T, G>), dim3(tile_numbers(a) * a.c.hkv * a.n_splits), dim3(64 * kWavesQ), 0,
-                     st, a);
+  constexpr int BYTES = QaLayout<G>::BYTES;
+  GL_CHECK(allow_lds(&qcache_attn_kernel<T, G>, BYTES));
+  const unsigned numbers = tile_numbers(a), heads = numbers * a.c.hkv, groups = heads * a.n_splits;
+  const TileDivs f{FixedDiv::by(a.n_splits, groups), FixedDiv::by(a.c.hkv, heads),
+                   FixedDiv::by(a.group, (unsigned long long)a.c.T * a.group), (65535u + a.group) / a.group};
+  hipLaunchKernelGGL((qcache_attn_kernel<T, G>), dim3(groups), dim3(64 * kWavesQ), BYTES, st, a, f);
   return hipGetLastError();
 }
 template <typename T, int G>
@@ -513,8 +647,13 @@ QCachePlan qcache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv,
   const long tiles = seqs * ((c.T * group + seqs * 16 - 1) / (seqs * 16));
   p.attn.rows = 16;
   p.attn.long_first = false;
-  const long want = 4L * n_cu / std::max(1L, tiles * c.hkv);
-  const long most = keys <= 1024 ? 1 : keys / 512;
+#ifndef GL_QWANT
+#define GL_QWANT 4L
+#define GL_QLEAST 512
+#define GL_QWHOLE 1024
+#endif
+  const long want = GL_QWANT * n_cu / std::max(1L, tiles * c.hkv);
+  const long most = keys <= GL_QWHOLE ? 1 : keys / GL_QLEAST;
   const long launch = (1L << 22) / ((long)c.n_seqs * c.hkv);
   p.attn.n_splits = static_cast<int>(std::max(1L, std::min({want, most, (long)kMaxSplits, launch})));
   const long even = (keys + p.attn.n_splits - 1) / p.attn.n_splits;

@@ -89,23 +89,36 @@ __device__ inline int k_scale(int row, int G, int i) { return row * G + i; }
 __device__ inline int v_word(int row, int G, int col8) { return ((row >> 2) * 4 * G + col8) * 4 + (row & 3); }
 __device__ inline int v_scale(int row, int G, int i) { return ((row >> 2) * G + i) * 4 + (row & 3); }
 
+// The constants of raw numbers: a register each, since and-or takes one constant from
+// elsewhere only (as a literal each would be an operation of its own).
+struct QuantMagic {
+  unsigned bf128 = 0x43004300u;  // bf16 128
+  unsigned h1024 = 0x64006400u, h64 = 0x54005400u;  // fp16 1024, 64
+  __device__ inline QuantMagic() {
+    asm("" : "+v"(bf128));
+    asm("" : "+v"(h1024));
+    asm("" : "+v"(h64));
+  }
+};
 // Two numbers n, n' (in bits 0-3 and 16-19 of w >> shift) as bf16 128 + n, 128 + n'.
-__device__ inline unsigned pair_bf16(unsigned w, int shift) { return ((w >> shift) & 0x000f000fu) | 0x43004300u; }
+__device__ inline unsigned pair_bf16(unsigned w, int shift, const QuantMagic& c) {
+  return ((w >> shift) & 0x000f000fu) | c.bf128;
+}
 // A word's columns as a bf16 operand of 128 + n.
-__device__ inline bf16x8 raw8_bf16(unsigned w) {
-  return __builtin_bit_cast(bf16x8, u32x4{pair_bf16(w, 0), pair_bf16(w, 4), pair_bf16(w, 8), pair_bf16(w, 12)});
+__device__ inline bf16x8 raw8_bf16(unsigned w, const QuantMagic& c) {
+  return __builtin_bit_cast(bf16x8, u32x4{pair_bf16(w, 0, c), pair_bf16(w, 4, c), pair_bf16(w, 8, c), pair_bf16(w, 12, c)});
 }
 // Upper halves of two floats (bf16 values) as a pair.
 __device__ inline unsigned upper_pair(float lo, float hi) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, hi), __builtin_bit_cast(unsigned, lo), 0x07060302u);
 }
 // A word's columns as a bf16 operand of n - 8.
-__device__ inline unsigned exact_pair(unsigned w, int shift) {
-  const unsigned p = pair_bf16(w, shift);
+__device__ inline unsigned exact_pair(unsigned w, int shift, const QuantMagic& c) {
+  const unsigned p = pair_bf16(w, shift, c);
   return upper_pair(__builtin_bit_cast(float, p << 16) - 136.0f, __builtin_bit_cast(float, p & 0xffff0000u) - 136.0f);
 }
-__device__ inline bf16x8 exact8_bf16(unsigned w) {
-  return __builtin_bit_cast(bf16x8, u32x4{exact_pair(w, 0), exact_pair(w, 4), exact_pair(w, 8), exact_pair(w, 12)});
+__device__ inline bf16x8 exact8_bf16(unsigned w, const QuantMagic& c) {
+  return __builtin_bit_cast(bf16x8, u32x4{exact_pair(w, 0, c), exact_pair(w, 4, c), exact_pair(w, 8, c), exact_pair(w, 12, c)});
 }
 
 }  // namespace glacier
