@@ -11,14 +11,19 @@ struct KeySplit {
   int per, active;  // keys of a split, at least one unit; splits that have keys, at least one
 };
 // Of keys 0 .. kend - 1 (none where kend is 0): split_keys of them a split, more
-// where that would take more than n_splits, and as many splits as that evenly.
+// where that would take more than n_splits, and as many splits as that evenly, all
+// counted in units.  up(a, b): a / b rounded up, a below 2^24, b at least 1.
+template <typename F>
+constexpr KeySplit split_with(int kend, int n_splits, int split_keys, F up) {
+  auto one = [](int n) { return n < 1 ? 1 : n; };
+  const int keys = (kend + kSplitUnit - 1) / kSplitUnit, given = (split_keys + kSplitUnit - 1) / kSplitUnit;
+  const int least = one(up(keys, n_splits));
+  const int active = one(up(keys, given > least ? given : least));
+  const int per = one(up(keys, active));
+  return {per * kSplitUnit, one(up(keys, per))};
+}
 constexpr KeySplit split_of(int kend, int n_splits, int split_keys) {
-  auto units = [](int keys) { return keys <= kSplitUnit ? kSplitUnit : (keys + kSplitUnit - 1) / kSplitUnit * kSplitUnit; };
-  auto splits = [](int keys, int per) { return keys <= per ? 1 : (keys + per - 1) / per; };
-  const int least = units((kend + n_splits - 1) / n_splits);
-  const int active = splits(kend, split_keys > least ? split_keys : least);
-  const int per = units((kend + active - 1) / active);
-  return {per, splits(kend, per)};
+  return split_with(kend, n_splits, split_keys, [](int a, int b) { return (a + b - 1) / b; });
 }
 
 }  // namespace glacier

@@ -63,14 +63,24 @@ struct TileKeys {
   int kend;  // keys 0 .. kend - 1
   int per, active;  // keys of a split, and how many splits have any
 };
+// a / b rounded up (0 <= a < 2^24, b >= 1): the reciprocal's product is off by at most
+// two downwards and one upwards, which the remainder tells; an integer division is 30
+// instructions.
+__device__ inline int div_up(int a, int b) {
+  const int q = static_cast<int>(static_cast<float>(a) * __builtin_amdgcn_rcpf(static_cast<float>(b)));
+  const int rest = a - q * b;
+  return q + (rest > 0 ? 1 : 0) + (rest > b ? 1 : 0) + (rest > 2 * b ? 1 : 0) - (rest <= -b ? 1 : 0);
+}
 __device__ inline TileKeys keys_up_to(const CacheAttn& a, const CacheSeq& s, int last) {
   TileKeys k;
   const long cap = (long)a.c.max_pages << a.c.page_shift;
   const long end = (long)s.pos0 + last + 1;
   k.kend = static_cast<int>(end < 0 ? 0 : end < cap ? end : cap);
-  const KeySplit split = split_of(k.kend, a.n_splits, a.split_keys);
-  k.per = split.per;
-  k.active = split.active;
+  KeySplit split{(k.kend + kSplitUnit - 1) / kSplitUnit * kSplitUnit, 1};  // (n_splits 1: what split_with gives)
+  if (split.per == 0) split.per = kSplitUnit;
+  if (a.n_splits > 1) split = split_with(k.kend, a.n_splits, a.split_keys, div_up);
+  k.per = __builtin_amdgcn_readfirstlane(split.per);
+  k.active = __builtin_amdgcn_readfirstlane(split.active);
   return k;
 }
 __device__ inline TileKeys tile_keys(const CacheAttn& a, const CacheSeq& s, int tile) {

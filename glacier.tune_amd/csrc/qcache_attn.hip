@@ -33,38 +33,33 @@
 namespace glacier {
 namespace {
 
-#ifndef GL_QW
-#define GL_QW 4
-#endif
-constexpr int kWavesQ = GL_QW;
 [[maybe_unused]] constexpr int kKeysQ = 32;  // keys of a wave's block: one k-step of the second product
-#ifndef GL_QSTAGES
-#define GL_QSTAGES 2
-#endif
-#ifndef GL_QOCC
-#define GL_QOCC (G <= 4 ? 2 : 1)
-#endif
+constexpr int kWavesQ = 4;
 
-// A wave's blocks in LDS, a ring of STAGES: for each tile of 16 keys the words and then
-// the scales of K and of V, as they lie in the page.
-template <int G>
+// LDS of a workgroup: its queries, operands of the first product (and -136 sum(q), where
+// its sums begin), then for each wave one block of K and one of V, words and then scales
+// of two tiles of 16 keys, as they lie in the pages.
+template <typename T, int G>
 struct QaLayout {
+  static constexpr int WAVES = kWavesQ;
+  static constexpr bool KEEP = sizeof(T) == 2;  // the queries stay in registers (fp32: three times as many)
+
   static constexpr int NV = (G + 3) / 4;    // blocks of 16 words of a token of V
   static constexpr bool HALF = G <= 2;      // two lanes share a word
   static constexpr int NB = HALF ? 4 : 8 * NV;  // 16-column products
   static constexpr int DP = 32 * G;
+  static constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;  // of a query
+  static constexpr int QUERY = 1024 * (TERMS == 3 ? 3 : 2);  // bytes of a group's operands
   static constexpr int WORDS = 256 * G, SCALES = 32 * G;  // bytes, of 16 keys
-  static constexpr int KS = WORDS, V = KS + SCALES, VS = V + WORDS;  // behind K's words
-  static constexpr int TILE = VS + SCALES, BLOCK = 2 * TILE;
+  static constexpr int SIDE = 2 * (WORDS + SCALES);
   static constexpr int ND = (WORDS + 1023) / 1024;  // DMA instructions of a tile's words
-  static constexpr int LOADS = 4 * (ND + 1);        // of a block
-  static constexpr int STAGES = GL_QSTAGES;
+  static constexpr int LOADS = 2 * (ND + 1);        // of a side
+  static constexpr int RING = G * QUERY + WAVES * 2 * SIDE;
   static constexpr int OS = DP + 4;         // row stride (floats) of a wave's sums in the join
   static constexpr int WAVE = 16 * (OS + 2);
-  static constexpr int RING = kWavesQ * STAGES * BLOCK, JOIN = kWavesQ * WAVE * 4;
+  static constexpr int JOIN = WAVES * WAVE * 4;
   static constexpr int BYTES = RING > JOIN ? RING : JOIN;
   static_assert(BYTES <= 160 * 1024, "exceeds the LDS of a CU");
-  static_assert((STAGES - 1) * LOADS < 64, "more loads in flight than are counted");
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -127,6 +122,16 @@ struct LdsWords<0, OFF> {
   return ((((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u) >> 15) * 0xffffu;
 }
 
+// 32-bit LDS address.
+[[maybe_unused]] __device__ inline unsigned lds_at(unsigned char* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((GLACIER_LDS unsigned char*)p));
+}
+// Two floats rounded to bf16, the first in the lower half.
+[[maybe_unused]] __device__ inline unsigned pair_of(float a, float b) {
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, bf16x2{(bf16)a, (bf16)b});
+}
+
 // Division of x by a number known before the launch: one multiplication while x d is
 // below 2^32 for every x of the call (the product's error, below x d / 2^32, stays
 // under one step then), else a division.  A dozen divisions of 30 instructions each
@@ -150,10 +155,10 @@ struct TileDivs {
 };
 
 template <typename T, int G>
-__global__ __launch_bounds__(64 * kWavesQ, GL_QOCC) void qcache_attn_kernel(CacheAttn a, TileDivs f) {
+__global__ __launch_bounds__((64 * QaLayout<T, G>::WAVES), G <= 4 ? 3 : 2) void qcache_attn_kernel(CacheAttn a, TileDivs f) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using L = QaLayout<G>;
-  constexpr int NV = L::NV, NB = L::NB;
+  using L = QaLayout<T, G>;
+  constexpr int NV = L::NV, NB = L::NB, WAVES = L::WAVES, TERMS = L::TERMS;
   constexpr bool F32 = sizeof(T) == 4, HALF = L::HALF;
   extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
@@ -175,168 +180,191 @@ __global__ __launch_bounds__(64 * kWavesQ, GL_QOCC) void qcache_attn_kernel(Cach
 
   const int part_bytes = quant_row_bytes(D) << c.page_shift, words_bytes = (16 * G) << c.page_shift;
   const long head_at = (long)kvh * part_bytes;
-  // this lane's places in a tile of its ring (bytes): words and scales of K and V
-  unsigned char* const ring = smem + w * L::STAGES * L::BLOCK;
-  const unsigned ring_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>((GLACIER_LDS unsigned char*)ring));
-  const unsigned k_at = ring_at + (col * 4 + g) * G * 4, ks_at = ring_at + L::KS + 8 * G * g;
+  const auto* const table = (const __attribute__((address_space(4))) int32_t*)(
+      reinterpret_cast<uintptr_t>(c.table + (long)b * c.table_stride));
+  constexpr int STEP = WAVES * kKeysQ;
+  const int first = k0 + w * kKeysQ;
+  // The table's entries of the block to be requested next (two pages of 16, or one).
+  // They are looked up a block ahead, by scalar loads, and not looked at before they are
+  // needed: any wait for LDS is one for them too.
+  int entry[2];
+  auto look_up = [&](int j) __attribute__((always_inline)) {
+    entry[0] = entry[1] = -1;
+    if (j < k1) entry[0] = table[min(j >> c.page_shift, c.max_pages - 1)];
+    if (c.page_shift == 4 && j + 16 < k1) entry[1] = table[min((j + 16) >> 4, c.max_pages - 1)];
+  };
+  look_up(first);
+
+  // this lane's row: its last key and its query
+  const int over = f.few_of(head0 + col, a.group), tok = tok0 + over, head = kvh * a.group + head0 + col - over * a.group;
+  const bool has_row = r0 + col < n_rows;
+  const int limit = has_row ? s.pos0 + tok : -1;
+  {
+    // columns 32 i + 8 g .. of groups i = w, w + WAVES, ..
+    const T* const q = static_cast<const T*>(a.q) +
+                       (has_row ? (long)(s.tok0 + tok) * a.hq + head : (long)(s.tok0 + tok0) * a.hq) * D;
+    bf16x8 minus;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) minus[e] = (bf16)-136.0f;
+#pragma unroll
+    for (int i0 = 0; i0 < G; i0 += WAVES) {
+      const int i = i0 + w, at = 32 * i + 8 * g;
+      if (i >= G) break;
+      i32x4 raw[F32 ? 2 : 1];
+#pragma unroll
+      for (int x = 0; x < (F32 ? 2 : 1); ++x) {
+        raw[x] = *reinterpret_cast<const i32x4*>(q + (at < D ? at + 4 * x : 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[x][e] = has_row && at < D ? raw[x][e] : 0;
+      }
+      unsigned char* const to = smem + i * L::QUERY + 16 * lane;
+      if constexpr (F32) {
+        bf16x8 term[3];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_bit_cast(f32x4, raw[e / 4])[e % 4];
+          term[0][e] = (bf16)x;
+          const float r1 = x - (float)term[0][e];
+          term[1][e] = (bf16)r1;
+          term[2][e] = (bf16)(r1 - (float)term[1][e]);
+        }
+#pragma unroll
+        for (int x = 0; x < 3; ++x) *reinterpret_cast<bf16x8*>(to + 1024 * x) = term[x];
+      } else {
+        const bf16x8 x = __builtin_bit_cast(bf16x8, raw[0]);
+        *reinterpret_cast<bf16x8*>(to) = x;
+        *reinterpret_cast<f32x4*>(to + 1024) = Mfma<bf16>::mma(minus, x, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+      }
+    }
+  }
+  __syncthreads();
+
+  // this lane's places (bytes): the queries, words and scales of K and V
+  unsigned char* const mine_at = smem + G * L::QUERY + w * 2 * L::SIDE;
+  const unsigned q_at = lds_at(smem) + 16 * lane;
+  const unsigned side_at = lds_at(mine_at);
+  const unsigned k_at = side_at + (col * 4 + g) * G * 4, ks_at = side_at + 2 * L::WORDS + 8 * G * g;
   unsigned v_at[NV], vs_at[NV];
 #pragma unroll
   for (int x = 0; x < NV; ++x) {
     const int word = min(HALF ? col >> 1 : 16 * x + col, 4 * G - 1);
-    v_at[x] = ring_at + L::V + (g * 4 * G + word) * 16;
-    vs_at[x] = ring_at + L::VS + (g * G + word / 4) * 8;
+    v_at[x] = side_at + L::SIDE + (g * 4 * G + word) * 16;
+    vs_at[x] = side_at + L::SIDE + 2 * L::WORDS + (g * G + word / 4) * 8;
   }
   const unsigned pick = HALF && (col & 1) ? 0x07060302u : 0x05040100u;  // which halves of a pair of words
-  const auto* const table = (const __attribute__((address_space(4))) int32_t*)(
-      reinterpret_cast<uintptr_t>(c.table + (long)b * c.table_stride));
-  // The table's entries of the block to be requested next.  They are looked up a block
-  // ahead, by scalar loads, and not looked at before they are needed: any wait for LDS
-  // is one for them too.
-  int entry[2];
-  auto look_up = [&](int j) __attribute__((always_inline)) {
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int key = j + 16 * p;
-      entry[p] = -1;
-      if (key < k1) entry[p] = table[min(key >> c.page_shift, c.max_pages - 1)];
-    }
-  };
-  // requests block j into slot `to` of the ring (zeros for a tile without a page);
-  // which of its tiles have a page
-  auto load = [&](int to, int j) __attribute__((always_inline)) {
-    unsigned found = 0;
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int in_page = (j + 16 * p) & ((1 << c.page_shift) - 1);
-      const bool held = static_cast<unsigned>(entry[p]) < static_cast<unsigned>(c.n_pages);
-      const long at = (held ? entry[p] : 0) * c.page_stride + head_at;
-      const int bytes = held ? part_bytes : 0;
-      found |= held ? 1u << p : 0u;
-      unsigned char* const slot = ring + to * L::BLOCK + p * L::TILE;
-#pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const auto rs = wave_rsrc(static_cast<const char*>(side ? c.v_pages : c.k_pages) + at, bytes);
-        unsigned char* const dst = slot + (side ? L::V : 0);
-#pragma unroll
-        for (int n = 0; n < L::ND; ++n)
-          if (L::WORDS % 1024 == 0 || lane < (L::WORDS - 1024 * n) / 16)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (GLACIER_LDS void*)(dst + 1024 * n), 16,
-                                                     16 * lane + 1024 * n, in_page * 16 * G, 0, 0);
-        if (lane < L::SCALES / 16)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (GLACIER_LDS void*)(dst + L::WORDS), 16, 16 * lane,
-                                                   words_bytes + in_page * 2 * G, 0, 0);
-      }
-    }
-    return found;
-  };
 
-  constexpr int STEP = kWavesQ * kKeysQ, AHEAD = L::STAGES - 1;
-  const int first = k0 + w * kKeysQ, blocks = first < k1 ? (k1 - first + STEP - 1) / STEP : 0;
-  unsigned there;  // two bits a block: its tiles that have a page, this block's lowest
-  auto request = [&](int i) __attribute__((always_inline)) {
-    there |= load(i % L::STAGES, first + i * STEP) << 2 * AHEAD;
+  // A block's pages: K's and V's two tiles of 16 keys, nothing where there is no page.
+  // (V's begin as many bytes behind K's as the pages do.)
+  long page_at[2];
+  int page_bytes[2], rows[2];
+  unsigned found = 0, there = 0;  // which tiles of the block requested last, and of this one, have a page
+  auto aim = [&](int j) __attribute__((always_inline)) {
+    found = 0;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (p == 1 && c.page_shift != 4) {  // the same page
+        page_at[1] = page_at[0];
+        found |= j + 16 < k1 ? found << 1 : 0;
+      } else {
+        const bool held = static_cast<unsigned>(entry[p]) < static_cast<unsigned>(c.n_pages);
+        page_at[p] = (held ? entry[p] : 0) * c.page_stride + head_at;
+        found |= held ? 1u << p : 0u;
+      }
+      page_bytes[p] = found >> p & 1 ? part_bytes : 0;
+      rows[p] = (j + 16 * p) & ((1 << c.page_shift) - 1);
+    }
   };
-  // the first blocks of a walk (past its end: loads of nothing, so that the compiler
-  // sees how many are under way when it waits for the queries)
+  auto request = [&](const void* pages, unsigned char* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const auto rs = wave_rsrc(static_cast<const char*>(pages) + page_at[p], page_bytes[p]);
+#pragma unroll
+      for (int n = 0; n < L::ND; ++n)
+        if (L::WORDS % 1024 == 0 || lane < (L::WORDS - 1024 * n) / 16)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (GLACIER_LDS void*)(to + p * L::WORDS + 1024 * n), 16,
+                                                   16 * lane + 1024 * n, rows[p] * 16 * G, 0, 0);
+      if (lane < L::SCALES / 16)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (GLACIER_LDS void*)(to + 2 * L::WORDS + p * L::SCALES), 16,
+                                                 16 * lane, words_bytes + rows[p] * 2 * G, 0, 0);
+    }
+  };
   auto start = [&]() __attribute__((always_inline)) {
-    there = 0;
-    look_up(first);
+    aim(first);
+    request(c.k_pages, mine_at);
+    request(c.v_pages, mine_at + L::SIDE);
+    look_up(first + STEP);
+  };
+  start();
+  LdsWords<4, 0> qw[G][TERMS], base[G];
+  auto queries = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      request(i);
-      look_up(first + (i + 1) * STEP);
-      there >>= 2;
+    for (int i = 0; i < G; ++i) {
+#pragma unroll
+      for (int x = 0; x < TERMS; ++x) qw[i][x].issue(q_at + i * L::QUERY + 1024 * x);
+      if constexpr (!F32) base[i].issue(q_at + i * L::QUERY + 1024);
     }
   };
-
-  // this lane's row: its last key and its query, columns 32 i + 8 g .. of each group
-  const int over = f.few_of(head0 + col, a.group), tok = tok0 + over, head = kvh * a.group + head0 + col - over * a.group;
-  const bool has_row = r0 + col < n_rows;
-  const int limit = has_row ? s.pos0 + tok : -1;
-  const T* const q = static_cast<const T*>(a.q) +
-                     (has_row ? (long)(s.tok0 + tok) * a.hq + head : (long)(s.tok0 + tok0) * a.hq) * D;
-  constexpr int TERMS = F32 ? 3 : 1;
-  bf16x8 qf[TERMS][G];
-  f32x4 base[F32 ? 1 : G];  // -136 sum(q) of each group, by a product of its own
-  i32x4 raw[G][F32 ? 2 : 1];
+  auto queries_settled = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < G; ++i)
+    for (int i = 0; i < G; ++i) {
 #pragma unroll
-    for (int x = 0; x < (F32 ? 2 : 1); ++x)
-      raw[i][x] = *reinterpret_cast<const i32x4*>(q + (32 * i + 8 * g < D ? 32 * i + 8 * g + 4 * x : 0));
-  __builtin_amdgcn_sched_barrier(0);  // (requested before the keys, or its wait is for them too)
-  start();
-  bf16x8 minus;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) minus[e] = (bf16)-136.0f;
-#pragma unroll
-  for (int i = 0; i < G; ++i) {
-    const bool ok = has_row && 32 * i + 8 * g < D;
-#pragma unroll
-    for (int x = 0; x < (F32 ? 2 : 1); ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) raw[i][x][e] = ok ? raw[i][x][e] : 0;
-    if constexpr (F32) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = __builtin_bit_cast(f32x4, raw[i][e / 4])[e % 4];
-        qf[0][i][e] = (bf16)x;
-        const float r1 = x - (float)qf[0][i][e];
-        qf[1][i][e] = (bf16)r1;
-        qf[2][i][e] = (bf16)(r1 - (float)qf[1][i][e]);
-      }
-    } else {
-      qf[0][i] = __builtin_bit_cast(bf16x8, raw[i][0]);
-      base[i] = Mfma<bf16>::mma(minus, qf[0][i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+      for (int x = 0; x < TERMS; ++x) qw[i][x].settled();
+      if constexpr (!F32) base[i].settled();
     }
+  };
+  if constexpr (L::KEEP) {
+    queries();
+    lgkm<0>();
+    queries_settled();
   }
 
   const QuantMagic magic;
   f32x4 acc[NB];
   float m, l;
   const int first_limit = s.pos0 + tok0;  // the tile's first row sees keys up to here
-  auto take = [&](int slot, const int (&here)[2], int j, auto careful) __attribute__((always_inline)) {
-    const unsigned base_at = slot * L::BLOCK;
+  // One block.  What it has read of LDS is requested anew for the next block at once, K's
+  // before its products and V's before its own, so that either has most of a block's time
+  // to come; the counts are of what may still be under way.
+  auto take = [&](int j, auto careful) __attribute__((always_inline)) {
+    vmw<L::LOADS>();  // K has come
     LdsWords<G, 0> kw[2];
     LdsWords<2 * G, 0> ks[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      kw[p].issue(k_at + base_at + p * L::TILE);
-      ks[p].issue(ks_at + base_at + p * L::TILE);
+      kw[p].issue(k_at + p * L::WORDS);
+      ks[p].issue(ks_at + p * L::SCALES);
     }
+    if constexpr (!L::KEEP) queries();
     lgkm<0>();
 #pragma unroll
     for (int p = 0; p < 2; ++p) kw[p].settled(), ks[p].settled();
-    look_up(j + L::STAGES * kWavesQ * kKeysQ);
+    if constexpr (!L::KEEP) queries_settled();
+    there = found;
+    const int here[2] = {there & 1 ? min(16, k1 - j) : 0, there & 2 ? min(16, k1 - j - 16) : 0};
     const bool whole = j + kKeysQ - 1 <= first_limit && here[0] == 16 && here[1] == 16;
+    aim(j + STEP);
+    request(c.k_pages, mine_at);
+    look_up(j + 2 * STEP);
     // S^T: keys 16 p + 4 g + r of this block, row col
     f32x4 st[2];
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      st[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < 2; ++p) st[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
         f32x4 d;
         if constexpr (F32) {
           const bf16x8 kf = exact8_bf16(kw[p][i], magic);
-          d = Mfma<bf16>::mma(kf, qf[2][i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-          d = Mfma<bf16>::mma(kf, qf[1][i], d);
-          d = Mfma<bf16>::mma(kf, qf[0][i], d);
+          d = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int x = TERMS - 1; x >= 0; --x) d = Mfma<bf16>::mma(kf, __builtin_bit_cast(bf16x8, qw[i][x].w), d);
         } else {
-          d = Mfma<bf16>::mma(raw8_bf16(kw[p][i], magic), qf[0][i], base[i]);
+          d = Mfma<bf16>::mma(raw8_bf16(kw[p][i], magic), __builtin_bit_cast(bf16x8, qw[i][0].w),
+                              __builtin_bit_cast(f32x4, base[i].w));
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) st[p][r] = fmaf(half_at(ks[p][(r * G + i) / 2], (r * G + i) % 2), d[r], st[p][r]);
-      }
-    }
-    LdsWords<4, 0> vw[2][NV];
-    LdsWords<2, 0> vs[2][NV];
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int y = 0; y < NV; ++y) {
-        vw[p][y].issue(v_at[y] + base_at + p * L::TILE);
-        vs[p][y].issue(vs_at[y] + base_at + p * L::TILE);
       }
 #pragma unroll
     for (int p = 0; p < 2; ++p)
@@ -366,18 +394,38 @@ __global__ __launch_bounds__(64 * kWavesQ, GL_QOCC) void qcache_attn_kernel(Cach
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[n][r] *= alpha;
     }
+    // the weights, and their bf16 terms by pairs
+    constexpr int PT = F32 ? 3 : 2;
+    u32x4 pf[PT];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float x = weight(st[e / 4][e % 4] - mn), y = weight(st[e / 4][e % 4 + 1] - mn);
+      l += x;
+      l += y;
+#pragma unroll
+      for (int z = 0; z < PT; ++z) {
+        const unsigned pair = pair_of(x, y);
+        pf[z][e / 2] = pair;
+        x -= __builtin_bit_cast(float, pair << 16);
+        y -= __builtin_bit_cast(float, pair & 0xffff0000u);
+      }
+    }
+    vmw<L::LOADS>();  // V has come
+    LdsWords<4, 0> vw[2][NV];
+    LdsWords<2, 0> vs[2][NV];
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        st[p][r] = weight(st[p][r] - mn);
-        l += st[p][r];
+      for (int y = 0; y < NV; ++y) {
+        vw[p][y].issue(v_at[y] + p * L::WORDS);
+        vs[p][y].issue(vs_at[y] + p * L::SCALES);
       }
     lgkm<0>();
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
       for (int y = 0; y < NV; ++y) vw[p][y].settled(), vs[p][y].settled();
+    request(c.v_pages, mine_at + L::SIDE);
     // scales of V that count: not those of keys that are not there
     if (!whole) {
 #pragma unroll
@@ -397,17 +445,6 @@ __global__ __launch_bounds__(64 * kWavesQ, GL_QOCC) void qcache_attn_kernel(Cach
           for (int u = 0; u < 2; ++u) vs[p][y].keep(u, ~nan_halves(vs[p][y][u]));
     }
     // O^T += V^T P^T
-    constexpr int PT = F32 ? 3 : 2;
-    bf16x8 pf[PT];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float rest = st[e / 4][e % 4];
-#pragma unroll
-      for (int z = 0; z < PT; ++z) {
-        pf[z][e] = (bf16)rest;
-        rest -= (float)pf[z][e];
-      }
-    }
 #pragma unroll
     for (int y = 0; y < NV; ++y) {
       float off[2][4][2];  // of a token: -1032 s and -72 s
@@ -443,7 +480,8 @@ __global__ __launch_bounds__(64 * kWavesQ, GL_QOCC) void qcache_attn_kernel(Cach
             }
           const int n = 8 * y + 4 * z + e;
 #pragma unroll
-          for (int t = PT - 1; t >= 0; --t) acc[n] = Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, vf), pf[t], acc[n]);
+          for (int t = PT - 1; t >= 0; --t)
+            acc[n] = Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pf[t]), acc[n]);
         }
       }
     }
@@ -453,18 +491,7 @@ __global__ __launch_bounds__(64 * kWavesQ, GL_QOCC) void qcache_attn_kernel(Cach
     l = 0.0f;
 #pragma unroll
     for (int n = 0; n < NB; ++n) acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < blocks; ++i) {
-      if (i + AHEAD < blocks) {
-        request(i + AHEAD);
-        vmw<AHEAD * L::LOADS>();
-      } else {
-        vm_wait_v((blocks - 1 - i) * L::LOADS);
-      }
-      const int j = first + i * STEP;
-      const int here[2] = {there & 1 ? min(16, k1 - j) : 0, there & 2 ? max(0, min(16, k1 - j - 16)) : 0};
-      take(i % L::STAGES, here, j, careful);
-      there >>= 2;
-    }
+    for (int j = first; j < k1; j += STEP) take(j, careful);
   };
   walk(std::false_type{});
   unsigned odd = 0;
@@ -473,10 +500,12 @@ __global__ __launch_bounds__(64 * kWavesQ, GL_QOCC) void qcache_attn_kernel(Cach
 #pragma unroll
     for (int r = 0; r < 4; ++r) odd |= has_row ? not_finite(acc[n][r]) : 0;
   if (__any(odd != 0)) {
+    vmw<0>();  // (the walk requests a block past its last one: nothing)
+    look_up(first);
     start();
     walk(std::true_type{});
     // a lane's sums of one block belong to one group of columns
-    for (int j = k0 + w * kKeysQ; j < k1; j += kWavesQ * kKeysQ)
+    for (int j = first; j < k1; j += STEP)
       for (int key = j; key < min(k1, j + kKeysQ); ++key) {
         const int at = cache_page(c, b, key);
         if (at < 0) continue;
@@ -526,16 +555,16 @@ __global__ __launch_bounds__(64 * kWavesQ, GL_QOCC) void qcache_attn_kernel(Cach
   }
   __syncthreads();
   constexpr int CPR = L::DP / 4;
-  for (int idx = threadIdx.x; idx < 16 * CPR; idx += 64 * kWavesQ) {
+  for (int idx = threadIdx.x; idx < 16 * CPR; idx += 64 * WAVES) {
     const int at_row = idx / CPR, d = 4 * (idx % CPR), r = r0 + at_row;
     if (r >= n_rows || d >= D) continue;
     float mx = kLeast;
 #pragma unroll
-    for (int u = 0; u < kWavesQ; ++u) mx = fmaxf(mx, all[u * L::WAVE + 16 * L::OS + at_row]);
+    for (int u = 0; u < WAVES; ++u) mx = fmaxf(mx, all[u * L::WAVE + 16 * L::OS + at_row]);
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float total = 0.0f;
 #pragma unroll
-    for (int u = 0; u < kWavesQ; ++u) {
+    for (int u = 0; u < WAVES; ++u) {
       const float* reg = all + u * L::WAVE;
       const float part = weight(reg[16 * L::OS + at_row] - mx);
       total += part * reg[16 * (L::OS + 1) + at_row];
@@ -595,12 +624,12 @@ __global__ __launch_bounds__(kExpandThreads) void qcache_expand_kernel(CacheView
 
 template <typename T, int G>
 hipError_t attend(const CacheAttn& a, hipStream_t st) {
-  constexpr int BYTES = QaLayout<G>::BYTES;
+  constexpr int BYTES = QaLayout<T, G>::BYTES, WAVES = QaLayout<T, G>::WAVES;
   GL_CHECK(allow_lds(&qcache_attn_kernel<T, G>, BYTES));
   const unsigned numbers = tile_numbers(a), heads = numbers * a.c.hkv, groups = heads * a.n_splits;
   const TileDivs f{FixedDiv::by(a.n_splits, groups), FixedDiv::by(a.c.hkv, heads),
                    FixedDiv::by(a.group, (unsigned long long)a.c.T * a.group), (65535u + a.group) / a.group};
-  hipLaunchKernelGGL((qcache_attn_kernel<T, G>), dim3(groups), dim3(64 * kWavesQ), BYTES, st, a, f);
+  hipLaunchKernelGGL((qcache_attn_kernel<T, G>), dim3(groups), dim3(64 * WAVES), BYTES, st, a, f);
   return hipGetLastError();
 }
 template <typename T, int G>
@@ -647,13 +676,8 @@ QCachePlan qcache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv,
   const long tiles = seqs * ((c.T * group + seqs * 16 - 1) / (seqs * 16));
   p.attn.rows = 16;
   p.attn.long_first = false;
-#ifndef GL_QWANT
-#define GL_QWANT 4L
-#define GL_QLEAST 512
-#define GL_QWHOLE 1024
-#endif
-  const long want = GL_QWANT * n_cu / std::max(1L, tiles * c.hkv);
-  const long most = keys <= GL_QWHOLE ? 1 : keys / GL_QLEAST;
+  const long want = 4L * n_cu / std::max(1L, tiles * c.hkv);
+  const long most = keys <= 512 ? 1 : keys / 256;
   const long launch = (1L << 22) / ((long)c.n_seqs * c.hkv);
   p.attn.n_splits = static_cast<int>(std::max(1L, std::min({want, most, (long)kMaxSplits, launch})));
   const long even = (keys + p.attn.n_splits - 1) / p.attn.n_splits;
