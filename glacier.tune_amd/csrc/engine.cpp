@@ -1566,8 +1566,11 @@ QuantLayout quant_layout_of(long long out, long long in, int group, int offsets)
   if (out % 4 != 0) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "out_features must be a multiple of 4");
   if (in % 32 != 0 || in % group != 0)
     fail(GLACIER_ATTN_ERR_UNSUPPORTED, "in_features must be a multiple of 32 and of group");
-  if (out * in >= (1LL << 31)) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
-  return quant_layout(out, in, group, offsets != 0);
+  // (the kernels count bytes of packed weights, and of 64 rows of x, in 32 bits)
+  if (out * in >= (1LL << 31) || in >= (1LL << 24)) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
+  const QuantLayout l = quant_layout(out, in, group, offsets != 0);
+  if (l.bytes >= (1LL << 31)) fail(GLACIER_ATTN_ERR_UNSUPPORTED, "tensor too large");
+  return l;
 }
 QuantLayout quant_layout_of(const glacier_quant_weights* w) {
   if (w == nullptr) fail(GLACIER_ATTN_ERR_INVALID_ARGUMENT, "w is NULL");
@@ -1611,11 +1614,16 @@ QuantProj quant_proj_of(const glacier_quant_proj_desc* desc, const glacier_lora_
   }
   return q;
 }
-// x A_p of every projection (in its place also without an adapter).
+// The workspace: the terms of fp32 x, then the parts of x A_p of every projection with
+// an adapter.
+size_t quant_terms_bytes(const QuantProj& q) {
+  return q.a.io_bf16 ? 0 : ((size_t)6 * q.a.T * q.a.in + 255) / 256 * 256;
+}
 size_t quant_proj_workspace(const QuantProj& q) {
-  bool any = false;
-  for (int p = 0; p < q.a.n_proj; ++p) any = any || q.a.p[p].a != nullptr;
-  return any ? sizeof(float) * q.a.n_proj * (size_t)q.a.T * q.a.rank : 0;
+  size_t n = 0;
+  for (int p = 0; p < q.a.n_proj; ++p) n += q.a.p[p].a != nullptr ? 1 : 0;
+  return quant_terms_bytes(q) +
+         (n > 0 ? sizeof(float) * n * quant_low_splits(q.a.T, q.a.in) * (size_t)q.a.T * q.a.rank : 0);
 }
 void need_quant_tensors(const QuantProj& q, const void* x) {
   const ProjLaunch& a = q.a;
@@ -2251,7 +2259,8 @@ int glacier_proj_quant_forward(glacier_attn_ctx* ctx, const glacier_quant_proj_d
     need(ctx, "ctx");
     q.a.x = x;
     glacier::need_workspace(workspace, workspace_bytes, glacier::quant_proj_workspace(q));
-    q.low = static_cast<float*>(workspace);
+    q.terms = workspace;
+    q.low = reinterpret_cast<float*>(static_cast<char*>(workspace) + glacier::quant_terms_bytes(q));
     std::lock_guard<std::mutex> g(ctx->eng->lock());
     glacier::DeviceScope on(ctx->eng->device());
     ctx->eng->QuantProjForward(q);

@@ -1,221 +1,366 @@
 // proj_quant.hip -- y_p = x W_p^T + bias_p + s_p (x A_p) B_p with base weights in 4 bits
 // and group scales: a step of an answer (few tokens), or a prompt.
 //
-// Reading the weights bounds it up to some tens of tokens, so they are read once, 16
-// bytes a lane, each word being what one lane feeds to one MFMA: 16 outputs by 32
-// columns by 16 tokens.  A workgroup takes 16 outputs and up to 16 NT tokens; its
-// waves share out the columns and are joined through LDS, where biases and the
-// adapters' products are added.  x comes from L2, where every workgroup finds it.
+// Reading the weights bounds it up to some tens of tokens, so they are read once a
+// workgroup, 16 bytes a lane, each word being what one lane feeds to one MFMA: 16 outputs
+// by 32 columns by 16 tokens.
 //   bf16: weights as 128 + n (one operation per two), the sum begun at -136 sum(x),
 //   which is one more product, with a constant; the scales are applied to the sums of
 //   a group.  The sums are 17 to 136 times the product's terms, which costs 4 to 8 of
 //   fp32's 24 bits.
-//   fp32: weights as n - 8, x in three bf16 terms (24 bits).
-// x A_p comes from the kernel of the bf16 projections (proj_lora.hip), in a launch
-// before.
+//   fp32: weights as n - 8, x in three bf16 terms (24 bits), which a launch before writes.
+// x A_p comes from a launch before, for more than 16 tokens from the kernel of the bf16
+// projections (proj_lora.hip); (x A_p) B_p by fp32 products into the same sums.
+#include "lds_mfma.hpp"
 #include "quant_page.hpp"
+
+#include <algorithm>
 
 namespace glacier {
 namespace {
 
 struct QuantSpec {
   const char* w;
-  const float *bias, *l, *b;
+  const float *bias, *l, *b;  // l: the parts of x A_p [splits][T][rank], or null
   float s;
-  int out, first;  // first: its first tile of 16 outputs
+  int out, first;  // first: its first tile of 16 RT outputs
   void* y;
 };
 struct QuantCall {
   const void* x;
-  int T, in, blocks, rank, n, tiles, token_blocks;
+  int T, in, blocks, rank, splits, n, tiles, token_blocks;
   QuantSpec p[kMaxProj];
 };
 
-// A wave's part of a block of 128 columns.
-template <typename IO, int NT, int GP, bool OFF>
-struct WBlock {
-  u32x4 w;
-  unsigned s[2 * GP], o[OFF ? 2 * GP : 1];  // of outputs 4 g ..: halves r GP + group
-  typename std::conditional<sizeof(IO) == 2, bf16x8, f32x4[2]>::type x[NT][4];
-};
-
+#if defined(__HIP_DEVICE_COMPILE__)
 template <int N>
-__device__ inline void load_u32(const char* p, unsigned* to) {  // N = 2, 4 or 8
+__device__ inline void load_u32(__amdgpu_buffer_rsrc_t rs, int voff, int soff, unsigned* to) {  // N = 2, 4 or 8
   if constexpr (N == 2) {
-    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
-    to[0] = v[0], to[1] = v[1];
+    const auto v = __builtin_amdgcn_raw_buffer_load_b64(rs, voff, soff, 0);
+    to[0] = static_cast<unsigned>(v[0]), to[1] = static_cast<unsigned>(v[1]);
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(p + 4 * i);
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(rs, voff + 4 * i, soff, 0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) to[i + e] = v[e];
+      for (int e = 0; e < 4; ++e) to[i + e] = static_cast<unsigned>(v[e]);
     }
   }
 }
+#endif
 
-// GP: groups of a block of 128 columns; OFF: weights have offsets
-template <typename IO, int NT, int KS, int GP, bool OFF>
-__global__ __launch_bounds__(64 * KS) void quant_proj_kernel(QuantCall a) {
+// A workgroup takes 16 RT RW outputs of 16 NT tokens.  RW waves take 16 RT outputs each and
+// walk the columns together, a block of 128 a step; KW such sets take every KW-th block
+// and are joined at the end.  x's operands of a block (NT of 1 KB for each 32 columns,
+// three times as many for fp32's terms) come by LDS DMA in the order in which lanes read
+// them (no bank conflicts, one read an operand), two steps ahead, one barrier a step; a
+// wave's weights come into its registers a step ahead.
+template <int NT, int RT, int RW, int KW, int GP, bool OFF, int TERMS>
+struct TileCfg {
+  static constexpr int SLOT = 4096 * NT * TERMS, SLOTS = 3, WAVES = RW * KW;
+  static constexpr int STRIDE = 20;  // floats of a token's 16 outputs in the join
+  static constexpr int RING = KW * SLOTS * SLOT, JOIN = KW > 1 ? WAVES * RT * NT * 16 * STRIDE * 4 : 0;
+  static constexpr int BYTES = RING > JOIN ? RING : JOIN;
+  // -136 sum(x) into the sums of every tile of outputs (one more product each), or kept
+  // apart and scaled with them (vector instructions, once a group)
+  static constexpr bool CHAIN = TERMS == 1 && !OFF && (GP == 4 || RT == 1);
+  static constexpr bool SUMS = TERMS == 1 ? !CHAIN : OFF;  // sums of x of their own
+  // loads of a step: a wave's share of x's operands, then its weights
+  static constexpr int XLOADS = 4 * NT * TERMS / RW, HALVES = GP == 4 ? 2 : 1, WLOADS = RT * (1 + HALVES * (OFF ? 2 : 1));
+};
+
+template <int NT, int RT, int RW, int KW, int GP, bool OFF, int TERMS>
+__global__ __launch_bounds__(64 * RW * KW) void quant_tile_kernel(QuantCall a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using B = WBlock<IO, NT, GP, OFF>;
-  constexpr bool F32 = sizeof(IO) == 4;
-  constexpr int STRIDE = 20;  // floats of a token's 16 outputs in LDS
-  __shared__ __align__(16) float red[KS * 16 * NT * STRIDE];
-  const int w = wave_id(), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-  // the token blocks of a tile of outputs follow each other on one XCD
-  const int id = blockIdx.x, round = id / (8 * a.token_blocks);
-  const int number = round * 8 + id % 8, t0 = id / 8 % a.token_blocks * 16 * NT;
-  if (number >= a.tiles) return;
+  using C = TileCfg<NT, RT, RW, KW, GP, OFF, TERMS>;
+  using IO = typename std::conditional<TERMS == 1, bf16, float>::type;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int w = wave_id() % RW, kw = wave_id() / RW, lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  int number = blockIdx.x, t0 = 0;
+  if (a.token_blocks > 1) {
+    const int round = number / (8 * a.token_blocks), rest = number - round * 8 * a.token_blocks;
+    number = round * 8 + rest % 8;
+    t0 = rest / 8 * 16 * NT;
+  }
+  number = RW * number + w;
+  const bool has_tile = number < a.tiles;
+  if (!has_tile) number = a.tiles - 1;  // (its wave takes part in the barriers)
   int p = 0;
   while (p + 1 < a.n && number >= a.p[p + 1].first) ++p;
   const QuantSpec& job = a.p[p];
-  const int tile = number - job.first;
-  const long tiles = (job.out + 15) / 16;
-  const char* const words = job.w + (long)tile * a.blocks * 1024 + lane * 16;
-  const char* const scales = job.w + tiles * a.blocks * 1024 + (long)tile * a.blocks * (32 * GP) + g * (8 * GP);
-  const char* const offsets = scales + tiles * a.blocks * (32 * GP);
-  const IO* x[NT];
+  const int tile = (number - job.first) * RT, tiles = (job.out + 15) / 16;
+  const auto wr = wave_rsrc(job.w, static_cast<int>((long)tiles * a.blocks * (1024 + (OFF ? 64 : 32) * GP)));
+  __amdgpu_buffer_rsrc_t xr[TERMS];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) x[n] = static_cast<const IO*>(a.x) + (long)min(t0 + 16 * n + col, a.T - 1) * a.in;
-  auto load = [&](B& to, int blk) __attribute__((always_inline)) {
-    to.w = *reinterpret_cast<const u32x4*>(words + (long)blk * 1024);
-    load_u32<2 * GP>(scales + (long)blk * (32 * GP), to.s);
-    if constexpr (OFF) load_u32<2 * GP>(offsets + (long)blk * (32 * GP), to.o);
+  for (int z = 0; z < TERMS; ++z)
+    xr[z] = wave_rsrc(static_cast<const bf16*>(a.x) + ((long)z * a.T + t0) * a.in, 0x7fffffff);
+  const int scales = tiles * a.blocks * 1024, offsets = scales + tiles * a.blocks * 32 * GP;
+  int x_at[NT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int k = min(128 * blk + 32 * i + 8 * g, a.in - 8);
+  for (int n = 0; n < NT; ++n) x_at[n] = (min(16 * n + col, a.T - 1 - t0) * a.in + 8 * g) * 2;
+  unsigned char* const ring = smem + kw * C::SLOTS * C::SLOT;
+  // operands (n, w), (n, w + RW), .. of the block of a step: this lane's 16 bytes
+  auto request = [&](int slot, int step) __attribute__((always_inline)) {
+    const int blk = min(step * KW + kw, a.blocks - 1);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if constexpr (F32) {
-          to.x[n][i][0] = *reinterpret_cast<const f32x4*>(x[n] + k);
-          to.x[n][i][1] = *reinterpret_cast<const f32x4*>(x[n] + k + 4);
-        } else {
-          to.x[n][i] = *reinterpret_cast<const bf16x8*>(x[n] + k);
-        }
-      }
+    for (int i0 = 0; i0 < 4; i0 += RW) {
+      const int i = i0 + w, k = 2 * min(128 * blk + 32 * i, a.in - 32);
+#pragma unroll
+      for (int z = 0; z < TERMS; ++z)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              xr[z], (GLACIER_LDS void*)(ring + slot * C::SLOT + (4 * (NT * z + n) + i) * 1024), 16, x_at[n], k, 0, 0);
+    }
+  };
+  struct Words {
+    u32x4 w[RT];
+    unsigned s[RT][2 * GP], o[RT][OFF ? 2 * GP : 1];
+  };
+  auto load = [&](Words& to, int step) __attribute__((always_inline)) {
+    const int blk = min(step * KW + kw, a.blocks - 1);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int at = min(tile + r, tiles - 1) * a.blocks + blk;
+      to.w[r] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, 16 * lane, at * 1024, 0));
+      load_u32<2 * GP>(wr, 8 * GP * g, scales + at * 32 * GP, to.s[r]);
+      if constexpr (OFF) load_u32<2 * GP>(wr, 8 * GP * g, offsets + at * 32 * GP, to.o[r]);
     }
   };
   const QuantMagic magic;
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  f32x4 y[NT];
+  f32x4 y[RT][NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) y[n] = zero;
-  bf16x8 minus, ones;
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) minus[e] = (bf16)-136.0f, ones[e] = (bf16)1.0f;
-  auto take = [&](B& from, int blk) __attribute__((always_inline)) {
-    if (128 * blk + 128 > a.in) {  // columns past the last one
+    for (int n = 0; n < NT; ++n) y[r][n] = zero;
+  bf16x8 minus;  // of sums of x (fp32: 1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (128 * blk + 32 * i >= a.in)
+  for (int e = 0; e < 8; ++e) minus[e] = (bf16)(TERMS == 1 ? -136.0f : 1.0f);
+  const unsigned ring_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>((GLACIER_LDS unsigned char*)ring)) + 16 * lane;
+  auto take = [&](const Words& from, unsigned slot_at) __attribute__((always_inline)) {
+    u32x4 f[2][NT * TERMS];
+    auto read = [&](int i) __attribute__((always_inline)) {
+      if constexpr (TERMS == 1) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if constexpr (F32)
-              from.x[n][i][0] = from.x[n][i][1] = zero;
-            else
-              from.x[n][i] = frag_zero<bf16>();
-          }
-    }
+        for (int n = 0; n < NT; ++n)
+          asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(f[i % 2][n]) : "v"(slot_at), "i"((4 * n + i) * 1024));
+      } else {  // (the compiler lets a sum pass through their registers: its write is waited for)
 #pragma unroll
-    for (int q = 0; q < GP; ++q) {
-      f32x4 d[NT], d0[NT];  // of the group: products, and -136 sum(x) (fp32: sum(x))
-      if constexpr (F32) {
+        for (int n = 0; n < NT; ++n)
+          asm volatile(
+              "s_nop 7\n\tds_read_b128 %0, %3 offset:%4\n\tds_read_b128 %1, %3 offset:%5\n\tds_read_b128 %2, %3 offset:%6"
+              : "=&v"(f[i % 2][n]), "=&v"(f[i % 2][NT + n]), "=&v"(f[i % 2][2 * NT + n])
+              : "v"(slot_at), "i"((4 * n + i) * 1024), "i"((4 * (NT + n) + i) * 1024), "i"((4 * (2 * NT + n) + i) * 1024));
+      }
+    };
+    read(0);
+    f32x4 d[RT][NT], d0[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) d[n] = d0[n] = zero;
-#pragma unroll
-        for (int i = q * 4 / GP; i < (q + 1) * 4 / GP; ++i) {
-          const bf16x8 wf = exact8_bf16(from.w[i], magic);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            bf16x8 h, m, l;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float v = from.x[n][i][e / 4][e % 4];
-              h[e] = (bf16)v;
-              const float r1 = v - (float)h[e];
-              m[e] = (bf16)r1;
-              l[e] = (bf16)(r1 - (float)m[e]);
-            }
-            d[n] = Mfma<bf16>::mma(wf, l, d[n]);
-            d[n] = Mfma<bf16>::mma(wf, m, d[n]);
-            d[n] = Mfma<bf16>::mma(wf, h, d[n]);
-            if constexpr (OFF) {
-              d0[n] = Mfma<bf16>::mma(ones, l, d0[n]);
-              d0[n] = Mfma<bf16>::mma(ones, m, d0[n]);
-              d0[n] = Mfma<bf16>::mma(ones, h, d0[n]);
-            }
-          }
-        }
+    for (int i = 0; i < 4; ++i) {
+      if (i < 3) {
+        read(i + 1);
+        lgkm<NT * TERMS>();
       } else {
+        lgkm<0>();
+      }
+#pragma unroll
+      for (int n = 0; n < NT * TERMS; ++n) tie_v(f[i % 2][n]);
+      if (i * GP % 4 == 0) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) d0[n] = zero;
 #pragma unroll
-        for (int i = q * 4 / GP; i < (q + 1) * 4 / GP; ++i)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) d0[n] = Mfma<bf16>::mma(minus, from.x[n][i], d0[n]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) d[n] = d0[n];
-#pragma unroll
-        for (int i = q * 4 / GP; i < (q + 1) * 4 / GP; ++i) {
-          const bf16x8 wf = raw8_bf16(from.w[i], magic);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) d[n] = Mfma<bf16>::mma(wf, from.x[n][i], d[n]);
-        }
+          for (int n = 0; n < NT; ++n) d[r][n] = zero;
       }
+      auto add = [&](const bf16x8& wf, f32x4 (&to)[NT]) __attribute__((always_inline)) {  // smallest terms first
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float s = half_at(from.s[(r * GP + q) / 2], (r * GP + q) % 2);
+        for (int z = TERMS - 1; z >= 0; --z)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) y[n][r] = fmaf(s, d[n][r], y[n][r]);
-        if constexpr (OFF) {
-          const float o = half_at(from.o[(r * GP + q) / 2], (r * GP + q) % 2) * (F32 ? 1.0f : -1.0f / 136.0f);
+          for (int n = 0; n < NT; ++n) to[n] = Mfma<bf16>::mma(wf, __builtin_bit_cast(bf16x8, f[i % 2][NT * z + n]), to[n]);
+      };
+      if constexpr (C::SUMS) add(minus, d0);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) y[n][r] = fmaf(o, d0[n][r], y[n][r]);
-        }
+      for (int r = 0; r < RT; ++r) {
+        if constexpr (C::CHAIN) add(minus, d[r]);
+        if constexpr (TERMS == 1)
+          add(raw8_bf16(from.w[r][i], magic), d[r]);
+        else
+          add(exact8_bf16(from.w[r][i], magic), d[r]);
+      }
+      if ((i + 1) * GP % 4 == 0) {  // a group's end
+        const int q = i * GP / 4;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float s = half_at(from.s[r][(e * GP + q) / 2], (e * GP + q) % 2);
+            float o = s;  // of -136 sum(x)
+            if constexpr (OFF) {
+              o = half_at(from.o[r][(e * GP + q) / 2], (e * GP + q) % 2);
+              if constexpr (TERMS == 1) o = fmaf(o, -1.0f / 136.0f, s);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              y[r][n][e] = fmaf(s, d[r][n][e], y[r][n][e]);
+              if constexpr (C::SUMS) y[r][n][e] = fmaf(o, d0[n][e], y[r][n][e]);
+            }
+          }
       }
     }
   };
-  B u, v;
-  int blk = w;
-  if (blk < a.blocks) load(u, blk);
-  for (; blk < a.blocks; blk += 2 * KS) {  // two blocks a turn, each loaded while the other is worked on
-    if (blk + KS < a.blocks) load(v, blk + KS);
-    take(u, blk);
-    if (blk + KS >= a.blocks) break;
-    if (blk + 2 * KS < a.blocks) load(u, blk + 2 * KS);
-    take(v, blk + KS);
+  // (columns past the last one: x's last ones again, which meet scales of zero)
+  const int steps = (a.blocks + KW - 1) / KW;
+  Words u, v;
+  request(0, 0);
+  request(1, 1);
+  load(u, 0);
+  auto turn = [&](int step, int slot, const Words& now, Words& next) __attribute__((always_inline)) {
+    vmw<C::XLOADS + C::WLOADS>();  // this block of x has come, but for what other waves asked for
+    wg_barrier();
+    request(slot == 0 ? 2 : slot - 1, step + 2);
+    load(next, step + 1);
+    if (KW == 1 || step * KW + kw < a.blocks) take(now, ring_at + slot * C::SLOT);
+  };
+  int slot = 0;
+  for (int step = 0; step < steps; step += 2) {
+    turn(step, slot, u, v);
+    slot = slot == 2 ? 0 : slot + 1;
+    if (step + 1 >= steps) break;
+    turn(step + 1, slot, v, u);
+    slot = slot == 2 ? 0 : slot + 1;
   }
+  vmw<0>();
+  if (job.l != nullptr) {  // (x A) B by fp32 products of four ranks
+    const long step = (long)a.T * a.rank;
+    for (int j0 = 4 * kw; j0 < a.rank; j0 += 4 * KW) {
+      const int j = j0 + g, jc = min(j, a.rank - 1);
+      float low[NT], up[RT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) store4(red + ((w * NT + n) * 16 + col) * STRIDE + 4 * g, y[n]);
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < 64 * NT; idx += 64 * KS) {
-    const int t = t0 + idx / 4, o = 16 * tile + 4 * (idx % 4);
-    if (t >= a.T || o >= job.out) continue;
-    f32x4 sum = zero;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const f32x4 part = *reinterpret_cast<const f32x4*>(red + (k * NT * 16 + idx / 4) * STRIDE + 4 * (idx % 4));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += part[e];
-    }
-    if (job.l != nullptr) {
-      f32x4 low = zero;
-      const float* const l = job.l + (long)t * a.rank;
-      for (int j = 0; j < a.rank; ++j) {
-        const f32x4 bj = *reinterpret_cast<const f32x4*>(job.b + (long)j * job.out + o);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) low[e] = fmaf(l[j], bj[e], low[e]);
+      for (int r = 0; r < RT; ++r) {
+        up[r] = job.b[(long)jc * job.out + min(16 * (tile + r) + col, job.out - 1)];
+        up[r] = j < a.rank ? up[r] : 0.0f;
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = fmaf(job.s, low[e], sum[e]);
+      for (int n = 0; n < NT; ++n) {
+        const float* const l = job.l + (long)min(t0 + 16 * n + col, a.T - 1) * a.rank + jc;
+        low[n] = 0.0f;
+#pragma unroll 8
+        for (int z = 0; z < a.splits; ++z) low[n] += l[z * step];
+        low[n] = j < a.rank ? job.s * low[n] : 0.0f;
+      }
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) y[r][n] = Mfma<float>::mma(up[r], low[n], y[r][n]);
     }
+  }
+  auto put = [&](int r, int n, f32x4 sum) __attribute__((always_inline)) {
+    const int t = t0 + 16 * n + col, o = 16 * (tile + r) + 4 * g;
+    if (!has_tile || t >= a.T || o >= job.out) return;
     if (job.bias != nullptr)
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += job.bias[o + e];
     store4(static_cast<IO*>(job.y) + (long)t * job.out + o, sum);
+  };
+  if constexpr (KW == 1) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) put(r, n, y[r][n]);
+  } else {
+    __syncthreads();
+    float* const mine = reinterpret_cast<float*>(smem) + w * (KW * RT * NT * 16 * C::STRIDE) + col * C::STRIDE + 4 * g;
+#pragma unroll
+    for (int x = 0; x < RT * NT; ++x) store4(mine + (kw * RT * NT + x) * 16 * C::STRIDE, y[x / NT][x % NT]);
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < RT * NT; ++x) {
+      if (x % KW != kw) continue;
+      f32x4 sum = zero;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) sum += *reinterpret_cast<const f32x4*>(mine + (k * RT * NT + x) * 16 * C::STRIDE);
+      put(x / NT, x % NT, sum);
+    }
   }
 #endif
+}
+
+// ---- x A of few tokens -----------------------------------------------------
+// Parts of x A_p over columns z kLowCols .. of x and rows of A_p each: [splits][T][rank]
+// of every projection.  Of 32 columns a lane holds eight of one token and the eight rows
+// of A that go with them, of one rank each: eight fp32 products of four.  The waves'
+// sums are added in order.
+constexpr int kLowCols = 256, kLowTokens = 16;
+struct LowCall {
+  const void* x;
+  const float* a[kMaxProj];
+  float* l[kMaxProj];
+  int T, in, rank, splits;
+};
+template <typename IO, int NR>  // NR: tiles of 16 ranks
+__global__ __launch_bounds__(256) void quant_low_kernel(LowCall c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __shared__ __align__(16) float part[4][NR][16][20];
+  const int z = blockIdx.x, w = wave_id(), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  const float* const a = c.a[blockIdx.y];
+  const int t = min(col, c.T - 1);
+  float x[2][8], v[2][NR][8];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int k = z * kLowCols + 64 * w + 32 * u, kc = min(k, c.in - 32) + 8 * g;  // (in is a multiple of 32)
+    load8(static_cast<const IO*>(c.x) + (long)t * c.in + kc, x[u]);
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int s = 0; s < 8; ++s) v[u][r][s] = a[(long)(kc + s) * c.rank + min(16 * r + col, c.rank - 1)];
+    if (k >= c.in)
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        x[u][s] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) v[u][r][s] = 0.0f;
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int s = 0; s < 8; ++s) sum = Mfma<float>::mma(v[u][r][s], x[u][s], sum);
+    store4(part[w][r][col] + 4 * g, sum);  // token col, ranks 16 r + 4 g ..
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 256 * NR; i += 256) {
+    const int j = i % 16, at = i / 16 % 16, r = i / 256;
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum += part[u][r][at][j];
+    if (at < c.T && 16 * r + j < c.rank) c.l[blockIdx.y][((long)z * c.T + at) * c.rank + 16 * r + j] = sum;
+  }
+#endif
+}
+
+// ---- fp32 x in three bf16 terms, [3][T][in] ---------------------------------
+// Cut, not rounded: 8 bits a term, so that the three are x exactly and none overflows.
+// What is not finite stays in the first.
+__global__ __launch_bounds__(256) void quant_terms_kernel(const float* x, bf16* to, long n) {
+  for (long i = 8 * ((long)blockIdx.x * 256 + threadIdx.x); i < n; i += 8L * 256 * gridDim.x) {
+    float v[8], h[8];
+    load8(x + i, v);
+#pragma unroll
+    for (int z = 0; z < 3; ++z) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool finite = fabsf(v[e]) < INFINITY;
+        h[e] = finite ? __uint_as_float(__float_as_uint(v[e]) & 0xffff0000u) : v[e];
+        v[e] = finite ? v[e] - h[e] : 0.0f;
+      }
+      store8(to + z * n + i, h);
+    }
+  }
 }
 
 // ---- laying out ------------------------------------------------------------
@@ -246,29 +391,71 @@ __global__ __launch_bounds__(256) void quant_pack_kernel(QuantPack a, QuantLayou
       row < a.out && i < groups ? from[row * groups + i] : static_cast<unsigned short>(0);
 }
 
-template <typename IO, int NT, int KS, int GP, bool OFF>
-hipError_t project(const QuantCall& c, hipStream_t st) {
-  hipLaunchKernelGGL((quant_proj_kernel<IO, NT, KS, GP, OFF>), dim3((c.tiles + 7) / 8 * 8 * c.token_blocks),
-                     dim3(64 * KS), 0, st, c);
+template <int NT, int RT, int RW, int KW, int GP, bool OFF, int TERMS>
+hipError_t tiled(QuantCall c, hipStream_t st) {
+  using C = TileCfg<NT, RT, RW, KW, GP, OFF, TERMS>;
+  c.token_blocks = (c.T + 16 * NT - 1) / (16 * NT);
+  c.tiles = 0;
+  for (int p = 0; p < c.n; ++p) {
+    c.p[p].first = c.tiles;
+    c.tiles += (c.p[p].out + 16 * RT - 1) / (16 * RT);
+  }
+  const int groups = (c.tiles + RW - 1) / RW, tb = c.token_blocks;
+  GL_CHECK(allow_lds((&quant_tile_kernel<NT, RT, RW, KW, GP, OFF, TERMS>), C::BYTES));
+  hipLaunchKernelGGL((quant_tile_kernel<NT, RT, RW, KW, GP, OFF, TERMS>), dim3(tb > 1 ? (groups + 7) / 8 * 8 * tb : groups),
+                     dim3(64 * C::WAVES), C::BYTES, st, c);
   return hipGetLastError();
 }
-template <typename IO, int NT, int KS>
+template <int TERMS, int NT, int RT, int RW, int KW>
 hipError_t by_group(const QuantCall& c, int group, bool off, hipStream_t st) {
-  if (group == 32) return off ? project<IO, NT, KS, 4, true>(c, st) : project<IO, NT, KS, 4, false>(c, st);
-  if (group == 64) return off ? project<IO, NT, KS, 2, true>(c, st) : project<IO, NT, KS, 2, false>(c, st);
-  return off ? project<IO, NT, KS, 1, true>(c, st) : project<IO, NT, KS, 1, false>(c, st);
+  if (group == 32) return off ? tiled<NT, RT, RW, KW, 4, true, TERMS>(c, st) : tiled<NT, RT, RW, KW, 4, false, TERMS>(c, st);
+  if (group == 64) return off ? tiled<NT, RT, RW, KW, 2, true, TERMS>(c, st) : tiled<NT, RT, RW, KW, 2, false, TERMS>(c, st);
+  return off ? tiled<NT, RT, RW, KW, 1, true, TERMS>(c, st) : tiled<NT, RT, RW, KW, 1, false, TERMS>(c, st);
 }
+// The shape of a workgroup, by how many tiles of 16 outputs by 16 tokens a call has: few
+// tiles are cut along the columns, many share the operands of x, and the weights, of a
+// workgroup.  In us, the shape named RT RW KW after NT, [tokens] in -> outputs:
+//   below 512     1: 1 2 4   [1] 3584 -> 4608: 11.0 (with 1 4 4: 13.2, 1 4 1: 18.1);
+//                            fp32: 15.6 (18.0, 24.7)
+//     and rows of 8192 or more, up to 16 tokens, bf16
+//                 1: 1 1 8   [1] 18944 -> 3584: 13.1 (1 2 4: 20.9); [16]: 23.7 (24.7); but
+//                            [1] 3584 -> 4608: 16.2.  (fp32's operands would take twice
+//                            the LDS that there is)
+//   below 1200    1: 1 4 4   [64] 3584 -> 3584: 9.6 (1 2 4: 13.4, 1 4 1: 11.5);
+//                            fp32 [32] 3584 -> 4608: 33.0 (45.6, 40.3)
+//   below 3000    1: 1 4 1   [16] 3584 -> 37888: 22.3 (1 2 4: 27.5, 1 4 4: 24.6); [128]
+//                            3584 -> 3584: 14.4; fp32 [16] 3584 -> 37888: 45.6 (2: 2 4 1:
+//                            63.3)
+//   more          2: 2 4 1   [24] 3584 -> 37888: 31.6 (1: 1 4 1: 32.9), [512] 3584 -> 4608:
+//                            44.6; fp32 the latter: 121.7 (1: 1 4 1: 143.9)
+//   40000 and more, bf16
+//                 4: 2 4 1   [512] 3584 -> 37888: 202 (2: 2 4 1: 213), but [512] 3584 ->
+//                            4608: 51
+template <int TERMS>
+hipError_t by_shape(const QuantCall& c, int group, bool off, hipStream_t st) {
+  long units = 0;
+  for (int p = 0; p < c.n; ++p) units += (c.p[p].out + 15) / 16;
+  units *= (c.T + 15) / 16;
+  if constexpr (TERMS == 1)
+    if (c.T <= 16 && units < 512 && c.blocks >= 64) return by_group<TERMS, 1, 1, 1, 8>(c, group, off, st);
+  if (units < 512) return by_group<TERMS, 1, 1, 2, 4>(c, group, off, st);
+  if (units < 1200) return by_group<TERMS, 1, 1, 4, 4>(c, group, off, st);
+  if (units < 3000) return by_group<TERMS, 1, 1, 4, 1>(c, group, off, st);
+  if constexpr (TERMS == 1)
+    if (units >= 40000) return by_group<TERMS, 4, 2, 4, 1>(c, group, off, st);
+  return by_group<TERMS, 2, 2, 4, 1>(c, group, off, st);
+}
+
 template <typename IO>
-hipError_t by_shape(QuantCall c, int group, bool off, int n_cu, hipStream_t st) {
-  constexpr int MOST = sizeof(IO) == 2 ? 4 : 2;
-  const int nt = c.T <= 16 ? 1 : c.T <= 32 || MOST == 2 ? 2 : 4;
-  c.token_blocks = (c.T + 16 * nt - 1) / (16 * nt);
-  const bool deep = (long)c.tiles * c.token_blocks < 4L * n_cu;
-  if (nt == 1) return deep ? by_group<IO, 1, 8>(c, group, off, st) : by_group<IO, 1, 4>(c, group, off, st);
-  if (nt == 2) return deep ? by_group<IO, 2, 8>(c, group, off, st) : by_group<IO, 2, 4>(c, group, off, st);
-  if constexpr (MOST == 4)
-    return deep ? by_group<IO, 4, 8>(c, group, off, st) : by_group<IO, 4, 4>(c, group, off, st);
-  return hipErrorInvalidValue;
+hipError_t low(const LowCall& c, int n, hipStream_t st) {
+  const dim3 grid(c.splits, n);
+  if (c.rank <= 16)
+    hipLaunchKernelGGL((quant_low_kernel<IO, 1>), grid, dim3(256), 0, st, c);
+  else if (c.rank <= 32)
+    hipLaunchKernelGGL((quant_low_kernel<IO, 2>), grid, dim3(256), 0, st, c);
+  else
+    hipLaunchKernelGGL((quant_low_kernel<IO, 4>), grid, dim3(256), 0, st, c);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -280,6 +467,8 @@ hipError_t launch_quant_pack(const QuantPack& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+int quant_low_splits(int T, int in) { return T <= kLowTokens ? (in + kLowCols - 1) / kLowCols : 1; }
+
 hipError_t launch_quant_proj(const QuantProj& q, int n_cu, hipStream_t st) {
   const ProjLaunch& a = q.a;
   QuantCall c{};
@@ -288,17 +477,31 @@ hipError_t launch_quant_proj(const QuantProj& q, int n_cu, hipStream_t st) {
   c.in = a.in;
   c.blocks = (a.in + 127) / 128;
   c.rank = a.rank;
+  c.splits = quant_low_splits(a.T, a.in);
   c.n = a.n_proj;
+  LowCall low_call{a.x, {}, {}, a.T, a.in, a.rank, c.splits};
   float* l[kMaxProj] = {};
+  int adapters = 0;
   for (int p = 0; p < a.n_proj; ++p) {
     const ProjSpec& s = a.p[p];
-    if (s.a != nullptr) l[p] = q.low + (long)p * a.T * a.rank;
-    c.p[p] = QuantSpec{static_cast<const char*>(s.w), s.bias, l[p], s.b, s.scaling, s.out, c.tiles, s.y};
-    c.tiles += (s.out + 15) / 16;
+    if (s.a != nullptr) {
+      l[p] = q.low + (long)adapters * c.splits * a.T * a.rank;
+      low_call.a[adapters] = s.a;
+      low_call.l[adapters++] = l[p];
+    }
+    c.p[p] = QuantSpec{static_cast<const char*>(s.w), s.bias, l[p], s.b, s.scaling, s.out, 0, s.y};
   }
-  GL_CHECK(launch_lowrank_forward(a, l, st));
-  return a.io_bf16 ? by_shape<bf16>(c, q.group, q.offsets, n_cu, st)
-                   : by_shape<float>(c, q.group, q.offsets, n_cu, st);
+  if (adapters > 0 && a.T <= kLowTokens)
+    GL_CHECK(a.io_bf16 ? low<bf16>(low_call, adapters, st) : low<float>(low_call, adapters, st));
+  else if (adapters > 0)
+    GL_CHECK(launch_lowrank_forward(a, l, st));
+  if (a.io_bf16) return by_shape<1>(c, q.group, q.offsets, st);
+  const long n = (long)a.T * a.in;
+  c.x = q.terms;
+  hipLaunchKernelGGL(quant_terms_kernel, dim3(static_cast<unsigned>(std::min((n + 2047) / 2048, 8L * n_cu))), dim3(256), 0,
+                     st, static_cast<const float*>(a.x), static_cast<bf16*>(q.terms), n);
+  GL_CHECK(hipGetLastError());
+  return by_shape<3>(c, q.group, q.offsets, st);
 }
 
 }  // namespace glacier

@@ -59,13 +59,16 @@ struct QuantPack {
 };
 hipError_t launch_quant_pack(const QuantPack& a, hipStream_t st);
 
-// a: x, T, in, rank, io_bf16 and the projections, w packed; low: [n_proj][T][rank]
-// for x A_p, or null without adapters.
+// Parts in which x A_p is left for the products.
+int quant_low_splits(int T, int in);
+// a: x, T, in, rank, io_bf16 and the projections, w packed; low: [adapters][parts][T]
+// [rank] for x A_p, or null without adapters; terms: bf16 [3][T][in] for fp32 x.
 struct QuantProj {
   ProjLaunch a;
   int group;
   bool offsets;
   float* low;
+  void* terms;
 };
 hipError_t launch_quant_proj(const QuantProj& q, int n_cu, hipStream_t st);
 

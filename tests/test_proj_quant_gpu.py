@@ -230,3 +230,35 @@ def test_an_answer_in_4_bits(eng):
         # (a rounding of q, k or v to bf16 that falls the other way may move a number of
         # the cache by a step: the norm is looked at, and few of them move)
         assert float((got[turn].cpu().double() - want).norm() / want.norm()) < 2.0 ** -6
+
+
+# tokens, outputs: by their number of tiles of 16 by 16 each takes another kernel
+SHAPES = {"deep": (5, 36), "few": (33, 132), "hundreds": (130, 1000), "thousand": (300, 1300), "thousands": (300, 4100),
+          "most": (1300, 8200)}
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("group,offsets", [(32, False), (32, True), (64, False), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("shape", sorted(SHAPES))
+def test_shapes_and_groups(eng, shape, group, offsets, dt):
+    (T, out), dt, g = SHAPES[shape], DTYPES[dt], torch.Generator().manual_seed(12)
+    cols = 8192 + group if shape == "deep" else {32: 352, 64: 320, 128: 384}[group]
+    w = qh.Weights(out, cols, group, offsets, 13)
+    x = torch.randn(T, cols, generator=g).to(dt)
+    kw = {"a": torch.randn(cols, 7, generator=g), "b": torch.randn(7, out, generator=g), "scaling": 0.5,
+          "bias": torch.randn(out, generator=g)}
+    pr = {"w": _pack(eng, w), "out": out, **{k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in kw.items()}}
+    y, = eng.proj_quant_forward(x.cuda(), [pr], rank=7, group=group, mins=offsets)
+    ch.check("y", y, *qh.project_ref(x, w, dt, **kw))
+
+
+def test_fp32_of_every_size(eng):
+    # x down to 2^-100 and up to where eight times it is still finite: three bf16 terms
+    # hold all of it
+    w, g = qh.Weights(64, 256, 64, False, 14), torch.Generator().manual_seed(15)
+    x = torch.randn(9, 256, generator=g)
+    x *= torch.tensor([2.0 ** e for e in (-100, -60, -20, 0, 20, 60, 100, 1, 2)])[:, None]
+    x[7:] = 0.0
+    x[7, 5], x[8, 200] = torch.finfo(torch.float32).max / 16, -torch.finfo(torch.float32).max / 16
+    y, = eng.proj_quant_forward(x.cuda(), [{"w": _pack(eng, w), "out": 64}], group=64)
+    ch.check("y", y, *qh.project_ref(x, w, torch.float32))
