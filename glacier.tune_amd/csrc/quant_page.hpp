@@ -34,17 +34,15 @@ __device__ inline f16 quant_scale(float s) {
   return (f16)fminf(fmaxf(__builtin_bit_cast(float, u), -kQuantScaleMax), kQuantScaleMax);
 }
 
-// The number of x: floor(x / s + 1/2) + 8 within 0 .. 15.  inv: about 1 / s; the
-// product may land on the wrong side of a border, which the remainder tells (it is
-// exact there: x and n s agree in their leading bits).
-__device__ inline unsigned quant_number(float x, float s, float inv) {
-  const float t = fminf(fmaxf(x * inv, -9.0f), 8.0f);
-  float n = floorf(t + 0.5f);
-  const float r = fmaf(-n, s, x), half = 0.5f * fabsf(s);
-  const float over = s < 0.0f ? -r : r;  // (x / s - n) |s|
-  n += over >= half ? 1.0f : 0.0f;
-  n -= over < -half ? 1.0f : 0.0f;
-  return static_cast<unsigned>(fminf(fmaxf(n + 8.0f, 0.0f), 15.0f));
+// The number of x: floor(x / s + 1/2) + 8 within 0 .. 15.  size: |s|; sign: s's sign bit;
+// inv: about 1 / |s|.  The product may land on the wrong side of a border: it is held
+// below it (by more than its error), and the remainder tells whether x has passed it (it
+// is exact there: x and n s agree in their leading bits).
+__device__ inline unsigned quant_number(float x, unsigned sign, float size, float inv) {
+  x = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) ^ sign);
+  const float n = floorf(fmaf(x, inv, 0.5f - 0x1p-18f));
+  const float up = fmaf(-n, size, x) >= 0.5f * size ? 9.0f : 8.0f;
+  return static_cast<unsigned>(fminf(fmaxf(n + up, 0.0f), 15.0f));
 }
 
 // Eight columns (of a group of 32 that four neighbouring lanes hold) as a word and
@@ -68,10 +66,11 @@ __device__ inline unsigned quantise8(const float (&x)[8], f16& scale) {
               : quant_scale((top >= -low ? top : low) * -0.125f);
   const float s = (float)scale;
   if (odd || s == 0.0f) return kQuantZero;
-  const float inv = 1.0f / s;
+  const unsigned sign = __builtin_bit_cast(unsigned, s) & 0x80000000u;
+  const float size = fabsf(s), inv = 1.0f / size;
   unsigned w = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w |= quant_number(x[e], s, inv) << (4 * (e / 2) + 16 * (e % 2));
+  for (int e = 0; e < 8; ++e) w |= quant_number(x[e], sign, size, inv) << (4 * (e / 2) + 16 * (e % 2));
   return w;
 }
 

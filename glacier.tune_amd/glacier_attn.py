@@ -565,16 +565,32 @@ def qcache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, 
     if len(shape) != 3 or k_pages.dtype is not torch.uint8:
         raise TypeError("k_pages must be uint8 [n_pages, n_heads_kv, quant_page_bytes(page_size, head_dim)]")
     n_pages, hkv, size = shape
-    if head_dim <= 0 or size % quant_page_bytes(1, head_dim) != 0:
+    row = quant_page_bytes(1, head_dim)
+    if head_dim <= 0 or size % row != 0:
         raise TypeError(f"a page's head of {size} bytes holds no whole tokens of {head_dim} columns")
-    if dtype not in (torch.float32, torch.bfloat16):
+    io = IO_BF16 if dtype is torch.bfloat16 else IO_F32
+    if io == IO_F32 and dtype is not torch.float32:
         raise TypeError(f"unsupported tensor dtype {dtype}")
     stride = _pages(k_pages, v_pages, device)
     batch = _batch_args(cu_tokens, kv_lens, page_table, total_tokens, max_new, max_kv, device)
     _need_32_bits(n_pages, hkv, size, head_dim)
-    return (KvCache(k_pages.data_ptr(), v_pages.data_ptr(), stride, n_pages,
-                    size // quant_page_bytes(1, head_dim), hkv, head_dim,
-                    IO_F32 if dtype is torch.float32 else IO_BF16), batch)
+    return KvCache(k_pages.data_ptr(), v_pages.data_ptr(), stride, n_pages, size // row, hkv, head_dim, io), batch
+
+
+_packed_sizes = {}
+
+
+def _packed_bytes(out, cols, group, offsets):
+    """Bytes of packed 4-bit weights, asked for once for each size; Unsupported for one
+    that is not taken."""
+    size = _packed_sizes.get((out, cols, group, offsets))
+    if size is None:
+        _need_32_bits(out, cols, group)
+        size = load().glacier_proj_quant_bytes(ctypes.byref(QuantWeights(out, cols, group, offsets)))
+        if size == 0:
+            _check(ERR_UNSUPPORTED)
+        _packed_sizes[out, cols, group, offsets] = size
+    return size
 
 
 def quantise_rows(w, group=32):
@@ -1086,9 +1102,12 @@ class GpuAttentionEngine:
             if q.dim() != 3:
                 raise TypeError("q must be [T, Hq, D]")
             hq = q.shape[1]
-            q_rot = _torch_mod.empty_like(q) if q_rot is None else q_rot
             qp = _address(q, "q", (T, hq, d), dt, dev)
-            rp = _address(q_rot, "q_rot", (T, hq, d), dt, dev)
+            if q_rot is None:
+                q_rot = _torch_mod.empty_like(q)
+                rp = q_rot.data_ptr()
+            else:
+                rp = _address(q_rot, "q_rot", (T, hq, d), dt, dev)
         self._bind_device_stream()
         rc = _lib.glacier_attn_qcache_append(self._h, ctypes.byref(cache), ctypes.byref(batch), kp, vp,
                                              float(rope_freq_base or 0.0), hq, qp, rp)
@@ -1105,9 +1124,11 @@ class GpuAttentionEngine:
         dev, T = self.device_ordinal, int(total_tokens)
         cache, batch = qcache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, T, 0, 0, dev,
                                    int(head_dim), dtype)
-        shape, torch = (T, cache.n_heads_kv, cache.head_dim), _torch_mod
-        k = torch.empty(shape, dtype=dtype, device=dev) if k is None else k
-        v = torch.empty(shape, dtype=dtype, device=dev) if v is None else v
+        shape = (T, cache.n_heads_kv, cache.head_dim)
+        if k is None:
+            k = k_pages.new_empty(shape, dtype=dtype)
+        if v is None:
+            v = k_pages.new_empty(shape, dtype=dtype)
         kp, vp = _address(k, "k", shape, dtype, dev), _address(v, "v", shape, dtype, dev)
         self._bind_device_stream()
         rc = _lib.glacier_attn_qcache_read(self._h, ctypes.byref(cache), ctypes.byref(batch), kp, vp)
@@ -1160,9 +1181,7 @@ class GpuAttentionEngine:
             raise TypeError(f"scales must be [{rows}, {cols} / group]")
         _need_32_bits(rows, cols)
         w = QuantWeights(rows, cols, cols // scales.shape[1], int(offsets is not None))
-        size = load().glacier_proj_quant_bytes(ctypes.byref(w))
-        if size == 0:
-            _check(ERR_UNSUPPORTED)
+        size = _packed_bytes(rows, cols, w.group, w.offsets)
         packed = torch.empty(size, dtype=torch.uint8, device=dev) if packed is None else packed
         args = (_address(numbers, "numbers", (rows, cols // 2), torch.uint8, dev),
                 _address(scales, "scales", scales.shape if len(scales) == rows else (rows, scales.shape[1]),
@@ -1188,22 +1207,22 @@ class GpuAttentionEngine:
         _need_32_bits(T, n_in, rank)
         desc = QuantProjDesc(T, n_in, int(group), int(bool(mins)), int(rank), self._io_of(x))
         xp = _address(x, "x", (T, n_in), dt, dev)
-        L, ys, arr = load(), [], (LoraProj * len(projs))()
+        L, ys, arr, mins = load(), [], (LoraProj * len(projs))(), desc.offsets
         for i, pr in enumerate(projs):
-            get = pr.get
-            n_out, y = int(pr["out"]), get("y")
-            _need_32_bits(n_out)
+            get, n_out = pr.get, int(pr["out"])
+            size = _packed_bytes(n_out, n_in, desc.group, mins)
+            bias, a, b, y = get("bias"), get("a"), get("b"), get("y")
             if y is None:
-                y = torch.empty((T, n_out), dtype=dt, device=dev)
+                y = x.new_empty((T, n_out))
+                yp = y.data_ptr()
+            else:
+                yp = _address(y, (i, "y"), (T, n_out), dt, dev)
             ys.append(y)
-            size = L.glacier_proj_quant_bytes(ctypes.byref(QuantWeights(n_out, n_in, desc.group, desc.offsets)))
-            if size == 0:
-                _check(ERR_UNSUPPORTED)
             arr[i] = (_address(pr["w"], (i, "w"), (size,), torch.uint8, dev),
-                      _optional(get("bias"), (i, "bias"), (n_out,), f32, dev),
-                      _optional(get("a"), (i, "a"), (n_in, rank), f32, dev),
-                      _optional(get("b"), (i, "b"), (rank, n_out), f32, dev), float(get("scaling", 0.0)), n_out,
-                      _address(y, (i, "y"), (T, n_out), dt, dev), None, None, None)
+                      None if bias is None else _address(bias, (i, "bias"), (n_out,), f32, dev),
+                      None if a is None else _address(a, (i, "a"), (n_in, rank), f32, dev),
+                      None if b is None else _address(b, (i, "b"), (rank, n_out), f32, dev),
+                      float(get("scaling", 0.0)), n_out, yp, None, None, None)
         size = L.glacier_proj_quant_workspace(ctypes.byref(desc), arr, len(projs))
         work = None if size == 0 else self._workspace(size)
         self._bind_device_stream()
