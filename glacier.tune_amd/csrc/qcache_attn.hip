@@ -659,20 +659,24 @@ constexpr size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 QCachePlan qcache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, int n_cu) {
   QCachePlan p{};
   p.attn = cache_attn_plan(c, hq, max_new, max_kv, n_cu);
-  // Expanded pages lie in the workspace for whatever the table's rows can name (max_kv
-  // is a hint only): up to 2^30 bytes of K and V, else tiles of 16 rows read the 4-bit
-  // pages however long the chunks are.
+  // Pages are written out for chunks that many tiles of 16 rows would read again: from a
+  // mean of 256 rows a sequence on.  28/4 heads of 128 over 8192 keys, in us: 4 sequences
+  // of 16 tokens 43.4 (written out: 63.2), of 32 66.0 (73.6), of 64 116 (84.4); 16 of 16
+  // 117 (153), of 32 214 (189); 32/8 heads in fp32, 4 of 32 over 2048: 36.2 (70.4).  They
+  // lie in the workspace for whatever the table's rows can name (max_kv is a hint only):
+  // up to 2^30 bytes of K and V, else tiles of 16 rows read the 4-bit pages however long
+  // the chunks are.
+  const long group = hq / c.hkv, cap = (long)c.max_pages << c.page_shift;
+  const long seqs = std::min(c.T, c.n_seqs);
   const size_t k_bytes = (size_t)c.n_seqs * c.max_pages * c.hkv * ((size_t)c.D << c.page_shift) * (c.io_bf16 ? 2 : 4);
-  p.expand = p.attn.rows > 16 && k_bytes <= (size_t)1 << 29;
+  p.expand = p.attn.rows > 16 && c.T * group > 256 * seqs && k_bytes <= (size_t)1 << 29;
   if (p.expand) {
     p.k_bytes = up256(k_bytes);
     p.table_bytes = up256(sizeof(int32_t) * c.n_seqs * c.max_pages);
     p.bytes = 2 * p.k_bytes + p.table_bytes + p.attn.bytes;
     return p;
   }
-  const long group = hq / c.hkv, cap = (long)c.max_pages << c.page_shift;
   const long keys = max_kv > 0 && max_kv < cap ? max_kv : cap;
-  const long seqs = std::min(c.T, c.n_seqs);
   const long tiles = seqs * ((c.T * group + seqs * 16 - 1) / (seqs * 16));
   p.attn.rows = 16;
   p.attn.long_first = false;

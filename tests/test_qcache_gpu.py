@@ -368,3 +368,20 @@ def test_lengths_past_the_table(eng):
         eng.qcache_append(*(torch.randn(41, 2, 64, device="cuda").bfloat16() for _ in range(2)),
                           p.k_pages, p.v_pages, torch.tensor([0, 1, 1], device="cuda").int(), p.kv_lens, table)
         assert torch.equal(before, p.both)
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("seqs,hq,hkv,d,page,pad", [
+    ([(90, 400), (75, 1500)], 28, 4, 128, 16, 3), ([(300, 300)], 14, 2, 64, 32, 0), ([(60, 61), (40, 700)], 8, 1, 96, 16, 2),
+    ([(200, 900), (1, 800), (0, 40)], 16, 4, 256, 16, 1)])
+def test_chunks_of_many_rows(eng, seqs, hq, hkv, d, page, pad, dt):
+    # a mean of more than 256 rows (token, head of the group) a sequence
+    p = qh.QPaged(seqs, hq, hkv, d, page, DTYPES[dt], 23, pad)
+    assert p.tokens * (hq // hkv) > 256 * len(seqs)
+    out = torch.full((p.tokens, hq, d), 7.0, device="cuda", dtype=DTYPES[dt])
+    lse = torch.full((hq, p.tokens), 7.0, device="cuda")
+    ref = qh.attend_ref(p)
+    eng.qcache_forward(p.q.cuda(), *p.arrays(), max_new=max(n for n, _ in seqs), max_kv=max(n for _, n in seqs), out=out, lse=lse)
+    ch.check("out", out, ref[0], ref[1])
+    ch.check("lse", lse, ref[2], ref[3])
+    assert not pad or ((out[-pad:] == 7.0).all() and (lse[:, -pad:] == 7.0).all())
