@@ -2256,9 +2256,9 @@ int glacier_proj_quant_forward(glacier_attn_ctx* ctx, const glacier_quant_proj_d
   return guarded([&] {
     glacier::QuantProj q = glacier::quant_proj_of(desc, proj, n_proj);
     glacier::need_quant_tensors(q, x);
-    need(ctx, "ctx");
     q.a.x = x;
     glacier::need_workspace(workspace, workspace_bytes, glacier::quant_proj_workspace(q));
+    need(ctx, "ctx");
     q.terms = workspace;
     q.low = reinterpret_cast<float*>(static_cast<char*>(workspace) + glacier::quant_terms_bytes(q));
     std::lock_guard<std::mutex> g(ctx->eng->lock());

@@ -29,6 +29,7 @@ struct QuantSpec {
 struct QuantCall {
   const void* x;
   int T, in, blocks, rank, splits, n, tiles, token_blocks;
+  int abreast;  // workgroups of one token block that are numbered in a row
   QuantSpec p[kMaxProj];
 };
 
@@ -77,10 +78,10 @@ __global__ __launch_bounds__(64 * RW * KW) void quant_tile_kernel(QuantCall a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int w = wave_id() % RW, kw = wave_id() / RW, lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   int number = blockIdx.x, t0 = 0;
-  if (a.token_blocks > 1) {
-    const int round = number / (8 * a.token_blocks), rest = number - round * 8 * a.token_blocks;
-    number = round * 8 + rest % 8;
-    t0 = rest / 8 * 16 * NT;
+  if (a.token_blocks > 1) {  // (a tile's token blocks on one XCD, whose L2 has its weights then)
+    const int round = number / (a.abreast * a.token_blocks), rest = number - round * a.abreast * a.token_blocks;
+    number = round * a.abreast + rest % a.abreast;
+    t0 = rest / a.abreast * 16 * NT;
   }
   number = RW * number + w;
   const bool has_tile = number < a.tiles;
@@ -400,9 +401,11 @@ hipError_t tiled(QuantCall c, hipStream_t st) {
     c.p[p].first = c.tiles;
     c.tiles += (c.p[p].out + 16 * RT - 1) / (16 * RT);
   }
-  const int groups = (c.tiles + RW - 1) / RW, tb = c.token_blocks;
+  const int groups = (c.tiles + RW - 1) / RW;
+  c.abreast = std::min(groups, 8);
+  const int grid = (groups + c.abreast - 1) / c.abreast * c.abreast * c.token_blocks;
   GL_CHECK(allow_lds((&quant_tile_kernel<NT, RT, RW, KW, GP, OFF, TERMS>), C::BYTES));
-  hipLaunchKernelGGL((quant_tile_kernel<NT, RT, RW, KW, GP, OFF, TERMS>), dim3(tb > 1 ? (groups + 7) / 8 * 8 * tb : groups),
+  hipLaunchKernelGGL((quant_tile_kernel<NT, RT, RW, KW, GP, OFF, TERMS>), dim3(grid),
                      dim3(64 * C::WAVES), C::BYTES, st, c);
   return hipGetLastError();
 }

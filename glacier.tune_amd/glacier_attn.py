@@ -1164,7 +1164,7 @@ class GpuAttentionEngine:
     @staticmethod
     def quant_bytes(out_features, in_features, group=32, offsets=False):
         """Bytes of packed 4-bit weights (0: not a size that is taken)."""
-        _need_32_bits(out_features, in_features)
+        _need_32_bits(out_features, in_features, group)
         return load().glacier_proj_quant_bytes(
             ctypes.byref(QuantWeights(int(out_features), int(in_features), int(group), int(bool(offsets)))))
 
@@ -1182,12 +1182,11 @@ class GpuAttentionEngine:
         _need_32_bits(rows, cols)
         w = QuantWeights(rows, cols, cols // scales.shape[1], int(offsets is not None))
         size = _packed_bytes(rows, cols, w.group, w.offsets)
-        packed = torch.empty(size, dtype=torch.uint8, device=dev) if packed is None else packed
-        args = (_address(numbers, "numbers", (rows, cols // 2), torch.uint8, dev),
-                _address(scales, "scales", scales.shape if len(scales) == rows else (rows, scales.shape[1]),
-                         torch.float16, dev),
-                _optional(offsets, "offsets", scales.shape, torch.float16, dev),
-                _address(packed, "packed", (size,), torch.uint8, dev))
+        np_ = _address(numbers, "numbers", (rows, cols // 2), torch.uint8, dev)
+        sp = _address(scales, "scales", (rows, scales.shape[1]), torch.float16, dev)
+        op = _optional(offsets, "offsets", scales.shape, torch.float16, dev)
+        packed = numbers.new_empty(size) if packed is None else packed
+        args = (np_, sp, op, _address(packed, "packed", (size,), torch.uint8, dev))
         self._bind_device_stream()
         rc = _lib.glacier_proj_quant_pack(self._h, ctypes.byref(w), *args)
         if rc != OK:

@@ -96,12 +96,12 @@ int glacier_attn_qcache_forward(glacier_attn_ctx *ctx, const glacier_kv_cache *c
  * (n - 8) s + o where there are offsets, n of 4 bits, s and o fp16. */
 typedef struct glacier_quant_weights {
   int32_t out_features;  /* a multiple of 4 */
-  int32_t in_features;   /* a multiple of 32 and of group */
+  int32_t in_features;   /* a multiple of 32 and of group, below 2^24 */
   int32_t group;         /* 32, 64 or 128 */
   int32_t offsets;       /* 0, or 1: weights have offsets */
 } glacier_quant_weights;
 
-/* Bytes of packed weights (0 if w is not valid).  Their layout, rows padded to a
+/* Bytes of packed weights, below 2^31 (0 if w is not valid).  Their layout, rows padded to a
  * multiple of 16 and columns to one of 128 with zeros:
  *   [out / 16][in / 128][64] entries of four 32-bit words: word i of entry 16 c + r
  *     holds row r's columns 32 i + 8 c .. of the block, in a cache word's order
@@ -134,7 +134,10 @@ size_t glacier_proj_quant_workspace(const glacier_quant_proj_desc *desc, const g
  * projections of x [T][in]: as glacier_proj_forward, with proj[p].w the packed
  * weights.  x, y, lora_a, lora_b and w 16-byte aligned; outputs share no memory
  * with inputs or each other.  workspace: at least glacier_proj_quant_workspace
- * bytes, 256-byte aligned, the call's own until it has run. */
+ * bytes, 256-byte aligned, the call's own until it has run.  Sums of eight (bf16
+ * tensors: 143) times a group's |x| pass through fp32: a token for which they pass
+ * its range, or with a value that is not finite, gets outputs that are not finite;
+ * no other token is touched. */
 int glacier_proj_quant_forward(glacier_attn_ctx *ctx, const glacier_quant_proj_desc *desc, const void *x,
                                const glacier_lora_proj *proj, int n_proj, void *workspace,
                                size_t workspace_bytes);
