@@ -370,18 +370,117 @@ def test_lengths_past_the_table(eng):
         assert torch.equal(before, p.both)
 
 
+def _written_out(eng, p):
+    """Whether a call without hints writes the pages out first: from a mean of 256 rows
+    (token, head of the group) a sequence on, where tiles of more than 16 rows are taken."""
+    cache, batch = ga.qcache_args(*p.arrays(), p.tokens, 0, 0, 0, p.d, p.dtype)
+    size = ga._lib.glacier_attn_qcache_workspace(eng._h, ga.ctypes.byref(cache), ga.ctypes.byref(batch), p.hq)
+    assert p.tokens * (p.hq // p.hkv) > 256 * len(p.seqs)
+    return size >= 2 * p.table.numel() * p.page * p.hkv * p.d * p.q.element_size()
+
+
 @pytest.mark.parametrize("dt", sorted(DTYPES))
 @pytest.mark.parametrize("seqs,hq,hkv,d,page,pad", [
     ([(90, 400), (75, 1500)], 28, 4, 128, 16, 3), ([(300, 300)], 14, 2, 64, 32, 0), ([(60, 61), (40, 700)], 8, 1, 96, 16, 2),
     ([(200, 900), (1, 800), (0, 40)], 16, 4, 256, 16, 1)])
 def test_chunks_of_many_rows(eng, seqs, hq, hkv, d, page, pad, dt):
-    # a mean of more than 256 rows (token, head of the group) a sequence
-    p = qh.QPaged(seqs, hq, hkv, d, page, DTYPES[dt], 23, pad)
-    assert p.tokens * (hq // hkv) > 256 * len(seqs)
+    # with hints in tiles of 16 rows, without them written out
+    p = qh.QPaged(seqs, hq, hkv, d, page, DTYPES[dt], 23, pad, columns=16384 // page)
+    assert _written_out(eng, p) == (dt == "bf16" or 64 < d <= 128)
     out = torch.full((p.tokens, hq, d), 7.0, device="cuda", dtype=DTYPES[dt])
     lse = torch.full((hq, p.tokens), 7.0, device="cuda")
     ref = qh.attend_ref(p)
-    eng.qcache_forward(p.q.cuda(), *p.arrays(), max_new=max(n for n, _ in seqs), max_kv=max(n for _, n in seqs), out=out, lse=lse)
-    ch.check("out", out, ref[0], ref[1])
-    ch.check("lse", lse, ref[2], ref[3])
+    for hints in (dict(max_new=max(n for n, _ in seqs), max_kv=max(n for _, n in seqs)), {}):
+        eng.qcache_forward(p.q.cuda(), *p.arrays(), out=out, lse=lse, **hints)
+        ch.check("out", out, ref[0], ref[1])
+        ch.check("lse", lse, ref[2], ref[3])
     assert not pad or ((out[-pad:] == 7.0).all() and (lse[:, -pad:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_many_rows_without_a_key(eng, dt):
+    p = qh.QPaged([(25, 30), (20, 20)], 28, 2, 96, 16, DTYPES[dt], 24, columns=1024)
+    assert _written_out(eng, p)
+    p.kv_lens[1] = 5
+    out, lse = eng.qcache_forward(p.q.cuda(), *p.arrays(), save=True)
+    assert not out[25:40].any() and (lse[:, 25:40] == -math.inf).all()
+    assert out[40].any() and not out.isnan().any()
+    ref = qh.attend_ref(p)
+    ch.check("out", out[:25], ref[0][:25], ref[1][:25])
+    p.kv_lens[0] = -3
+    out, lse = eng.qcache_forward(p.q.cuda(), *p.arrays(), save=True)
+    assert not out[:40].any() and (lse[:, :40] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_many_rows_and_bad_pages(eng, dt):
+    p = qh.QPaged([(24, 100), (19, 70), (20, 64)], 28, 2, 128, 16, DTYPES[dt], 25, columns=1024)
+    assert _written_out(eng, p)
+    p.table[0, 2], p.table[1, 0], p.table[2, 1] = -1, p.n_pages, 2 ** 31 - 1
+    gone = [(0, j) for j in range(32, 48)] + [(1, j) for j in range(16)] + [(2, j) for j in range(16, 32)]
+    out, lse = eng.qcache_forward(p.q.cuda(), *p.arrays(), save=True)
+    ref, far = ch.attend_ref(p, hidden=gone), qh.attend_ref(p)
+    ch.check("out", out, ref[0], ref[1] + far[1])
+    ch.check("lse", lse, ref[2], ref[3] + far[3])
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_many_rows_and_keys_that_are_not_finite(eng, dt, d):
+    def change(p):
+        p.v[0][33, 0, 5] = math.nan
+        p.k[1][50, 0, 3] = math.inf
+
+    args = ([(28, 40), (23, 52)], 28, 2, d, 16, DTYPES[dt], 26)
+    p, clean = qh.QPaged(*args, change=change, columns=1024), qh.QPaged(*args)
+    out, lse = eng.qcache_forward(p.q.cuda(), *p.arrays(), save=True)
+    want, bound, *_ = qh.attend_ref(clean)
+    odd = torch.zeros_like(out, dtype=torch.bool)
+    odd[21:28, :14, :32] = True  # positions 33 .. 39 of 12 .. 39
+    odd[49:, :14] = True  # positions 50, 51 of 29 .. 51
+    assert torch.equal(out.isnan(), odd)
+    ch.check("out", torch.where(odd, 0.0, out), torch.where(odd.cpu(), 0.0, want), bound)
+    assert lse[:14, 49:].isnan().all() and not lse[14:].isnan().any() and not lse[:, :49].isnan().any()
+
+
+@pytest.mark.parametrize("cu", [[0, 25, 3, 40], [-7, 2, 900, 3], [44, 4, 1, 0], [0, 2 ** 31 - 1, -2 ** 31, 60]])
+def test_many_rows_and_wrong_offsets(eng, cu):
+    p = qh.QPaged([(20, 30), (20, 40), (20, 50)], 28, 2, 64, 16, torch.bfloat16, 27, columns=1024)
+    assert _written_out(eng, p)
+    wrong = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    rows = torch.full((62, 28, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+    eng.qcache_forward(p.q.cuda(), p.k_pages, p.v_pages, wrong, p.kv_lens, p.table, out=rows[1:61])
+    torch.cuda.synchronize()
+    assert (rows[0] == 7.0).all() and (rows[61] == 7.0).all()
+
+
+def test_two_engines_and_threads(eng):
+    # an engine and a stream each, called from two threads at once
+    import threading
+
+    sets = [qh.QPaged([(1, 300), (2, 90)], 8, 2, 128, 16, torch.bfloat16, 40 + i) for i in range(2)]
+    want = [eng.qcache_forward(p.q.cuda(), *p.arrays())[0] for p in sets]
+    own = [ga.GpuAttentionEngine(0, ga.PREC_BF16) for _ in sets]
+    got, failed = [None, None], []
+
+    def run(i):
+        try:
+            p, q, stream = sets[i], sets[i].q.cuda(), torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(stream):
+                outs = [own[i].qcache_forward(q, *p.arrays())[0] for _ in range(20)]
+            stream.synchronize()
+            got[i] = outs
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    assert all(torch.equal(o, w) for outs, w in zip(got, want) for o in outs)
+    for e in own:
+        e.close()
