@@ -4,11 +4,13 @@
 // HBM-bound: each row is read once and written once.  A wave takes one token, or a
 // share of its heads when there are few tokens.  A lane holds eight columns of a
 // head, so a group of 32 is four neighbouring lanes: its largest element is found in
-// two exchanges, and a lane's eight numbers are one word of the page.  Two steps' rows
-// are in flight, the first from before the token's place is known, and the angles of a
-// lane's columns stay in its registers.  5272 tokens of 32 query and 8 KV heads of 128
-// (bf16): 30.7 us for 114 MB (3.7 TB/s; with the rows asked for step by step and the
-// angles read from LDS 38), read back in 8.0.
+// two exchanges, and a lane's eight numbers are one word of the page.  A step's rows are
+// in flight while the one before is worked on, the first from before the token's place
+// is known, and the angles of a lane's columns stay in its registers.  5272 tokens of 32
+// query and 8 KV heads of 128 (bf16): 26.4 us for 114 MB (4.3 TB/s), 1600 operations a
+// token; with the rows asked for step by step and the angles read from LDS 38, with
+// queries in a key's layout, which forms each angle's product twice, and elements rounded
+// from 64 bits to bf16 at once 29.4.  Read back in 8.0.
 //
 // The rotation is formed in 64 bits: a key that fp32 rounding moves over the border
 // between two numbers would be held a whole step off, so that the cache's contents
@@ -31,11 +33,20 @@ __device__ inline double2 turn64(double rev, int pos) {
   return make_double2(c, s);
 }
 
-// Eight columns of a row as they are loaded, and the eight that they are rotated with.
+// Of a query a lane holds four columns of the first half and the four that they are
+// rotated with; of a key eight columns in a row (a word) and their eight partners.
 template <typename IO>
 struct Columns {
   Piece<IO, 4> own[2], other[2];
 };
+
+// x rounded to fp32, kept so: rounded to bf16 from there (the compiler rounds some
+// elements from 64 bits otherwise, by eight operations each).
+__device__ inline float rounded(double x) {
+  float r = (float)x;
+  asm("" : "+v"(r));
+  return r;
+}
 
 template <typename IO, int G>
 __global__ __launch_bounds__(64 * kWavesQa) void qcache_append_kernel(CacheAppend a, TurnRates rates) {
@@ -46,39 +57,81 @@ __global__ __launch_bounds__(64 * kWavesQa) void qcache_append_kernel(CacheAppen
   const int unit = blockIdx.x * kWavesQa + wave;
   const int t = unit / a.parts, part = unit - t * a.parts;
   if (t >= c.T) return;
-  const int half = c.D / 2, heads = a.hq + 2 * c.hkv, turned = a.hq + c.hkv;
+  const int half = c.D / 2, held = 2 * c.hkv, q_steps = (a.hq + H - 1) / H, steps = q_steps + (held + H - 1) / H;
   const int col8 = lane % L, slot = lane / L, col = 8 * col8;
+  // queries: pairs (pair + e, half + pair + e) (half is a multiple of 4)
+  const bool has_pair = slot < H && 4 * col8 < half;
+  const int pair = has_pair ? 4 * col8 : 0;
+  const IO* const q = static_cast<const IO*>(a.q) + (long)t * a.hq * c.D;
+  auto load_q = [&](Piece<IO, 4> (&to)[2], int step) __attribute__((always_inline)) {
+    const IO* const src = q + (long)min(step * H + slot, a.hq - 1) * c.D + pair;
+    to[0].load(src), to[1].load(src + half);
+  };
+  // keys and values, keys first: columns col .. and, rotated, their partners
   const bool in_row = slot < H && col < c.D;
-  // (half is a multiple of 4: four columns have their partners together)
   const int at0 = in_row ? col : 0, at1 = at0 + 4;
   const int to0 = at0 < half ? at0 + half : at0 - half, to1 = at1 < half ? at1 + half : at1 - half;
-  auto load = [&](Columns<IO>& to, int h0) __attribute__((always_inline)) {
-    const int h = min(h0 + slot, heads - 1);
-    const IO* const src = h < a.hq ? static_cast<const IO*>(a.q) + ((long)t * a.hq + h) * c.D
-                          : h < turned ? static_cast<const IO*>(a.k) + ((long)t * c.hkv + (h - a.hq)) * c.D
-                                       : static_cast<const IO*>(a.v) + ((long)t * c.hkv + (h - turned)) * c.D;
+  auto load_kv = [&](Columns<IO>& to, int step) __attribute__((always_inline)) {
+    const int h0 = (step - q_steps) * H, h = min(h0 + slot, held - 1);
+    const IO* const src = h < c.hkv ? static_cast<const IO*>(a.k) + ((long)t * c.hkv + h) * c.D
+                                    : static_cast<const IO*>(a.v) + ((long)t * c.hkv + (h - c.hkv)) * c.D;
     to.own[0].load(src + at0), to.own[1].load(src + at1);
-    if (a.rotate && h0 < turned) to.other[0].load(src + to0), to.other[1].load(src + to1);
+    if (a.rotate && h0 < c.hkv) to.other[0].load(src + to0), to.other[1].load(src + to1);
   };
-  // two steps' rows in flight, from before the search for the token's place
-  const int first = part * H, stride = a.parts * H;
-  Columns<IO> one, two;
-  load(one, first);
-  if (first + stride < heads) load(two, first + stride);
+  // a step's rows are in flight while the one before is worked on, the first ones from
+  // before the search for the token's place
+  int step = part;
+  const int first_kv = step >= q_steps ? step : step + (q_steps - step + a.parts - 1) / a.parts * a.parts;
+  Piece<IO, 4> one[2], two[2];
+  Columns<IO> next;
+  if (step < q_steps) load_q(one, step);
+  if (step + a.parts < q_steps) load_q(two, step + a.parts);
+  if (first_kv < steps) load_kv(next, first_kv);
   const CacheSeq s = seq_of_token(c, lane, t);
   if (s.b >= c.n_seqs || t < s.tok0) return;  // behind the last sequence
   const int pos = s.pos0 + (t - s.tok0);
   const int page = cache_page(c, s.b, pos);
   const int row = pos & ((1 << c.page_shift) - 1);
-  // the angles of this lane's columns, the same in every head
-  double co[8], si[8];
+  double2* const turn = turns[wave];
   if (a.rotate) {
-    double2* const turn = turns[wave];
     const int second = lane + 64;
     const double lo = rates.rev[lane < half ? lane : 0], hi = rates.rev[second < half ? second : 0];
     if (lane < half) turn[lane] = turn64(lo, pos);
     if (second < half) turn[second] = turn64(hi, pos);
     wave_lds_order();
+  }
+  if (step < q_steps) {
+    double2 cs[4];  // the angles of this lane's pairs, the same in every head
+#pragma unroll
+    for (int e = 0; e < 4; ++e) cs[e] = turn[pair + e];
+    IO* const q_rot = static_cast<IO*>(a.q_rot) + (long)t * a.hq * c.D;
+    auto take = [&](const Piece<IO, 4> (&from)[2], int at) __attribute__((always_inline)) {
+      const int h = at * H + slot;
+      float x[4], y[4], u[4], v[4];
+      from[0].get(x), from[1].get(y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const double xd = x[e], yd = y[e];
+        u[e] = rounded(fma(xd, cs[e].x, -yd * cs[e].y));
+        v[e] = rounded(fma(yd, cs[e].x, xd * cs[e].y));
+      }
+      if (!has_pair || h >= a.hq) return;
+      Piece<IO, 4> to[2];
+      to[0].set(u), to[1].set(v);
+      to[0].store(q_rot + (long)h * c.D + pair), to[1].store(q_rot + (long)h * c.D + pair + half);
+    };
+    for (; step < q_steps; step += 2 * a.parts) {
+      const int then = step + a.parts;
+      take(one, step);
+      if (then >= q_steps) break;
+      if (then + a.parts < q_steps) load_q(one, then + a.parts);
+      take(two, then);
+      if (then + 2 * a.parts < q_steps) load_q(two, then + 2 * a.parts);
+    }
+  }
+  if (page < 0) return;  // (held nowhere)
+  double co[8], si[8];
+  if (a.rotate && (first_kv - q_steps) * H < c.hkv) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int at = (e < 4 ? at0 : at1) + e % 4;
@@ -87,9 +140,11 @@ __global__ __launch_bounds__(64 * kWavesQa) void qcache_append_kernel(CacheAppen
     }
   }
   const long part_bytes = (long)quant_row_bytes(c.D) << c.page_shift;
-  auto take = [&](const Columns<IO>& from, int h0) __attribute__((always_inline)) {
-    const int h = h0 + slot;
-    const bool here = slot < H && h < heads, is_q = h < a.hq, is_k = !is_q && h < turned;
+  for (step = first_kv; step < steps; step += a.parts) {
+    const Columns<IO> from = next;
+    if (step + a.parts < steps) load_kv(next, step + a.parts);
+    const int h0 = (step - q_steps) * H, h = h0 + slot;
+    const bool here = slot < H && h < held, is_k = h < c.hkv;
     float x[8];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
@@ -98,7 +153,7 @@ __global__ __launch_bounds__(64 * kWavesQa) void qcache_append_kernel(CacheAppen
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[4 * p + e] = in_row ? own[e] : 0.0f;
     }
-    if (a.rotate && h0 < turned) {
+    if (a.rotate && h0 < c.hkv) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         float other[4];
@@ -107,28 +162,19 @@ __global__ __launch_bounds__(64 * kWavesQa) void qcache_append_kernel(CacheAppen
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * p + e;
           const float r = (float)fma((double)x[i], co[i], (double)other[e] * si[i]);
-          x[i] = in_row && (is_q || is_k) ? r : x[i];
+          x[i] = in_row && is_k ? r : x[i];
         }
       }
     }
-    if (here && is_q && in_row) store8(static_cast<IO*>(a.q_rot) + ((long)t * a.hq + h) * c.D + col, x);
-    if (h0 + H <= a.hq || page < 0) return;  // (the wave's heads are queries, or held nowhere)
     // (all lanes: a group's lanes exchange their largest elements)
     f16 scale;
     const unsigned w = quantise8(x, scale);
-    if (!here || is_q) return;
-    const int kv = h - (is_k ? a.hq : turned);
+    if (!here) continue;
+    const int kv = is_k ? h : h - c.hkv;
     char* const to = static_cast<char*>(is_k ? c.k_pages : c.v_pages) + page * c.page_stride + kv * part_bytes;
     f16* const scales = reinterpret_cast<f16*>(to + ((16L * G) << c.page_shift));
     reinterpret_cast<unsigned*>(to)[is_k ? k_word(row, G, col8) : v_word(row, G, col8)] = w;
     if (col8 % 4 == 0) scales[is_k ? k_scale(row, G, col8 / 4) : v_scale(row, G, col8 / 4)] = scale;
-  };
-  for (int h0 = first; h0 < heads; h0 += 2 * stride) {
-    take(one, h0);
-    if (h0 + stride >= heads) break;
-    if (h0 + 2 * stride < heads) load(one, h0 + 2 * stride);
-    take(two, h0 + stride);
-    if (h0 + 3 * stride < heads) load(two, h0 + 3 * stride);
   }
 }
 
@@ -166,7 +212,7 @@ __global__ __launch_bounds__(64 * kWavesQa) void qcache_read_kernel(QCacheRead a
 template <typename IO, int G>
 hipError_t append(CacheAppend& a, const TurnRates& r, int n_cu, hipStream_t st) {
   constexpr int H = 16 / G;
-  a.parts = turn_parts(a.c.T, (a.hq + 2 * a.c.hkv + H - 1) / H, n_cu);
+  a.parts = turn_parts(a.c.T, (a.hq + H - 1) / H + (2 * a.c.hkv + H - 1) / H, n_cu);
   const long units = (long)a.c.T * a.parts;
   hipLaunchKernelGGL((qcache_append_kernel<IO, G>), dim3((units + kWavesQa - 1) / kWavesQa), dim3(64 * kWavesQa), 0,
                      st, a, r);

@@ -48,26 +48,26 @@ __device__ inline unsigned quant_number(float x, unsigned sign, float size, floa
 // Eight columns (of a group of 32 that four neighbouring lanes hold) as a word and
 // the group's scale.
 __device__ inline unsigned quantise8(const float (&x)[8], f16& scale) {
-  float top = x[0], low = x[0];
-  unsigned odd = 0;
+  float top = x[0], low = x[0], zero = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     top = fmaxf(top, x[e]);
     low = fminf(low, x[e]);
-    odd |= (__builtin_bit_cast(unsigned, x[e]) & 0x7f800000u) == 0x7f800000u ? 1u : 0u;
+    zero = fmaf(x[e], 0.0f, zero);  // NaN where an element is not finite
   }
 #pragma unroll
   for (int d = 1; d < 4; d *= 2) {
     top = fmaxf(top, __shfl_xor(top, d));
     low = fminf(low, __shfl_xor(low, d));
-    odd |= __shfl_xor(odd, d);
+    zero += __shfl_xor(zero, d);
   }
+  const bool odd = zero != 0.0f;
   scale = odd ? __builtin_bit_cast(f16, static_cast<unsigned short>(kQuantNan))
               : quant_scale((top >= -low ? top : low) * -0.125f);
   const float s = (float)scale;
   if (odd || s == 0.0f) return kQuantZero;
   const unsigned sign = __builtin_bit_cast(unsigned, s) & 0x80000000u;
-  const float size = fabsf(s), inv = 1.0f / size;
+  const float size = fabsf(s), inv = __builtin_amdgcn_rcpf(size);
   unsigned w = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) w |= quant_number(x[e], sign, size, inv) << (4 * (e / 2) + 16 * (e % 2));
