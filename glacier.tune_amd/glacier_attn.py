@@ -26,6 +26,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 
 import numpy as np
 
@@ -578,6 +579,7 @@ def qcache_args(k_pages, v_pages, cu_tokens, kv_lens, page_table, total_tokens, 
 
 
 _packed_sizes = {}
+_LORA_PROJ = struct.Struct("@4Pfi4P")  # a LoraProj's fields, written at once
 
 
 def _packed_bytes(out, cols, group, offsets):
@@ -1206,7 +1208,7 @@ class GpuAttentionEngine:
         _need_32_bits(T, n_in, rank)
         desc = QuantProjDesc(T, n_in, int(group), int(bool(mins)), int(rank), self._io_of(x))
         xp = _address(x, "x", (T, n_in), dt, dev)
-        L, ys, arr, mins = load(), [], (LoraProj * len(projs))(), desc.offsets
+        L, ys, arr, mins, put = load(), [], (LoraProj * len(projs))(), desc.offsets, _LORA_PROJ.pack_into
         for i, pr in enumerate(projs):
             get, n_out = pr.get, int(pr["out"])
             size = _packed_bytes(n_out, n_in, desc.group, mins)
@@ -1217,11 +1219,11 @@ class GpuAttentionEngine:
             else:
                 yp = _address(y, (i, "y"), (T, n_out), dt, dev)
             ys.append(y)
-            arr[i] = (_address(pr["w"], (i, "w"), (size,), torch.uint8, dev),
-                      None if bias is None else _address(bias, (i, "bias"), (n_out,), f32, dev),
-                      None if a is None else _address(a, (i, "a"), (n_in, rank), f32, dev),
-                      None if b is None else _address(b, (i, "b"), (rank, n_out), f32, dev),
-                      float(get("scaling", 0.0)), n_out, yp, None, None, None)
+            put(arr, i * _LORA_PROJ.size, _address(pr["w"], (i, "w"), (size,), torch.uint8, dev),
+                0 if bias is None else _address(bias, (i, "bias"), (n_out,), f32, dev),
+                0 if a is None else _address(a, (i, "a"), (n_in, rank), f32, dev),
+                0 if b is None else _address(b, (i, "b"), (rank, n_out), f32, dev),
+                get("scaling", 0.0), n_out, yp, 0, 0, 0)
         size = L.glacier_proj_quant_workspace(ctypes.byref(desc), arr, len(projs))
         work = None if size == 0 else self._workspace(size)
         self._bind_device_stream()

@@ -282,3 +282,10 @@ def test_front_end_checks_products():
                  (n, s, s[:, :1]), (n, s, None, torch.zeros(size - 1, dtype=torch.uint8))):
         with pytest.raises((TypeError, ga.Unsupported)):
             pack(types.SimpleNamespace(device_ordinal=-1), *args)
+
+
+def test_a_projection_is_written_at_once():
+    arr = (ga.LoraProj * 2)()
+    ga._LORA_PROJ.pack_into(arr, ga._LORA_PROJ.size, 1, 2, 3, 4, -1.5, 6, 7, 8, 9, 10)
+    assert ga._LORA_PROJ.size == ctypes.sizeof(ga.LoraProj) and not arr[0].w
+    assert [getattr(arr[1], f) for f, _ in ga.LoraProj._fields_] == [1, 2, 3, 4, -1.5, 6, 7, 8, 9, 10]
