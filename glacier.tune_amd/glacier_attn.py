@@ -16,7 +16,9 @@ GpuLoraEngine.Forward.cs:205-245, and LoraAdapter.Backward, LoraAdapter.cs:190-2
 `qk_norm_forward` / `qk_norm_backward` are the per-head norms of queries and keys
 with the rotation (include/glacier_norm.h); `cache_append` and `cache_forward`
 the paged key/value cache that answers with the tuned model
-(include/glacier_cache.h).  Errors raise: InvalidArgument (a ValueError, where the C#
+(include/glacier_cache.h); `qcache_append`, `qcache_read` and `qcache_forward` the
+same cache in 4 bits, `quant_pack` and `proj_quant_forward` projections with 4-bit
+base weights (include/glacier_quant.h).  Errors raise: InvalidArgument (a ValueError, where the C#
 engine throws ArgumentOutOfRangeException), Unsupported (the shape stays on
 the CPU path), DeviceError, OutOfMemory.  There is no fallback: if the
 library is missing or the device fails, the call raises.
