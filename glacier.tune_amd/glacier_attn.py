@@ -603,6 +603,8 @@ def quantise_rows(w, group=32):
     largest magnitude of each group to n = 0."""
     torch = _torch()
 
+    if w.dim() != 2 or group <= 0 or w.shape[1] % group != 0:
+        raise TypeError(f"w must be [out, in] with whole groups of {group} columns, got {tuple(w.shape)}")
     g = w.float().unflatten(1, (-1, group))
     top, low = g.amax(-1), g.amin(-1)
     s = (torch.where(top >= -low, top, low) / -8.0).half()

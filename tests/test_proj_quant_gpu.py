@@ -262,3 +262,26 @@ def test_fp32_of_every_size(eng):
     x[7, 5], x[8, 200] = torch.finfo(torch.float32).max / 16, -torch.finfo(torch.float32).max / 16
     y, = eng.proj_quant_forward(x.cuda(), [{"w": _pack(eng, w), "out": 64}], group=64)
     ch.check("y", y, *qh.project_ref(x, w, torch.float32))
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+@pytest.mark.parametrize("T", [3001, 50001])
+def test_many_tokens_of_few_outputs(eng, dt, T):
+    dt, w = DTYPES[dt], qh.Weights(20, 96, 32, True, 16)
+    x = torch.randn(T, 96, generator=torch.Generator().manual_seed(17)).to(dt)
+    kw = {"a": torch.randn(96, 3), "b": torch.randn(3, 20), "scaling": 1.0}
+    pr = {"w": _pack(eng, w), "out": 20, "a": kw["a"].cuda(), "b": kw["b"].cuda(), "scaling": 1.0}
+    y, = eng.proj_quant_forward(x.cuda(), [pr], rank=3, mins=True)
+    ch.check("y", y, *qh.project_ref(x, w, dt, **kw))
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_one_weight_in_two_projections(eng, dt):
+    # one W, A and B twice, and tensors that begin inside others
+    dt, w = DTYPES[dt], qh.Weights(64, 128, 64, False, 18)
+    packed, rows = _pack(eng, w), torch.randn(7, 128).to(dt).cuda()
+    a, b = torch.randn(128, 9).cuda(), torch.randn(9, 64).cuda()
+    pr = {"w": packed, "out": 64, "a": a, "b": b, "scaling": 0.25}
+    one, two = eng.proj_quant_forward(rows[2:], [dict(pr), dict(pr, scaling=-0.25)], rank=9, group=64)
+    for y, s in ((one, 0.25), (two, -0.25)):
+        ch.check("y", y, *qh.project_ref(rows[2:].cpu(), w, dt, a=a.cpu(), b=b.cpu(), scaling=s))

@@ -484,3 +484,32 @@ def test_two_engines_and_threads(eng):
     assert all(torch.equal(o, w) for outs, w in zip(got, want) for o in outs)
     for e in own:
         e.close()
+
+
+@pytest.mark.parametrize("dt", sorted(DTYPES))
+def test_captured_chunks_that_are_written_out(eng, dt):
+    # two graphs, whose workspaces hold the pages written out, side by side, with lengths
+    # that change between the replays
+    sets, graphs, outs, streams = [], [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seed in (51, 52):
+        p = qh.QPaged([(24, 90), (20, 300)], 28, 2, 128, 16, DTYPES[dt], seed, columns=1024)
+        assert _written_out(eng, p)
+        sets.append((p, p.q.cuda()))
+    for (p, q), stream in zip(sets, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(eng.qcache_forward(q, *p.arrays(), save=True))
+        graphs.append(graph)
+    for turn in range(4):
+        for p, _ in sets:
+            p.kv_lens -= torch.tensor([9 * turn, 40], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        got = [(o.clone(), x.clone()) for o, x in outs]
+        for (p, q), (o, x) in zip(sets, got):
+            want = eng.qcache_forward(q, *p.arrays(), save=True)
+            assert torch.equal(o, want[0]) and torch.equal(x, want[1])

@@ -289,3 +289,14 @@ def test_a_projection_is_written_at_once():
     ga._LORA_PROJ.pack_into(arr, ga._LORA_PROJ.size, 1, 2, 3, 4, -1.5, 6, 7, 8, 9, 10)
     assert ga._LORA_PROJ.size == ctypes.sizeof(ga.LoraProj) and not arr[0].w
     assert [getattr(arr[1], f) for f, _ in ga.LoraProj._fields_] == [1, 2, 3, 4, -1.5, 6, 7, 8, 9, 10]
+
+
+def test_rows_to_be_quantised():
+    torch = pytest.importorskip("torch")
+    for w, group in ((torch.zeros(4, 40), 32), (torch.zeros(32), 32), (torch.zeros(4, 64), 0), (torch.zeros(4, 64), 128)):
+        with pytest.raises(TypeError):
+            ga.quantise_rows(w, group)
+    numbers, scales = ga.quantise_rows(torch.tensor([[0.0, -4.0, 4.0, 1.0]]).repeat(4, 16), 32)
+    assert (scales == -0.5).all() and (numbers[:, 0] == (8 | 15 << 4)).all() and (numbers[:, 1] == (0 | 6 << 4)).all()
+    numbers, scales = ga.quantise_rows(torch.zeros(4, 64), 64)
+    assert not scales.any() and (numbers == 0x88).all()
