@@ -35,6 +35,7 @@ namespace {
 
 [[maybe_unused]] constexpr int kKeysQ = 32;  // keys of a wave's block: one k-step of the second product
 constexpr int kWavesQ = 4;
+[[maybe_unused]] constexpr float kSlack = 8.0f;
 
 // LDS of a workgroup: its queries, operands of the first product (and -136 sum(q), where
 // its sums begin), then for each wave one block of K and one of V, words and then scales
@@ -384,7 +385,10 @@ __global__ __launch_bounds__((64 * QaLayout<T, G>::WAVES), G <= 4 ? 3 : 2) void 
     for (int p = 0; p < 2; ++p)
 #pragma unroll
       for (int r = 0; r < 4; ++r) top = fmaxf(top, st[p][r]);
-    const float mn = fmaxf(m, col_max_swap(top));
+    // The running maximum follows a row's scores only where they leave it by more than
+    // kSlack: weights reach 2^kSlack then, which fp32 sums hold as well, and most blocks
+    // of a tile of several rows scale nothing.
+    const float high = col_max_swap(top), mn = high > m + kSlack ? high : m;
     if (__any(mn != m)) {
       const float alpha = weight(m - mn);
       m = mn;
