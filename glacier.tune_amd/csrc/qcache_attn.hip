@@ -149,11 +149,84 @@ struct FixedDiv {
 struct TileDivs {
   FixedDiv splits, heads, group;
   unsigned few;  // 2^16 / group, rounded up
+  bool by_length;  // tiles as work_by_length has them
   // x / group for x < group + 15
   __device__ inline int few_of(int x, int of) const {
     return of >= 16 ? (x >= of ? 1 : 0) : static_cast<int>(static_cast<unsigned>(x) * few >> 16);
   }
 };
+
+// Sum of x over this lane and those before it.
+[[maybe_unused]] __device__ inline int lanes_up_to(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // 1, 2, 4, 8 lanes before, in a row of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // the row before's last lane, into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // lane 31, into rows 2 and 3
+  return x;
+}
+
+// What a workgroup takes: a tile of 16 rows from r0 of sequence s on, one split of its
+// keys, one KV head.
+struct TileWork {
+  CacheSeq s;
+  int r0, split, kvh;  // r0: -1 if there is none
+  int per, active;  // of the keys, where `last` (else not known yet)
+  bool last;  // the sequence's last tile
+};
+// As everywhere: tiles are numbered through all sequences, a tile's splits from another
+// one on.
+[[maybe_unused]] __device__ inline TileWork work_by_number(const CacheAttn& a, const TileDivs& f, int lane, int block) {
+  const CacheView& c = a.c;
+  TileWork x{{c.n_seqs, 0, 0, 0}, -1, 0, 0, 0, 0, false};
+  const int rest = f.splits.of(block), number = f.heads.of(rest);
+  x.kvh = rest - number * c.hkv;
+  x.split = block - rest * a.n_splits + number;
+  x.split -= f.splits.of(x.split) * a.n_splits;
+  x.s = find_seq(c, lane, number, [&](int b, int to) { return (to * a.group >> 4) + b; });
+  if (x.s.b < c.n_seqs) x.r0 = 16 * (number - (x.s.tok0 * a.group >> 4) - x.s.b);
+  return x;
+}
+// Every lane works out how many splits the last tile of one of up to 64 sequences has, so
+// that workgroups without work come last: a launch holds one for every split that a tile
+// may have, and an empty one among others costs them up to 9 ns.  us a call, by number
+// and so: 32 sequences of 4096 keys, groups of 7 and 15 heads, 29.6, 27.2 and 31.3, 28.7;
+// 64 of up to 4096, 14/2 heads of 64, 19.3, 17.4; 8 of up to 16000, 32/8 heads of 128,
+// 33.2, 30.7; groups of one head 25.9, 26.5; 4 chunks of 32 tokens over 8192 64.1, 66.9.
+[[maybe_unused]] __device__ inline TileWork work_by_length(const CacheAttn& a, const TileDivs& f, int lane, int block) {
+  const CacheView& c = a.c;
+  TileWork x{{c.n_seqs, 0, 0, 0}, -1, 0, 0, 0, 0, false};
+  const int item = f.heads.of(block);
+  x.kvh = block - item * c.hkv;
+  const int i = min(lane, c.n_seqs - 1);
+  const int from = clamp_row(c.cu[i], c.T), n = lane < c.n_seqs ? max(0, clamp_row(c.cu[i + 1], c.T) - from) : 0;
+  const int pos0 = c.kv_lens[i] - n, tiles = (n * a.group + 15) >> 4;
+  const long cap = (long)c.max_pages << c.page_shift, len = (long)pos0 + n;
+  const int kend = static_cast<int>(len < 0 ? 0 : len < cap ? len : cap);
+  KeySplit k{max(1, (kend + kSplitUnit - 1) / kSplitUnit) * kSplitUnit, 1};
+  if (a.n_splits > 1) k = split_with(kend, a.n_splits, a.split_keys, div_up);
+  const int items = tiles * k.active, end = lanes_up_to(items);
+  const unsigned long long mine = __ballot(item >= end - items && item < end);
+  if (mine == 0) return x;
+  const int b = __ffsll(mine) - 1, count = __builtin_amdgcn_readlane(tiles, b);
+  x.s.b = b;
+  x.s.tok0 = __builtin_amdgcn_readlane(from, b);
+  x.s.n = __builtin_amdgcn_readlane(n, b);
+  x.s.pos0 = __builtin_amdgcn_readlane(pos0, b);
+  x.per = __builtin_amdgcn_readlane(k.per, b);
+  x.active = __builtin_amdgcn_readlane(k.active, b);
+  x.split = item - __builtin_amdgcn_readlane(end - items, b);
+  int tile = 0;
+  if (count > 1) {
+    tile = __builtin_amdgcn_readfirstlane(div_up(x.split + 1, x.active) - 1);
+    x.split -= tile * x.active;
+  }
+  x.last = tile == count - 1;
+  // (more work than the launch has room for, as wrong offsets may have it, can wrap around)
+  x.r0 = tile >= 0 && tile < count && x.split >= 0 && x.split < x.active ? 16 * tile : -1;
+  return x;
+}
 
 template <typename T, int G>
 __global__ __launch_bounds__((64 * QaLayout<T, G>::WAVES), G <= 4 ? 3 : 2) void qcache_attn_kernel(CacheAttn a, TileDivs f) {
@@ -164,18 +237,19 @@ __global__ __launch_bounds__((64 * QaLayout<T, G>::WAVES), G <= 4 ? 3 : 2) void 
   extern __shared__ __align__(16) unsigned char smem[];
   const CacheView& c = a.c;
   const int w = wave_id(), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15, D = c.D;
-  const int rest = f.splits.of(blockIdx.x), number = f.heads.of(rest);
-  const int kvh = rest - number * c.hkv;
-  int split = blockIdx.x - rest * a.n_splits + number;  // (a tile's splits from another one on)
-  split -= f.splits.of(split) * a.n_splits;
-  const CacheSeq s = find_seq(c, lane, number, [&](int b, int to) { return (to * a.group >> 4) + b; });
-  const int b = s.b;
-  if (b >= c.n_seqs) return;
-  const int r0 = 16 * (number - (s.tok0 * a.group >> 4) - b), n_rows = s.n * a.group;
+  const TileWork x = f.by_length ? work_by_length(a, f, lane, blockIdx.x) : work_by_number(a, f, lane, blockIdx.x);
+  const CacheSeq& s = x.s;
+  const int b = s.b, r0 = x.r0, split = x.split, kvh = x.kvh, n_rows = s.n * a.group;
   if (r0 < 0 || r0 >= n_rows) return;
   const int tok0 = f.group.of(r0), head0 = r0 - tok0 * a.group;  // the tile's first row
   const int last = min(s.n - 1, tok0 + f.few_of(head0 + 15, a.group));
-  const TileKeys tk = keys_up_to(a, s, last);
+  TileKeys tk;
+  if (x.last) {
+    const long cap = (long)c.max_pages << c.page_shift, end = (long)s.pos0 + s.n;
+    tk = {static_cast<int>(end < 0 ? 0 : end < cap ? end : cap), x.per, x.active};
+  } else {
+    tk = keys_up_to(a, s, last);
+  }
   if (split >= tk.active) return;
   const int k0 = split * tk.per, k1 = min(tk.kend, k0 + tk.per);
 
@@ -632,9 +706,11 @@ template <typename T, int G>
 hipError_t attend(const CacheAttn& a, hipStream_t st) {
   constexpr int BYTES = QaLayout<T, G>::BYTES, WAVES = QaLayout<T, G>::WAVES;
   GL_CHECK(allow_lds(&qcache_attn_kernel<T, G>, BYTES));
-  const unsigned numbers = tile_numbers(a), heads = numbers * a.c.hkv, groups = heads * a.n_splits;
-  const TileDivs f{FixedDiv::by(a.n_splits, groups), FixedDiv::by(a.c.hkv, heads),
-                   FixedDiv::by(a.group, (unsigned long long)a.c.T * a.group), (65535u + a.group) / a.group};
+  const unsigned groups = tile_numbers(a) * a.c.hkv * a.n_splits;
+  // by length: several sequences, mostly of one tile (else few workgroups are empty)
+  const bool by_length = a.c.n_seqs > 1 && a.c.n_seqs <= 64 && (long)a.c.T * a.group <= 16L * a.c.n_seqs;
+  const TileDivs f{FixedDiv::by(a.n_splits, groups), FixedDiv::by(a.c.hkv, groups),
+                   FixedDiv::by(a.group, (unsigned long long)a.c.T * a.group), (65535u + a.group) / a.group, by_length};
   hipLaunchKernelGGL((qcache_attn_kernel<T, G>), dim3(groups), dim3(64 * WAVES), BYTES, st, a, f);
   return hipGetLastError();
 }
