@@ -3,7 +3,9 @@
 //
 // Reading the weights bounds it up to some tens of tokens, so they are read once a
 // workgroup, 16 bytes a lane, each word being what one lane feeds to one MFMA: 16 outputs
-// by 32 columns by 16 tokens.
+// by 32 columns by 16 tokens.  [1] 3584 -> 18944 twice (76 MB) 18.1 us, 4.2 TB/s with
+// start and end; 16 tokens, groups of 128 with offsets, 20.9; 64 tokens 43.5; 512 tokens
+// 202 to 224, 620 to 690 TFLOP/s.
 //   bf16: weights as 128 + n (one operation per two), the sum begun at -136 sum(x),
 //   which is one more product, with a constant; the scales are applied to the sums of
 //   a group.  The sums are 17 to 136 times the product's terms, which costs 4 to 8 of
