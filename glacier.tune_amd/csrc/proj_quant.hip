@@ -431,12 +431,13 @@ hipError_t by_group(const QuantCall& c, int group, bool off, hipStream_t st) {
 //   below 3000    1: 1 4 1   [16] 3584 -> 37888: 22.3 (1 2 4: 27.5, 1 4 4: 24.6); [128]
 //                            3584 -> 3584: 14.4; fp32 [16] 3584 -> 37888: 45.6 (2: 2 4 1:
 //                            63.3)
-//   more          2: 2 4 1   [24] 3584 -> 37888: 30.9 (1: 1 4 1: 32.9), [512] 3584 -> 4608:
-//                            44.6; fp32 the latter: 121.7 (1: 1 4 1: 143.9)
-//   40000 and more, bf16
-//                 4: 2 4 1   [512] 3584 -> 37888: 202 (2: 2 4 1: 213; with weights that
+//   more          2: 2 4 1   [24] 3584 -> 37888: 30.9 (1: 1 4 1: 32.9), [512] 4096 -> 6144:
+//                            48; fp32 [512] 3584 -> 4608: 121.7 (1: 1 4 1: 143.9)
+//   35000 and more, bf16
+//                 4: 2 4 1   [256] 3584 -> 37888: 117 (2: 2 4 1: 127), but [200]: 117 (109)
+//                            and [103]: 76 (68); [512]: 202 (213; with weights that
 //                            are not in the last-level cache 224; 4: 2 8 1 248, 4: 4 2 1
-//                            263), but [512] 3584 -> 4608: 51.  690 TFLOP/s: matrix
+//                            263), but [512] 4096 -> 6144: 55.  690 TFLOP/s: matrix
 //                            instructions are busy 41% of the time, vector ones 52%, and
 //                            two waves a SIMD, in step, hardly overlap them
 template <int TERMS>
@@ -450,7 +451,7 @@ hipError_t by_shape(const QuantCall& c, int group, bool off, hipStream_t st) {
   if (units < 1200) return by_group<TERMS, 1, 1, 4, 4>(c, group, off, st);
   if (units < 3000) return by_group<TERMS, 1, 1, 4, 1>(c, group, off, st);
   if constexpr (TERMS == 1)
-    if (units >= 40000) return by_group<TERMS, 4, 2, 4, 1>(c, group, off, st);
+    if (units >= 35000) return by_group<TERMS, 4, 2, 4, 1>(c, group, off, st);
   return by_group<TERMS, 2, 2, 4, 1>(c, group, off, st);
 }
 
