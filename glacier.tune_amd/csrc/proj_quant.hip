@@ -64,12 +64,19 @@ struct TileCfg {
   static constexpr int STRIDE = 20;  // floats of a token's 16 outputs in the join
   static constexpr int RING = KW * SLOTS * SLOT, JOIN = KW > 1 ? WAVES * RT * NT * 16 * STRIDE * 4 : 0;
   static constexpr int BYTES = RING > JOIN ? RING : JOIN;
+  // Offsets of groups of 32, four to a block: one fp32 product for it, of them and the
+  // sums of x, which every tile's sums begin with (bf16: -136 of them; fp32: they do not).
+  // Larger groups: the sums of x are kept apart and scaled with the others, vector
+  // instructions once a group.  [103] 3584 -> 37888 and [16], with offsets, groups of 32:
+  // 81 and 24.5 us (kept apart: 109 and 28).
+  static constexpr bool FOLD = OFF && GP == 4;
   // -136 sum(x) into the sums of every tile of outputs (one more product each), or kept
-  // apart and scaled with them (vector instructions, once a group)
+  // apart and scaled with them
   static constexpr bool CHAIN = TERMS == 1 && !OFF && (GP == 4 || RT == 1);
-  static constexpr bool SUMS = TERMS == 1 ? !CHAIN : OFF;  // sums of x of their own
+  static constexpr bool SUMS = !FOLD && (TERMS == 1 ? !CHAIN : OFF);  // sums of x of their own
   // loads of a step: a wave's share of x's operands, then its weights
-  static constexpr int XLOADS = 4 * NT * TERMS / RW, HALVES = GP == 4 ? 2 : 1, WLOADS = RT * (1 + HALVES * (OFF ? 2 : 1));
+  static constexpr int XLOADS = 4 * NT * TERMS / RW, HALVES = GP == 4 ? 2 : 1;
+  static constexpr int WLOADS = RT * (1 + HALVES * (OFF && !FOLD ? 2 : 1) + (FOLD ? 1 : 0));
 };
 
 template <int NT, int RT, int RW, int KW, int GP, bool OFF, int TERMS>
@@ -118,7 +125,7 @@ __global__ __launch_bounds__(64 * RW * KW) void quant_tile_kernel(QuantCall a) {
   };
   struct Words {
     u32x4 w[RT];
-    unsigned s[RT][2 * GP], o[RT][OFF ? 2 * GP : 1];
+    unsigned s[RT][2 * GP], o[RT][OFF && !C::FOLD ? 2 * GP : 1];
   };
   auto load = [&](Words& to, int step) __attribute__((always_inline)) {
     const int blk = min(step * KW + kw, a.blocks - 1);
@@ -127,7 +134,10 @@ __global__ __launch_bounds__(64 * RW * KW) void quant_tile_kernel(QuantCall a) {
       const int at = min(tile + r, tiles - 1) * a.blocks + blk;
       to.w[r] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, 16 * lane, at * 1024, 0));
       load_u32<2 * GP>(wr, 8 * GP * g, scales + at * 32 * GP, to.s[r]);
-      if constexpr (OFF) load_u32<2 * GP>(wr, 8 * GP * g, offsets + at * 32 * GP, to.o[r]);
+      if constexpr (C::FOLD)  // row col, group g
+        to.o[r][0] = __builtin_amdgcn_raw_buffer_load_b16(wr, 8 * col + 2 * g, offsets + at * 128, 0);
+      else if constexpr (OFF)
+        load_u32<2 * GP>(wr, 8 * GP * g, offsets + at * 32 * GP, to.o[r]);
     }
   };
   const QuantMagic magic;
@@ -144,21 +154,38 @@ __global__ __launch_bounds__(64 * RW * KW) void quant_tile_kernel(QuantCall a) {
   auto take = [&](const Words& from, unsigned slot_at) __attribute__((always_inline)) {
     u32x4 f[2][NT * TERMS];
     auto read = [&](int i) __attribute__((always_inline)) {
-      if constexpr (TERMS == 1) {
+      u32x4(&to)[NT * TERMS] = f[i % 2];
+      if constexpr (TERMS == 1 && !C::FOLD) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(f[i % 2][n]) : "v"(slot_at), "i"((4 * n + i) * 1024));
-      } else {  // (the compiler lets a sum pass through their registers: its write is waited for)
+          asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(to[n]) : "v"(slot_at), "i"((4 * n + i) * 1024));
+      // (else the compiler lets sums pass through the operands' registers: their writes are
+      // waited for)
+      } else if constexpr (TERMS == 1 && NT == 1) {
+        asm volatile("s_nop 7\n\tds_read_b128 %0, %1 offset:%2" : "=&v"(to[0]) : "v"(slot_at), "i"(i * 1024));
+      } else if constexpr (TERMS == 1 && NT == 2) {
+        asm volatile("s_nop 7\n\tds_read_b128 %0, %2 offset:%3\n\tds_read_b128 %1, %2 offset:%4"
+                     : "=&v"(to[0]), "=&v"(to[1])
+                     : "v"(slot_at), "i"(i * 1024), "i"((4 + i) * 1024));
+      } else if constexpr (TERMS == 1) {
+        static_assert(NT == 4, "reads of one, two or four operands");
+        asm volatile(
+            "s_nop 7\n\tds_read_b128 %0, %4 offset:%5\n\tds_read_b128 %1, %4 offset:%6\n\tds_read_b128 %2, %4 offset:%7\n\t"
+            "ds_read_b128 %3, %4 offset:%8"
+            : "=&v"(to[0]), "=&v"(to[1]), "=&v"(to[2]), "=&v"(to[3])
+            : "v"(slot_at), "i"(i * 1024), "i"((4 + i) * 1024), "i"((8 + i) * 1024), "i"((12 + i) * 1024));
+      } else {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
           asm volatile(
               "s_nop 7\n\tds_read_b128 %0, %3 offset:%4\n\tds_read_b128 %1, %3 offset:%5\n\tds_read_b128 %2, %3 offset:%6"
-              : "=&v"(f[i % 2][n]), "=&v"(f[i % 2][NT + n]), "=&v"(f[i % 2][2 * NT + n])
+              : "=&v"(to[n]), "=&v"(to[NT + n]), "=&v"(to[2 * NT + n])
               : "v"(slot_at), "i"((4 * n + i) * 1024), "i"((4 * (NT + n) + i) * 1024), "i"((4 * (2 * NT + n) + i) * 1024));
       }
     };
     read(0);
     f32x4 d[RT][NT], d0[NT];
+    float of_x[NT];  // of group g's columns and token col
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i < 3) {
@@ -183,10 +210,16 @@ __global__ __launch_bounds__(64 * RW * KW) void quant_tile_kernel(QuantCall a) {
 #pragma unroll
           for (int n = 0; n < NT; ++n) to[n] = Mfma<bf16>::mma(wf, __builtin_bit_cast(bf16x8, f[i % 2][NT * z + n]), to[n]);
       };
-      if constexpr (C::SUMS) add(minus, d0);
+      if constexpr (C::SUMS || C::FOLD) add(minus, d0);
+      if constexpr (C::FOLD)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) of_x[n] = i == 0 || g == i ? d0[n][0] : of_x[n];
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         if constexpr (C::CHAIN) add(minus, d[r]);
+        if constexpr (C::FOLD && TERMS == 1)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) d[r][n] = d0[n];
         if constexpr (TERMS == 1)
           add(raw8_bf16(from.w[r][i], magic), d[r]);
         else
@@ -200,7 +233,7 @@ __global__ __launch_bounds__(64 * RW * KW) void quant_tile_kernel(QuantCall a) {
           for (int e = 0; e < 4; ++e) {
             const float s = half_at(from.s[r][(e * GP + q) / 2], (e * GP + q) % 2);
             float o = s;  // of -136 sum(x)
-            if constexpr (OFF) {
+            if constexpr (OFF && !C::FOLD) {
               o = half_at(from.o[r][(e * GP + q) / 2], (e * GP + q) % 2);
               if constexpr (TERMS == 1) o = fmaf(o, -1.0f / 136.0f, s);
             }
@@ -212,6 +245,13 @@ __global__ __launch_bounds__(64 * RW * KW) void quant_tile_kernel(QuantCall a) {
           }
       }
     }
+    if constexpr (C::FOLD)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float o = half_at(from.o[r][0], 0) * (TERMS == 1 ? -1.0f / 136.0f : 1.0f);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) y[r][n] = Mfma<float>::mma(o, of_x[n], y[r][n]);
+      }
   };
   // (columns past the last one: x's last ones again, which meet scales of zero)
   const int steps = (a.blocks + KW - 1) / KW;
