@@ -26,4 +26,20 @@ constexpr KeySplit split_of(int kend, int n_splits, int split_keys) {
   return split_with(kend, n_splits, split_keys, [](int a, int b) { return (a + b - 1) / b; });
 }
 
+// Work numbered by the sequences' lengths: how many (tile, split) pairs a sequence of
+// `tiles` tiles stands for, `last` the splits of its last one.  An earlier tile may have
+// more splits than the last: past n_splits splits of split_keys a split grows by whole
+// units, so that one key more can leave fewer (4 of 256: 1024 keys take 4, 1025 take 3).
+// Sequences of several tiles therefore stand for all that a tile may have.
+constexpr int items_of(int tiles, int last, int n_splits) { return tiles > 1 ? tiles * n_splits : tiles * last; }
+struct TileItem {
+  int tile, split;
+};
+// The x-th of them.  down(a): a / n_splits.
+template <typename F>
+constexpr TileItem item_at(int x, int tiles, int n_splits, F down) {
+  const int tile = tiles > 1 ? down(x) : 0;
+  return {tile, x - tile * n_splits};
+}
+
 }  // namespace glacier
