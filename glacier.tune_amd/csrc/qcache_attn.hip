@@ -751,11 +751,11 @@ QCachePlan qcache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv,
   // 117 (153), of 32 214 (189); 32/8 heads in fp32, 4 of 32 over 2048: 36.2 (70.4).  They
   // lie in the workspace for whatever the table's rows can name (max_kv is a hint only):
   // up to 2^30 bytes of K and V, else tiles of 16 rows read the 4-bit pages however long
-  // the chunks are.
+  // the chunks are.  (Nor is there anything to write out of tables without a column.)
   const long group = hq / c.hkv, cap = (long)c.max_pages << c.page_shift;
   const long seqs = std::min(c.T, c.n_seqs);
   const size_t k_bytes = (size_t)c.n_seqs * c.max_pages * c.hkv * ((size_t)c.D << c.page_shift) * (c.io_bf16 ? 2 : 4);
-  p.expand = p.attn.rows > 16 && c.T * group > 256 * seqs && k_bytes <= (size_t)1 << 29;
+  p.expand = p.attn.rows > 16 && c.T * group > 256 * seqs && k_bytes > 0 && k_bytes <= (size_t)1 << 29;
   if (p.expand) {
     p.k_bytes = up256(k_bytes);
     p.table_bytes = up256(sizeof(int32_t) * c.n_seqs * c.max_pages);
