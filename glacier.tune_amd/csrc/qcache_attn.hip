@@ -42,6 +42,10 @@ namespace {
 [[maybe_unused]] constexpr int kKeysQ = 32;  // keys of a wave's block: one k-step of the second product
 constexpr int kWavesQ = 4;
 [[maybe_unused]] constexpr float kSlack = 8.0f;
+// Queries are multiplied as 2^-13 of themselves (exactly, but below 2^-113, whose products no
+// softmax sees), so that 32 of them times 143, of either sign, stay within fp32 whatever they
+// are, as they do over a cache in bf16 or fp32.  The scores' scale gives it back.
+constexpr float kQueryShare = 0x1p-13f;
 
 // LDS of a workgroup: its queries, operands of the first product (and -136 sum(q), where
 // its sums begin), then for each wave one block of K and one of V, words and then scales
@@ -300,7 +304,7 @@ __global__ __launch_bounds__((64 * QaLayout<T, G>::WAVES), G <= 4 ? 3 : 2) void 
         bf16x8 term[3];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float x = __builtin_bit_cast(f32x4, raw[e / 4])[e % 4];
+          const float x = kQueryShare * __builtin_bit_cast(f32x4, raw[e / 4])[e % 4];
           term[0][e] = (bf16)x;
           const float r1 = x - (float)term[0][e];
           term[1][e] = (bf16)r1;
@@ -309,7 +313,9 @@ __global__ __launch_bounds__((64 * QaLayout<T, G>::WAVES), G <= 4 ? 3 : 2) void 
 #pragma unroll
         for (int x = 0; x < 3; ++x) *reinterpret_cast<bf16x8*>(to + 1024 * x) = term[x];
       } else {
-        const bf16x8 x = __builtin_bit_cast(bf16x8, raw[0]);
+        bf16x8 x = __builtin_bit_cast(bf16x8, raw[0]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (bf16)(kQueryShare * (float)x[e]);
         *reinterpret_cast<bf16x8*>(to) = x;
         *reinterpret_cast<f32x4*>(to + 1024) = Mfma<bf16>::mma(minus, x, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
       }
@@ -706,7 +712,8 @@ __global__ __launch_bounds__(kExpandThreads) void qcache_expand_kernel(CacheView
 }
 
 template <typename T, int G>
-hipError_t attend(const CacheAttn& a, hipStream_t st) {
+hipError_t attend(CacheAttn a, hipStream_t st) {
+  a.scale_log2 /= kQueryShare;
   constexpr int BYTES = QaLayout<T, G>::BYTES, WAVES = QaLayout<T, G>::WAVES;
   GL_CHECK(allow_lds(&qcache_attn_kernel<T, G>, BYTES));
   const unsigned groups = tile_numbers(a) * a.c.hkv * a.n_splits;
