@@ -14,6 +14,7 @@
 // x A_p comes from a launch before, for more than 16 tokens from the kernel of the bf16
 // projections (proj_lora.hip); (x A_p) B_p by fp32 products into the same sums.
 #include "lds_mfma.hpp"
+#include "quant_grid.hpp"
 #include "quant_page.hpp"
 
 #include <algorithm>
@@ -31,7 +32,6 @@ struct QuantSpec {
 struct QuantCall {
   const void* x;
   int T, in, blocks, rank, splits, n, tiles, token_blocks;
-  int abreast;  // workgroups of one token block that are numbered in a row
   QuantSpec p[kMaxProj];
 };
 
@@ -86,13 +86,9 @@ __global__ __launch_bounds__(64 * RW * KW) void quant_tile_kernel(QuantCall a) {
   using IO = typename std::conditional<TERMS == 1, bf16, float>::type;
   extern __shared__ __align__(16) unsigned char smem[];
   const int w = wave_id() % RW, kw = wave_id() / RW, lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-  int number = blockIdx.x, t0 = 0;
-  if (a.token_blocks > 1) {  // (a tile's token blocks on one XCD, whose L2 has its weights then)
-    const int round = number / (a.abreast * a.token_blocks), rest = number - round * a.abreast * a.token_blocks;
-    number = round * a.abreast + rest % a.abreast;
-    t0 = rest / a.abreast * 16 * NT;
-  }
-  number = RW * number + w;
+  const QuantPlace place = quant_place(blockIdx.x, (a.tiles + RW - 1) / RW, a.token_blocks);
+  const int t0 = place.block * 16 * NT;
+  int number = RW * place.set + w;
   const bool has_tile = number < a.tiles;
   if (!has_tile) number = a.tiles - 1;  // (its wave takes part in the barriers)
   int p = 0;
@@ -443,9 +439,7 @@ hipError_t tiled(QuantCall c, hipStream_t st) {
     c.p[p].first = c.tiles;
     c.tiles += (c.p[p].out + 16 * RT - 1) / (16 * RT);
   }
-  const int groups = (c.tiles + RW - 1) / RW;
-  c.abreast = std::min(groups, 8);
-  const int grid = (groups + c.abreast - 1) / c.abreast * c.abreast * c.token_blocks;
+  const int grid = quant_grid((c.tiles + RW - 1) / RW, c.token_blocks);
   GL_CHECK(allow_lds((&quant_tile_kernel<NT, RT, RW, KW, GP, OFF, TERMS>), C::BYTES));
   hipLaunchKernelGGL((quant_tile_kernel<NT, RT, RW, KW, GP, OFF, TERMS>), dim3(grid),
                      dim3(64 * C::WAVES), C::BYTES, st, c);
