@@ -80,7 +80,8 @@ struct CachePlan {
 };
 CachePlan cache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv, int n_cu);
 hipError_t launch_cache_attn(const CacheAttn& a, hipStream_t st);
-// Joins the splits' sums of tiles of at most 32 rows (a.n_splits > 1).
+// Joins the splits' sums row by row (a.n_splits > 1): those of tiles of at most 32 rows, and
+// of 128 rows with more than kCacheTileJoin splits.
 hipError_t launch_cache_join(const CacheAttn& a, hipStream_t st);
 
 constexpr int kCacheWideRows = 128;  // rows of a tile of cache_attn_wide.hip

@@ -3,14 +3,17 @@
 // Tiles, splits and the join are those of cache_attn.hip: 16 rows are (token, head of
 // the group) pairs of one KV head, a workgroup's four waves take 32 keys at a time in
 // turn, each with its own running maximum and sum, joined through LDS at the end.  K
-// and V go from the pages into registers and, unpacked there, straight into the
-// matrix cores: a word of a page holds what one lane feeds to one MFMA, and pages are
-// laid out so that a lane's words lie together.
+// and V come from the pages by LDS DMA, as they lie there, into an area of each wave,
+// and are unpacked in registers, straight into the matrix cores: a word of a page holds
+// what one lane feeds to one MFMA, and pages are laid out so that a lane's words lie
+// together.
 //
 // S^T = K Q^T, 16 keys by 16 rows, 32 columns (one group) at a time.
 //   bf16: K as 128 + n (one operation per two elements), the sum begun at -136 sum(q),
 //   and the scales applied to the product: S += s (K' q - 136 sum q).  The sums are 17
-//   to 136 times the product's terms, which costs 4 to 8 of fp32's 24 bits.
+//   to 136 times the product's terms, which costs 4 to 8 of fp32's 24 bits: a score is
+//   then off by some 2^-20 of its terms' length, far below what rounding its operands
+//   to bf16 has cost, and n - 8 instead takes four operations for one.
 //   fp32: K as n - 8, q in three bf16 terms (24 bits).
 // O^T += V^T P^T, 32 tokens at a time.  Two tokens' words, their halves exchanged, hold
 // eight columns of both: a lane's words are the operands of eight products (columns 8 x
@@ -18,8 +21,8 @@
 // word's halves).
 //   V as bf16 (n - 8) s, exact (five bits by three): (1024 + n) s - 1032 s, or (64 + n) s
 //   - 72 s, where the sum in brackets is an fp16 value by one OR, formed by fp32
-//   operations that take fp16 operands, of whose results the upper halves are kept.  The weights in two bf16 terms (16 bits of
-//   them; fp32: three).
+//   operations that take fp16 operands, of whose results the upper halves are kept.
+//   The weights in two bf16 terms (16 bits of them; fp32: three).
 //
 // A held value is NaN only by its scale (it is never infinite).  Where a sum is not
 // finite the wave walks its keys once more with such scales of V cleared, and gives

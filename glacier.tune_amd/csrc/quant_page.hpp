@@ -6,7 +6,8 @@
 // three, so a held value is exact in bf16 and in fp16, and no kernel rounds it.  A
 // word's eight numbers lie so that (word >> 4 j) & 0x000f000f are neighbouring
 // columns 2 j and 2 j + 1 in the two halves of a register: one more OR makes them
-// floats 128 + n (bf16) or 16 + n (fp16, shifted), exact, without a conversion.
+// floats 128 + n (bf16) or 1024 + n (fp16; bits 4 to 7 of a half 64 + n), exact, without
+// a conversion.
 #pragma once
 
 #include "attn_common.hpp"
@@ -14,7 +15,7 @@
 
 namespace glacier {
 
-constexpr float kQuantScaleMax = 2688.0f;  // five bits; 24 times it is an fp16 value
+constexpr float kQuantScaleMax = 2688.0f;  // the format's largest scale: 21 x 2^7, five bits
 constexpr unsigned kQuantNan = 0x7e00u;    // scale of a group that is not finite
 constexpr unsigned kQuantZero = 0x88888888u;  // a word of zeros
 
