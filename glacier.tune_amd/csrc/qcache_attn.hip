@@ -11,9 +11,10 @@
 // S^T = K Q^T, 16 keys by 16 rows, 32 columns (one group) at a time.
 //   bf16: K as 128 + n (one operation per two elements), the sum begun at -136 sum(q),
 //   and the scales applied to the product: S += s (K' q - 136 sum q).  The sums are 17
-//   to 136 times the product's terms, which costs 4 to 8 of fp32's 24 bits: a score is
-//   then off by some 2^-20 of its terms' length, far below what rounding its operands
-//   to bf16 has cost, and n - 8 instead takes four operations for one.
+//   to 136 times the product's terms, which costs 4 to 8 of fp32's 24 bits: scores of
+//   random queries are off by 7 x 2^-24 of their terms' length (root of squares; direct
+//   sums 1 x 2^-24), far below what rounding q to bf16 has cost.  n - 8 instead would take
+//   five operations more for two elements, where unpacking is what bounds single tokens.
 //   fp32: K as n - 8, q in three bf16 terms (24 bits).
 // O^T += V^T P^T, 32 tokens at a time.  Two tokens' words, their halves exchanged, hold
 // eight columns of both: a lane's words are the operands of eight products (columns 8 x
@@ -761,7 +762,10 @@ QCachePlan qcache_attn_plan(const CacheView& c, int hq, int max_new, int max_kv,
   // 117 (153), of 32 214 (189); 32/8 heads in fp32, 4 of 32 over 2048: 36.2 (70.4).  They
   // lie in the workspace for whatever the table's rows can name (max_kv is a hint only):
   // up to 2^30 bytes of K and V, else tiles of 16 rows read the 4-bit pages however long
-  // the chunks are.  (Nor is there anything to write out of tables without a column.)
+  // the chunks are.  (Nor is there anything to write out of tables without a column.)  What
+  // the mean and the table's width cost: 2048 tokens over 8192 beside 57 single ones over 4096
+  // 588, 325 and 40 in two calls; 17 of 128 over 2048 in a table of 32768 tokens 210, of 2048
+  // 125; 2048 over 2048 in one of 131072, whose whole width the launch covers, 90, of 2048 75.
   const long group = hq / c.hkv, cap = (long)c.max_pages << c.page_shift;
   const long seqs = std::min(c.T, c.n_seqs);
   const size_t k_bytes = (size_t)c.n_seqs * c.max_pages * c.hkv * ((size_t)c.D << c.page_shift) * (c.io_bf16 ? 2 : 4);

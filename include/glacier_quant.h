@@ -83,9 +83,13 @@ int glacier_attn_qcache_read(glacier_attn_ctx *ctx, const glacier_kv_cache *cach
 size_t glacier_attn_qcache_workspace(glacier_attn_ctx *ctx, const glacier_kv_cache *cache,
                                      const glacier_cache_batch *batch, int32_t n_heads_q);
 
-/* glacier_attn_cache_forward over 4-bit pages, which are read exactly: weights
- * multiply V as two bf16 terms, 16 bits of them (bf16 tensors), or to fp32 rounding
- * (fp32 tensors).  A NaN in the pages reaches only the rows that see its token. */
+/* glacier_attn_cache_forward over 4-bit pages, which are read exactly.  fp32 tensors:
+ * to fp32 rounding.  bf16 tensors: a score, and so lse, is an fp32 sum of terms (128
+ * + n) s q and -136 s q, whose additions are off by 2^-24 of sums of up to 143 |s| |q|
+ * each (random queries: the score by 2^-21 of its terms' length, as a root mean
+ * square), and weights multiply V as two bf16 terms, 16 bits of them.  Queries may have
+ * any finite size for which q k stays within fp32.  A NaN in the pages reaches only the
+ * rows that see its token. */
 int glacier_attn_qcache_forward(glacier_attn_ctx *ctx, const glacier_kv_cache *cache,
                                 const glacier_cache_batch *batch, int32_t n_heads_q, const void *q,
                                 void *out, float *lse, void *workspace, size_t workspace_bytes);
@@ -121,8 +125,9 @@ typedef struct glacier_quant_proj_desc {
   int32_t group;         /* of every projection's weights */
   int32_t offsets;       /* likewise */
   int32_t rank;          /* 1..GLACIER_PROJ_MAX_RANK when any adapter is given */
-  int32_t io_dtype;      /* GLACIER_ATTN_IO_*: x and y.  F32: to fp32 rounding; BF16: fp32
-                            sums, each output rounded once */
+  int32_t io_dtype;      /* GLACIER_ATTN_IO_*: x and y.  F32: to fp32 rounding; BF16: fp32 sums
+                            of terms (128 + n) s x and -136 s x, whose additions are off by
+                            2^-24 of sums of up to 143 |s| |x| each; each output rounded once */
 } glacier_quant_proj_desc;
 
 /* Bytes of device workspace glacier_proj_quant_forward needs (0 if it needs none,
