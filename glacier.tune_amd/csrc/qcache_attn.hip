@@ -46,9 +46,9 @@ namespace {
 [[maybe_unused]] constexpr int kKeysQ = 32;  // keys of a wave's block: one k-step of the second product
 constexpr int kWavesQ = 4;
 [[maybe_unused]] constexpr float kSlack = 8.0f;
-// Queries are multiplied as 2^-13 of themselves (exactly, but below 2^-113, whose products no
-// softmax sees), so that 32 of them times 143, of either sign, stay within fp32 whatever they
-// are, as they do over a cache in bf16 or fp32.  The scores' scale gives it back.
+// Queries are multiplied as 2^-13 of themselves (exactly, but for bits below 2^-120 of q, which
+// no softmax sees), so that 32 of them times 143, of either sign, stay within fp32 whatever
+// they are, as they do over a cache in bf16 or fp32.  The scores' scale gives it back.
 constexpr float kQueryShare = 0x1p-13f;
 
 // LDS of a workgroup: its queries, operands of the first product (and -136 sum(q), where
