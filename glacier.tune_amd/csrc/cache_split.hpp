@@ -26,20 +26,21 @@ constexpr KeySplit split_of(int kend, int n_splits, int split_keys) {
   return split_with(kend, n_splits, split_keys, [](int a, int b) { return (a + b - 1) / b; });
 }
 
-// Work numbered by the sequences' lengths: how many (tile, split) pairs a sequence of
-// `tiles` tiles stands for, `last` the splits of its last one.  An earlier tile may have
-// more splits than the last: past n_splits splits of split_keys a split grows by whole
-// units, so that one key more can leave fewer (4 of 256: 1024 keys take 4, 1025 take 3).
-// Sequences of several tiles therefore stand for all that a tile may have.
-constexpr int items_of(int tiles, int last, int n_splits) { return tiles > 1 ? tiles * n_splits : tiles * last; }
-struct TileItem {
-  int tile, split;
-};
-// The x-th of them.  down(a): a / n_splits.
+// Work numbered by the sequences' lengths: how many splits each tile of a sequence of `tiles`
+// tiles and kend keys stands for; `last`: those that its last tile has.  An earlier tile,
+// which sees fewer keys, may have more than the last: a split has split_keys keys as long as
+// n_splits of them reach, and grows by whole units then, so that one key more can leave fewer
+// (4 of 256: 1024 keys take 4, 1025 take 3).  Splits of split_keys that the keys would take,
+// n_splits at most, are the most that a tile of so many keys or fewer has; while n_splits
+// reach they are the last one's.  (n_splits for each tile would do, but leaves workgroups
+// without work: 8 sequences of 4 tokens over 300 keys beside 24 single ones over up to 8192,
+// 28/4 heads of 128, 28.7 us so and 33 with n_splits.)
 template <typename F>
-constexpr TileItem item_at(int x, int tiles, int n_splits, F down) {
-  const int tile = tiles > 1 ? down(x) : 0;
-  return {tile, x - tile * n_splits};
+constexpr int splits_a_tile(int tiles, int last, int kend, int n_splits, int split_keys, F up) {
+  if (tiles <= 1 || n_splits == 1) return last;
+  const int keys = (kend + kSplitUnit - 1) / kSplitUnit, given = (split_keys + kSplitUnit - 1) / kSplitUnit;
+  const int most = up(keys, given < 1 ? 1 : given);
+  return most < 1 ? 1 : most < n_splits ? most : n_splits;
 }
 
 }  // namespace glacier

@@ -202,7 +202,7 @@ struct TileWork {
   if (x.s.b < c.n_seqs) x.r0 = 16 * (number - (x.s.tok0 * a.group >> 4) - x.s.b);
   return x;
 }
-// Every lane works out how many splits the tiles of one of up to 64 sequences have (items_of),
+// Every lane works out how many splits the tiles of one of up to 64 sequences have (splits_a_tile),
 // so that workgroups without work come last: a launch holds one for every split that a tile
 // may have, and an empty one among others costs them up to 9 ns.  us a call, by number
 // and so: 32 sequences of 4096 keys, groups of 7 and 15 heads, 29.6, 27.2 and 31.3, 28.7;
@@ -220,7 +220,8 @@ struct TileWork {
   const int kend = static_cast<int>(len < 0 ? 0 : len < cap ? len : cap);
   KeySplit k{max(1, (kend + kSplitUnit - 1) / kSplitUnit) * kSplitUnit, 1};
   if (a.n_splits > 1) k = split_with(kend, a.n_splits, a.split_keys, div_up);
-  const int items = items_of(tiles, k.active, a.n_splits), end = lanes_up_to(items);
+  const int each = splits_a_tile(tiles, k.active, kend, a.n_splits, a.split_keys, div_up);
+  const int items = tiles * each, end = lanes_up_to(items);
   const unsigned long long mine = __ballot(item >= end - items && item < end);
   if (mine == 0) return x;
   const int b = __ffsll(mine) - 1, count = __builtin_amdgcn_readlane(tiles, b);
@@ -230,12 +231,16 @@ struct TileWork {
   x.s.pos0 = __builtin_amdgcn_readlane(pos0, b);
   x.per = __builtin_amdgcn_readlane(k.per, b);
   x.active = __builtin_amdgcn_readlane(k.active, b);
-  const int at = item - __builtin_amdgcn_readlane(end - items, b);
-  const TileItem i_at = item_at(at, count, a.n_splits, [&](int y) { return f.splits.of(y); });
-  x.split = i_at.split;
-  x.last = i_at.tile == count - 1;
+  const int per_tile = __builtin_amdgcn_readlane(each, b);
+  x.split = item - __builtin_amdgcn_readlane(end - items, b);
+  int tile = 0;
+  if (count > 1) {
+    tile = __builtin_amdgcn_readfirstlane(div_up(x.split + 1, per_tile) - 1);
+    x.split -= tile * per_tile;
+  }
+  x.last = tile == count - 1;
   // (more work than the launch has room for, as wrong offsets may have it, can wrap around)
-  x.r0 = at >= 0 && i_at.tile < count && x.split >= 0 && x.split < a.n_splits ? 16 * i_at.tile : -1;
+  x.r0 = tile >= 0 && tile < count && x.split >= 0 && x.split < per_tile ? 16 * tile : -1;
   return x;
 }
 

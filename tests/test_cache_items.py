@@ -1,7 +1,8 @@
 """Which workgroup takes which split of which tile where the work of a 4-bit cache's attention
 is numbered by the sequences' lengths (glacier.tune_amd/csrc/cache_split.hpp), compiled for
-the CPU: every split that the join counts is taken once, whatever max_kv said, and a launch
-by number of tiles has room for all of them."""
+the CPU: every split that the join counts is taken once, whatever max_kv said, a launch by
+number of tiles has room for all of them, and where max_kv holds none is taken in vain but
+those that only a sequence's last tile has."""
 import os
 import shutil
 import subprocess
@@ -34,12 +35,14 @@ static bool check(const std::vector<Seq>& seqs, int group, int n_splits, int spl
     const int tiles = (s.n * group + 15) / 16;
     const int last = split_of(std::max(0, s.kv), n_splits, split_keys).active;
     std::vector<int> taken(tiles * n_splits, 0);
-    const int items = items_of(tiles, last, n_splits);
-    for (int x = 0; x < items; ++x) {
-      const TileItem i = item_at(x, tiles, n_splits, [&](int a) { return a / n_splits; });
-      if (i.tile < 0 || i.tile >= tiles || i.split < 0 || i.split >= n_splits) return false;
-      ++taken[i.tile * n_splits + i.split];
+    const int each = splits_a_tile(tiles, last, std::max(0, s.kv), n_splits, split_keys,
+                                   [](int a, int b) { return (a + b - 1) / b; });
+    const int items = tiles * each;
+    if (each < 1 || each > n_splits || (s.kv <= n_splits * split_keys && each != last)) {
+      std::printf("%d keys: %d splits a tile, %d of the last (%d of %d)\\n", s.kv, each, last, n_splits, split_keys);
+      return false;
     }
+    for (int x = 0; x < items; ++x) ++taken[x / each * n_splits + x % each];
     for (int t = 0; t < tiles; ++t) {
       const int active = split_of(keys_of(t, s.n, s.kv, group), n_splits, split_keys).active;
       for (int u = 0; u < n_splits; ++u)
